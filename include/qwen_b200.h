@@ -381,6 +381,130 @@ int qwen_gemm_bf16(const void* A, const void* B, void* C, int M, int N, int K, i
  * scratch (4 x rows x ceil(n / 512) x k words) and synchronizes `stream`. */
 int qwen_row_topk(const float* logits, int rows, int n, int ld, int k, float* values, int* ids, void* stream);
 
+/* ---- drafted-token decoding over a K/V cache (no reference counterpart) ---- */
+/* The operators of one step of decoding with drafted tokens, on caller-owned
+ * device memory: rows enter a cache in 16 or 8 bits and are read back, the
+ * drafted tokens' queries attend to the cache and to their own branch, the
+ * drafted tokens are checked against the target's probabilities, and the kept
+ * branch's rows move up behind the context.  (The reference decodes one token
+ * per step over a bf16 cache, main.cu:141-145.)
+ *
+ * Common rules.  Every pointer that a call takes is device memory of the
+ * current device, 16-byte aligned where it holds rows (k, v, q, out, the
+ * cache) and 4-byte aligned elsewhere; the calls are asynchronous on `stream`
+ * (a cudaStream_t of the current device, NULL = legacy default stream), allocate
+ * nothing, copy nothing from or to the host and may be captured.  Lengths,
+ * trees and counts are read on the device, so a captured call follows them;
+ * whatever they hold, nothing outside the described buffers is touched.
+ * Sequences are the rows 0 .. n_seqs - 1 of the view (at most 65535).
+ *
+ * A tree of n_nodes drafted tokens (1 .. 64) is given by parents[seq][node]:
+ * -1 for a root, else a smaller node index.  Any other value marks an absent
+ * node (a padded entry), and nodes below an absent node are absent too. */
+#define QWEN_BF16 0
+#define QWEN_FP16 1
+#define QWEN_FP32 2
+#define QWEN_E4M3 3   /* 8-bit floating point, 4 exponent and 3 mantissa bits, largest value 448 */
+#define QWEN_INT8 4   /* -127 .. 127 */
+
+/* One layer (or any set of heads) of a cache: position p of head h of sequence
+ * s is the head_dim elements at k + s * seq_stride + h * head_stride + p *
+ * head_dim (elements; strides are positive multiples of head_dim, heads and
+ * sequences do not overlap).  dtype QWEN_BF16, QWEN_FP16, QWEN_E4M3 or QWEN_INT8.
+ * The 8-bit types have one fp32 scale per row at k_scale + (s * seq_stride +
+ * h * head_stride) / head_dim + p; a row's values are code * scale.  The scale
+ * pointers are NULL for the 16-bit types.  head_dim is 64 or 128. */
+typedef struct {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    long long seq_stride, head_stride;
+    int dtype, n_seqs, n_kv_heads, head_dim, capacity;
+} qwen_kv_cache_t;
+
+/* The view of layer `layer` of a handle's batch slots (qwen_batch_init first;
+ * slot = sequence), or with layer = -1 of all layers at once (their heads one
+ * after the other).  The handle owns the memory. */
+int qwen_batch_cache(qwen_t* ctx, int layer, qwen_kv_cache_t* out);
+
+/* Rows into the cache: token t (0 .. n_tokens-1) of sequence s, at k + (s *
+ * n_tokens + t) * ld elements (head h at + h * head_dim; ld a multiple of 8,
+ * at least n_kv_heads * head_dim), becomes position start[s] + t, for t <
+ * counts[s] (counts NULL: all).  src_dtype QWEN_BF16, QWEN_FP16 or QWEN_FP32.
+ * A row of an 8-bit cache with largest magnitude a (at least 2^-60) gets the
+ * scale a / 448 (QWEN_E4M3) or a / 127 (QWEN_INT8), rounded once to fp32, and
+ * each code is the nearest one to x * 448 / a (x * 127 / a), ties to even; a
+ * row that holds an infinity or NaN gets the scale NaN (and reads back as NaN).
+ * 16-bit caches take the values rounded to their type.  Positions outside the
+ * cache are not written; start[s] < 0 leaves sequence s as it was. */
+int qwen_kv_append(const qwen_kv_cache_t* cache, const void* k, const void* v, int src_dtype, long long ld, int n_tokens,
+                   const int* start, const int* counts, void* stream);
+
+/* qwen_kv_append's inverse: positions start[s] + t, t < counts[s], to rows
+ * (s * n_tokens + t) of k and v (ld elements apart, dst_dtype), each value code
+ * * scale in fp32 rounded once to dst_dtype.  Rows of positions outside the
+ * cache, of t >= counts[s] and of sequences with start[s] < 0 stay as they were. */
+int qwen_kv_read(const qwen_kv_cache_t* cache, void* k, void* v, int dst_dtype, long long ld, int n_tokens, const int* start,
+                 const int* counts, void* stream);
+
+/* The kept branch's rows: position start[s] + i receives what position start[s]
+ * + path[s][i] held before the call, for i < n_path[s] (path is [n_seqs][n_nodes],
+ * n_nodes 1 .. 64; any order and repeats are allowed).  Entries outside 0 ..
+ * n_nodes-1 and positions outside the cache are left out; start[s] < 0 or
+ * n_path[s] <= 0 leaves sequence s as it was.  With qwen_tree_verify's path and
+ * n_path, and start = the length that qwen_tree_attention was given, the cache
+ * then holds start[s] + n_path[s] positions. */
+int qwen_kv_keep(const qwen_kv_cache_t* cache, const int* start, const int* path, const int* n_path, int n_nodes, void* stream);
+
+/* Bytes of workspace that qwen_tree_attention needs for these sizes. */
+int qwen_tree_attention_workspace(const qwen_kv_cache_t* cache, int n_nodes, int n_heads, size_t* bytes);
+
+/* Attention of a tree of drafted tokens over a cache whose positions lens[s] +
+ * i already hold the nodes' own K and V (qwen_kv_append): node i of sequence s
+ * attends to positions 0 .. lens[s]-1, to its ancestors and to itself,
+ * o = sum_j softmax_j(scale * q . k_j) v_j, and query head h to K/V head
+ * h / (n_heads / n_kv_heads).  One root and no other node is an ordinary decode
+ * step; a chain of nodes is a causal step of several tokens.  q and out are
+ * [n_seqs][n_nodes][n_heads][head_dim] with ldq and ldo elements between nodes
+ * (multiples of 8, at least n_heads * head_dim), dtype QWEN_BF16 or QWEN_FP16, that of
+ * a 16-bit cache; out is not q.  Rows of absent nodes become 0; nodes whose
+ * position lies outside the cache, and all nodes of sequences with lens[s] < 0,
+ * are absent.  What positions that a node does not see hold (NaN included) has
+ * no influence on it.  Scores, softmax statistics and sums are fp32; the
+ * weights enter the product with V in 16 bits.  workspace: as many bytes as
+ * qwen_tree_attention_workspace says, contents free, 16-byte aligned; calls
+ * that may overlap need one each. */
+int qwen_tree_attention(const qwen_kv_cache_t* cache, const void* q, void* out, int dtype, long long ldq, long long ldo, int n_nodes,
+                        int n_heads, const int* lens, const int* parents, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Which drafted tokens the target model keeps, and the token after them.
+ * logits: the target's, [n_seqs][n_nodes][vocab], rows ld elements apart
+ * (logits_dtype QWEN_FP32, QWEN_BF16 or QWEN_FP16); row i is the distribution p =
+ * softmax(logits / temperature) of the token after node i.  Node 0 is the last
+ * token already known (the only root that the walk starts from); tokens[s][i]
+ * is node i's token.  From node 0 on, the present children of the reached node are
+ * tried in index order; a child with token x is kept, and becomes the reached
+ * node, if
+ *     uniforms[s][child] * left * q(x) < rest(x),
+ * where rest = p and left = 1 at first, and after a refusal
+ *     rest = max(rest - left * q, 0), left = the sum of rest:
+ * the kept tokens and the one after them are then distributed as the target's
+ * own samples, if every child was drawn from q, its parent's row of draft
+ * ([n_seqs][n_nodes][vocab] fp32 probabilities, rows ld_draft apart).  draft
+ * NULL: the children are the drafter's chosen tokens, q(x) = 1 for the child's
+ * token alone, so a refusal takes x out of rest.  When no child is kept,
+ * next[s] is the smallest token whose running sum of rest exceeds
+ * uniforms[s][0] * left (of p, if nothing is left).  uniforms ([n_seqs][n_nodes]
+ * fp32) lie in [0, 1).  temperature 0: p is 1 at the largest logit (ties to the
+ * smaller token), draft and uniforms are not read and may be NULL.  Tokens cut
+ * by top-k or top-p enter with logits of -inf.  A row with a NaN, a +inf or
+ * nothing above -inf has no distribution: no child is kept there and next[s] =
+ * -1.  Outputs: path[s][n_nodes] the kept nodes from node 0 on, then -1;
+ * n_path[s] their number (0, and next -1, if node 0 is not a root); next[s].
+ * temperature is 0 or within 1e-6 .. 1e6. */
+int qwen_tree_verify(const void* logits, int logits_dtype, long long ld, const float* draft, long long ld_draft, const int* tokens,
+                     const int* parents, const float* uniforms, int n_seqs, int n_nodes, int vocab, float temperature, int* path,
+                     int* n_path, int* next, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,361 @@
+// draft_ops.cu — the C ABI of the drafted-token operators (qwen_kv_append,
+// qwen_kv_read, qwen_kv_keep, qwen_tree_attention, qwen_tree_verify): argument
+// checks, variant choice and launches.  No reference counterpart (the
+// reference decodes one token per step, main.cu:141-145).
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <climits>
+#include <cmath>
+#include <initializer_list>
+#include <string>
+
+#include "../../include/qwen_b200.h"
+#include "kv_rows.cuh"
+#include "tree_attention.cuh"
+#include "tree_verify.cuh"
+
+int qwen_internal_fail(int code, const std::string& msg);
+
+namespace {
+
+int fail(int code, const std::string& msg) { return qwen_internal_fail(code, msg); }
+#define CU(call)                                                                                        \
+    do {                                                                                                \
+        cudaError_t e_ = (call);                                                                        \
+        if (e_ != cudaSuccess) return fail(QWEN_E_CUDA, std::string(#call) + ": " + cudaGetErrorString(e_)); \
+    } while (0)
+#define TRY(call)                          \
+    do {                                   \
+        int rc_ = (call);                  \
+        if (rc_ != QWEN_OK) return rc_;    \
+    } while (0)
+
+// ---- argument checks -----------------------------------------------------------
+struct Ptr {
+    const void* p;
+    const char* name;
+    size_t align;
+    bool used;   // false: may be anything
+};
+// NULL and alignment first (no GPU needed), then: device memory of the current device, *dev.
+int check_ptrs(std::initializer_list<Ptr> ptrs, int* dev) {
+    for (const Ptr& a : ptrs) {
+        if (!a.used) continue;
+        if (!a.p) return fail(QWEN_E_ARG, std::string(a.name) + " is NULL");
+        if ((uintptr_t)a.p % a.align) return fail(QWEN_E_ARG, std::string(a.name) + " must be " + std::to_string(a.align) + "-byte aligned");
+    }
+    CU(cudaGetDevice(dev));
+    for (const Ptr& a : ptrs) {
+        if (!a.used) continue;
+        cudaPointerAttributes at;
+        const cudaError_t e = cudaPointerGetAttributes(&at, a.p);
+        if (e != cudaSuccess) cudaGetLastError();   // not left behind for the caller's next query
+        if (e != cudaSuccess || (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged))
+            return fail(QWEN_E_ARG, std::string(a.name) + " is not device memory");
+        if (at.type == cudaMemoryTypeDevice && at.device != *dev)
+            return fail(QWEN_E_ARG, std::string(a.name) + " lies on another device than the current one");
+    }
+    return QWEN_OK;
+}
+bool is16(int t) { return t == QWEN_BF16 || t == QWEN_FP16; }
+bool is8(int t) { return t == QWEN_E4M3 || t == QWEN_INT8; }
+
+int check_view(const qwen_kv_cache_t* c) {
+    if (!c) return fail(QWEN_E_ARG, "NULL cache view");
+    if (!is16(c->dtype) && !is8(c->dtype)) return fail(QWEN_E_ARG, "cache dtype must be QWEN_BF16, QWEN_FP16, QWEN_E4M3 or QWEN_INT8");
+    if (c->head_dim != 64 && c->head_dim != 128) return fail(QWEN_E_UNSUPPORTED, "head_dim must be 64 or 128");
+    if (c->n_seqs < 1 || c->n_seqs > 65535) return fail(QWEN_E_ARG, "n_seqs out of [1, 65535]");
+    if (c->n_kv_heads < 1 || c->n_kv_heads > 65535) return fail(QWEN_E_ARG, "n_kv_heads out of [1, 65535]");
+    if (c->capacity < 1 || c->capacity > 1 << 30) return fail(QWEN_E_ARG, "capacity out of [1, 2^30]");
+    const long long row = (long long)c->capacity * c->head_dim;
+    if (c->head_stride % c->head_dim || c->seq_stride % c->head_dim || (c->n_kv_heads > 1 && c->head_stride < row) ||
+        (c->n_seqs > 1 && c->seq_stride < row) || c->head_stride < 0 || c->seq_stride < 0)
+        return fail(QWEN_E_ARG, "strides must be multiples of head_dim and at least capacity * head_dim");
+    if (is16(c->dtype) && (c->k_scale || c->v_scale)) return fail(QWEN_E_ARG, "a 16-bit cache has no scales");
+    return QWEN_OK;
+}
+// The view's pointers, as check_ptrs takes them.
+#define QB_VIEW_PTRS(c)                                                                                              \
+    Ptr{(c)->k, "cache k", 16, true}, Ptr{(c)->v, "cache v", 16, true}, Ptr{(c)->k_scale, "cache k_scale", 4, is8((c)->dtype)}, \
+        Ptr{(c)->v_scale, "cache v_scale", 4, is8((c)->dtype)}
+qb::kv::Cache device_view(const qwen_kv_cache_t* c) {
+    return qb::kv::Cache{(uint8_t*)c->k, (uint8_t*)c->v, c->k_scale, c->v_scale, c->seq_stride, c->head_stride, c->capacity};
+}
+int sm_count(int dev, int* n) {
+    static std::atomic<int> known[64];
+    if (dev < 0 || dev >= 64) return fail(QWEN_E_ARG, "device index beyond 63");
+    int v = known[dev].load();
+    if (!v) {
+        CU(cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev));
+        known[dev].store(v);
+    }
+    *n = v;
+    return QWEN_OK;
+}
+// Sets a kernel's shared-memory limit once per device (not a stream operation: allowed during capture).
+template <typename K>
+int smem_limit(K kernel, std::atomic<uint64_t>& done, int dev, int bytes) {
+    if (!((done.load() >> dev) & 1)) {
+        CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        done.fetch_or(1ull << dev);
+    }
+    return QWEN_OK;
+}
+
+// ---- cache rows -------------------------------------------------------------------
+template <template <int, int, int> class F, typename... A>
+int by_types(int rows, int store, int dim, A... a) {
+#define QB_STORES(R, D)                                                      \
+    switch (store) {                                                         \
+        case QWEN_BF16: return F<R, QWEN_BF16, D>::go(a...);                 \
+        case QWEN_FP16: return F<R, QWEN_FP16, D>::go(a...);                 \
+        case QWEN_E4M3: return F<R, QWEN_E4M3, D>::go(a...);                 \
+        default: return F<R, QWEN_INT8, D>::go(a...);                        \
+    }
+#define QB_ROWS(D)                                                           \
+    switch (rows) {                                                          \
+        case QWEN_BF16: QB_STORES(QWEN_BF16, D)                              \
+        case QWEN_FP16: QB_STORES(QWEN_FP16, D)                              \
+        default: QB_STORES(QWEN_FP32, D)                                     \
+    }
+    if (dim == 64) { QB_ROWS(64) }
+    QB_ROWS(128)
+#undef QB_ROWS
+#undef QB_STORES
+}
+
+template <int R, int S, int D>
+struct Append {
+    static int go(const qwen_kv_cache_t* c, const void* k, const void* v, long long ld, int n_tokens, const int* start, const int* counts,
+                  cudaStream_t st) {
+        const unsigned rows = (unsigned)c->n_kv_heads * (unsigned)n_tokens, per = qb::kv::Place<D>::kRows;
+        qb::kv::append_kernel<R, S, D><<<dim3((rows + per - 1) / per, c->n_seqs, 2), qb::kv::kThreads, 0, st>>>(
+            device_view(c), (const uint8_t*)k, (const uint8_t*)v, ld, c->n_kv_heads, n_tokens, start, counts);
+        CU(cudaGetLastError());
+        return QWEN_OK;
+    }
+};
+template <int R, int S, int D>
+struct Read {
+    static int go(const qwen_kv_cache_t* c, void* k, void* v, long long ld, int n_tokens, const int* start, const int* counts, cudaStream_t st) {
+        const unsigned rows = (unsigned)c->n_kv_heads * (unsigned)n_tokens, per = qb::kv::Place<D>::kRows;
+        qb::kv::read_kernel<R, S, D><<<dim3((rows + per - 1) / per, c->n_seqs, 2), qb::kv::kThreads, 0, st>>>(
+            device_view(c), (uint8_t*)k, (uint8_t*)v, ld, c->n_kv_heads, n_tokens, start, counts);
+        CU(cudaGetLastError());
+        return QWEN_OK;
+    }
+};
+
+int check_rows(const qwen_kv_cache_t* c, const void* k, const void* v, int dtype, long long ld, int n_tokens, const int* start,
+               const int* counts) {
+    int dev = 0;
+    TRY(check_view(c));
+    if (!is16(dtype) && dtype != QWEN_FP32) return fail(QWEN_E_ARG, "rows must be QWEN_BF16, QWEN_FP16 or QWEN_FP32");
+    if (n_tokens < 1 || n_tokens > c->capacity) return fail(QWEN_E_ARG, "n_tokens out of [1, capacity]");
+    if ((long long)n_tokens * c->n_kv_heads >= 1ll << 31) return fail(QWEN_E_UNSUPPORTED, "n_tokens * n_kv_heads must be below 2^31");
+    if (ld % 8 || ld < (long long)c->n_kv_heads * c->head_dim) return fail(QWEN_E_ARG, "ld must be a multiple of 8 and hold every head");
+    return check_ptrs({QB_VIEW_PTRS(c), {k, "k", 16, true}, {v, "v", 16, true}, {start, "start", 4, true}, {counts, "counts", 4, counts != nullptr}},
+                      &dev);
+}
+
+// ---- tree attention ----------------------------------------------------------------
+// The kernel's variant: blocks of 16 rows where the item has no more, else of 32.
+int attention_rows(int m) { return m <= 16 ? 16 : 32; }
+
+struct Plan {
+    int rows, row_blocks, shares;
+    size_t bytes;
+};
+int check_tree(const qwen_kv_cache_t* c, int n_nodes, int n_heads) {
+    if (n_nodes < 1 || n_nodes > qb::ta::kMaxNodes) return fail(QWEN_E_ARG, "n_nodes out of [1, 64]");
+    if (n_heads < 1 || n_heads % c->n_kv_heads) return fail(QWEN_E_ARG, "n_heads must be a positive multiple of n_kv_heads");
+    if (n_heads / c->n_kv_heads > 1 << 14) return fail(QWEN_E_UNSUPPORTED, "more than 2^14 query heads for each K/V head");
+    return QWEN_OK;
+}
+int attention_plan(const qwen_kv_cache_t* c, int n_nodes, int n_heads, int dev, Plan* p) {
+    const long long m = (long long)n_nodes * (n_heads / c->n_kv_heads);
+    int nsm = 0;
+    TRY(sm_count(dev, &nsm));
+    p->rows = attention_rows((int)m);
+    p->row_blocks = (int)((m + p->rows - 1) / p->rows);
+    // two CTAs an SM, but no more than there can be tiles (64 keys at least)
+    const double most = (double)c->n_seqs * c->n_kv_heads * p->row_blocks * ((c->capacity + 63) / 64);
+    p->shares = (int)std::min((double)(2 * nsm), most);
+    p->bytes = (size_t)2 * p->shares * p->rows * (c->head_dim + 2) * sizeof(float);
+    return QWEN_OK;
+}
+
+template <int QT, int STORE, int D, int MT>
+int attention_launch(const qb::ta::Params& P, const Plan& plan, int dev, cudaStream_t st) {
+    using L = qb::ta::Layout<STORE, D, MT>;
+    static std::atomic<uint64_t> done{0};
+    auto kernel = qb::ta::attention_kernel<QT, STORE, D, MT>;
+    TRY(smem_limit(kernel, done, dev, L::kSmem));
+    kernel<<<plan.shares, qb::ta::kThreads, L::kSmem, st>>>(P, plan.row_blocks);
+    CU(cudaGetLastError());
+    if (plan.shares == 1) return QWEN_OK;
+    constexpr int kJoinRows = qb::ta::kJoinThreads / (D / 4);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(plan.shares, L::kRows / kJoinRows);
+    cfg.blockDim = dim3(qb::ta::kJoinThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    CU(cudaLaunchKernelEx(&cfg, qb::ta::combine_kernel<QT, L::KT, D, L::kRows>, P, plan.row_blocks));
+    return QWEN_OK;
+}
+template <int QT, int STORE>
+int attention_by_shape(int dim, const qb::ta::Params& P, const Plan& plan, int dev, cudaStream_t st) {
+    if (dim == 64) return plan.rows == 16 ? attention_launch<QT, STORE, 64, 1>(P, plan, dev, st) : attention_launch<QT, STORE, 64, 2>(P, plan, dev, st);
+    return plan.rows == 16 ? attention_launch<QT, STORE, 128, 1>(P, plan, dev, st) : attention_launch<QT, STORE, 128, 2>(P, plan, dev, st);
+}
+
+// ---- verification --------------------------------------------------------------------
+template <int T>
+int verify_launch(const qb::tv::Params& P, int n_seqs, int cluster, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)n_seqs * cluster);
+    cfg.blockDim = dim3(qb::tv::kThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    CU(cudaLaunchKernelEx(&cfg, qb::tv::verify_kernel<T>, P));
+    return QWEN_OK;
+}
+
+}  // namespace
+
+extern "C" int qwen_kv_append(const qwen_kv_cache_t* cache, const void* k, const void* v, int src_dtype, long long ld, int n_tokens,
+                              const int* start, const int* counts, void* stream) {
+    TRY(check_rows(cache, k, v, src_dtype, ld, n_tokens, start, counts));
+    return by_types<Append>(src_dtype, cache->dtype, cache->head_dim, cache, k, v, ld, n_tokens, start, counts, (cudaStream_t)stream);
+}
+
+extern "C" int qwen_kv_read(const qwen_kv_cache_t* cache, void* k, void* v, int dst_dtype, long long ld, int n_tokens, const int* start,
+                            const int* counts, void* stream) {
+    TRY(check_rows(cache, k, v, dst_dtype, ld, n_tokens, start, counts));
+    return by_types<Read>(dst_dtype, cache->dtype, cache->head_dim, cache, k, v, ld, n_tokens, start, counts, (cudaStream_t)stream);
+}
+
+extern "C" int qwen_kv_keep(const qwen_kv_cache_t* cache, const int* start, const int* path, const int* n_path, int n_nodes, void* stream) {
+    int dev = 0;
+    TRY(check_view(cache));
+    if (n_nodes < 1 || n_nodes > qb::kv::kMaxNodes) return fail(QWEN_E_ARG, "n_nodes out of [1, 64]");
+    TRY(check_ptrs({QB_VIEW_PTRS(cache), {start, "start", 4, true}, {path, "path", 4, true}, {n_path, "n_path", 4, true}}, &dev));
+    const dim3 grid(cache->n_kv_heads, cache->n_seqs);
+    const auto c = device_view(cache);
+    const cudaStream_t st = (cudaStream_t)stream;
+    const bool k8 = is8(cache->dtype), wide = cache->head_dim == 128;
+    if (k8 && wide) qb::kv::keep_kernel<128, true><<<grid, qb::kv::kKeepThreads, 0, st>>>(c, start, path, n_path, n_nodes, 1);
+    else if (k8) qb::kv::keep_kernel<64, true><<<grid, qb::kv::kKeepThreads, 0, st>>>(c, start, path, n_path, n_nodes, 1);
+    else if (wide) qb::kv::keep_kernel<256, false><<<grid, qb::kv::kKeepThreads, 0, st>>>(c, start, path, n_path, n_nodes, 2);
+    else qb::kv::keep_kernel<128, false><<<grid, qb::kv::kKeepThreads, 0, st>>>(c, start, path, n_path, n_nodes, 2);
+    CU(cudaGetLastError());
+    return QWEN_OK;
+}
+
+extern "C" int qwen_tree_attention_workspace(const qwen_kv_cache_t* cache, int n_nodes, int n_heads, size_t* bytes) {
+    if (!bytes) return fail(QWEN_E_ARG, "NULL argument");
+    TRY(check_view(cache));
+    TRY(check_tree(cache, n_nodes, n_heads));
+    int dev = 0;
+    CU(cudaGetDevice(&dev));
+    Plan p;
+    TRY(attention_plan(cache, n_nodes, n_heads, dev, &p));
+    *bytes = p.bytes;
+    return QWEN_OK;
+}
+
+extern "C" int qwen_tree_attention(const qwen_kv_cache_t* cache, const void* q, void* out, int dtype, long long ldq, long long ldo, int n_nodes,
+                                   int n_heads, const int* lens, const int* parents, float scale, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+    TRY(check_view(cache));
+    if (!is16(dtype)) return fail(QWEN_E_ARG, "q and out must be QWEN_BF16 or QWEN_FP16");
+    if (is16(cache->dtype) && cache->dtype != dtype) return fail(QWEN_E_ARG, "q and a 16-bit cache must have the same type");
+    TRY(check_tree(cache, n_nodes, n_heads));
+    const long long width = (long long)n_heads * cache->head_dim;
+    if (ldq % 8 || ldo % 8 || ldq < width || ldo < width) return fail(QWEN_E_ARG, "ldq and ldo must be multiples of 8 and hold every head");
+    if (!std::isfinite(scale)) return fail(QWEN_E_ARG, "scale must be finite");
+    if (q == out) return fail(QWEN_E_ARG, "out must not be q");
+    int dev = 0;
+    TRY(check_ptrs({QB_VIEW_PTRS(cache), {q, "q", 16, true}, {out, "out", 16, true}, {lens, "lens", 4, true}, {parents, "parents", 4, true},
+                    {workspace, "workspace", 16, true}}, &dev));
+    Plan plan;
+    TRY(attention_plan(cache, n_nodes, n_heads, dev, &plan));
+    if (workspace_bytes < plan.bytes) return fail(QWEN_E_ARG, "workspace is smaller than qwen_tree_attention_workspace says");
+    qb::ta::Params P;
+    P.cache = device_view(cache);
+    P.q = (const uint8_t*)q;
+    P.out = (uint8_t*)out;
+    P.lens = lens;
+    P.parents = parents;
+    P.work = (float*)workspace;
+    P.ldq = ldq;
+    P.ldo = ldo;
+    P.n_seqs = cache->n_seqs;
+    P.n_kv_heads = cache->n_kv_heads;
+    P.group = n_heads / cache->n_kv_heads;
+    P.n_nodes = n_nodes;
+    P.scale_log2 = scale * 1.4426950408889634f;
+    const cudaStream_t st = (cudaStream_t)stream;
+    const int dim = cache->head_dim;
+    const bool bf = dtype == QWEN_BF16;
+    switch (cache->dtype) {
+        case QWEN_E4M3: return bf ? attention_by_shape<QWEN_BF16, QWEN_E4M3>(dim, P, plan, dev, st) : attention_by_shape<QWEN_FP16, QWEN_E4M3>(dim, P, plan, dev, st);
+        case QWEN_INT8: return bf ? attention_by_shape<QWEN_BF16, QWEN_INT8>(dim, P, plan, dev, st) : attention_by_shape<QWEN_FP16, QWEN_INT8>(dim, P, plan, dev, st);
+        default: return bf ? attention_by_shape<QWEN_BF16, QWEN_BF16>(dim, P, plan, dev, st) : attention_by_shape<QWEN_FP16, QWEN_FP16>(dim, P, plan, dev, st);
+    }
+}
+
+extern "C" int qwen_tree_verify(const void* logits, int logits_dtype, long long ld, const float* draft, long long ld_draft, const int* tokens,
+                                const int* parents, const float* uniforms, int n_seqs, int n_nodes, int vocab, float temperature, int* path,
+                                int* n_path, int* next, void* stream) {
+    if (!is16(logits_dtype) && logits_dtype != QWEN_FP32) return fail(QWEN_E_ARG, "logits must be QWEN_FP32, QWEN_BF16 or QWEN_FP16");
+    if (n_seqs < 1 || n_seqs > 65535) return fail(QWEN_E_ARG, "n_seqs out of [1, 65535]");
+    if (n_nodes < 1 || n_nodes > qb::tv::kMaxNodes) return fail(QWEN_E_ARG, "n_nodes out of [1, 64]");
+    if (vocab < 1 || vocab > 1 << 30) return fail(QWEN_E_ARG, "vocab out of [1, 2^30]");
+    if (ld < vocab || (draft && ld_draft < vocab)) return fail(QWEN_E_ARG, "ld and ld_draft must hold a row");
+    if (!(temperature == 0.0f || (temperature >= 1e-6f && temperature <= 1e6f))) return fail(QWEN_E_ARG, "temperature must be 0 or within 1e-6 .. 1e6");
+    const size_t elem = logits_dtype == QWEN_FP32 ? 4 : 2;
+    const bool greedy = temperature == 0.0f;
+    int dev = 0, nsm = 0;
+    TRY(check_ptrs({{logits, "logits", elem, true}, {draft, "draft", 4, draft && !greedy}, {tokens, "tokens", 4, n_nodes > 1},
+                    {parents, "parents", 4, true}, {uniforms, "uniforms", 4, !greedy}, {path, "path", 4, true}, {n_path, "n_path", 4, true},
+                    {next, "next", 4, true}}, &dev));
+    TRY(sm_count(dev, &nsm));
+    qb::tv::Params P;
+    P.logits = logits;
+    P.draft = greedy ? nullptr : draft;
+    P.tokens = tokens;
+    P.parents = parents;
+    P.uniforms = uniforms;
+    P.path = path;
+    P.n_path = n_path;
+    P.next = next;
+    P.ld = ld;
+    P.ld_draft = ld_draft;
+    P.n_nodes = n_nodes;
+    P.vocab = vocab;
+    const bool rows16 = ((uintptr_t)logits | (size_t)ld * elem) % 16 == 0;
+    P.vec = rows16 && (!P.draft || ((uintptr_t)draft | (size_t)ld_draft * 4) % 16 == 0);
+    P.temperature = temperature;
+    // as many CTAs for a sequence as the SMs allow, a whole run of 128 tokens for each warp
+    int cluster = 1;
+    while (cluster < qb::tv::kMaxCluster && (long long)n_seqs * cluster * 2 <= nsm && vocab >= cluster * 2 * qb::tv::kWarps * 128) cluster *= 2;
+    const cudaStream_t st = (cudaStream_t)stream;
+    switch (logits_dtype) {
+        case QWEN_BF16: return verify_launch<QWEN_BF16>(P, n_seqs, cluster, st);
+        case QWEN_FP16: return verify_launch<QWEN_FP16>(P, n_seqs, cluster, st);
+        default: return verify_launch<QWEN_FP32>(P, n_seqs, cluster, st);
+    }
+}

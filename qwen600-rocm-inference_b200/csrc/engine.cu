@@ -1065,6 +1065,24 @@ extern "C" int qwen_batch_read_logits(qwen_t* c, int rows, float* logits_host) {
     return QWEN_OK;
 }
 
+extern "C" int qwen_batch_cache(qwen_t* c, int layer, qwen_kv_cache_t* out) {
+    if (!c || !out) return fail(QWEN_E_ARG, "NULL argument");
+    if (!c->b_max) return fail(QWEN_E_STATE, "qwen_batch_init first");
+    if (layer < -1 || layer >= N_LAYERS) return fail(QWEN_E_ARG, "layer out of [-1, N_LAYERS)");
+    const size_t at = (size_t)std::max(layer, 0) * kGroups * SEQ_LEN * HEAD_DIM;
+    out->k = c->bkc + at;
+    out->v = c->bvc + at;
+    out->k_scale = out->v_scale = nullptr;
+    out->seq_stride = (long long)slot_elems();
+    out->head_stride = (long long)SEQ_LEN * HEAD_DIM;
+    out->dtype = QWEN_BF16;
+    out->n_seqs = c->b_max;
+    out->n_kv_heads = layer < 0 ? N_LAYERS * kGroups : kGroups;
+    out->head_dim = HEAD_DIM;
+    out->capacity = SEQ_LEN;
+    return QWEN_OK;
+}
+
 extern "C" int qwen_set_prefill_parts(qwen_t* c, int parts) {
     if (!c) return fail(QWEN_E_ARG, "NULL handle");
     if (parts < 1 || parts > 3) return fail(QWEN_E_ARG, "parts must be 1, 2 or 3");

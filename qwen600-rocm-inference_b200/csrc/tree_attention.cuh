@@ -1,0 +1,657 @@
+// tree_attention.cuh — attention of a tree of drafted tokens over a K/V cache
+// (qwen_tree_attention).  No reference counterpart (the reference's attention
+// serves one token over a bf16 cache, qwen_model.cuh:551-614).
+//
+// Mathematics.  Node i of sequence s attends to positions [0, len) and to len + j
+// for its ancestors-or-self j, a 64-bit mask.  One pass over the keys with the
+// running maximum m and sum l of the softmax (base 2, scale * log2 e folded into
+// the scores); O += P V with P = 2^(score - m), scaled down when m rises.
+//
+// The rows of a work item are the n_nodes * group (query head, node) pairs that
+// share a K/V head, so each K/V byte is read once for all of them.  The items
+// (sequence, K/V head, block of rows) are laid end to end in units of key tiles, and
+// CTA i takes the i-th of G equal shares of that line: ragged lengths balance
+// by themselves, and a single long sequence spreads over all SMs.  An item that
+// crosses a share's border leaves partial (m, l, O) in the workspace, two slots a
+// CTA, and combine_kernel joins them in the order of the keys, so results do not
+// depend on timing.  The shares are computed on the device from lens.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "../../include/qwen_b200.h"
+#include "kv_rows.cuh"
+#include "ptx.cuh"
+
+namespace qb {
+namespace ta {
+
+constexpr int kMaxNodes = 64;
+
+struct Params {
+    kv::Cache cache;
+    const uint8_t* q;
+    uint8_t* out;
+    const int *lens, *parents;
+    float* work;
+    long long ldq, ldo;
+    int n_seqs, n_kv_heads, group, n_nodes;
+    float scale_log2;   // scale * log2(e)
+};
+
+// ---- the line of key tiles -----------------------------------------------------
+// Positions that sequence s has, its nodes' among them (0: nothing is present).
+__device__ __forceinline__ int seq_end(const Params& P, int len) {
+    return len < 0 || len >= P.cache.capacity ? 0 : min(len + min(P.n_nodes, P.cache.capacity - len), P.cache.capacity);
+}
+template <int KT>
+__device__ __forceinline__ int seq_tiles(const Params& P, int len) { return max(1, (seq_end(P, len) + KT - 1) / KT); }
+
+// All lanes of a warp: the number of tiles on the line, units = items per sequence.
+template <int KT>
+__device__ __forceinline__ long long line_tiles(const Params& P, int units) {
+    long long n = 0;
+    for (int s = threadIdx.x & 31; s < P.n_seqs; s += 32) n += seq_tiles<KT>(P, P.lens[s]);
+    #pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(~0u, n, o);
+    return n * units;
+}
+// All lanes of a warp: the sequence that tile x of the line belongs to, and the
+// tiles before it.  x is below line_tiles.
+template <int KT>
+__device__ __forceinline__ int line_find(const Params& P, int units, long long x, long long& before) {
+    const int lane = threadIdx.x & 31;
+    before = 0;
+    for (int s0 = 0; s0 < P.n_seqs; s0 += 32) {
+        const long long n = s0 + lane < P.n_seqs ? (long long)seq_tiles<KT>(P, P.lens[s0 + lane]) * units : 0;
+        long long inc = n;
+        #pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(~0u, inc, o);
+            if (lane >= o) inc += y;
+        }
+        const uint32_t hit = __ballot_sync(~0u, n > 0 && before + inc > x);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            before += __shfl_sync(~0u, inc - n, l);
+            return s0 + l;
+        }
+        before += __shfl_sync(~0u, inc, 31);
+    }
+    return P.n_seqs - 1;
+}
+// First tile of share i of G.
+__device__ __forceinline__ long long share(long long tiles, int i, int G) { return tiles * i / G; }
+// The share that tile x lies in.
+__device__ __forceinline__ int share_of(long long tiles, long long x, int G) { return (int)(((x + 1) * G - 1) / tiles); }
+
+// ---- the tree --------------------------------------------------------------------
+// One warp: anc[i] = the nodes that node i sees (itself and its ancestors), 0 if it
+// is absent.  Six rounds of doubling the step; two nodes a lane.
+__device__ __forceinline__ void tree_masks(const Params& P, int seq, int len, uint64_t* anc, int8_t* up) {
+    const int lane = threadIdx.x & 31, N = P.n_nodes;
+    constexpr int8_t kNone = -1, kAbsent = -2;
+    #pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int i = lane + 32 * k;
+        int p = kAbsent;
+        if (i < N) {
+            p = P.parents[(size_t)seq * N + i];
+            if (p < -1 || p >= i || len < 0 || (long long)len + i >= P.cache.capacity) p = kAbsent;
+        }
+        up[i] = (int8_t)p;
+        anc[i] = 1ull << i;
+    }
+    __syncwarp();
+    for (int step = 1; step < N; step <<= 1) {
+        uint64_t a[2];
+        int8_t u[2];
+        #pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int i = lane + 32 * k, p = up[i];
+            a[k] = anc[i] | (p >= 0 ? anc[p] : 0);
+            u[k] = p >= 0 ? up[p] : (int8_t)p;
+        }
+        __syncwarp();
+        #pragma unroll
+        for (int k = 0; k < 2; k++) { anc[lane + 32 * k] = a[k]; up[lane + 32 * k] = u[k]; }
+        __syncwarp();
+    }
+    #pragma unroll
+    for (int k = 0; k < 2; k++)
+        if (up[lane + 32 * k] != kNone) anc[lane + 32 * k] = 0;
+    __syncwarp();
+}
+
+// ---- fragments ---------------------------------------------------------------------
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr) : "memory");
+}
+template <bool BF>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    } else {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+}
+// Two 8-bit codes to an fp16 pair (exact).  The pair is bytes (B0, B1) of w.
+template <int STORE, int B0, int B1>
+__device__ __forceinline__ uint32_t codes_f16x2(uint32_t w) {
+    if constexpr (STORE == QWEN_INT8) {
+        // 0x6400 | u is 1024 + u; u = code + 128
+        const uint32_t h = __byte_perm(w ^ 0x80808080u, 0x64646464u, 0x4040u | B0 | (B1 << 8));
+        const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    } else {
+        uint32_t h;
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)__byte_perm(w, 0, B0 | (B1 << 4))));
+        return h;
+    }
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) { return BF ? cvt_bf16x2(lo, hi) : kv::half2_bits(lo, hi); }
+
+// ---- few rows: warp-level tensor cores ------------------------------------------------
+// Bound by the cache's bytes (a row of 128 bf16 values is worth 22 cycles of an SM's
+// share of the memory bandwidth, its products with 16 query rows about 4).  Four
+// warps; each owns KW keys of a tile, its own ring of kStages cp.async stages and its own (m, l, O) over all
+// rows, so the loop has no block barrier; the four are joined at the end of an
+// item.  16-bit caches multiply in the cache's type.  8-bit codes become fp16
+// (exact for both types): queries are scaled by a power of two per row into
+// fp16's range (bf16 queries; the factor returns with the score), a key's scale
+// multiplies its scores, a value row's scale its weights, divided by a power of
+// two that is at least the largest scale so far, so the weights stay within
+// fp16.  P is rounded to 16 bits (half a step: 2^-9 or 2^-12 relative) as
+// the product with V takes it; l sums it unrounded.
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kStages = 3;
+
+template <int STORE, int D, int MT>
+struct Layout {
+    static constexpr int kEs = STORE == QWEN_E4M3 || STORE == QWEN_INT8 ? 1 : 2;
+    static constexpr bool k8 = kEs == 1;
+    static constexpr int kRow = D * kEs;                       // bytes of a cache row
+    static constexpr int KW = kRow == 256 ? 16 : 32;           // keys of a warp's part of a tile
+    static constexpr int KT = kWarps * KW;                     // keys of a tile
+    static constexpr int kRows = 16 * MT;                      // query rows of an item
+    static constexpr int kPart = KW * kRow;                    // bytes of K (or V) of a warp's stage
+    static constexpr int kScale = k8 ? 2 * KW * 4 : 0;         // its scales
+    static constexpr int kStage = 2 * kPart + kScale;
+    static constexpr int kRing = kWarps * kStages * kStage;
+    static constexpr int kJoin = kWarps * kRows * (D + 2) * 4; // the warps' (O, m, l) at the end of an item (over the ring)
+    static constexpr int kQ = kRing > kJoin ? kRing : kJoin;   // query rows, 16 bits
+    static constexpr int kAnc = kQ + kRows * D * 2;            // tree masks
+    static constexpr int kUp = kAnc + kMaxNodes * 8;
+    static constexpr int kQf = kUp + kMaxNodes;                // the rows' powers of two
+    static constexpr int kSmem = kQf + kRows * 4;
+    static constexpr int kSlot = kRows * (D + 2);              // floats of a workspace slot: O, then (m, l) pairs
+    static_assert(kRing % 16 == 0 && kJoin % 16 == 0 && kStage % 16 == 0, "rows of 16-byte pieces");
+    static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two CTAs an SM");
+};
+// Byte of 16-byte piece c of row r, so that 8 rows of one piece (or 8 pieces) meet no bank twice.
+template <int ROW>
+__device__ __forceinline__ int swz(int r, int c) {
+    if constexpr (ROW >= 128) return r * ROW + ((c ^ (r & 7)) << 4);
+    else return r * ROW + ((c ^ ((r >> 1) & 3)) << 4);
+}
+
+// grid G (shares), kThreads threads, Layout::kSmem bytes.  row_blocks: blocks of
+// kRows rows an item's K/V head has.
+template <int QT, int STORE, int D, int MT>
+__global__ void __launch_bounds__(kThreads, 2) attention_kernel(const Params P, int row_blocks) {
+    using L = Layout<STORE, D, MT>;
+    constexpr bool BF = QT == QWEN_BF16 && !L::k8;       // type of the products
+    constexpr int KW = L::KW, NT = KW / 8, DT = D / 8, KS = D / 16;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j = lane & 3;
+    uint8_t* ring = smem + warp * kStages * L::kStage;
+    uint64_t* anc = reinterpret_cast<uint64_t*>(smem + L::kAnc);
+    float* qf = reinterpret_cast<float*>(smem + L::kQf);
+    pdl_wait();
+    pdl_launch_dependents();   // after the wait: what the joining kernel reads early (lens) is then complete
+
+    const int units = P.n_kv_heads * row_blocks, G = gridDim.x;
+    const long long tiles = line_tiles<L::KT>(P, units);
+    long long at = share(tiles, blockIdx.x, G);
+    const long long to = share(tiles, blockIdx.x + 1, G);
+    if (at >= to) return;
+    long long before;
+    int seq = line_find<L::KT>(P, units, at, before);
+    bool first_item = true;
+    const int M = P.n_nodes * P.group;
+    while (at < to) {
+        const int len = P.lens[seq], end = seq_end(P, len), n = seq_tiles<L::KT>(P, len);
+        const int unit = (int)((at - before) / n), t0 = (int)((at - before) - (long long)unit * n);
+        const int t1 = (int)min((long long)n, t0 + (to - at));
+        const int h = unit / row_blocks, r_base = (unit - h * row_blocks) * L::kRows;
+        const size_t head = (size_t)seq * P.cache.seq_stride + (size_t)h * P.cache.head_stride;
+        const uint8_t *kb = P.cache.k + head * L::kEs, *vb = P.cache.v + head * L::kEs;
+        const float *ksb = L::k8 ? P.cache.ks + head / D : nullptr, *vsb = L::k8 ? P.cache.vs + head / D : nullptr;
+
+        auto load = [&](int t, int s) {   // this warp's part of tile t into stage s; positions >= end as zeros
+            uint8_t* st = ring + s * L::kStage;
+            const int k0 = t * L::KT + warp * KW;
+            constexpr int kChunks = L::kRow / 16, kPer = KW * kChunks / 32;
+            #pragma unroll
+            for (int i = 0; i < kPer; i++) {
+                const int c = lane + 32 * i, r = c / kChunks, p = c % kChunks;
+                const bool live = k0 + r < end;
+                const size_t off = live ? (size_t)(k0 + r) * L::kRow + p * 16 : 0;
+                cp_async16(smem_addr(st + swz<L::kRow>(r, p)), kb + off, live);
+                cp_async16(smem_addr(st + L::kPart + swz<L::kRow>(r, p)), vb + off, live);
+            }
+            if constexpr (L::k8) {
+                static_assert(KW == 32, "one scale a lane");
+                const bool live = k0 + lane < end;
+                const size_t off = live ? k0 + lane : 0;
+                cp_async4(smem_addr(st + 2 * L::kPart + 4 * lane), ksb + off, live);
+                cp_async4(smem_addr(st + 2 * L::kPart + 4 * KW + 4 * lane), vsb + off, live);
+            }
+        };
+        #pragma unroll
+        for (int s = 0; s < kStages - 1; s++) {
+            if (t0 + s < t1) load(t0 + s, s);
+            cp_async_commit();
+        }
+        // queries to shared memory, 16 bits; for 8-bit caches fp16 with the dims of each 16 in
+        // the order in which the K codes come out of ldmatrix: 4j, 4j+1 at 2j, 4j+2, 4j+3 at 8 + 2j
+        if (warp == 0) tree_masks(P, seq, len, anc, reinterpret_cast<int8_t*>(smem + L::kUp));
+        {
+            constexpr int kLanes = D / 8;   // 8 elements a thread
+            const int part = tid % kLanes;
+            for (int r = tid / kLanes; r < L::kRows; r += kThreads / kLanes) {
+                const int row = r_base + r, node = row / P.group, hq = h * P.group + row % P.group;
+                uint4 w = make_uint4(0, 0, 0, 0);
+                if (row < M) w = *reinterpret_cast<const uint4*>(P.q + (((size_t)seq * P.n_nodes + node) * (size_t)P.ldq + (size_t)hq * D + part * 8) * 2);
+                if constexpr (!L::k8) {
+                    *reinterpret_cast<uint4*>(smem + L::kQ + swz<D * 2>(r, part)) = w;
+                } else {
+                    uint32_t x[4] = {w.x, w.y, w.z, w.w};
+                    if constexpr (QT == QWEN_BF16) {
+                        uint32_t m = 0;
+                        #pragma unroll
+                        for (int i = 0; i < 4; i++) m = max(m, max(x[i] & 0x7fffu, (x[i] >> 16) & 0x7fffu));
+                        #pragma unroll
+                        for (int o = 1; o < kLanes; o <<= 1) m = max(m, __shfl_xor_sync(~0u, m, o));
+                        // 2^e <= the row's largest magnitude < 2^(e+1); infinities and NaN go through as they are
+                        const int e = min(max((int)(m >> 7), 1), 253);
+                        const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+                        #pragma unroll
+                        for (int i = 0; i < 4; i++) x[i] = kv::half2_bits(bf_lo(x[i]) * down, bf_hi(x[i]) * down);
+                        if (part == 0) qf[r] = __uint_as_float((uint32_t)e << 23);
+                    } else if (part == 0) {
+                        qf[r] = 1.0f;
+                    }
+                    // this thread's 8 dims are the first or second half of a 16: pairs p = 0..3 (dims 2p, 2p+1) of it
+                    const int half = part & 1, chunk = part & ~1;
+                    #pragma unroll
+                    for (int p = 0; p < 4; p++) {
+                        const int d = 8 * half + 2 * p, jj = d >> 2, k = (d & 2) ? 8 + 2 * jj : 2 * jj;
+                        *reinterpret_cast<uint32_t*>(smem + L::kQ + swz<D * 2>(r, chunk + (k >> 3)) + (k & 7) * 2) = x[p];
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        uint64_t see[2 * MT];     // what this lane's rows see of the tree
+        float c[2 * MT];          // their score factors
+        #pragma unroll
+        for (int i = 0; i < 2 * MT; i++) {
+            const int r = 16 * (i >> 1) + g + 8 * (i & 1), row = r_base + r;
+            see[i] = row < M ? anc[row / P.group] : 0;
+            c[i] = L::k8 ? P.scale_log2 * qf[r] : P.scale_log2;
+        }
+        uint32_t qa[MT == 1 ? KS : 1][4];   // one block of rows: its fragments stay in registers
+        auto q_frag = [&](int mt, int ks, uint32_t (&a)[4]) {
+            const int r = 16 * mt + (lane & 15), p = 2 * ks + (lane >> 4);
+            ldsm_x4(smem_addr(smem + L::kQ + swz<D * 2>(r, p)), a[0], a[1], a[2], a[3]);
+        };
+        if constexpr (MT == 1) {
+            #pragma unroll
+            for (int ks = 0; ks < KS; ks++) q_frag(0, ks, qa[ks]);
+        }
+
+        float o[MT][DT][4], m[2 * MT], l[2 * MT];
+        #pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+            #pragma unroll
+            for (int d = 0; d < DT; d++)
+                #pragma unroll
+                for (int e = 0; e < 4; e++) o[mt][d][e] = 0.f;
+        #pragma unroll
+        for (int i = 0; i < 2 * MT; i++) { m[i] = -INFINITY; l[i] = 0.f; }
+        uint32_t ve = 1;   // 8-bit caches: O is in units of 2^(ve - 127)
+
+        for (int t = t0; t < t1; t++) {
+            {
+                const int ahead = t + kStages - 1;
+                if (ahead < t1) load(ahead, (ahead - t0) % kStages);
+                cp_async_commit();
+            }
+            cp_async_wait<kStages - 1>();
+            __syncwarp();
+            uint8_t* st = ring + (t - t0) % kStages * L::kStage;
+            const int k0 = t * L::KT + warp * KW;
+            if (k0 < end) {
+                // ---- scores ----
+                float s[MT][NT][4];
+                #pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+                    #pragma unroll
+                    for (int i = 0; i < NT; i++)
+                        #pragma unroll
+                        for (int e = 0; e < 4; e++) s[mt][i][e] = 0.f;
+                #pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    uint32_t a[MT][4];
+                    #pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        if constexpr (MT == 1) { a[0][0] = qa[ks][0]; a[0][1] = qa[ks][1]; a[0][2] = qa[ks][2]; a[0][3] = qa[ks][3]; }
+                        else q_frag(mt, ks, a[mt]);
+                    }
+                    if constexpr (!L::k8) {
+                        #pragma unroll
+                        for (int i = 0; i < NT; i += 2) {   // keys 8i .. 8i+15, dims 16 ks .. +15
+                            uint32_t b[4];
+                            ldsm_x4(smem_addr(st + swz<L::kRow>(8 * i + (lane & 7) + ((lane >> 4) << 3), 2 * ks + ((lane >> 3) & 1))), b[0], b[1], b[2], b[3]);
+                            #pragma unroll
+                            for (int mt = 0; mt < MT; mt++) {
+                                mma16816<BF>(s[mt][i], a[mt], b[0], b[1]);
+                                mma16816<BF>(s[mt][i + 1], a[mt], b[2], b[3]);
+                            }
+                        }
+                    } else {                                // four key groups of one 16-byte piece
+                        uint32_t b[4];
+                        ldsm_x4(smem_addr(st + swz<L::kRow>(lane, ks)), b[0], b[1], b[2], b[3]);
+                        #pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const uint32_t b0 = codes_f16x2<STORE, 0, 1>(b[i]), b1 = codes_f16x2<STORE, 2, 3>(b[i]);
+                            #pragma unroll
+                            for (int mt = 0; mt < MT; mt++) mma16816<BF>(s[mt][i], a[mt], b0, b1);
+                        }
+                    }
+                }
+                const bool tail = k0 + KW > len;   // the same for the warp: some keys are the tree's, or past the end
+                float vs[NT][2];
+                if constexpr (L::k8) {
+                    const float* sc = reinterpret_cast<const float*>(st + 2 * L::kPart);
+                    #pragma unroll
+                    for (int i = 0; i < NT; i++) {
+                        const float2 ks2 = *reinterpret_cast<const float2*>(sc + 8 * i + 2 * j);
+                        const float2 vs2 = *reinterpret_cast<const float2*>(sc + KW + 8 * i + 2 * j);
+                        vs[i][0] = vs2.x;
+                        vs[i][1] = vs2.y;
+                        #pragma unroll
+                        for (int mt = 0; mt < MT; mt++) {
+                            s[mt][i][0] *= c[2 * mt] * ks2.x; s[mt][i][1] *= c[2 * mt] * ks2.y;
+                            s[mt][i][2] *= c[2 * mt + 1] * ks2.x; s[mt][i][3] *= c[2 * mt + 1] * ks2.y;
+                        }
+                    }
+                } else {
+                    #pragma unroll
+                    for (int i = 0; i < NT; i++)
+                        #pragma unroll
+                        for (int mt = 0; mt < MT; mt++) {
+                            s[mt][i][0] *= c[2 * mt]; s[mt][i][1] *= c[2 * mt];
+                            s[mt][i][2] *= c[2 * mt + 1]; s[mt][i][3] *= c[2 * mt + 1];
+                        }
+                }
+                auto sees = [&](int row, int key) {   // key: position
+                    const int node = key - len;
+                    return node < 0 || (node < kMaxNodes && ((see[row] >> node) & 1));
+                };
+                if (tail) {
+                    #pragma unroll
+                    for (int mt = 0; mt < MT; mt++)
+                        #pragma unroll
+                        for (int i = 0; i < NT; i++)
+                            #pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                if (!sees(2 * mt + (e >> 1), k0 + 8 * i + 2 * j + (e & 1))) s[mt][i][e] = -INFINITY;
+                }
+                // ---- softmax ----
+                uint32_t up = 0;    // 8-bit: the rise of ve
+                if constexpr (L::k8) {
+                    uint32_t e = __float_as_uint(reinterpret_cast<const float*>(st + 2 * L::kPart)[KW + lane]) >> 23 & 0xffu;
+                    e = e == 255u ? 0u : min(e + 1, 253u);
+                    e = __reduce_max_sync(~0u, e);
+                    if (e > ve) { up = e - ve; ve = e; }
+                }
+                const float vinv = L::k8 ? __uint_as_float((254u - ve) << 23) : 1.0f;
+                float f[2 * MT];
+                bool moved = up != 0;
+                #pragma unroll
+                for (int r = 0; r < 2 * MT; r++) {
+                    float mx = -INFINITY;
+                    #pragma unroll
+                    for (int i = 0; i < NT; i++) mx = fmaxf(mx, fmaxf(s[r >> 1][i][2 * (r & 1)], s[r >> 1][i][2 * (r & 1) + 1]));
+                    mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+                    const float mn = fmaxf(m[r], mx);
+                    const float base = mn == -INFINITY ? 0.f : mn;
+                    f[r] = exp2_approx(m[r] - base);
+                    moved |= mn > m[r];
+                    m[r] = mn;
+                    float sum = 0.f;
+                    #pragma unroll
+                    for (int i = 0; i < NT; i++)
+                        #pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            float& x = s[r >> 1][i][2 * (r & 1) + e];
+                            x = exp2_approx(x - base);
+                            sum += x;
+                            if constexpr (L::k8) x *= !tail || sees(r, k0 + 8 * i + 2 * j + e) ? vs[i][e] * vinv : 0.f;
+                        }
+                    l[r] = l[r] * f[r] + sum;
+                }
+                if (__any_sync(~0u, moved)) {
+                    const float w = L::k8 ? (up < 127u ? __uint_as_float((127u - up) << 23) : 0.f) : 1.0f;
+                    #pragma unroll
+                    for (int mt = 0; mt < MT; mt++)
+                        #pragma unroll
+                        for (int d = 0; d < DT; d++)
+                            #pragma unroll
+                            for (int e = 0; e < 4; e++) o[mt][d][e] *= f[2 * mt + (e >> 1)] * w;
+                }
+                uint8_t* sv = st + L::kPart;
+                // the dim of column e (0, 1) of this lane in column tile d
+                auto dim_of = [&](int d, int e) { return L::k8 ? (d >> 1) * 16 + 4 * j + 2 * e + (d & 1) : 8 * d + 2 * j + e; };
+                if (STORE != QWEN_INT8 && tail) {
+                    // An infinity or NaN in a V row of the tree may only reach the nodes that see the row, but 0 * NaN
+                    // in the product is NaN: such values are added here, to those, and zeroed before the product.
+                    const int from = max(len - k0, 0);
+                    bool odd = false;
+                    for (int i = lane; i < (KW - from) * (L::kRow / 4); i += 32) {
+                        const int r = from + i / (L::kRow / 4), b = i % (L::kRow / 4);
+                        const uint32_t w = *reinterpret_cast<const uint32_t*>(sv + swz<L::kRow>(r, b >> 2) + 4 * (b & 3));
+                        if constexpr (L::k8) {
+                            #pragma unroll
+                            for (int e = 0; e < 4; e++) odd |= ((w >> (8 * e)) & 0x7fu) == 0x7fu;
+                        } else {
+                            constexpr uint32_t kExp = QT == QWEN_BF16 ? 0x7f80u : 0x7c00u;
+                            odd |= (w & kExp) == kExp || ((w >> 16) & kExp) == kExp;
+                        }
+                    }
+                    if (__any_sync(~0u, odd)) {
+                        constexpr uint32_t kExp = L::k8 ? 0x7fu : QT == QWEN_BF16 ? 0x7f80u : 0x7c00u;
+                        for (int r = from; r < KW; r++)
+                            #pragma unroll
+                            for (int d = 0; d < DT; d++)
+                                #pragma unroll
+                                for (int e = 0; e < 2; e++) {
+                                    const int byte = dim_of(d, e) * L::kEs;
+                                    const uint8_t* p = sv + swz<L::kRow>(r, byte >> 4) + (byte & 15);
+                                    const uint32_t w = L::k8 ? *p : *reinterpret_cast<const uint16_t*>(p);
+                                    if ((w & kExp) != kExp) continue;
+                                    const float x = L::k8 ? NAN : QT == QWEN_BF16 ? bf2f((uint16_t)w) : __half2float(__ushort_as_half((uint16_t)w));
+                                    #pragma unroll
+                                    for (int q = 0; q < 2 * MT; q++)
+                                        if (sees(q, k0 + r)) o[q >> 1][d][2 * (q & 1) + e] += x;
+                                }
+                        __syncwarp();
+                        for (int i = lane; i < (KW - from) * (L::kRow / L::kEs); i += 32) {
+                            const int r = from + i / D, byte = i % D * L::kEs;
+                            uint8_t* p = sv + swz<L::kRow>(r, byte >> 4) + (byte & 15);
+                            if constexpr (L::k8) { if ((*p & kExp) == kExp) *p = 0; }
+                            else { uint16_t* w = reinterpret_cast<uint16_t*>(p); if ((*w & kExp) == kExp) *w = 0; }
+                        }
+                        __syncwarp();
+                    }
+                }
+                // ---- O += P V ----
+                #pragma unroll
+                for (int kk = 0; kk < KW / 16; kk++) {
+                    uint32_t a[MT][4];
+                    #pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        a[mt][0] = pack2<BF>(s[mt][2 * kk][0], s[mt][2 * kk][1]);
+                        a[mt][1] = pack2<BF>(s[mt][2 * kk][2], s[mt][2 * kk][3]);
+                        a[mt][2] = pack2<BF>(s[mt][2 * kk + 1][0], s[mt][2 * kk + 1][1]);
+                        a[mt][3] = pack2<BF>(s[mt][2 * kk + 1][2], s[mt][2 * kk + 1][3]);
+                    }
+                    #pragma unroll
+                    for (int p = 0; p < L::kRow / 16; p += 2) {   // two 16-byte pieces of the 16 keys' rows
+                        uint32_t b[4];
+                        ldsm_x4_t(smem_addr(sv + swz<L::kRow>(16 * kk + (lane & 15), p + (lane >> 4))), b[0], b[1], b[2], b[3]);
+                        #pragma unroll
+                        for (int mt = 0; mt < MT; mt++) {
+                            if constexpr (!L::k8) {
+                                mma16816<BF>(o[mt][p], a[mt], b[0], b[1]);
+                                mma16816<BF>(o[mt][p + 1], a[mt], b[2], b[3]);
+                            } else {
+                                #pragma unroll
+                                for (int q = 0; q < 2; q++) {
+                                    mma16816<BF>(o[mt][2 * (p + q)], a[mt], codes_f16x2<STORE, 0, 2>(b[2 * q]), codes_f16x2<STORE, 0, 2>(b[2 * q + 1]));
+                                    mma16816<BF>(o[mt][2 * (p + q) + 1], a[mt], codes_f16x2<STORE, 1, 3>(b[2 * q]), codes_f16x2<STORE, 1, 3>(b[2 * q + 1]));
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+            __syncwarp();   // the stage is free
+        }
+        cp_async_wait<0>();
+        __syncthreads();    // the rings are free: the warps' results go over them
+        float* join = reinterpret_cast<float*>(smem);               // [warp][row][D], then [warp][row][2]
+        float* join_ml = join + kWarps * L::kRows * D;
+        const float unit_v = L::k8 ? __uint_as_float(ve << 23) : 1.0f;
+        #pragma unroll
+        for (int r = 0; r < 2 * MT; r++) {
+            float sum = l[r];
+            sum += __shfl_xor_sync(~0u, sum, 1);
+            sum += __shfl_xor_sync(~0u, sum, 2);
+            const int row = 16 * (r >> 1) + g + 8 * (r & 1);
+            if (j == 0) {
+                join_ml[(warp * L::kRows + row) * 2] = m[r];
+                join_ml[(warp * L::kRows + row) * 2 + 1] = sum;
+            }
+            #pragma unroll
+            for (int d = 0; d < DT; d++)
+                #pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int dim = L::k8 ? (d >> 1) * 16 + 4 * j + 2 * e + (d & 1) : 8 * d + 2 * j + e;
+                    join[(warp * L::kRows + row) * D + dim] = o[r >> 1][d][2 * (r & 1) + e] * unit_v;
+                }
+        }
+        __syncthreads();
+        const bool whole = t0 == 0 && t1 == n;
+        float* slot = P.work + (size_t)(2 * blockIdx.x + (first_item ? 0 : 1)) * L::kSlot;
+        for (int i = tid; i < L::kRows * (D / 4); i += kThreads) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4, row = r_base + r;
+            if (row >= M) break;
+            const bool present = anc[row / P.group] != 0;
+            float mm = -INFINITY, ll = 0.f;
+            #pragma unroll
+            for (int w = 0; w < kWarps; w++) mm = fmaxf(mm, join_ml[(w * L::kRows + r) * 2]);
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+            #pragma unroll
+            for (int w = 0; w < kWarps; w++) {
+                const float mw = join_ml[(w * L::kRows + r) * 2], lw = join_ml[(w * L::kRows + r) * 2 + 1];
+                const float fw = mm == -INFINITY ? 1.0f : exp2_approx(mw - mm);
+                const float4 b = *reinterpret_cast<const float4*>(join + (w * L::kRows + r) * D + d);
+                ll += lw * fw;
+                a.x += b.x * fw; a.y += b.y * fw; a.z += b.z * fw; a.w += b.w * fw;
+            }
+            if (!present) { mm = -INFINITY; ll = 0.f; a = make_float4(0.f, 0.f, 0.f, 0.f); }
+            if (whole) {
+                const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+                const int node = row / P.group, hq = h * P.group + row % P.group;
+                uint8_t* dst = P.out + (((size_t)seq * P.n_nodes + node) * (size_t)P.ldo + (size_t)hq * D + d) * 2;
+                *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<QT == QWEN_BF16>(a.x * inv, a.y * inv), pack2<QT == QWEN_BF16>(a.z * inv, a.w * inv));
+            } else {
+                *reinterpret_cast<float4*>(slot + r * D + d) = a;
+                if (d == 0) *reinterpret_cast<float2*>(slot + L::kRows * D + 2 * r) = make_float2(mm, ll);
+            }
+        }
+        __syncthreads();
+        first_item = false;
+        at += t1 - t0;
+        if (at < to && at - before == (long long)n * units) { before = at; seq++; }
+    }
+}
+
+// Joins the partial results of the items that cross a border between shares:
+// block (i, y) takes the item that begins in share i and goes on in share i + 1, rows y * kJoinRows ..
+constexpr int kJoinThreads = 128;
+template <int QT, int KT, int D, int ROWS>
+__global__ void __launch_bounds__(kJoinThreads) combine_kernel(const Params P, int row_blocks) {
+    constexpr int kSlot = ROWS * (D + 2), kLanes = D / 4, kJoinRows = kJoinThreads / kLanes;
+    const int i = blockIdx.x, G = gridDim.x, units = P.n_kv_heads * row_blocks;
+    const long long tiles = line_tiles<KT>(P, units);
+    const long long from = share(tiles, i, G), edge = share(tiles, i + 1, G);
+    long long before = 0, s = edge, e = edge;   // the item at the border: its tiles
+    int seq = 0, unit = 0;
+    if (edge > from && edge < tiles) {
+        seq = line_find<KT>(P, units, edge, before);
+        const int n = seq_tiles<KT>(P, P.lens[seq]);
+        unit = (int)((edge - before) / n);
+        s = before + (long long)unit * n;
+        e = s + n;
+    }
+    pdl_wait();   // on every path: this kernel may not end before the one that it joins
+    if (s >= edge || s < from) return;          // it begins at the border, or before this share
+    const int last = share_of(tiles, e - 1, G);
+    const int h = unit / row_blocks, r = blockIdx.y * kJoinRows + threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
+    const int row = (unit - h * row_blocks) * ROWS + r;
+    if (row >= P.n_nodes * P.group) return;
+    // share i holds the item last (its second slot) unless it begins with it
+    const size_t first_slot = 2 * (size_t)i + (from < s ? 1 : 0);
+    float mm = -INFINITY, ll = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = i; k <= last; k++) {
+        if (k > i && share(tiles, k, G) == share(tiles, k + 1, G)) continue;
+        const float* slot = P.work + (k == i ? first_slot : 2 * (size_t)k) * kSlot;
+        const float2 ml = *reinterpret_cast<const float2*>(slot + ROWS * D + 2 * r);
+        const float4 b = *reinterpret_cast<const float4*>(slot + r * D + d);
+        const float mn = fmaxf(mm, ml.x);
+        const float f0 = mn == -INFINITY ? 1.0f : exp2_approx(mm - mn), f1 = mn == -INFINITY ? 1.0f : exp2_approx(ml.x - mn);
+        ll = ll * f0 + ml.y * f1;
+        a.x = a.x * f0 + b.x * f1; a.y = a.y * f0 + b.y * f1; a.z = a.z * f0 + b.z * f1; a.w = a.w * f0 + b.w * f1;
+        mm = mn;
+    }
+    const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+    const int node = row / P.group, hq = h * P.group + row % P.group;
+    uint8_t* dst = P.out + (((size_t)seq * P.n_nodes + node) * (size_t)P.ldo + (size_t)hq * D + d) * 2;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<QT == QWEN_BF16>(a.x * inv, a.y * inv), pack2<QT == QWEN_BF16>(a.z * inv, a.w * inv));
+}
+
+}  // namespace ta
+}  // namespace qb

@@ -87,6 +87,15 @@ _SIGS = {
     "qwen_batch_prefill": (_c.c_int, [_P, _c.c_int, _P, _c.c_int, _P]),
     "qwen_batch_step": (_c.c_int, [_P, _c.c_int, _P, _P, _P, _P, _P]),
     "qwen_batch_read_logits": (_c.c_int, [_P, _c.c_int, _P]),
+    "qwen_batch_cache": (_c.c_int, [_P, _c.c_int, _P]),
+    "qwen_kv_append": (_c.c_int, [_P, _P, _P, _c.c_int, _c.c_longlong, _c.c_int, _P, _P, _P]),
+    "qwen_kv_read": (_c.c_int, [_P, _P, _P, _c.c_int, _c.c_longlong, _c.c_int, _P, _P, _P]),
+    "qwen_kv_keep": (_c.c_int, [_P, _P, _P, _P, _c.c_int, _P]),
+    "qwen_tree_attention_workspace": (_c.c_int, [_P, _c.c_int, _c.c_int, _c.POINTER(_c.c_size_t)]),
+    "qwen_tree_attention": (_c.c_int, [_P, _P, _P, _c.c_int, _c.c_longlong, _c.c_longlong, _c.c_int, _c.c_int, _P, _P, _c.c_float, _P,
+                                       _c.c_size_t, _P]),
+    "qwen_tree_verify": (_c.c_int, [_P, _c.c_int, _c.c_longlong, _P, _c.c_longlong, _P, _P, _P, _c.c_int, _c.c_int, _c.c_int, _c.c_float,
+                                    _P, _P, _P, _P]),
     "qwen_tokenizer_load": (_c.c_int, [_c.c_char_p, _c.c_int, _c.POINTER(_P)]),
     "qwen_tokenizer_free": (None, [_P]),
     "qwen_tokenizer_info": (_c.c_int, [_P, _c.POINTER(_c.c_int), _c.POINTER(_c.c_int), _c.POINTER(_c.c_int), _c.POINTER(_c.c_int)]),
@@ -109,6 +118,17 @@ class Sampling(ctypes.Structure):
 
 
 GREEDY = Sampling(0.0, 1.0, 1)
+
+# element types of the drafted-token operators
+BF16, FP16, FP32, E4M3, INT8 = 0, 1, 2, 3, 4
+
+
+class KVCache(ctypes.Structure):
+    """qwen_kv_cache_t: a view of K/V rows in device memory (pointers as ints, None for
+    absent scales; strides in elements)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("seq_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong), ("dtype", ctypes.c_int), ("n_seqs", ctypes.c_int),
+                ("n_kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("capacity", ctypes.c_int)]
 
 
 def load_library(path=None):
@@ -235,6 +255,43 @@ def gemv_bf16_static(W_ptr, x_ptr, y_ptr, n, k, stream=0):
                                                 ctypes.c_void_p(stream)))
 
 
+# ---- drafted-token decoding over a K/V cache (device pointers, ints) ----
+def kv_append(cache, k_ptr, v_ptr, dtype, ld, n_tokens, start_ptr, counts_ptr=0, stream=0):
+    """K/V rows (s, t) of k and v (ld elements apart) -> positions start[s] + t of the cache, t < counts[s]."""
+    _check(load_library().qwen_kv_append(ctypes.byref(cache), k_ptr, v_ptr, dtype, ld, n_tokens, start_ptr, counts_ptr, stream))
+
+
+def kv_read(cache, k_ptr, v_ptr, dtype, ld, n_tokens, start_ptr, counts_ptr=0, stream=0):
+    """Positions start[s] + t of the cache, t < counts[s] -> rows (s, t) of k and v."""
+    _check(load_library().qwen_kv_read(ctypes.byref(cache), k_ptr, v_ptr, dtype, ld, n_tokens, start_ptr, counts_ptr, stream))
+
+
+def kv_keep(cache, start_ptr, path_ptr, n_path_ptr, n_nodes, stream=0):
+    """Position start[s] + i of the cache <- what position start[s] + path[s][i] held, i < n_path[s]."""
+    _check(load_library().qwen_kv_keep(ctypes.byref(cache), start_ptr, path_ptr, n_path_ptr, n_nodes, stream))
+
+
+def tree_attention_workspace(cache, n_nodes, n_heads):
+    """Bytes of workspace of tree_attention."""
+    n = ctypes.c_size_t()
+    _check(load_library().qwen_tree_attention_workspace(ctypes.byref(cache), n_nodes, n_heads, ctypes.byref(n)))
+    return n.value
+
+
+def tree_attention(cache, q_ptr, out_ptr, dtype, ldq, ldo, n_nodes, n_heads, lens_ptr, parents_ptr, scale, workspace_ptr, workspace_bytes,
+                   stream=0):
+    """Attention of the tree's nodes over positions 0 .. lens[s]-1, their ancestors and themselves (positions lens[s] + node)."""
+    _check(load_library().qwen_tree_attention(ctypes.byref(cache), q_ptr, out_ptr, dtype, ldq, ldo, n_nodes, n_heads, lens_ptr, parents_ptr,
+                                              scale, workspace_ptr, workspace_bytes, stream))
+
+
+def tree_verify(logits_ptr, dtype, ld, draft_ptr, ld_draft, tokens_ptr, parents_ptr, uniforms_ptr, n_seqs, n_nodes, vocab, temperature,
+                path_ptr, n_path_ptr, next_ptr, stream=0):
+    """Which drafted nodes the target's logits keep (path, n_path) and the token after them (next)."""
+    _check(load_library().qwen_tree_verify(logits_ptr, dtype, ld, draft_ptr, ld_draft, tokens_ptr, parents_ptr, uniforms_ptr, n_seqs, n_nodes,
+                                           vocab, temperature, path_ptr, n_path_ptr, next_ptr, stream))
+
+
 class Engine:
     """One model instance on one GPU (a qwen_t handle)."""
 
@@ -336,6 +393,12 @@ class Engine:
         out = np.zeros((int(rows), VOCAB_SIZE), dtype=np.float32)
         _check(self._lib.qwen_batch_read_logits(self._h, int(rows), _ptr(out)))
         return out
+
+    def batch_cache(self, layer=-1):
+        """KVCache view of one layer of the batch slots (-1: all layers' heads in one view)."""
+        c = KVCache()
+        _check(self._lib.qwen_batch_cache(self._h, int(layer), ctypes.byref(c)))
+        return c
 
     def set_prefill_parts(self, parts=3):
         """bf16 parts per activation in the tensor-core passes (3: fp32-exact, 2, 1)."""
