@@ -216,20 +216,53 @@ int attention_by_shape(int dim, const qb::ta::Params& P, const Plan& plan, int d
 }
 
 // ---- verification --------------------------------------------------------------------
+// CTAs for a sequence: as many as the SMs have for each of them, a run of 128
+// tokens at least for each warp; 16 (more than every GPU must offer) where the
+// device can hold that many such clusters.  Row buffers: two, one or none,
+// whichever fits.
+constexpr int kVerifySmem = 208 * 1024;
 template <int T>
-int verify_launch(const qb::tv::Params& P, int n_seqs, int cluster, cudaStream_t st) {
+int verify_launch(qb::tv::Params& P, int n_seqs, int nsm, int dev, cudaStream_t st) {
+    using namespace qb::tv;
+    static std::atomic<uint64_t> done{0};
+    static std::atomic<int> wide[64];   // clusters of 16 that fit at once, + 1
+    const auto kernel = verify_kernel<T, true>;
+    if (!((done.load() >> dev) & 1)) {
+        CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        CU(cudaFuncSetAttribute(verify_kernel<T, false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    }
+    TRY(smem_limit(kernel, done, dev, kVerifySmem));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)n_seqs * cluster);
-    cfg.blockDim = dim3(qb::tv::kThreads);
-    cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = cluster;
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    CU(cudaLaunchKernelEx(&cfg, qb::tv::verify_kernel<T>, P));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = st;
+    int n16 = wide[dev].load();
+    if (!n16) {
+        cfg.gridDim = dim3(16);
+        at[0].val.clusterDim.x = 16;
+        cfg.dynamicSmemBytes = kVerifySmem;
+        if (cudaOccupancyMaxActiveClusters(&n16, kernel, &cfg) != cudaSuccess) { cudaGetLastError(); n16 = 0; }
+        wide[dev].store(++n16);
+    }
+    const int runs = (P.vocab + kRun - 1) / kRun;
+    int cluster = 1;
+    while (cluster < kMaxCluster && (long long)n_seqs * cluster * 2 <= nsm && runs >= cluster * 2 * kWarps) cluster *= 2;
+    if (cluster == 16 && n_seqs > n16 - 1) cluster = 8;
+    const int parts = cluster * kWarps;
+    const int part_runs = (runs + parts - 1) / parts;
+    P.part_bytes = (part_runs + 1) / 2 * 2 * kRun * (T == QWEN_FP32 ? 4 : 2);   // whole steps of two runs
+    const long long row = (long long)kWarps * P.part_bytes;
+    P.buffers = 2 * row <= kVerifySmem ? 2 : row <= kVerifySmem ? 1 : 0;
+    at[0].val.clusterDim.x = cluster;
+    cfg.gridDim = dim3((unsigned)n_seqs * cluster);
+    cfg.dynamicSmemBytes = (size_t)(P.buffers * row);
+    if (P.buffers) CU(cudaLaunchKernelEx(&cfg, kernel, P));
+    else CU(cudaLaunchKernelEx(&cfg, verify_kernel<T, false>, P));
     return QWEN_OK;
 }
 
@@ -349,13 +382,10 @@ extern "C" int qwen_tree_verify(const void* logits, int logits_dtype, long long 
     const bool rows16 = ((uintptr_t)logits | (size_t)ld * elem) % 16 == 0;
     P.vec = rows16 && (!P.draft || ((uintptr_t)draft | (size_t)ld_draft * 4) % 16 == 0);
     P.temperature = temperature;
-    // as many CTAs for a sequence as the SMs allow, a whole run of 128 tokens for each warp
-    int cluster = 1;
-    while (cluster < qb::tv::kMaxCluster && (long long)n_seqs * cluster * 2 <= nsm && vocab >= cluster * 2 * qb::tv::kWarps * 128) cluster *= 2;
     const cudaStream_t st = (cudaStream_t)stream;
     switch (logits_dtype) {
-        case QWEN_BF16: return verify_launch<QWEN_BF16>(P, n_seqs, cluster, st);
-        case QWEN_FP16: return verify_launch<QWEN_FP16>(P, n_seqs, cluster, st);
-        default: return verify_launch<QWEN_FP32>(P, n_seqs, cluster, st);
+        case QWEN_BF16: return verify_launch<QWEN_BF16>(P, n_seqs, nsm, dev, st);
+        case QWEN_FP16: return verify_launch<QWEN_FP16>(P, n_seqs, nsm, dev, st);
+        default: return verify_launch<QWEN_FP32>(P, n_seqs, nsm, dev, st);
     }
 }

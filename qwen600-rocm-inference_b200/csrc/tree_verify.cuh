@@ -11,12 +11,27 @@
 // so rest is p without the refused tokens.)  Only the rows that the walk
 // reaches are read.
 //
-// One cluster of CTAs per sequence, every CTA a contiguous slice of the
-// vocabulary, every warp a contiguous part of that.  Statistics that decide a
-// comparison (largest logit, sum) are fp32 while nothing is refused; sums that
-// the drawn token's position depends on (the running sum crosses a border for
-// each of up to 10^5 tokens, so 24 bits would misplace about one draw in a
-// hundred) are fp64.
+// One cluster of CTAs per sequence, every warp a contiguous part of the
+// vocabulary (whole runs of 128 tokens).  A level of the walk is a chain of
+// latencies - the row's arrival, the largest logit and the sum, one exchange over
+// the cluster - so a warp keeps its part of the row in shared memory where that
+// fits, the first child's row is copied meanwhile (into a second buffer, or
+// piece by piece over the row that is being read), and every warp's statistics go
+// straight to every CTA through distributed shared memory: one cluster barrier a
+// pass.
+//
+// Statistics that decide a comparison (largest logit, sum) are fp32 while nothing
+// is refused.  Sums that the drawn token's position depends on are fp64: the
+// running sum crosses a border for each of up to 10^5 tokens, so 24 bits would
+// misplace about one draw in a hundred.  Their powers of two are a polynomial of
+// degree 8 in fp64 (relative error 2^-39, 13 fp64 operations a token; a table of
+// 256 roots with three operations took as long, on bank conflicts).
+//
+// Measured on a vocabulary of 151,936 in fp32: a chain of 8 nodes of one
+// sequence 22 us, 32 sequences with drafted probabilities 59 us (the rows that are
+// reached and the last drafted rows are 13 us of memory traffic; the longest of
+// the 32 walks is eight levels of 4.5 us: 2.6 us for a row's 38,000 tokens an SM,
+// 1.3 us for the exchange).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -27,8 +42,9 @@
 namespace qb {
 namespace tv {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kMaxNodes = 64, kMaxCluster = 8;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kRun = 128;
+constexpr uint64_t kWaitNs = 1000000000ull;   // longest wait for a copy from this GPU's own memory
+constexpr int kMaxNodes = 64, kMaxCluster = 16, kMaxParts = kMaxCluster * kWarps;
 
 struct Params {
     const void* logits;
@@ -38,12 +54,14 @@ struct Params {
     int *path, *n_path, *next;
     long long ld, ld_draft;
     int n_nodes, vocab, vec;   // vec: rows of logits and draft start on 16 bytes
+    int buffers, part_bytes;   // row buffers in shared memory (0: parts do not fit), bytes of a warp's part (whole steps)
     float temperature;
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void st_cluster(const void* local, uint32_t rank, uint64_t v) {
@@ -52,211 +70,399 @@ __device__ __forceinline__ void st_cluster(const void* local, uint32_t rank, uin
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
 }
 
-// What the CTAs of a cluster tell one another: two words each, two buffers in
-// turn (a buffer is written again only after the next exchange's barrier).
+// What the warps of a cluster tell one another: a word or two each, two buffers
+// in turn (a buffer is written again only after the next exchange's barrier).
 struct Shared {
-    uint64_t box[2][kMaxCluster][2];
-    double wsum[kWarps];             // sums of rest over the warps' parts, of the last sum pass
-    float wm[kWarps], wz[kWarps];
-    int wi[kWarps], wf[kWarps];
+    uint64_t box[2][kMaxParts];
+    double run_sum[kWarps];          // the owner's second look: its runs' sums, last weighted tokens, the token
+    int run_last[kWarps], found;
+    uint64_t arrived[2][kWarps];     // a row buffer's bulk copies, per warp
+    int late;                        // a wait for them ran out
     float lx[kMaxNodes], qx[kMaxNodes], u[kMaxNodes];
     int par[kMaxNodes], tok[kMaxNodes], gone[kMaxNodes];   // gone: refused tokens at this node (chosen drafts)
 };
 
+__device__ __forceinline__ float exp2_ftz(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// a warp's largest value (no NaN), by the order of its bits as a whole number
+__device__ __forceinline__ float max_lanes(float x) {
+    const int b = __float_as_int(x);
+    const int r = __reduce_max_sync(~0u, b < 0 ? b ^ 0x7fffffff : b);
+    return __int_as_float(r < 0 ? r ^ 0x7fffffff : r);
+}
+__device__ __forceinline__ float sum_lanes(float x) {
+    #pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
+    return x;
+}
 template <int T>
 __device__ __forceinline__ float load1(const void* p, size_t i) {
     if constexpr (T == QWEN_FP32) return __ldg((const float*)p + i);
     else if constexpr (T == QWEN_BF16) return bf2f(__ldg((const uint16_t*)p + i));
     else return __half2float(__ldg((const __half*)p + i));
 }
-// four consecutive values; past `end` they are `pad`
+// four values from 8 or 16 bytes
+template <int T>
+__device__ __forceinline__ void unpack4(const uint4& w, float (&x)[4]) {
+    if constexpr (T == QWEN_FP32) {
+        x[0] = __uint_as_float(w.x); x[1] = __uint_as_float(w.y); x[2] = __uint_as_float(w.z); x[3] = __uint_as_float(w.w);
+    } else if constexpr (T == QWEN_BF16) {
+        x[0] = bf_lo(w.x); x[1] = bf_hi(w.x); x[2] = bf_lo(w.y); x[3] = bf_hi(w.y);
+    } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), g = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+        x[0] = f.x; x[1] = f.y; x[2] = g.x; x[3] = g.y;
+    }
+}
+// four consecutive values of a row in global memory; past `end` they are `pad`
 template <int T>
 __device__ __forceinline__ void load4(const void* row, int i, int end, bool vec, float pad, float (&x)[4]) {
     if (vec && i + 4 <= end) {
+        uint4 w = make_uint4(0, 0, 0, 0);
         if constexpr (T == QWEN_FP32) {
-            const float4 a = __ldg(reinterpret_cast<const float4*>((const float*)row + i));
-            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+            w = __ldg(reinterpret_cast<const uint4*>((const float*)row + i));
         } else {
             const uint2 a = __ldg(reinterpret_cast<const uint2*>((const uint16_t*)row + i));
-            if constexpr (T == QWEN_BF16) {
-                x[0] = bf_lo(a.x); x[1] = bf_hi(a.x); x[2] = bf_lo(a.y); x[3] = bf_hi(a.y);
-            } else {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a.x)), g = __half22float2(*reinterpret_cast<const __half2*>(&a.y));
-                x[0] = f.x; x[1] = f.y; x[2] = g.x; x[3] = g.y;
-            }
+            w.x = a.x; w.y = a.y;
         }
+        unpack4<T>(w, x);
     } else {
         #pragma unroll
         for (int j = 0; j < 4; j++) x[j] = i + j < end ? load1<T>(row, i + j) : pad;
     }
 }
 
-// grid n_seqs * cluster CTAs, kThreads threads.
-template <int T>
+// grid n_seqs * cluster CTAs, kThreads threads, buffers * kWarps * part_bytes of
+// dynamic shared memory.  HELD: parts are held in row buffers (P.buffers > 0).
+template <int T, bool HELD>
 __global__ void __launch_bounds__(kThreads) verify_kernel(const Params P) {
+    constexpr int K = HELD ? 2 : 4;   // runs of a step: 4 K tokens a lane
+    constexpr int kEs = T == QWEN_FP32 ? 4 : 2;
     __shared__ Shared sh;
+    extern __shared__ __align__(16) uint8_t parts_mem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)cluster_rank(), size = (int)cluster_size(), seq = blockIdx.x / size;
     const int N = P.n_nodes, V = P.vocab;
     const bool greedy = P.temperature == 0.0f, vec = P.vec != 0;
-    // this warp's part of the vocabulary: whole runs of 128
-    const int runs = (V + 127) / 128, parts = size * kWarps, mine = rank * kWarps + warp;
-    const int lo = (int)((long long)runs * mine / parts) * 128, hi = min((int)((long long)runs * (mine + 1) / parts) * 128, V);
+    // this warp's part of the vocabulary
+    const int runs = (V + kRun - 1) / kRun, parts = size * kWarps, mine = rank * kWarps + warp;
+    const int r0 = (int)((long long)runs * mine / parts), r1 = (int)((long long)runs * (mine + 1) / parts);
+    const int lo = r0 * kRun, hi = min(r1 * kRun, V);
+
+    auto row_of = [&](int node) { return (const uint8_t*)P.logits + ((size_t)seq * N + node) * (size_t)P.ld * kEs; };
+    if (lane == 0) {
+        mbar_init(&sh.arrived[0][warp], 1);
+        mbar_init(&sh.arrived[1][warp], 1);
+        fence_barrier_init();
+    }
+    __syncwarp();
+    // Tokens from .. to-1 (from: a whole run) of this warp's part of a node's row into buffer b: by bulk copies, which take no
+    // issue slots from the arithmetic, where rows start on 16 bytes.  first: the first piece of the part.
+    uint32_t phase = 0;      // bit b: the parity that buffer b's next part completes
+    uint32_t coming = 0;     // bit b: a part is on its way
+    auto fetch = [&](int node, int b, int from, int to, bool first) {
+        uint8_t* dst = parts_mem + (size_t)(b * kWarps + warp) * P.part_bytes;
+        const uint8_t* row = row_of(node);
+        int k = from;        // tokens from here on are copied one by one
+        if (vec) {
+            const uint32_t n = (uint32_t)((to - from) * kEs) & ~15u, all = (uint32_t)((hi - lo) * kEs) & ~15u;
+            if (lane == 0) {
+                if (first && all) mbar_arrive_expect_tx(&sh.arrived[b][warp], all);
+                if (n) bulk_g2s(dst + (size_t)(from - lo) * kEs, row + (size_t)from * kEs, n, &sh.arrived[b][warp], policy_evict_last());
+            }
+            if (all) coming |= 1u << b;
+            k = from + (int)(n / kEs);
+        }
+        for (k += lane; k < to; k += 32) {
+            if constexpr (kEs == 4) reinterpret_cast<float*>(dst)[k - lo] = __ldg((const float*)row + k);
+            else reinterpret_cast<uint16_t*>(dst)[k - lo] = __ldg((const uint16_t*)row + k);
+        }
+    };
+    // Waits for buffer b's part; a wait that runs out marks the sequence (next = -1) and goes on.
+    auto landed = [&](int b) {
+        if (coming >> b & 1) {
+            if (!mbar_wait(&sh.arrived[b][warp], phase >> b & 1, kWaitNs)) sh.late = 1;
+            phase ^= 1u << b;
+            coming &= ~(1u << b);
+        }
+        __syncwarp();
+    };
+    if constexpr (HELD) {
+        fetch(0, 0, lo, hi, true);
+        // behind the part's end: -inf up to a whole step
+        for (int b = 0; b < P.buffers; b++) {
+            uint8_t* dst = parts_mem + (size_t)(b * kWarps + warp) * P.part_bytes;
+            for (int k = hi - lo + lane; k < P.part_bytes / kEs; k += 32) {
+                if constexpr (T == QWEN_FP32) reinterpret_cast<float*>(dst)[k] = -INFINITY;
+                else reinterpret_cast<uint16_t*>(dst)[k] = T == QWEN_BF16 ? 0xff80 : 0xfc00;
+            }
+        }
+    }
 
     if (tid < N) {
         sh.par[tid] = P.parents[(size_t)seq * N + tid];
         sh.tok[tid] = N > 1 ? P.tokens[(size_t)seq * N + tid] : 0;
         sh.u[tid] = greedy ? 0.f : P.uniforms[(size_t)seq * N + tid];
     }
-    __syncthreads();
+    if (tid == 0) { sh.found = INT_MAX; sh.late = 0; }
     int* path = P.path + (size_t)seq * N;
     if (rank == 0 && tid < N) path[tid] = -1;
+    __syncthreads();         // (path's -1 come before its entries)
     if (sh.par[0] != -1) {   // the same for the whole cluster
         if (rank == 0 && tid == 0) { P.n_path[seq] = 0; P.next[seq] = -1; }
+        if constexpr (HELD) landed(0);
         return;
     }
-    __syncthreads();         // path's -1 before its entries (rank 0, thread 0 writes them)
+    // every node's logit (and drafted probability) in its parent's row
+    if (tid < N && !greedy) {
+        const int up = sh.par[tid], x = sh.tok[tid];
+        const bool in = up >= 0 && up < tid && x >= 0 && x < V;
+        sh.lx[tid] = in ? load1<T>(row_of(up), x) : -INFINITY;
+        sh.qx[tid] = in && P.draft ? __ldg(P.draft + ((size_t)seq * N + up) * (size_t)P.ld_draft + x) : 1.0f;
+    }
     cluster_sync();          // every CTA runs before another writes to its box
 
     const float c32 = greedy ? 0.f : 1.4426950408889634f / P.temperature;
-    const double it64 = greedy ? 0.0 : 1.0 / (double)P.temperature;
-    int turn = 0;
-    // every CTA's two words to every CTA; sh.box[result] then holds them by rank
-    auto exchange = [&](uint64_t a, uint64_t b) {
-        const int buf = turn & 1;
-        turn++;
-        if (tid < size) {
-            st_cluster(&sh.box[buf][rank][0], tid, a);
-            st_cluster(&sh.box[buf][rank][1], tid, b);
-        }
-        __syncwarp();
-        cluster_sync();
-        return buf;
-    };
+    const double c64 = greedy ? 1.0 : 1.4426950408889634074 / (double)P.temperature;
+    const unsigned dmin = (unsigned)__double2hiint(-1000.0 / c64);   // high word of the lowest x - M that counts
+    int turn = 0, held = 0;  // held: the buffer with the reached node's row
+    int other = -1;          // two buffers: the node whose row is on its way into the second
+    int inside = 0;          // one buffer: the node whose row it holds or receives
 
     int at = 0, count = 1;
     if (rank == 0 && tid == 0) path[0] = 0;
     for (;;) {
-        const void* row = (const uint8_t*)P.logits + ((size_t)seq * N + at) * (size_t)P.ld * (T == QWEN_FP32 ? 4 : 2);
+        const uint8_t* row = row_of(at);
         const float* qrow = P.draft && !greedy ? P.draft + ((size_t)seq * N + at) * (size_t)P.ld_draft : nullptr;
-        if (tid < N && tid > at && sh.par[tid] == at) {
-            const int x = sh.tok[tid];
-            const bool in = x >= 0 && x < V;
-            sh.lx[tid] = in ? load1<T>(row, x) : -INFINITY;
-            sh.qx[tid] = in && qrow ? __ldg(qrow + x) : 1.0f;
+        // the children, and the first of them
+        uint64_t children = __ballot_sync(~0u, lane > at && lane < N && sh.par[lane] == at) |
+                            (uint64_t)__ballot_sync(~0u, lane + 32 > at && lane + 32 < N && sh.par[lane + 32] == at) << 32;
+        const int child = __ffsll((long long)children) - 1;
+        const bool next_row = child >= 0;
+        if constexpr (HELD) {
+            landed(held);
+            if (next_row && P.buffers == 2) {
+                landed(held ^ 1);
+                fetch(child, held ^ 1, lo, hi, true);
+                other = child;
+            }
+        } else if (next_row && vec && hi > lo) {   // as far as the L2
+            const int n = (hi - lo) * kEs & ~15;
+            if (lane == 0 && n) bulk_prefetch_l2(row_of(child) + (size_t)lo * kEs, n);
         }
+        const uint8_t* part = parts_mem + (size_t)(held * kWarps + warp) * P.part_bytes;
+        // one step's logits: runs i0 / kRun .., tokens i0 + kRun k + 4 lane + j at x[4 k + j]; -inf past the end
+        auto step = [&](int i0, auto& x) {
+            #pragma unroll
+            for (int k = 0; k < (int)sizeof(x) / 16; k++) {
+                float y[4];
+                if constexpr (HELD) {
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    const uint8_t* p = part + (size_t)(i0 - lo + kRun * k + 4 * lane) * kEs;
+                    if constexpr (kEs == 4) {
+                        w = *reinterpret_cast<const uint4*>(p);
+                    } else {
+                        const uint2 a = *reinterpret_cast<const uint2*>(p);
+                        w.x = a.x; w.y = a.y;
+                    }
+                    unpack4<T>(w, y);
+                } else {
+                    load4<T>(row, i0 + kRun * k + 4 * lane, hi, vec, -INFINITY, y);
+                }
+                #pragma unroll
+                for (int j = 0; j < 4; j++) x[4 * k + j] = y[j];
+            }
+        };
         // ---- largest logit (its first place) and, unless greedy, the fp32 sum ----
         float m = -INFINITY, z = 0.f;
         int mi = INT_MAX, bad = 0;
-        for (int i0 = lo; i0 < hi; i0 += 512) {
-            float x[4][4];
-            #pragma unroll
-            for (int k = 0; k < 4; k++) load4<T>(row, i0 + 128 * k + 4 * lane, hi, vec, -INFINITY, x[k]);
-            float m4 = m;
-            #pragma unroll
-            for (int k = 0; k < 4; k++)
+        for (int i0 = lo; i0 < hi; i0 += K * kRun) {
+            float x[4 * K];
+            step(i0, x);
+            if (greedy) {
                 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if (x[k][j] > m4) { m4 = x[k][j]; mi = i0 + 128 * k + 4 * lane + j; }
-                    bad |= x[k][j] != x[k][j];
+                for (int j = 0; j < 4 * K; j++) {
+                    if (x[j] > m) { m = x[j]; mi = i0 + kRun * (j >> 2) + 4 * lane + (j & 3); }
+                    bad |= x[j] != x[j];
                 }
-            if (!greedy && m4 > -INFINITY) {
-                z *= exp2f((m - m4) * c32);
+            } else {             // (a NaN makes z NaN; before any logit above -inf z stays 0)
+                float t[4 * K];
                 #pragma unroll
-                for (int k = 0; k < 4; k++)
+                for (int j = 0; j < 4 * K; j++) t[j] = x[j];
+                #pragma unroll
+                for (int o = 2 * K; o > 0; o >>= 1)
                     #pragma unroll
-                    for (int j = 0; j < 4; j++) z += exp2f((x[k][j] - m4) * c32);
+                    for (int j = 0; j < o; j++) t[j] = fmaxf(t[j], t[j + o]);
+                const float top = fmaxf(m, t[0]), from = top > -INFINITY ? top : 0.f;
+                #pragma unroll
+                for (int j = 0; j < 4 * K; j++) t[j] = exp2_ftz((x[j] - from) * c32);
+                #pragma unroll
+                for (int o = 2 * K; o > 0; o >>= 1)
+                    #pragma unroll
+                    for (int j = 0; j < o; j++) t[j] += t[j + o];
+                z = fmaf(z, exp2_ftz((m - from) * c32), t[0]);
+                m = top;
             }
-            m = m4;
+            // one buffer: the next row over what has been read, in pieces of four steps (smaller ones cost more to issue)
+            if (HELD && next_row && P.buffers == 1 && (((i0 - lo) / (K * kRun) & 3) == 3 || i0 + K * kRun >= hi)) {
+                const int piece = i0 - ((i0 - lo) / (K * kRun) & 3) * (K * kRun);
+                __syncwarp();
+                fetch(child, 0, piece, min(i0 + K * kRun, hi), piece == lo);
+            }
         }
-        auto join = [&](float m2, float z2, int i2) {
-            const float mm = fmaxf(m, m2);
-            if (mm > -INFINITY) z = (m > -INFINITY ? z * exp2f((m - mm) * c32) : 0.f) + (m2 > -INFINITY ? z2 * exp2f((m2 - mm) * c32) : 0.f);
-            mi = m2 > m ? i2 : m2 == m ? min(mi, i2) : mi;
-            m = mm;
-        };
-        #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float m2 = __shfl_xor_sync(~0u, m, o), z2 = __shfl_xor_sync(~0u, z, o);
-            const int i2 = __shfl_xor_sync(~0u, mi, o);
-            join(m2, z2, i2);
+        if (HELD && next_row && P.buffers == 1) inside = child;
+        if (!greedy) bad = z != z;
+        // the warp's, then the cluster's: the largest first, then the sums on its scale.  A warp that met a NaN says +inf.
+        float M = max_lanes(__any_sync(~0u, bad) ? INFINITY : m);
+        {
+            uint64_t* box = sh.box[turn & 1];
+            turn++;
+            uint32_t low;
+            if (greedy) low = __reduce_min_sync(~0u, m == M ? mi : INT_MAX);
+            else low = __float_as_uint(sum_lanes(m > -INFINITY && M < INFINITY ? z * exp2_ftz((m - M) * c32) : 0.f));
+            if (lane < size) st_cluster(box + mine, lane, (uint64_t)__float_as_uint(M) << 32 | low);
+            cluster_sync();
+            uint64_t w[kMaxParts / 32];
+            m = -INFINITY;
+            #pragma unroll
+            for (int k = 0; k < kMaxParts / 32; k++) {
+                w[k] = lane + 32 * k < parts ? box[lane + 32 * k] : 0xff80000000000000ull;   // -inf
+                m = fmaxf(m, __uint_as_float((uint32_t)(w[k] >> 32)));
+            }
+            M = max_lanes(m);
+            z = 0.f;
+            mi = INT_MAX;
+            #pragma unroll
+            for (int k = 0; k < kMaxParts / 32; k++) {
+                const float mk = __uint_as_float((uint32_t)(w[k] >> 32));
+                if (greedy) { if (mk == M) mi = min(mi, (int)(uint32_t)w[k]); }
+                else if (mk > -INFINITY) z += __uint_as_float((uint32_t)w[k]) * exp2_ftz((mk - M) * c32);
+            }
+            if (greedy) mi = __reduce_min_sync(~0u, mi);
+            else z = sum_lanes(z);
         }
-        bad = __any_sync(~0u, bad);
-        if (lane == 0) { sh.wm[warp] = m; sh.wz[warp] = z; sh.wi[warp] = mi; sh.wf[warp] = bad; }
-        __syncthreads();
-        m = -INFINITY; z = 0.f; mi = INT_MAX; bad = 0;
-        for (int w = 0; w < kWarps; w++) { join(sh.wm[w], sh.wz[w], sh.wi[w]); bad |= sh.wf[w]; }
-        int buf = exchange((uint64_t)__float_as_uint(m) << 32 | __float_as_uint(z), (uint64_t)(uint32_t)mi << 32 | (uint32_t)bad);
-        m = -INFINITY; z = 0.f; mi = INT_MAX; bad = 0;
-        for (int r = 0; r < size; r++) {
-            const uint64_t a = sh.box[buf][r][0], b = sh.box[buf][r][1];
-            join(__uint_as_float((uint32_t)(a >> 32)), __uint_as_float((uint32_t)a), (int)(b >> 32));
-            bad |= (int)(b & 1);
-        }
-        const float M = m;
-        const bool none = bad || !(M > -INFINITY) || M == INFINITY;
+        const bool none = !(M > -INFINITY) || M == INFINITY;
 
         // ---- children in index order ----
         int kept = -1, n_gone = 0;
-        double Z = z, left = 1.0, S = 0.0, total = 0.0;
+        // Z: the sum; left, S and rest are Z times those of the walk's definition
+        double Z = z, left = Z, S = 0.0;
         bool summed = false;
-        // rest's sum over the vocabulary (fp64), unnormalised while S is 0; the warps' sums stay in sh.wsum
-        auto weight = [&](float x, float q) {
-            const double e = exp(((double)x - (double)M) * it64);
-            return S > 0.0 ? fmax(e / Z - S * (double)q, 0.0) : e;
+        const double M64 = M;
+        // weights 2^(c (x - M)) = 2^n 2^f, |f| <= 1/2, of K tokens; in[j]: the weight counts (not below 2^-1000).  The steps go
+        // over all K in turn, so that each fp64 operation finds the others' in the pipe
+        auto powers = [&](const auto& x, auto& e, auto& in) {
+            constexpr int K = sizeof(x) / sizeof(float);
+            double d[K], f[K];
+            int n[K];
+            #pragma unroll
+            for (int j = 0; j < K; j++) d[j] = (double)x[j] - M64;
+            #pragma unroll
+            for (int j = 0; j < K; j++) f[j] = fma(d[j], c64, 6755399441055744.0);   // + 1.5 * 2^52: the nearest whole number in the low word
+            #pragma unroll
+            for (int j = 0; j < K; j++) { n[j] = __double2loint(f[j]); f[j] -= 6755399441055744.0; }
+            #pragma unroll
+            for (int j = 0; j < K; j++) f[j] = fma(d[j], c64, -f[j]);
+            constexpr double kC[8] = {1.5310079402249296e-05, 1.5403455852453838e-04, 1.3333450568000645e-03, 9.618129159402558e-03,
+                                      5.550410941205933e-02, 2.402265069581299e-01, 6.931471805459335e-01, 1.0};
+            #pragma unroll
+            for (int j = 0; j < K; j++) e[j] = fma(f[j], 1.3255224878668817e-06, kC[0]);
+            #pragma unroll
+            for (int i = 1; i < 8; i++)
+                #pragma unroll
+                for (int j = 0; j < K; j++) e[j] = fma(f[j], e[j], kC[i]);
+            #pragma unroll
+            for (int j = 0; j < K; j++) {
+                e[j] = __hiloint2double(__double2hiint(e[j]) + (n[j] << 20), __double2loint(e[j]));
+                in[j] = (unsigned)__double2hiint(d[j]) < dmin;   // d > -1000 / c by its high word (d is 0 or negative)
+            }
+        };
+        auto power = [&](float x) {
+            const float a[1] = {x};
+            double e[1];
+            bool in[1];
+            powers(a, e, in);
+            return in[0] ? e[0] : 0.0;
+        };
+        // what is left of the tokens' weights, where in[j] (S > 0: with draft)
+        auto weights = [&](const auto& x, const auto& q, auto& e, auto& in) {
+            powers(x, e, in);
+            if (S > 0.0) {
+                #pragma unroll
+                for (int j = 0; j < (int)(sizeof(x) / sizeof(float)); j++) {
+                    e[j] = fma(-S, (double)q[j], e[j]);
+                    in[j] = in[j] && __double2hiint(e[j]) >= 0;
+                }
+            }
         };
         auto is_gone = [&](int i) {
             for (int g = 0; g < n_gone; g++) if (sh.gone[g] == i) return true;
             return false;
         };
+        const uint64_t* sums = nullptr;   // the parts' sums of rest, of the last sum pass
         auto sum_pass = [&]() {
-            double s = 0.0;
+            if (HELD && P.buffers == 1 && inside != at) {
+                landed(0);
+                fetch(at, 0, lo, hi, true);
+                landed(0);
+                inside = at;
+            }
+            double sum[8] = {};
             bool any = false;
             for (int g = 0; g < n_gone; g++) any |= sh.gone[g] >= lo && sh.gone[g] < hi;
-            for (int i0 = lo; i0 < hi; i0 += 256) {
-                float x[2][4], q[2][4];
-                #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    load4<T>(row, i0 + 128 * k + 4 * lane, hi, vec, -INFINITY, x[k]);
-                    if (S > 0.0) load4<QWEN_FP32>(qrow, i0 + 128 * k + 4 * lane, hi, vec, 0.f, q[k]);
+            for (int i0 = lo; i0 < hi; i0 += 2 * kRun) {
+                float x[8], q[8];
+                double e[8];
+                bool in[8];
+                step(i0, x);
+                if (S > 0.0) {
+                    #pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        float y[4];
+                        load4<QWEN_FP32>(qrow, i0 + kRun * k + 4 * lane, hi, vec, 0.f, y);
+                        #pragma unroll
+                        for (int j = 0; j < 4; j++) q[4 * k + j] = y[j];
+                    }
+                }
+                weights(x, q, e, in);
+                if (any) {
+                    #pragma unroll
+                    for (int j = 0; j < 8; j++) if (is_gone(i0 + kRun * (j >> 2) + 4 * lane + (j & 3))) in[j] = false;
                 }
                 #pragma unroll
-                for (int k = 0; k < 2; k++)
-                    #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int i = i0 + 128 * k + 4 * lane + j;
-                        if (i < hi && !(any && is_gone(i))) s += weight(x[k][j], S > 0.0 ? q[k][j] : 0.f);
-                    }
+                for (int j = 0; j < 8; j++) if (in[j]) sum[j] += e[j];
             }
+            double s = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
             #pragma unroll
             for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-            __syncthreads();   // readers of an earlier pass's wsum
-            if (lane == 0) sh.wsum[warp] = s;
-            __syncthreads();
-            double cta = 0.0;
-            for (int w = 0; w < kWarps; w++) cta += sh.wsum[w];
-            buf = exchange((uint64_t)__double_as_longlong(cta), 0);
+            uint64_t* box = sh.box[turn & 1];
+            turn++;
+            if (lane < size) st_cluster(box + mine, lane, (uint64_t)__double_as_longlong(s));
+            cluster_sync();
             double t = 0.0;
-            for (int r = 0; r < size; r++) t += __longlong_as_double((long long)sh.box[buf][r][0]);
+            for (int i = lane; i < parts; i += 32) t += __longlong_as_double((long long)box[i]);
+            #pragma unroll
+            for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
+            sums = box;
             return t;
         };
-        for (int i = at + 1; i < N && kept < 0 && !none; i++) {
-            if (sh.par[i] != at) continue;
-            const int x = sh.tok[i];
+        for (; children && kept < 0 && !none; children &= children - 1) {
+            const int i = __ffsll((long long)children) - 1, x = sh.tok[i];
             if (x < 0 || x >= V) continue;
             if (greedy) {
                 if (x == mi) kept = i;
                 continue;
             }
-            const double p = exp(((double)sh.lx[i] - (double)M) * it64) / Z;
-            const double q = sh.qx[i], rest = qrow ? fmax(p - S * q, 0.0) : is_gone(x) ? 0.0 : p;
+            const double e = power(sh.lx[i]), q = sh.qx[i];
+            const double rest = qrow ? fmax(fma(-S, q, e), 0.0) : is_gone(x) ? 0.0 : e;
             if ((double)sh.u[i] * left * q < rest) {
                 kept = i;
             } else if (qrow) {
-                if (!summed) Z = sum_pass();   // p to 64 bits from here on
+                if (!summed) left = Z = sum_pass();   // to 64 bits from here on
                 S += left;
                 left = sum_pass();
-                total = left;
                 summed = true;
             } else if (!is_gone(x)) {
                 left -= rest;
@@ -270,7 +476,14 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Params P) {
             at = kept;
             if (rank == 0 && tid == 0) path[count] = kept;
             count++;
-            __syncthreads();   // lx, qx are rewritten
+            if (HELD && P.buffers == 2 && kept == other) {
+                held ^= 1;
+            } else if (HELD && (P.buffers == 2 || kept != inside)) {
+                landed(held);
+                fetch(kept, held, lo, hi, true);
+                inside = kept;
+            }
+            other = -1;
             continue;
         }
         // ---- no child is kept: the token after the path ----
@@ -278,82 +491,126 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Params P) {
             if (rank == 0 && tid == 0) P.next[seq] = none ? -1 : mi;
             break;
         }
-        if (!summed) total = sum_pass();
+        double total = summed ? left : sum_pass();
         if (!(total > 0.0)) {   // nothing is left: p itself
             S = 0.0;
             n_gone = 0;
             total = sum_pass();
         }
-        // the part that the running sum crosses the target in, or else the last with any weight
-        double target = (double)sh.u[0] * total;
-        int owner = -1, last = 0;
-        double before = 0.0, mine_before = 0.0;
-        for (int r = 0; r < size; r++) {
-            const double s = __longlong_as_double((long long)sh.box[buf][r][0]);
-            if (s > 0.0) last = r;
-            if (owner < 0 && before + s > target) { owner = r; mine_before = before; }
-            before += s;
+        // the part in which the running sum crosses the target, or else the last one with any weight
+        const double target = (double)sh.u[0] * total;
+        double run;              // the sum before the owner's part
+        int owner;
+        bool over;               // nothing crosses: the last token with any weight
+        {
+            double part_sum[kMaxParts / 32], mine_sum = 0.0;
+            const int per = (parts + 31) / 32;
+            int last = -1;
+            #pragma unroll
+            for (int k = 0; k < kMaxParts / 32; k++) {
+                const int p = lane * per + k;
+                part_sum[k] = k < per && p < parts ? __longlong_as_double((long long)sums[p]) : 0.0;
+                mine_sum += part_sum[k];
+                if (part_sum[k] > 0.0) last = p;
+            }
+            double inc = mine_sum;
+            #pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double y = __shfl_up_sync(~0u, inc, o);
+                if (lane >= o) inc += y;
+            }
+            double before = inc - mine_sum;
+            int first = INT_MAX;
+            double first_run = 0.0;
+            #pragma unroll
+            for (int k = 0; k < kMaxParts / 32; k++) {
+                if (first == INT_MAX && part_sum[k] > 0.0 && before + part_sum[k] > target) { first = lane * per + k; first_run = before; }
+                before += part_sum[k];
+            }
+            owner = __reduce_min_sync(~0u, first);
+            last = __reduce_max_sync(~0u, last);
+            over = owner == INT_MAX;
+            if (over) owner = last;
+            run = __shfl_sync(~0u, first_run, min(owner / per, 31));
         }
-        const bool over = owner < 0;
-        if (over) owner = last;
-        if (rank == owner) {
-            int w = -1;
-            last = 0;
-            double run = over ? -INFINITY : mine_before;   // over: nothing crosses, the last weight is taken
-            for (int k = 0; k < kWarps; k++) {
-                if (sh.wsum[k] > 0.0) last = k;
-                if (w < 0 && run + sh.wsum[k] > target) w = k;
-                else if (w < 0) run += sh.wsum[k];
-            }
-            if (w < 0) { w = last; run = -INFINITY; }
-            if (warp == w) {
-                int found = -1, last_i = -1;
-                for (int i0 = lo; i0 < hi && found < 0; i0 += 128) {
-                    float x[4], q[4] = {0.f, 0.f, 0.f, 0.f};
-                    double e[4];
-                    load4<T>(row, i0 + 4 * lane, hi, vec, -INFINITY, x);
-                    if (S > 0.0) load4<QWEN_FP32>(qrow, i0 + 4 * lane, hi, vec, 0.f, q);
-                    double s = 0.0;
+        if (owner / kWarps == rank) {
+            // the CTA's warps share the owner's part: run k of each round of kWarps runs
+            const int o0 = (int)((long long)runs * owner / parts) * kRun, o1 = min((int)((long long)runs * (owner + 1) / parts) * kRun, V);
+            const uint8_t* opart = parts_mem + (size_t)(held * kWarps + owner % kWarps) * P.part_bytes;
+            int best = -1;             // the last token with any weight
+            bool done = false;
+            for (int b = o0; b < o1 && !done; b += kWarps * kRun) {
+                const int i = b + warp * kRun + 4 * lane;
+                float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, q[4] = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (HELD) {
                     #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int i = i0 + 4 * lane + j;
-                        e[j] = i < hi && !is_gone(i) ? weight(x[j], q[j]) : 0.0;
-                        if (e[j] > 0.0) last_i = i;
-                        s += e[j];
-                    }
-                    double inc = s;
-                    #pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const double y = __shfl_up_sync(~0u, inc, o);
-                        if (lane >= o) inc += y;
-                    }
-                    const uint32_t cross = __ballot_sync(~0u, run + inc > target);
-                    if (cross) {
-                        const int l = __ffs(cross) - 1;
-                        int f = -1;
-                        if (lane == l) {
-                            double a = run + (inc - s);
-                            #pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                a += e[j];
-                                if (f < 0 && e[j] > 0.0 && a > target) f = i0 + 4 * lane + j;
-                            }
-                            if (f < 0) f = last_i;   // the rounding of inc - s
+                    for (int j = 0; j < 4; j++)
+                        if (i + j < o1) {
+                            if constexpr (T == QWEN_FP32) x[j] = reinterpret_cast<const float*>(opart)[i + j - o0];
+                            else if constexpr (T == QWEN_BF16) x[j] = bf2f(reinterpret_cast<const uint16_t*>(opart)[i + j - o0]);
+                            else x[j] = __half2float(reinterpret_cast<const __half*>(opart)[i + j - o0]);
                         }
-                        found = __shfl_sync(~0u, f, l);
-                        if (found < 0) break;
-                    }
-                    run += __shfl_sync(~0u, inc, 31);
+                } else {
+                    load4<T>(row, i, o1, vec, -INFINITY, x);
                 }
+                if (S > 0.0) load4<QWEN_FP32>(qrow, i, o1, vec, 0.f, q);
+                double e[4], s = 0.0;
+                bool in[4];
+                int mine_last = -1;
+                weights(x, q, e, in);
                 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) last_i = max(last_i, __shfl_xor_sync(~0u, last_i, o));
-                if (lane == 0) P.next[seq] = found >= 0 ? found : last_i;
+                for (int j = 0; j < 4; j++) {
+                    if (!in[j] || i + j >= o1 || is_gone(i + j)) e[j] = 0.0;
+                    if (e[j] > 0.0) mine_last = i + j;
+                    s += e[j];
+                }
+                double inc = s;
+                #pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double y = __shfl_up_sync(~0u, inc, o);
+                    if (lane >= o) inc += y;
+                }
+                const int warp_last = __reduce_max_sync(~0u, mine_last);
+                if (lane == 31) { sh.run_sum[warp] = inc; sh.run_last[warp] = warp_last; }
+                __syncthreads();
+                // the sums before this warp's run and behind the round (the same additions in every warp)
+                double upto = lane < kWarps ? sh.run_sum[lane] : 0.0;
+                best = max(best, __reduce_max_sync(~0u, lane < kWarps ? sh.run_last[lane] : -1));
+                #pragma unroll
+                for (int o = 1; o < kWarps; o <<= 1) {
+                    const double y = __shfl_up_sync(~0u, upto, o);
+                    if (lane >= o) upto += y;
+                }
+                const double behind = __shfl_sync(~0u, upto, (warp + 31) & 31), round = __shfl_sync(~0u, upto, kWarps - 1);
+                const double before = run + (warp ? behind : 0.0);
+                if (!over) {
+                    const uint32_t cross = __ballot_sync(~0u, s > 0.0 && before + inc > target);
+                    if (cross && lane == __ffs(cross) - 1) {
+                        double a = before + (inc - s);
+                        int f = -1;
+                        #pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            a += e[j];
+                            if (f < 0 && e[j] > 0.0 && a > target) f = i + j;
+                        }
+                        atomicMin(&sh.found, f >= 0 ? f : mine_last);   // (the rounding of inc - s)
+                    }
+                }
+                run += round;
+                __syncthreads();
+                done = sh.found != INT_MAX;   // (the next round's first barrier comes before another write)
             }
+            if (tid == 0) P.next[seq] = sh.found != INT_MAX ? sh.found : best;
         }
         break;
     }
     if (rank == 0 && tid == 0) P.n_path[seq] = count;
+    if constexpr (HELD) {
+        landed(0);
+        landed(1);
+    }
     cluster_sync();   // no CTA leaves while another may still write to its box
+    if (tid == 0 && sh.late) P.next[seq] = -1;
 }
 
 }  // namespace tv

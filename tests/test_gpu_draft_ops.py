@@ -571,6 +571,14 @@ def test_verify_walks(qb, temp, with_draft, b, t, vocab, dtype, pad):
         assert got[1].max() > 1      # the cases do keep drafted tokens
 
 
+@pytest.mark.parametrize("b,dtype,pad", [(150, "fp32", 0), (75, "fp32", 1), (37, "fp32", 0), (20, "bf16", 0)])
+def test_verify_rows_beyond_shared_memory(qb, b, dtype, pad):
+    """So many sequences that a warp's part of a row no longer fits beside another's, or at all."""
+    case = _drafted(b, b, 3, 151936, _types(qb)[dtype][1], b % 2 == 0, 0.7)
+    got = _check_verify(qb, *case, 0.7, pad)
+    assert got[1].max() > 1
+
+
 @pytest.mark.parametrize("with_draft", [False, True])
 def test_verify_edges_of_the_uniforms(qb, with_draft):
     """Uniforms of 0 and of the largest number below 1; tokens with no probability; masked vocabularies; repeated siblings."""
