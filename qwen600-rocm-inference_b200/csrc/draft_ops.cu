@@ -14,6 +14,7 @@
 #include "../../include/qwen_b200.h"
 #include "kv_rows.cuh"
 #include "tree_attention.cuh"
+#include "tree_attention_tc.cuh"
 #include "tree_verify.cuh"
 
 int qwen_internal_fail(int code, const std::string& msg);
@@ -161,8 +162,11 @@ int check_rows(const qwen_kv_cache_t* c, const void* k, const void* v, int dtype
 }
 
 // ---- tree attention ----------------------------------------------------------------
-// The kernel's variant: blocks of 16 rows where the item has no more, else of 32.
-int attention_rows(int m) { return m <= 16 ? 16 : 32; }
+// The kernel's variant, by the query rows of a K/V head (nodes times query heads):
+// up to 16 and up to 32 the warp-level kernel, in one block of rows; above, where it
+// would read the cache once for every 32 rows, the tensor-memory kernel with one
+// block of 128 rows or, above 128, two.
+int attention_rows(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : m <= 128 ? 128 : 256; }
 
 struct Plan {
     int rows, row_blocks, shares;
@@ -180,13 +184,31 @@ int attention_plan(const qwen_kv_cache_t* c, int n_nodes, int n_heads, int dev, 
     TRY(sm_count(dev, &nsm));
     p->rows = attention_rows((int)m);
     p->row_blocks = (int)((m + p->rows - 1) / p->rows);
-    // two CTAs an SM, but no more than there can be tiles (64 keys at least)
-    const double most = (double)c->n_seqs * c->n_kv_heads * p->row_blocks * ((c->capacity + 63) / 64);
-    p->shares = (int)std::min((double)(2 * nsm), most);
+    // two CTAs an SM (the tensor-memory kernel: one), but no more than there can be tiles (64 keys at least, 128)
+    const int keys = p->rows <= 32 ? 64 : 128;
+    const double most = (double)c->n_seqs * c->n_kv_heads * p->row_blocks * ((c->capacity + keys - 1) / keys);
+    p->shares = (int)std::min((double)(p->rows <= 32 ? 2 * nsm : nsm), most);
     p->bytes = (size_t)2 * p->shares * p->rows * (c->head_dim + 2) * sizeof(float);
     return QWEN_OK;
 }
 
+// The kernel that joins the shares' partial results, launched so that it may start its set-up early.
+template <int QT, int KT, int D, int ROWS>
+int join_launch(const qb::ta::Params& P, const Plan& plan, cudaStream_t st) {
+    if (plan.shares == 1) return QWEN_OK;
+    constexpr int kJoinRows = qb::ta::kJoinThreads / (D / 4);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(plan.shares, ROWS / kJoinRows);
+    cfg.blockDim = dim3(qb::ta::kJoinThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    CU(cudaLaunchKernelEx(&cfg, qb::ta::combine_kernel<QT, KT, D, ROWS>, P, plan.row_blocks));
+    return QWEN_OK;
+}
 template <int QT, int STORE, int D, int MT>
 int attention_launch(const qb::ta::Params& P, const Plan& plan, int dev, cudaStream_t st) {
     using L = qb::ta::Layout<STORE, D, MT>;
@@ -195,24 +217,30 @@ int attention_launch(const qb::ta::Params& P, const Plan& plan, int dev, cudaStr
     TRY(smem_limit(kernel, done, dev, L::kSmem));
     kernel<<<plan.shares, qb::ta::kThreads, L::kSmem, st>>>(P, plan.row_blocks);
     CU(cudaGetLastError());
-    if (plan.shares == 1) return QWEN_OK;
-    constexpr int kJoinRows = qb::ta::kJoinThreads / (D / 4);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(plan.shares, L::kRows / kJoinRows);
-    cfg.blockDim = dim3(qb::ta::kJoinThreads);
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    CU(cudaLaunchKernelEx(&cfg, qb::ta::combine_kernel<QT, L::KT, D, L::kRows>, P, plan.row_blocks));
-    return QWEN_OK;
+    return join_launch<QT, L::KT, D, L::kRows>(P, plan, st);
+}
+template <int QT, int STORE, int D, bool PAIR>
+int attention_tc_launch(const qb::ta::Params& P, const Plan& plan, int dev, cudaStream_t st) {
+    using L = qb::ta::TcLayout<STORE, D, PAIR>;
+    static std::atomic<uint64_t> done{0};
+    auto kernel = qb::ta::attention_tc_kernel<QT, STORE, D, PAIR>;
+    TRY(smem_limit(kernel, done, dev, L::kSmem));
+    kernel<<<plan.shares, qb::ta::kTcThreads, L::kSmem, st>>>(P, plan.row_blocks);
+    CU(cudaGetLastError());
+    return join_launch<QT, qb::ta::kTcKT, D, L::kRows>(P, plan, st);
+}
+template <int QT, int STORE, int D>
+int attention_by_rows(const qb::ta::Params& P, const Plan& plan, int dev, cudaStream_t st) {
+    switch (plan.rows) {
+        case 16: return attention_launch<QT, STORE, D, 1>(P, plan, dev, st);
+        case 32: return attention_launch<QT, STORE, D, 2>(P, plan, dev, st);
+        case 128: return attention_tc_launch<QT, STORE, D, false>(P, plan, dev, st);
+        default: return attention_tc_launch<QT, STORE, D, true>(P, plan, dev, st);
+    }
 }
 template <int QT, int STORE>
 int attention_by_shape(int dim, const qb::ta::Params& P, const Plan& plan, int dev, cudaStream_t st) {
-    if (dim == 64) return plan.rows == 16 ? attention_launch<QT, STORE, 64, 1>(P, plan, dev, st) : attention_launch<QT, STORE, 64, 2>(P, plan, dev, st);
-    return plan.rows == 16 ? attention_launch<QT, STORE, 128, 1>(P, plan, dev, st) : attention_launch<QT, STORE, 128, 2>(P, plan, dev, st);
+    return dim == 64 ? attention_by_rows<QT, STORE, 64>(P, plan, dev, st) : attention_by_rows<QT, STORE, 128>(P, plan, dev, st);
 }
 
 // ---- verification --------------------------------------------------------------------

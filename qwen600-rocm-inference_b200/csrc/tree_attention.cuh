@@ -636,15 +636,32 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(const Params P, i
     const size_t first_slot = 2 * (size_t)i + (from < s ? 1 : 0);
     float mm = -INFINITY, ll = 0.f;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = i; k <= last; k++) {
-        if (k > i && share(tiles, k, G) == share(tiles, k + 1, G)) continue;
-        const float* slot = P.work + (k == i ? first_slot : 2 * (size_t)k) * kSlot;
-        const float2 ml = *reinterpret_cast<const float2*>(slot + ROWS * D + 2 * r);
-        const float4 b = *reinterpret_cast<const float4*>(slot + r * D + d);
-        const float mn = fmaxf(mm, ml.x);
-        const float f0 = mn == -INFINITY ? 1.0f : exp2_approx(mm - mn), f1 = mn == -INFINITY ? 1.0f : exp2_approx(ml.x - mn);
-        ll = ll * f0 + ml.y * f1;
-        a.x = a.x * f0 + b.x * f1; a.y = a.y * f0 + b.y * f1; a.z = a.z * f0 + b.z * f1; a.w = a.w * f0 + b.w * f1;
+    constexpr int kAhead = 8;   // partial results loaded at once
+    for (int k0 = i; k0 <= last; k0 += kAhead) {
+        float2 ml[kAhead];
+        float4 b[kAhead];
+        #pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            const int k = k0 + j;
+            ml[j] = make_float2(-INFINITY, 0.f);
+            b[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k > last || (k > i && share(tiles, k, G) == share(tiles, k + 1, G))) continue;
+            const float* slot = P.work + (k == i ? first_slot : 2 * (size_t)k) * kSlot;
+            ml[j] = *reinterpret_cast<const float2*>(slot + ROWS * D + 2 * r);
+            b[j] = *reinterpret_cast<const float4*>(slot + r * D + d);
+        }
+        float mn = mm;
+        #pragma unroll
+        for (int j = 0; j < kAhead; j++) mn = fmaxf(mn, ml[j].x);
+        const float f0 = mn == -INFINITY ? 1.0f : exp2_approx(mm - mn);
+        ll *= f0;
+        a.x *= f0; a.y *= f0; a.z *= f0; a.w *= f0;
+        #pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            const float f1 = mn == -INFINITY ? 1.0f : exp2_approx(ml[j].x - mn);
+            ll += ml[j].y * f1;
+            a.x += b[j].x * f1; a.y += b[j].y * f1; a.z += b[j].z * f1; a.w += b[j].w * f1;
+        }
         mm = mn;
     }
     const float inv = ll == 0.f ? 0.f : 1.0f / ll;

@@ -1,0 +1,617 @@
+// tree_attention_tc.cuh — tree attention of many query rows a K/V head on the
+// sm_100a tensor cores (tcgen05.mma with accumulators in tensor memory); the
+// mathematics and the division of the work are tree_attention.cuh's.  No
+// reference counterpart.
+//
+// With 33 and more rows (nodes times query heads a K/V head) the warp-level
+// products no longer fit under the cache's bytes, and blocks of 32 rows would
+// read them several times.  Here an item has 128 rows (one block) or 256 (two),
+// tiles have 128 keys, and two streams of 128 softmax threads (a thread a row)
+// work in turn, so one stream's exponentials run while the tensor core
+// forms the other's products: with one block of rows the streams take
+// alternate key tiles (joined at the end of an item in tensor memory), with two
+// blocks each stream takes a block and both use every tile.  A tile costs a
+// stream 128 exponentials a row, 1024 cycles of an SM at 16 a cycle; its two
+// products 256 cycles each; its bytes (bf16, 128 dims) 2,800 cycles of an SM's
+// share of the memory bandwidth.  So one block is bound by memory, two by the
+// exponentials.
+//
+// Warps: 0-3 and 4-7 the streams (warp w reads the tensor-memory lanes 32 (w % 4) ..,
+// its rows), 8-11 producers, 12 issues the products.  S = Q K^T and P (16 bits,
+// written over S) and O are in tensor memory; Q, K and V in shared memory, rows of
+// 64 dims in the 128-byte swizzle: K is a K-major operand, V an MN-major one (its
+// rows are keys, so the product P V needs no transposed copy).  K and V
+// parts of tiles go through one ring in the order in which they are used.  16-bit
+// rows arrive by cp.async; 8-bit rows arrive in a thread-private staging ring, become
+// fp16 (exact) and are stored swizzled by the thread that loaded them.  Every
+// wait is bounded; where one runs out, the item's rows become NaN.
+#pragma once
+#include "gemm_tc.cuh"
+#include "tree_attention.cuh"
+
+namespace qb {
+namespace ta {
+
+constexpr int kTcThreads = 416, kTcKT = 128, kTcProducers = 128;
+constexpr int kScaleRing = 8;
+
+template <int STORE, int D, bool PAIR>
+struct TcLayout {
+    static constexpr bool k8 = STORE == QWEN_E4M3 || STORE == QWEN_INT8;
+    static constexpr int kRow = D * (k8 ? 1 : 2);          // bytes of a cache row
+    static constexpr int kHalf = kTcKT * D * 2;            // K or V of a tile, or 128 query rows: 16 bits
+    static constexpr int kBlocks = PAIR ? 2 : 1;           // blocks of 128 query rows
+    static constexpr int kRows = 128 * kBlocks;
+    static constexpr int kRing = D == 64 ? (k8 ? 6 : 8) : k8 ? (PAIR ? 3 : 4) : (PAIR ? 4 : 5);   // K / V parts in flight
+    static constexpr int kRawHalf = k8 ? kTcKT * D : 0;
+    static constexpr int kRawRing = k8 ? (D == 64 ? 4 : 3) : 0;
+    static constexpr int kQ = 0;
+    static constexpr int kKV = kQ + kBlocks * kHalf;
+    static constexpr int kRaw = kKV + kRing * kHalf;
+    static constexpr int kScales = kRaw + kRawRing * kRawHalf;                        // [ring][ks 128, vs 128]
+    static constexpr int kMl = kScales + (k8 ? kScaleRing * 2 * kTcKT * 4 : 0);       // [stream][row] (base, l)
+    static constexpr int kAnc = kMl + 2 * 128 * 8;
+    static constexpr int kUp = kAnc + kMaxNodes * 8;
+    static constexpr int kVe = kUp + kMaxNodes;                                       // [ring][producer warp] largest exponent of vs
+    static constexpr int kBar = kVe + kScaleRing * 4 * 4;
+    static constexpr int kBars = 2 * kRing + kScaleRing + 8;
+    static constexpr int kMisc = kBar + kBars * 8;                                    // tensor-memory address, fault, odd[8]
+    static constexpr int kSmem = kMisc + 48 + 1024;
+    static constexpr int kSlot = kRows * (D + 2);
+    static_assert(kSmem <= 227 * 1024, "one CTA's shared memory");
+    static_assert(2 * kSmem > 228 * 1024, "one CTA an SM: the kernel allocates all of tensor memory");
+};
+
+// Instruction descriptor, kind::f16: D fp32 (bits 4-5), A and B bf16 (1) or fp16 (0) at bits 7 and 10, B MN-major at
+// bit 16, N >> 3 at bit 17, M >> 4 at bit 24.
+template <bool BF>
+__host__ __device__ constexpr uint32_t tc_idesc(int N, bool mn_major_b) {
+    return (1u << 4) | (BF ? (1u << 7) | (1u << 10) : 0u) | (mn_major_b ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | (8u << 24);
+}
+// MN-major operand in the 128-byte swizzle: rows (keys) of 64 dims, 8 rows 1024 bytes, the next 64 dims `block` bytes on.
+__device__ __forceinline__ uint64_t mn_major_sw128_desc(uint32_t saddr, uint32_t block) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(block >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | ((uint64_t)1u << 46) |
+           ((uint64_t)2u << 61);
+}
+// D (tensor memory) += A (tensor memory, 128 rows x 16) . B
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+          "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tc_st32(uint32_t taddr, const float (&v)[32]) {
+    uint32_t a[16], b[16];
+    #pragma unroll
+    for (int i = 0; i < 16; i++) { a[i] = __float_as_uint(v[i]); b[i] = __float_as_uint(v[16 + i]); }
+    tc_st16(taddr, a);
+    tc_st16(taddr + 16, b);
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// A share of the line, item after item; every role walks it alike.
+struct Items {
+    long long at, to, before;
+    int seq, len, end, n, h, r_base, t0, t1, units, row_blocks;
+    // all lanes of a warp; false: nothing to do
+    __device__ __forceinline__ bool start(const Params& P, int blocks) {
+        row_blocks = blocks;
+        units = P.n_kv_heads * blocks;
+        const long long tiles = line_tiles<kTcKT>(P, units);
+        at = share(tiles, blockIdx.x, gridDim.x);
+        to = share(tiles, blockIdx.x + 1, gridDim.x);
+        if (at >= to) return false;
+        seq = line_find<kTcKT>(P, units, at, before);
+        return true;
+    }
+    template <int ROWS>
+    __device__ __forceinline__ void item(const Params& P) {
+        len = P.lens[seq];
+        end = seq_end(P, len);
+        n = seq_tiles<kTcKT>(P, len);
+        const int unit = (int)((at - before) / n);
+        t0 = (int)((at - before) - (long long)unit * n);
+        t1 = (int)min((long long)n, t0 + (to - at));
+        h = unit / row_blocks;
+        r_base = (unit - h * row_blocks) * ROWS;
+    }
+    __device__ __forceinline__ bool next() {
+        at += t1 - t0;
+        if (at >= to) return false;
+        if (at - before == (long long)n * units) { before = at; seq++; }
+        return true;
+    }
+};
+
+// grid G (shares; one CTA an SM), kTcThreads threads, TcLayout::kSmem bytes.
+template <int QT, int STORE, int D, bool PAIR>
+__global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Params P, int row_blocks) {
+    using L = TcLayout<STORE, D, PAIR>;
+    using namespace qb::tc;
+    constexpr bool BF = QT == QWEN_BF16 && !L::k8;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBar);   // [kRing] a K or V part is in place (128 producers)
+    uint64_t* empty = full + L::kRing;                              // [kRing] its products are done
+    uint64_t* scaled = empty + L::kRing;                            // [kScaleRing] a tile's scales are in place (128 producers)
+    uint64_t* sfull = scaled + kScaleRing;                          // [2] S of the stream
+    uint64_t* pfull = sfull + 2;                                    // [2] P of the stream, O rescaled (4 warps)
+    uint64_t* pvdone = sfull + 4;                                   // [2] P V of the stream
+    uint64_t* qfull = sfull + 6;                                    // the item's queries (8 warps)
+    uint64_t* drained = sfull + 7;                                  // all products are done, at the end
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
+    volatile int* fault = reinterpret_cast<int*>(smem + L::kMisc + 4);
+    volatile int* odd = fault + 1;                                  // [8] an item's V rows of the tree hold an infinity or NaN
+    uint64_t* anc = reinterpret_cast<uint64_t*>(smem + L::kAnc);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        for (int i = 0; i < L::kRing; i++) { mbar_init(&full[i], kTcProducers); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < kScaleRing; i++) mbar_init(&scaled[i], kTcProducers);
+        for (int i = 0; i < 2; i++) { mbar_init(&sfull[i], 1); mbar_init(&pfull[i], 4); mbar_init(&pvdone[i], 1); }
+        mbar_init(qfull, 8);
+        mbar_init(drained, 1);
+        fence_barrier_init();
+        *fault = 0;
+        for (int i = 0; i < 8; i++) odd[i] = 0;
+    }
+    if (warp == 12) tmem_alloc(tmem_slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    constexpr uint32_t kTmO = 256;   // S / P of stream s: columns 128 s .., O: 256 + 128 s ..
+    pdl_wait();
+    pdl_launch_dependents();         // after the wait: what the joining kernel reads early (lens) is then complete
+
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (ok && !mbar_wait(bar, parity, kWaitNs)) { ok = false; *fault = 1; }
+        return ok;
+    };
+    Items it;
+    const bool busy = it.start(P, row_blocks);   // the same for the whole CTA
+    if (busy && warp >= 8 && warp < 12) {
+        // ---------------- producers ----------------
+        const int pt = tid - 256;
+        uint32_t part = 0;           // K / V parts so far: slot part % kRing
+        uint32_t unsaid = 0;         // 16-bit rows: parts whose copies are committed but not yet announced
+        uint32_t item = 0, tile = 0; // tile: of the CTA so far
+        auto say = [&](uint32_t p) { fence_async_smem(); mbar_arrive(&full[p % L::kRing]); };
+        auto free_slot = [&](uint32_t p) {   // the slot of part p: all products with the part before it in it are done
+            if (p < (uint32_t)L::kRing) return true;
+            return wait(&empty[p % L::kRing], (p / L::kRing - 1) & 1u);
+        };
+        do {
+            it.item<L::kRows>(P);
+            const size_t head = (size_t)it.seq * P.cache.seq_stride + (size_t)it.h * P.cache.head_stride;
+            const uint8_t* base[2] = {P.cache.k + head * (L::k8 ? 1 : 2), P.cache.v + head * (L::k8 ? 1 : 2)};
+            if constexpr (!L::k8) {
+                constexpr int kChunks = D / 8, kPer = kTcKT * kChunks / kTcProducers, kStep = kTcProducers / kChunks;
+                const int c = pt % kChunks, r0 = pt / kChunks;
+                for (int t = it.t0; t < it.t1 && ok; t++) {
+                    const int k0 = t * kTcKT;
+                    #pragma unroll 1
+                    for (int kv = 0; kv < 2 && ok; kv++, part++) {
+                        if (part >= (uint32_t)L::kRing && unsaid && !mbar_try_wait(&empty[part % L::kRing], (part / L::kRing - 1) & 1u)) {
+                            cp_async_wait<0>();   // the ring is full: announce all that is coming before the wait for a slot
+                            for (; unsaid; unsaid--) say(part - unsaid);
+                        }
+                        if (!free_slot(part)) break;
+                        uint8_t* dst = smem + L::kKV + part % L::kRing * L::kHalf + (c >> 3) * (kTcKT * 128);
+                        #pragma unroll
+                        for (int i = 0; i < kPer; i++) {
+                            const int r = r0 + i * kStep;
+                            const bool live = k0 + r < it.end;
+                            const size_t off = live ? (size_t)(k0 + r) * L::kRow + c * 16 : 0;
+                            cp_async16(smem_addr(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)), base[kv] + off, live);
+                        }
+                        cp_async_commit();
+                        unsaid++;
+                        const bool tail = k0 + kTcKT > it.len;
+                        if (tail && kv == 1) {
+                            // rows of the tree: infinities and NaN would reach nodes that do not see them (0 * NaN): they go to the
+                            // softmax threads by another way (odd), and are zero in the product.  Every thread looks at its own copies.
+                            cp_async_wait<0>();
+                            constexpr uint32_t kExp = QT == QWEN_BF16 ? 0x7f80u : 0x7c00u;
+                            bool any = false;
+                            #pragma unroll 1
+                            for (int i = 0; i < kPer; i++) {
+                                const int r = r0 + i * kStep;
+                                if (k0 + r < it.len) continue;
+                                uint4* p = reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+                                uint4 w = *p;
+                                uint32_t x[4] = {w.x, w.y, w.z, w.w};
+                                bool hit = false;
+                                #pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    if ((x[e] & kExp) == kExp) { x[e] &= 0xffff0000u; hit = true; }
+                                    if (((x[e] >> 16) & kExp) == kExp) { x[e] &= 0xffffu; hit = true; }
+                                }
+                                if (hit) { *p = make_uint4(x[0], x[1], x[2], x[3]); any = true; }
+                            }
+                            if (any) odd[item & 7] = 1;
+                        }
+                        if (unsaid > 2) {
+                            cp_async_wait<2>();
+                            say(part + 1 - unsaid);
+                            unsaid--;
+                        }
+                    }
+                }
+            } else {
+                // raw part x (K and V in turn) of this item sits in staging slot x % kRawRing, copied by the thread that converts it
+                constexpr int kChunks = D / 16, kPer = kTcKT * kChunks / kTcProducers, kStep = kTcProducers / kChunks;
+                const int c = pt % kChunks, r0 = pt / kChunks, parts = 2 * (it.t1 - it.t0);
+                auto copy = [&](int x) {
+                    if (x < parts) {
+                        const int k0 = (it.t0 + (x >> 1)) * kTcKT;
+                        uint8_t* dst = smem + L::kRaw + x % L::kRawRing * L::kRawHalf + pt * 16;
+                        #pragma unroll
+                        for (int i = 0; i < kPer; i++) {
+                            const int r = r0 + i * kStep;
+                            const bool live = k0 + r < it.end;
+                            cp_async16(smem_addr(dst + i * kTcProducers * 16), base[x & 1] + (live ? (size_t)(k0 + r) * L::kRow + c * 16 : 0), live);
+                        }
+                        if (!(x & 1)) {   // the tile's scales come with K
+                            const bool live = k0 + pt < it.end;
+                            float* sc = reinterpret_cast<float*>(smem + L::kScales) + (tile + (x >> 1)) % kScaleRing * 2 * kTcKT + pt;
+                            cp_async4(smem_addr(sc), P.cache.ks + head / D + (live ? k0 + pt : 0), live);
+                            cp_async4(smem_addr(sc + kTcKT), P.cache.vs + head / D + (live ? k0 + pt : 0), live);
+                        }
+                    }
+                    cp_async_commit();
+                };
+                #pragma unroll
+                for (int x = 0; x < L::kRawRing - 1; x++) copy(x);
+                for (int x = 0; x < parts && ok; x++, part++) {
+                    copy(x + L::kRawRing - 1);
+                    cp_async_wait<L::kRawRing - 1>();
+                    if (!free_slot(part)) break;
+                    const int k0 = (it.t0 + (x >> 1)) * kTcKT;
+                    const bool tail = STORE == QWEN_E4M3 && (x & 1) && k0 + kTcKT > it.len;
+                    const uint8_t* src = smem + L::kRaw + x % L::kRawRing * L::kRawHalf + pt * 16;
+                    uint8_t* dst = smem + L::kKV + part % L::kRing * L::kHalf + (c >> 2) * (kTcKT * 128);
+                    #pragma unroll 4
+                    for (int i = 0; i < kPer; i++) {
+                        const int r = r0 + i * kStep;
+                        const uint4 w = *reinterpret_cast<const uint4*>(src + i * kTcProducers * 16);
+                        uint32_t q[4] = {w.x, w.y, w.z, w.w};
+                        if (tail && k0 + r >= it.len) {
+                            bool hit = false;
+                            #pragma unroll
+                            for (int e = 0; e < 16; e++)
+                                if (((q[e >> 2] >> (8 * (e & 3))) & 0x7fu) == 0x7fu) { q[e >> 2] &= ~(0xffu << (8 * (e & 3))); hit = true; }
+                            if (hit) odd[item & 7] = 1;
+                        }
+                        uint32_t o[8];
+                        #pragma unroll
+                        for (int e = 0; e < 4; e++) { o[2 * e] = codes_f16x2<STORE, 0, 1>(q[e]); o[2 * e + 1] = codes_f16x2<STORE, 2, 3>(q[e]); }
+                        const int ch = (2 * c) & 7;
+                        *reinterpret_cast<uint4*>(dst + r * 128 + ((ch ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                        *reinterpret_cast<uint4*>(dst + r * 128 + (((ch + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+                    }
+                    say(part);
+                    if (!(x & 1)) {   // the largest exponent of the value scales, a warp's 32 keys
+                        const uint32_t ring = (tile + (x >> 1)) % kScaleRing;
+                        const float vs = reinterpret_cast<const float*>(smem + L::kScales)[ring * 2 * kTcKT + kTcKT + pt];
+                        uint32_t e = __float_as_uint(vs) >> 23 & 0xffu;
+                        e = __reduce_max_sync(~0u, e == 255u ? 0u : min(e + 1, 253u));
+                        if (lane == 0) reinterpret_cast<volatile uint32_t*>(smem + L::kVe)[ring * 4 + (warp - 8)] = e;
+                        __syncwarp();
+                        mbar_arrive(&scaled[ring]);
+                    }
+                }
+                cp_async_wait<0>();
+                tile += it.t1 - it.t0;
+            }
+            item++;
+        } while (ok && it.next());
+        cp_async_wait<0>();
+        if (ok) for (; unsaid; unsaid--) say(part - unsaid);
+    } else if (busy && warp == 12) {
+        // ---------------- products ----------------
+        constexpr uint32_t id_s = tc_idesc<BF>(kTcKT, false), id_o = tc_idesc<BF>(D, true);
+        uint32_t part = 0, item = 0, steps[2] = {0, 0};   // steps of a stream so far
+        if (lane == 0) {
+            do {
+                it.item<L::kRows>(P);
+                const int nt = it.t1 - it.t0, nv = PAIR ? 2 * nt : nt;   // virtual steps: stream v & 1
+                if (!wait(qfull, item & 1u)) break;
+                tc_fence_after();
+                for (int v = 0; v < nv + 2 && ok; v++) {
+                    const int s = v & 1;
+                    if (v >= 2) {              // O += P V of step v - 2
+                        const int u = v - 2, t = PAIR ? u >> 1 : u;
+                        const uint32_t p = part + 2 * t + 1;
+                        if (!wait(&pfull[s], (steps[s] - 1) & 1u) || !wait(&full[p % L::kRing], p / L::kRing & 1u)) break;
+                        tc_fence_after();
+                        const uint32_t vb = smem_addr(smem + L::kKV + p % L::kRing * L::kHalf);
+                        #pragma unroll
+                        for (int k = 0; k < kTcKT / 16; k++)
+                            tc_mma_ts(tmem + kTmO + 128 * s, tmem + 128 * s + 8 * k, mn_major_sw128_desc(vb + k * 2048, kTcKT * 128), id_o,
+                                      (u >= 2 || k) ? 1u : 0u);
+                        if (!PAIR || s) mma_commit(&empty[p % L::kRing]);
+                        mma_commit(&pvdone[s]);
+                    }
+                    if (v < nv) {              // S = Q K^T of step v, over the P that the product above has read
+                        const int t = PAIR ? v >> 1 : v;
+                        const uint32_t p = part + 2 * t;
+                        if (v >= 2 && !wait(&pvdone[s], (steps[s] - 1) & 1u)) break;
+                        if (!wait(&full[p % L::kRing], p / L::kRing & 1u)) break;
+                        tc_fence_after();
+                        const uint32_t kb = smem_addr(smem + L::kKV + p % L::kRing * L::kHalf);
+                        const uint32_t qb = smem_addr(smem + L::kQ + (PAIR ? s : 0) * L::kHalf);
+                        #pragma unroll
+                        for (int k = 0; k < D / 16; k++)
+                            mma_bf16(tmem + 128 * s, kmajor_sw128_desc(qb + (k >> 2) * (128 * 128) + (k & 3) * 32),
+                                     kmajor_sw128_desc(kb + (k >> 2) * (kTcKT * 128) + (k & 3) * 32), id_s, k ? 1u : 0u);
+                        if (!PAIR || s) mma_commit(&empty[p % L::kRing]);
+                        mma_commit(&sfull[s]);
+                        steps[s]++;
+                    }
+                }
+                part += 2 * nt;
+                item++;
+            } while (ok && it.next());
+            mma_commit(drained);
+            if (!mbar_wait(drained, 0, kWaitNs)) *fault = 1;
+        }
+        __syncwarp();
+    } else if (busy && warp < 8) {
+        // ---------------- softmax ----------------
+        const int s = warp >> 2, rl = 32 * (warp & 3) + lane;              // stream, row of its block
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t ts = tmem + lanes + 128 * s, to = tmem + lanes + kTmO;
+        float2* ml = reinterpret_cast<float2*>(smem + L::kMl);
+        const int M = P.n_nodes * P.group;
+        const bool flip = P.scale_log2 < 0.f;                              // a negative scale: its sign goes to the queries
+        uint32_t item = 0, steps = 0, tile = 0;
+        bool first_item = true;
+        do {
+            it.item<L::kRows>(P);
+            const int nt = it.t1 - it.t0, mine = PAIR ? nt : (nt + 1 - s) >> 1;   // steps of this stream
+            named_bar(1, 256);                                             // the item before is written, its masks and queries are free
+            if (tid == 0) odd[(item - 1) & 7] = 0;
+            if (warp == 0) tree_masks(P, it.seq, it.len, anc, reinterpret_cast<int8_t*>(smem + L::kUp));
+            const int row = it.r_base + (PAIR ? 128 * s : 0) + rl;         // one block: both streams' threads rl share a row
+            float c = fabsf(P.scale_log2);                                 // (kept above 0: -inf * 0 would be NaN)
+            {
+                const int node = row / P.group, hq = it.h * P.group + row % P.group;
+                const uint4* src = reinterpret_cast<const uint4*>(P.q + (((size_t)it.seq * P.n_nodes + node) * (size_t)P.ldq + (size_t)hq * D) * 2);
+                const bool live = row < M;
+                float down = 1.0f;
+                if constexpr (L::k8 && QT == QWEN_BF16) {                  // into fp16's range, a power of two a row
+                    uint32_t m = 0;
+                    if (live) {
+                        #pragma unroll 4
+                        for (int i = 0; i < D / 8; i++) {
+                            const uint4 w = __ldg(src + i);
+                            const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+                            #pragma unroll
+                            for (int e = 0; e < 4; e++) m = max(m, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
+                        }
+                    }
+                    const int e = min(max((int)(m >> 7), 1), 253);
+                    down = __uint_as_float((uint32_t)(254 - e) << 23);
+                    c *= __uint_as_float((uint32_t)e << 23);
+                }
+                constexpr int kAll = D / 8;
+                const int i0 = PAIR ? 0 : s * (kAll / 2), i1 = PAIR ? kAll : i0 + kAll / 2;
+                uint8_t* dst = smem + L::kQ + (PAIR ? s : 0) * L::kHalf + rl * 128;
+                #pragma unroll 4
+                for (int i = i0; i < i1; i++) {
+                    uint4 w = live ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+                    if constexpr (L::k8 && QT == QWEN_BF16) {
+                        w.x = kv::half2_bits(bf_lo(w.x) * down, bf_hi(w.x) * down);
+                        w.y = kv::half2_bits(bf_lo(w.y) * down, bf_hi(w.y) * down);
+                        w.z = kv::half2_bits(bf_lo(w.z) * down, bf_hi(w.z) * down);
+                        w.w = kv::half2_bits(bf_lo(w.w) * down, bf_hi(w.w) * down);
+                    }
+                    if (flip) { w.x ^= 0x80008000u; w.y ^= 0x80008000u; w.z ^= 0x80008000u; w.w ^= 0x80008000u; }
+                    *reinterpret_cast<uint4*>(dst + (i >> 3) * (128 * 128) + (((i & 7) ^ (rl & 7)) << 4)) = w;
+                }
+            }
+            c = fmaxf(c, 1e-37f);
+            fence_async_smem();
+            named_bar(1, 256);                                             // masks
+            if (lane == 0) mbar_arrive(qfull);
+            const uint64_t see = row < M ? anc[row / P.group] : 0;
+            float top = -INFINITY, base = -INFINITY, l = 0.f;              // running maximum; what exponents are taken from
+            int ve_run = 37;                                               // 8 bits: largest exponent of a value scale so far, 2^-90 at least
+            for (int i = 0; i < mine; i++, steps++) {
+                const int tl = PAIR ? i : 2 * i + s, k0 = (it.t0 + tl) * kTcKT;
+                const float *ks = nullptr, *vs = nullptr;
+                if constexpr (L::k8) {
+                    const uint32_t ring = (tile + tl) % kScaleRing;
+                    wait(&scaled[ring], (tile + tl) / kScaleRing & 1u);
+                    ks = reinterpret_cast<const float*>(smem + L::kScales) + ring * 2 * kTcKT;
+                    vs = ks + kTcKT;
+                    const volatile uint32_t* v4 = reinterpret_cast<const volatile uint32_t*>(smem + L::kVe) + ring * 4;
+                    ve_run = max(ve_run, (int)max(max(v4[0], v4[1]), max(v4[2], v4[3])));
+                }
+                wait(&sfull[s], steps & 1u);
+                tc_fence_after();
+                const bool tail = k0 + kTcKT > it.len;
+                // column x of the tile: whether this row sees it
+                auto sees = [&](int x) {
+                    const int node = k0 + x - it.len;
+                    return node < 0 || (node < kMaxNodes && ((see >> node) & 1));
+                };
+                auto scores = [&](int c0, float (&v)[32]) {
+                    tmem_ld32(ts + c0, v);
+                    if constexpr (L::k8) {
+                        #pragma unroll
+                        for (int x = 0; x < 32; x += 4) {
+                            const float4 a = *reinterpret_cast<const float4*>(ks + c0 + x);
+                            v[x] *= a.x; v[x + 1] *= a.y; v[x + 2] *= a.z; v[x + 3] *= a.w;
+                        }
+                    }
+                    if (tail) {
+                        #pragma unroll
+                        for (int x = 0; x < 32; x++) if (!sees(c0 + x)) v[x] = -INFINITY;
+                    }
+                };
+                float mx = -INFINITY;
+                #pragma unroll 1
+                for (int c0 = 0; c0 < kTcKT; c0 += 32) {
+                    float v[32];
+                    scores(c0, v);
+                    #pragma unroll
+                    for (int x = 0; x < 32; x += 2) mx = max3(mx, v[x], v[x + 1]);
+                }
+                // c = 0 with an infinite score is NaN, as it should be; an all-masked tile stays -inf
+                top = fmaxf(top, mx == -INFINITY ? mx : mx * c);
+                const float want = L::k8 ? top + (float)(ve_run - 127) : top;
+                float f = 1.0f;
+                const bool move = want > base + 8.0f;                      // (from -inf: the first tile that has a key)
+                if (move) {
+                    f = exp2_approx(base - want);
+                    l *= f;
+                    base = want;
+                }
+                if (i > 0 && __any_sync(~0u, move)) {                      // O of the steps before is complete: S was formed after it
+                    #pragma unroll 1
+                    for (int c0 = 0; c0 < D; c0 += 32) {
+                        float o[32];
+                        tmem_ld32(to + 128 * s + c0, o);
+                        #pragma unroll
+                        for (int x = 0; x < 32; x++) o[x] *= f;
+                        tc_st32(to + 128 * s + c0, o);
+                    }
+                }
+                const float from = base == -INFINITY ? 0.f : base;
+                float sum = 0.f;
+                #pragma unroll 1
+                for (int c0 = 0; c0 < kTcKT; c0 += 32) {
+                    float v[32];
+                    scores(c0, v);
+                    uint32_t w[16];
+                    #pragma unroll
+                    for (int x = 0; x < 32; x += 2) {
+                        float a = exp2_approx(fmaf(v[x], c, -from)), b = exp2_approx(fmaf(v[x + 1], c, -from));
+                        sum += a + b;
+                        if constexpr (L::k8) {
+                            const float2 y = *reinterpret_cast<const float2*>(vs + c0 + x);
+                            a *= !tail || sees(c0 + x) ? y.x : 0.f;
+                            b *= !tail || sees(c0 + x + 1) ? y.y : 0.f;
+                        }
+                        w[x / 2] = pack2<BF>(a, b);
+                    }
+                    tc_st16(ts + c0 / 2, w);
+                }
+                l += sum;
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&pfull[s]);
+            }
+            tile += nt;
+            // ---- the item's rows ----
+            if (mine) wait(&pvdone[s], (steps - 1) & 1u);
+            tc_fence_after();
+            const bool whole = it.t0 == 0 && it.t1 == it.n;
+            float mm = base, ll = l, f0 = 1.0f, f1 = 0.0f;                 // this row of O is f0 O_s + f1 O_other
+            bool both = false;
+            if constexpr (!PAIR) {
+                ml[s * 128 + rl] = make_float2(mine ? base : -INFINITY, l);
+                tc_fence_before();
+                named_bar(1, 256);
+                tc_fence_after();
+                const float2 other = ml[(s ^ 1) * 128 + rl];
+                both = nt > 1;
+                mm = fmaxf(base, other.x);
+                f0 = base == -INFINITY ? (mm == -INFINITY ? 1.0f : 0.f) : exp2_approx(base - mm);
+                f1 = other.x == -INFINITY ? (mm == -INFINITY && both ? 1.0f : 0.f) : exp2_approx(other.x - mm);
+                ll = l * f0 + other.y * f1;
+            }
+            const bool odd_rows = odd[item & 7] != 0;                      // (every part of the item has been announced)
+            const bool live = row < M, present = see != 0;
+            const float inv = !present || ll == 0.f ? 0.f : 1.0f / ll;
+            const int node = row / P.group, hq = it.h * P.group + row % P.group;
+            uint8_t* dst = P.out + (((size_t)it.seq * P.n_nodes + node) * (size_t)P.ldo + (size_t)hq * D) * 2;
+            float* slot = P.work + (size_t)(2 * blockIdx.x + (first_item ? 0 : 1)) * L::kSlot;
+            const int r = row - it.r_base;
+            const int d0 = PAIR ? 0 : s * (D / 2), d1 = PAIR ? D : d0 + D / 2;
+            #pragma unroll 1
+            for (int c0 = d0; c0 < d1; c0 += 32) {
+                float o[32];
+                if (PAIR || mine) {
+                    tmem_ld32(to + 128 * s + c0, o);
+                    #pragma unroll
+                    for (int x = 0; x < 32; x++) o[x] *= f0;
+                } else {
+                    #pragma unroll
+                    for (int x = 0; x < 32; x++) o[x] = 0.f;
+                }
+                if (!PAIR && (both || !mine)) {   // the other stream has steps
+                    float b[32];
+                    tmem_ld32(to + 128 * (s ^ 1) + c0, b);
+                    #pragma unroll
+                    for (int x = 0; x < 32; x++) o[x] = fmaf(b[x], f1, o[x]);
+                }
+                if (odd_rows) {                   // infinities and NaN of the tree's V rows, for the rows that see them
+                    const size_t head = (size_t)it.seq * P.cache.seq_stride + (size_t)it.h * P.cache.head_stride;
+                    for (int j = 0; j < P.n_nodes; j++) {
+                        const long long pos = (long long)it.len + j;
+                        if (!((see >> j) & 1) || pos < (long long)it.t0 * kTcKT || pos >= (long long)it.t1 * kTcKT) continue;
+                        #pragma unroll
+                        for (int x = 0; x < 32; x++) {
+                            const size_t at = head + (size_t)pos * D + c0 + x;
+                            if constexpr (STORE == QWEN_E4M3) { if ((P.cache.v[at] & 0x7f) == 0x7f) o[x] += NAN; }
+                            else if constexpr (!L::k8) {
+                                const uint16_t w = reinterpret_cast<const uint16_t*>(P.cache.v)[at];
+                                constexpr uint32_t kExp = QT == QWEN_BF16 ? 0x7f80u : 0x7c00u;
+                                if ((w & kExp) == kExp) o[x] += QT == QWEN_BF16 ? bf2f(w) : __half2float(__ushort_as_half(w));
+                            }
+                        }
+                    }
+                }
+                if (*fault) {
+                    #pragma unroll
+                    for (int x = 0; x < 32; x++) o[x] = NAN;
+                }
+                if (!live) continue;
+                if (whole) {
+                    uint32_t w[16];
+                    #pragma unroll
+                    for (int x = 0; x < 16; x++) w[x] = present ? pack2<QT == QWEN_BF16>(o[2 * x] * inv, o[2 * x + 1] * inv) : 0u;
+                    #pragma unroll
+                    for (int x = 0; x < 4; x++)
+                        *reinterpret_cast<uint4*>(dst + (c0 + 8 * x) * 2) = make_uint4(w[4 * x], w[4 * x + 1], w[4 * x + 2], w[4 * x + 3]);
+                } else {
+                    #pragma unroll
+                    for (int x = 0; x < 32; x += 4)
+                        *reinterpret_cast<float4*>(slot + r * D + c0 + x) = present ? make_float4(o[x], o[x + 1], o[x + 2], o[x + 3])
+                                                                                     : make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (c0 == 0)
+                        *reinterpret_cast<float2*>(slot + L::kRows * D + 2 * r) = present ? make_float2(mm, ll) : make_float2(-INFINITY, 0.f);
+                }
+            }
+            tc_fence_before();
+            first_item = false;
+            item++;
+        } while (it.next());
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace ta
+}  // namespace qb
