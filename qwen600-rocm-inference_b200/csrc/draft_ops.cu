@@ -164,9 +164,9 @@ int check_rows(const qwen_kv_cache_t* c, const void* k, const void* v, int dtype
 // ---- tree attention ----------------------------------------------------------------
 // The kernel's variant, by the query rows of a K/V head (nodes times query heads):
 // up to 16 and up to 32 the warp-level kernel, in one block of rows; above, where it
-// would read the cache once for every 32 rows, the tensor-memory kernel with one
-// block of 128 rows or, above 128, two.
-int attention_rows(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : m <= 128 ? 128 : 256; }
+// would read the cache once for every 32 rows, the tensor-memory kernel in blocks
+// of 128.
+int attention_rows(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : 128; }
 
 struct Plan {
     int rows, row_blocks, shares;
@@ -193,12 +193,11 @@ int attention_plan(const qwen_kv_cache_t* c, int n_nodes, int n_heads, int dev, 
 }
 
 // The kernel that joins the shares' partial results, launched so that it may start its set-up early.
-template <int QT, int KT, int D, int ROWS>
+template <int QT, int KT, int D, int ROWS, bool ACROSS>
 int join_launch(const qb::ta::Params& P, const Plan& plan, cudaStream_t st) {
     if (plan.shares == 1) return QWEN_OK;
-    constexpr int kJoinRows = qb::ta::kJoinThreads / (D / 4);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(plan.shares, ROWS / kJoinRows);
+    cfg.gridDim = dim3(plan.shares, qb::ta::join_blocks<D, ROWS, ACROSS>());
     cfg.blockDim = dim3(qb::ta::kJoinThreads);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
@@ -206,7 +205,7 @@ int join_launch(const qb::ta::Params& P, const Plan& plan, cudaStream_t st) {
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    CU(cudaLaunchKernelEx(&cfg, qb::ta::combine_kernel<QT, KT, D, ROWS>, P, plan.row_blocks));
+    CU(cudaLaunchKernelEx(&cfg, qb::ta::combine_kernel<QT, KT, D, ROWS, ACROSS>, P, plan.row_blocks));
     return QWEN_OK;
 }
 template <int QT, int STORE, int D, int MT>
@@ -217,25 +216,24 @@ int attention_launch(const qb::ta::Params& P, const Plan& plan, int dev, cudaStr
     TRY(smem_limit(kernel, done, dev, L::kSmem));
     kernel<<<plan.shares, qb::ta::kThreads, L::kSmem, st>>>(P, plan.row_blocks);
     CU(cudaGetLastError());
-    return join_launch<QT, L::KT, D, L::kRows>(P, plan, st);
+    return join_launch<QT, L::KT, D, L::kRows, false>(P, plan, st);
 }
-template <int QT, int STORE, int D, bool PAIR>
+template <int QT, int STORE, int D>
 int attention_tc_launch(const qb::ta::Params& P, const Plan& plan, int dev, cudaStream_t st) {
-    using L = qb::ta::TcLayout<STORE, D, PAIR>;
+    using L = qb::ta::TcLayout<STORE, D>;
     static std::atomic<uint64_t> done{0};
-    auto kernel = qb::ta::attention_tc_kernel<QT, STORE, D, PAIR>;
+    auto kernel = qb::ta::attention_tc_kernel<QT, STORE, D>;
     TRY(smem_limit(kernel, done, dev, L::kSmem));
     kernel<<<plan.shares, qb::ta::kTcThreads, L::kSmem, st>>>(P, plan.row_blocks);
     CU(cudaGetLastError());
-    return join_launch<QT, qb::ta::kTcKT, D, L::kRows>(P, plan, st);
+    return join_launch<QT, qb::ta::kTcKT, D, qb::ta::kTcRows, true>(P, plan, st);
 }
 template <int QT, int STORE, int D>
 int attention_by_rows(const qb::ta::Params& P, const Plan& plan, int dev, cudaStream_t st) {
     switch (plan.rows) {
         case 16: return attention_launch<QT, STORE, D, 1>(P, plan, dev, st);
         case 32: return attention_launch<QT, STORE, D, 2>(P, plan, dev, st);
-        case 128: return attention_tc_launch<QT, STORE, D, false>(P, plan, dev, st);
-        default: return attention_tc_launch<QT, STORE, D, true>(P, plan, dev, st);
+        default: return attention_tc_launch<QT, STORE, D>(P, plan, dev, st);
     }
 }
 template <int QT, int STORE>

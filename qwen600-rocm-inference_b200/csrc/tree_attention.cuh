@@ -80,10 +80,19 @@ __device__ __forceinline__ int line_find(const Params& P, int units, long long x
     }
     return P.n_seqs - 1;
 }
-// First tile of share i of G.
-__device__ __forceinline__ long long share(long long tiles, int i, int G) { return tiles * i / G; }
-// The share that tile x lies in.
-__device__ __forceinline__ int share_of(long long tiles, long long x, int G) { return (int)(((x + 1) * G - 1) / tiles); }
+// a / b for a >= 0, b > 0: by 32 bits where they do (a 64-bit division takes some hundred instructions)
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+// The line cut into G shares: share i begins at tile i * tiles / G (rounded down).
+struct Shares {
+    long long tiles, whole;
+    uint32_t rest, G;
+    __device__ __forceinline__ Shares(long long n, int g) : tiles(n), whole(quotient(n, g)), rest((uint32_t)(n - whole * g)), G((uint32_t)g) {}
+    __device__ __forceinline__ long long begin(int i) const { return whole * i + (rest * (uint32_t)i) / G; }   // rest * i < G^2
+    // the share that tile x lies in: the last one that begins at x or before
+    __device__ __forceinline__ int of(long long x) const { return (int)quotient((x + 1) * G - 1, tiles); }
+};
 
 // ---- the tree --------------------------------------------------------------------
 // One warp: anc[i] = the nodes that node i sees (itself and its ancestors), 0 if it
@@ -121,6 +130,14 @@ __device__ __forceinline__ void tree_masks(const Params& P, int seq, int len, ui
     for (int k = 0; k < 2; k++)
         if (up[lane + 32 * k] != kNone) anc[lane + 32 * k] = 0;
     __syncwarp();
+}
+
+// Of the 64 positions len - before .. that begin `before` positions in front of the tree's first: bit x is set where a node that
+// sees the nodes `see` sees position x (all of the context, and those nodes).  see 0: an absent node, whose row is dropped.
+__device__ __forceinline__ uint64_t visible(uint64_t see, int before) {
+    if (before >= 64) return ~0ull;
+    if (before >= 0) return ((1ull << before) - 1) | (see << before);
+    return before > -64 ? see >> -before : 0ull;
 }
 
 // ---- fragments ---------------------------------------------------------------------
@@ -229,8 +246,9 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const Params P, 
 
     const int units = P.n_kv_heads * row_blocks, G = gridDim.x;
     const long long tiles = line_tiles<L::KT>(P, units);
-    long long at = share(tiles, blockIdx.x, G);
-    const long long to = share(tiles, blockIdx.x + 1, G);
+    const Shares shares(tiles, G);
+    long long at = shares.begin(blockIdx.x);
+    const long long to = shares.begin(blockIdx.x + 1);
     if (at >= to) return;
     long long before;
     int seq = line_find<L::KT>(P, units, at, before);
@@ -238,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const Params P, 
     const int M = P.n_nodes * P.group;
     while (at < to) {
         const int len = P.lens[seq], end = seq_end(P, len), n = seq_tiles<L::KT>(P, len);
-        const int unit = (int)((at - before) / n), t0 = (int)((at - before) - (long long)unit * n);
+        const int unit = (int)quotient(at - before, n), t0 = (int)((at - before) - (long long)unit * n);
         const int t1 = (int)min((long long)n, t0 + (to - at));
         const int h = unit / row_blocks, r_base = (unit - h * row_blocks) * L::kRows;
         const size_t head = (size_t)seq * P.cache.seq_stride + (size_t)h * P.cache.head_stride;
@@ -413,10 +431,12 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const Params P, 
                             s[mt][i][2] *= c[2 * mt + 1]; s[mt][i][3] *= c[2 * mt + 1];
                         }
                 }
-                auto sees = [&](int row, int key) {   // key: position
-                    const int node = key - len;
-                    return node < 0 || (node < kMaxNodes && ((see[row] >> node) & 1));
-                };
+                uint32_t vis[2 * MT];   // bit x: the row sees position k0 + x (KW <= 32)
+                if (tail) {
+                    #pragma unroll
+                    for (int r = 0; r < 2 * MT; r++) vis[r] = (uint32_t)visible(see[r], len - k0);
+                }
+                auto sees = [&](int row, int x) { return (vis[row] >> x & 1) != 0; };
                 if (tail) {
                     #pragma unroll
                     for (int mt = 0; mt < MT; mt++)
@@ -424,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const Params P, 
                         for (int i = 0; i < NT; i++)
                             #pragma unroll
                             for (int e = 0; e < 4; e++)
-                                if (!sees(2 * mt + (e >> 1), k0 + 8 * i + 2 * j + (e & 1))) s[mt][i][e] = -INFINITY;
+                                if (!sees(2 * mt + (e >> 1), 8 * i + 2 * j + (e & 1))) s[mt][i][e] = -INFINITY;
                 }
                 // ---- softmax ----
                 uint32_t up = 0;    // 8-bit: the rise of ve
@@ -457,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const Params P, 
                             float& x = s[r >> 1][i][2 * (r & 1) + e];
                             x = exp2_approx(x - base);
                             sum += x;
-                            if constexpr (L::k8) x *= !tail || sees(r, k0 + 8 * i + 2 * j + e) ? vs[i][e] * vinv : 0.f;
+                            if constexpr (L::k8) x *= !tail || sees(r, 8 * i + 2 * j + e) ? vs[i][e] * vinv : 0.f;
                         }
                     l[r] = l[r] * f[r] + sum;
                 }
@@ -503,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const Params P, 
                                     const float x = L::k8 ? NAN : QT == QWEN_BF16 ? bf2f((uint16_t)w) : __half2float(__ushort_as_half((uint16_t)w));
                                     #pragma unroll
                                     for (int q = 0; q < 2 * MT; q++)
-                                        if (sees(q, k0 + r)) o[q >> 1][d][2 * (q & 1) + e] += x;
+                                        if (sees(q, r)) o[q >> 1][d][2 * (q & 1) + e] += x;
                                 }
                         __syncwarp();
                         for (int i = lane; i < (KW - from) * (L::kRow / L::kEs); i += 32) {
@@ -609,65 +629,81 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const Params P, 
 }
 
 // Joins the partial results of the items that cross a border between shares:
-// block (i, y) takes the item that begins in share i and goes on in share i + 1, rows y * kJoinRows ..
+// blocks (i, y) take the item that begins in share i and goes on in share i + 1.
+// ACROSS: a slot holds O as [dim / 4][row] (the tensor-memory kernel: a thread a
+// row) and a thread here joins 16 dims of a row, lanes along the rows; otherwise O
+// is [row][dim] and a thread joins 4 dims, lanes along the dims.
 constexpr int kJoinThreads = 128;
-template <int QT, int KT, int D, int ROWS>
+template <int D, int ROWS, bool ACROSS>
+__host__ __device__ constexpr int join_blocks() { return ROWS * (ACROSS ? D / 16 : D / 4) / kJoinThreads; }
+template <int QT, int KT, int D, int ROWS, bool ACROSS>
 __global__ void __launch_bounds__(kJoinThreads) combine_kernel(const Params P, int row_blocks) {
-    constexpr int kSlot = ROWS * (D + 2), kLanes = D / 4, kJoinRows = kJoinThreads / kLanes;
+    constexpr int kSlot = ROWS * (D + 2), kVec = ACROSS ? 4 : 1, kAhead = ACROSS ? 4 : 8;   // float4s a thread; partial results loaded at once
     const int i = blockIdx.x, G = gridDim.x, units = P.n_kv_heads * row_blocks;
     const long long tiles = line_tiles<KT>(P, units);
-    const long long from = share(tiles, i, G), edge = share(tiles, i + 1, G);
+    const Shares shares(tiles, G);
+    const long long from = shares.begin(i), edge = shares.begin(i + 1);
     long long before = 0, s = edge, e = edge;   // the item at the border: its tiles
     int seq = 0, unit = 0;
     if (edge > from && edge < tiles) {
         seq = line_find<KT>(P, units, edge, before);
         const int n = seq_tiles<KT>(P, P.lens[seq]);
-        unit = (int)((edge - before) / n);
+        unit = (int)quotient(edge - before, n);
         s = before + (long long)unit * n;
         e = s + n;
     }
     pdl_wait();   // on every path: this kernel may not end before the one that it joins
     if (s >= edge || s < from) return;          // it begins at the border, or before this share
-    const int last = share_of(tiles, e - 1, G);
-    const int h = unit / row_blocks, r = blockIdx.y * kJoinRows + threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
+    const int last = shares.of(e - 1);
+    const int t = blockIdx.y * kJoinThreads + threadIdx.x;
+    const int h = unit / row_blocks, r = ACROSS ? t % ROWS : t / (D / 4), d = ACROSS ? t / ROWS * 16 : t % (D / 4) * 4;
     const int row = (unit - h * row_blocks) * ROWS + r;
     if (row >= P.n_nodes * P.group) return;
     // share i holds the item last (its second slot) unless it begins with it
     const size_t first_slot = 2 * (size_t)i + (from < s ? 1 : 0);
     float mm = -INFINITY, ll = 0.f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int kAhead = 8;   // partial results loaded at once
+    float4 a[kVec];
+    #pragma unroll
+    for (int v = 0; v < kVec; v++) a[v] = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int k0 = i; k0 <= last; k0 += kAhead) {
         float2 ml[kAhead];
-        float4 b[kAhead];
+        float4 b[kAhead][kVec];
         #pragma unroll
         for (int j = 0; j < kAhead; j++) {
             const int k = k0 + j;
             ml[j] = make_float2(-INFINITY, 0.f);
-            b[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (k > last || (k > i && share(tiles, k, G) == share(tiles, k + 1, G))) continue;
+            #pragma unroll
+            for (int v = 0; v < kVec; v++) b[j][v] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k > last || (k > i && shares.whole == 0 && shares.begin(k) == shares.begin(k + 1))) continue;   // (a share without a tile)
             const float* slot = P.work + (k == i ? first_slot : 2 * (size_t)k) * kSlot;
             ml[j] = *reinterpret_cast<const float2*>(slot + ROWS * D + 2 * r);
-            b[j] = *reinterpret_cast<const float4*>(slot + r * D + d);
+            #pragma unroll
+            for (int v = 0; v < kVec; v++) b[j][v] = *reinterpret_cast<const float4*>(ACROSS ? slot + ((d / 4 + v) * ROWS + r) * 4 : slot + r * D + d);
         }
         float mn = mm;
         #pragma unroll
         for (int j = 0; j < kAhead; j++) mn = fmaxf(mn, ml[j].x);
         const float f0 = mn == -INFINITY ? 1.0f : exp2_approx(mm - mn);
         ll *= f0;
-        a.x *= f0; a.y *= f0; a.z *= f0; a.w *= f0;
+        #pragma unroll
+        for (int v = 0; v < kVec; v++) { a[v].x *= f0; a[v].y *= f0; a[v].z *= f0; a[v].w *= f0; }
         #pragma unroll
         for (int j = 0; j < kAhead; j++) {
             const float f1 = mn == -INFINITY ? 1.0f : exp2_approx(ml[j].x - mn);
             ll += ml[j].y * f1;
-            a.x += b[j].x * f1; a.y += b[j].y * f1; a.z += b[j].z * f1; a.w += b[j].w * f1;
+            #pragma unroll
+            for (int v = 0; v < kVec; v++) {
+                a[v].x += b[j][v].x * f1; a[v].y += b[j][v].y * f1; a[v].z += b[j][v].z * f1; a[v].w += b[j][v].w * f1;
+            }
         }
         mm = mn;
     }
     const float inv = ll == 0.f ? 0.f : 1.0f / ll;
     const int node = row / P.group, hq = h * P.group + row % P.group;
     uint8_t* dst = P.out + (((size_t)seq * P.n_nodes + node) * (size_t)P.ldo + (size_t)hq * D + d) * 2;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<QT == QWEN_BF16>(a.x * inv, a.y * inv), pack2<QT == QWEN_BF16>(a.z * inv, a.w * inv));
+    #pragma unroll
+    for (int v = 0; v < kVec; v++)
+        *reinterpret_cast<uint2*>(dst + 8 * v) = make_uint2(pack2<QT == QWEN_BF16>(a[v].x * inv, a[v].y * inv), pack2<QT == QWEN_BF16>(a[v].z * inv, a[v].w * inv));
 }
 
 }  // namespace ta

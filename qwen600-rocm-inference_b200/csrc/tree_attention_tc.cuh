@@ -5,22 +5,20 @@
 //
 // With 33 and more rows (nodes times query heads a K/V head) the warp-level
 // products no longer fit under the cache's bytes, and blocks of 32 rows would
-// read them several times.  Here an item has 128 rows (one block) or 256 (two),
-// tiles have 128 keys, and two streams of 128 softmax threads (a thread a row)
-// work in turn, so one stream's exponentials run while the tensor core
-// forms the other's products: with one block of rows the streams take
-// alternate key tiles (joined at the end of an item in tensor memory), with two
-// blocks each stream takes a block and both use every tile.  A tile costs a
-// stream 128 exponentials a row, 1024 cycles of an SM at 16 a cycle; its two
-// products 256 cycles each; its bytes (bf16, 128 dims) 2,800 cycles of an SM's
-// share of the memory bandwidth.  So one block is bound by memory, two by the
-// exponentials.
+// read them several times.  Here an item has 128 rows, tiles have 128 keys, and
+// 256 softmax threads serve them, two a row (64 keys each; they agree on the row's
+// maximum through shared memory).  A tile's two products take 512 cycles each
+// (4,096 multiply-adds a cycle), its 16,384 exponentials 1,024 (16 a cycle), its bytes
+// (bf16, 128 dims) 2,800 of an SM's share of the memory bandwidth.  S and P have two
+// buffers each, so that the next tile's S is formed during a tile's exponentials.
+// (Two blocks of rows over shared tiles leave tensor memory for one S each: a
+// chain of products and exponentials without overlap, 2,800 cycles a block and tile.)
 //
-// Warps: 0-3 and 4-7 the streams (warp w reads the tensor-memory lanes 32 (w % 4) ..,
-// its rows), 8-11 producers, 12 issues the products.  S = Q K^T and P (16 bits,
-// written over S) and O are in tensor memory; Q, K and V in shared memory, rows of
-// 64 dims in the 128-byte swizzle: K is a K-major operand, V an MN-major one (its
-// rows are keys, so the product P V needs no transposed copy).  K and V
+// Warps: 0-7 softmax (warp w reads the tensor-memory lanes 32 (w % 4) .., its
+// rows; w / 4 picks the keys' half), 8-11 producers, 12 issues the products.  S = Q
+// K^T, P (16 bits) and O are in tensor memory; Q, K and V in shared memory, rows
+// of 64 dims in the 128-byte swizzle: K is a K-major operand, V an MN-major one
+// (its rows are keys, so the product P V needs no transposed copy).  K and V
 // parts of tiles go through one ring in the order in which they are used.  16-bit
 // rows arrive by cp.async; 8-bit rows arrive in a thread-private staging ring, become
 // fp16 (exact) and are stored swizzled by the thread that loaded them.  Every
@@ -32,32 +30,30 @@
 namespace qb {
 namespace ta {
 
-constexpr int kTcThreads = 416, kTcKT = 128, kTcProducers = 128;
+constexpr int kTcKT = 128, kTcRows = 128, kTcProducers = 128, kTcSoftmax = 256, kTcThreads = 416;
 constexpr int kScaleRing = 8;
 
-template <int STORE, int D, bool PAIR>
+template <int STORE, int D>
 struct TcLayout {
     static constexpr bool k8 = STORE == QWEN_E4M3 || STORE == QWEN_INT8;
     static constexpr int kRow = D * (k8 ? 1 : 2);          // bytes of a cache row
-    static constexpr int kHalf = kTcKT * D * 2;            // K or V of a tile, or 128 query rows: 16 bits
-    static constexpr int kBlocks = PAIR ? 2 : 1;           // blocks of 128 query rows
-    static constexpr int kRows = 128 * kBlocks;
-    static constexpr int kRing = D == 64 ? (k8 ? 6 : 8) : k8 ? (PAIR ? 3 : 4) : (PAIR ? 4 : 5);   // K / V parts in flight
+    static constexpr int kHalf = kTcKT * D * 2;            // K or V of a tile, or the query rows: 16 bits
+    static constexpr int kRing = D == 64 ? (k8 ? 6 : 8) : k8 ? 4 : 5;   // K / V parts in flight
     static constexpr int kRawHalf = k8 ? kTcKT * D : 0;
     static constexpr int kRawRing = k8 ? (D == 64 ? 4 : 3) : 0;
     static constexpr int kQ = 0;
-    static constexpr int kKV = kQ + kBlocks * kHalf;
+    static constexpr int kKV = kQ + kHalf;
     static constexpr int kRaw = kKV + kRing * kHalf;
     static constexpr int kScales = kRaw + kRawRing * kRawHalf;                        // [ring][ks 128, vs 128]
-    static constexpr int kMl = kScales + (k8 ? kScaleRing * 2 * kTcKT * 4 : 0);       // [stream][row] (base, l)
-    static constexpr int kAnc = kMl + 2 * 128 * 8;
+    static constexpr int kXm = kScales + (k8 ? kScaleRing * 2 * kTcKT * 4 : 0);       // [tile parity][half][row] maxima, then sums
+    static constexpr int kAnc = kXm + 2 * 2 * kTcRows * 4;
     static constexpr int kUp = kAnc + kMaxNodes * 8;
     static constexpr int kVe = kUp + kMaxNodes;                                       // [ring][producer warp] largest exponent of vs
     static constexpr int kBar = kVe + kScaleRing * 4 * 4;
     static constexpr int kBars = 2 * kRing + kScaleRing + 8;
     static constexpr int kMisc = kBar + kBars * 8;                                    // tensor-memory address, fault, odd[8]
     static constexpr int kSmem = kMisc + 48 + 1024;
-    static constexpr int kSlot = kRows * (D + 2);
+    static constexpr int kSlot = kTcRows * (D + 2);
     static_assert(kSmem <= 227 * 1024, "one CTA's shared memory");
     static_assert(2 * kSmem > 228 * 1024, "one CTA an SM: the kernel allocates all of tensor memory");
 };
@@ -104,6 +100,19 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
+// Bounded wait without a suspend-time hint: these waits are short, and a thread that sleeps wakes late.
+__device__ __forceinline__ bool mbar_spin(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
+    uint64_t since = 0;
+    for (uint32_t n = 0;; n++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((n & 255u) == 255u) {
+            const uint64_t now = global_ns();
+            if (!since) since = now;
+            else if (now - since > limit_ns) return false;
+        }
+    }
+}
+
 // A share of the line, item after item; every role walks it alike.
 struct Items {
     long long at, to, before;
@@ -112,23 +121,22 @@ struct Items {
     __device__ __forceinline__ bool start(const Params& P, int blocks) {
         row_blocks = blocks;
         units = P.n_kv_heads * blocks;
-        const long long tiles = line_tiles<kTcKT>(P, units);
-        at = share(tiles, blockIdx.x, gridDim.x);
-        to = share(tiles, blockIdx.x + 1, gridDim.x);
+        const Shares shares(line_tiles<kTcKT>(P, units), gridDim.x);
+        at = shares.begin(blockIdx.x);
+        to = shares.begin(blockIdx.x + 1);
         if (at >= to) return false;
         seq = line_find<kTcKT>(P, units, at, before);
         return true;
     }
-    template <int ROWS>
     __device__ __forceinline__ void item(const Params& P) {
         len = P.lens[seq];
         end = seq_end(P, len);
         n = seq_tiles<kTcKT>(P, len);
-        const int unit = (int)((at - before) / n);
+        const int unit = (int)quotient(at - before, n);
         t0 = (int)((at - before) - (long long)unit * n);
         t1 = (int)min((long long)n, t0 + (to - at));
         h = unit / row_blocks;
-        r_base = (unit - h * row_blocks) * ROWS;
+        r_base = (unit - h * row_blocks) * kTcRows;
     }
     __device__ __forceinline__ bool next() {
         at += t1 - t0;
@@ -139,9 +147,10 @@ struct Items {
 };
 
 // grid G (shares; one CTA an SM), kTcThreads threads, TcLayout::kSmem bytes.
-template <int QT, int STORE, int D, bool PAIR>
+// row_blocks: blocks of kTcRows rows that a K/V head has.
+template <int QT, int STORE, int D>
 __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Params P, int row_blocks) {
-    using L = TcLayout<STORE, D, PAIR>;
+    using L = TcLayout<STORE, D>;
     using namespace qb::tc;
     constexpr bool BF = QT == QWEN_BF16 && !L::k8;
     extern __shared__ uint8_t smem_raw[];
@@ -149,9 +158,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBar);   // [kRing] a K or V part is in place (128 producers)
     uint64_t* empty = full + L::kRing;                              // [kRing] its products are done
     uint64_t* scaled = empty + L::kRing;                            // [kScaleRing] a tile's scales are in place (128 producers)
-    uint64_t* sfull = scaled + kScaleRing;                          // [2] S of the stream
-    uint64_t* pfull = sfull + 2;                                    // [2] P of the stream, O rescaled (4 warps)
-    uint64_t* pvdone = sfull + 4;                                   // [2] P V of the stream
+    // [2]: the S / P buffer of a tile's parity
+    uint64_t* sfull = scaled + kScaleRing;                          // S formed
+    uint64_t* pfull = sfull + 2;                                    // P written, O rescaled (8 warps)
+    uint64_t* pvdone = sfull + 4;                                   // P V added
     uint64_t* qfull = sfull + 6;                                    // the item's queries (8 warps)
     uint64_t* drained = sfull + 7;                                  // all products are done, at the end
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
@@ -163,32 +173,33 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
     if (tid == 0) {
         for (int i = 0; i < L::kRing; i++) { mbar_init(&full[i], kTcProducers); mbar_init(&empty[i], 1); }
         for (int i = 0; i < kScaleRing; i++) mbar_init(&scaled[i], kTcProducers);
-        for (int i = 0; i < 2; i++) { mbar_init(&sfull[i], 1); mbar_init(&pfull[i], 4); mbar_init(&pvdone[i], 1); }
+        for (int i = 0; i < 2; i++) { mbar_init(&sfull[i], 1); mbar_init(&pfull[i], 8); mbar_init(&pvdone[i], 1); }
         mbar_init(qfull, 8);
         mbar_init(drained, 1);
         fence_barrier_init();
         *fault = 0;
         for (int i = 0; i < 8; i++) odd[i] = 0;
     }
-    if (warp == 12) tmem_alloc(tmem_slot, 512);
+    constexpr int kProducer = 8, kIssuer = 12;
+    if (warp == kIssuer) tmem_alloc(tmem_slot, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    constexpr uint32_t kTmO = 256;   // S / P of stream s: columns 128 s .., O: 256 + 128 s ..
+    constexpr uint32_t kTmO = 256, kTmP = 384;   // columns: S buffers 0 and 128, O 256, P buffers 384 and 448
     pdl_wait();
     pdl_launch_dependents();         // after the wait: what the joining kernel reads early (lens) is then complete
 
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (ok && !mbar_wait(bar, parity, kWaitNs)) { ok = false; *fault = 1; }
+        if (ok && !mbar_spin(bar, parity, kWaitNs)) { ok = false; *fault = 1; }
         return ok;
     };
     Items it;
     const bool busy = it.start(P, row_blocks);   // the same for the whole CTA
-    if (busy && warp >= 8 && warp < 12) {
+    if (busy && warp >= kProducer && warp < kIssuer) {
         // ---------------- producers ----------------
-        const int pt = tid - 256;
+        const int pt = tid - 32 * kProducer;
         uint32_t part = 0;           // K / V parts so far: slot part % kRing
         uint32_t unsaid = 0;         // 16-bit rows: parts whose copies are committed but not yet announced
         uint32_t item = 0, tile = 0; // tile: of the CTA so far
@@ -198,7 +209,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
             return wait(&empty[p % L::kRing], (p / L::kRing - 1) & 1u);
         };
         do {
-            it.item<L::kRows>(P);
+            it.item(P);
             const size_t head = (size_t)it.seq * P.cache.seq_stride + (size_t)it.h * P.cache.head_stride;
             const uint8_t* base[2] = {P.cache.k + head * (L::k8 ? 1 : 2), P.cache.v + head * (L::k8 ? 1 : 2)};
             if constexpr (!L::k8) {
@@ -223,29 +234,32 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                         }
                         cp_async_commit();
                         unsaid++;
-                        const bool tail = k0 + kTcKT > it.len;
-                        if (tail && kv == 1) {
+                        if (kv == 1 && k0 + kTcKT > it.len) {
                             // rows of the tree: infinities and NaN would reach nodes that do not see them (0 * NaN): they go to the
                             // softmax threads by another way (odd), and are zero in the product.  Every thread looks at its own copies.
+                            if (unsaid > 1) {
+                                cp_async_wait<1>();
+                                for (; unsaid > 1; unsaid--) say(part + 1 - unsaid);
+                            }
                             cp_async_wait<0>();
-                            constexpr uint32_t kExp = QT == QWEN_BF16 ? 0x7f80u : 0x7c00u;
+                            constexpr uint32_t kExp = QT == QWEN_BF16 ? 0x7f807f80u : 0x7c007c00u;
                             bool any = false;
-                            #pragma unroll 1
+                            #pragma unroll 4
                             for (int i = 0; i < kPer; i++) {
                                 const int r = r0 + i * kStep;
-                                if (k0 + r < it.len) continue;
                                 uint4* p = reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-                                uint4 w = *p;
-                                uint32_t x[4] = {w.x, w.y, w.z, w.w};
-                                bool hit = false;
-                                #pragma unroll
-                                for (int e = 0; e < 4; e++) {
-                                    if ((x[e] & kExp) == kExp) { x[e] &= 0xffff0000u; hit = true; }
-                                    if (((x[e] >> 16) & kExp) == kExp) { x[e] &= 0xffffu; hit = true; }
+                                const uint4 w = *p;
+                                // all ones where a 16-bit half is not finite
+                                uint4 m = make_uint4(__vcmpeq2(w.x & kExp, kExp), __vcmpeq2(w.y & kExp, kExp), __vcmpeq2(w.z & kExp, kExp),
+                                                     __vcmpeq2(w.w & kExp, kExp));
+                                if ((m.x | m.y | m.z | m.w) && k0 + r >= it.len) {
+                                    *p = make_uint4(w.x & ~m.x, w.y & ~m.y, w.z & ~m.z, w.w & ~m.w);
+                                    any = true;
                                 }
-                                if (hit) { *p = make_uint4(x[0], x[1], x[2], x[3]); any = true; }
                             }
                             if (any) odd[item & 7] = 1;
+                            say(part);
+                            unsaid = 0;
                         }
                         if (unsaid > 2) {
                             cp_async_wait<2>();
@@ -312,7 +326,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                         const float vs = reinterpret_cast<const float*>(smem + L::kScales)[ring * 2 * kTcKT + kTcKT + pt];
                         uint32_t e = __float_as_uint(vs) >> 23 & 0xffu;
                         e = __reduce_max_sync(~0u, e == 255u ? 0u : min(e + 1, 253u));
-                        if (lane == 0) reinterpret_cast<volatile uint32_t*>(smem + L::kVe)[ring * 4 + (warp - 8)] = e;
+                        if (lane == 0) reinterpret_cast<volatile uint32_t*>(smem + L::kVe)[ring * 4 + (warp - kProducer)] = e;
                         __syncwarp();
                         mbar_arrive(&scaled[ring]);
                     }
@@ -324,137 +338,150 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
         } while (ok && it.next());
         cp_async_wait<0>();
         if (ok) for (; unsaid; unsaid--) say(part - unsaid);
-    } else if (busy && warp == 12) {
-        // ---------------- products ----------------
+    } else if (busy && warp == kIssuer) {
+        // ---------------- products (lane 0), the items' tree masks (all) ----------------
         constexpr uint32_t id_s = tc_idesc<BF>(kTcKT, false), id_o = tc_idesc<BF>(D, true);
-        uint32_t part = 0, item = 0, steps[2] = {0, 0};   // steps of a stream so far
-        if (lane == 0) {
-            do {
-                it.item<L::kRows>(P);
-                const int nt = it.t1 - it.t0, nv = PAIR ? 2 * nt : nt;   // virtual steps: stream v & 1
-                if (!wait(qfull, item & 1u)) break;
+        uint32_t part = 0, item = 0;
+        uint32_t steps[2] = {0, 0};   // tiles of a buffer so far
+        bool going = true;
+        do {
+            it.item(P);
+            // every softmax thread has taken what it needs of the item before's masks (it announced that item's queries after)
+            tree_masks(P, it.seq, it.len, anc, reinterpret_cast<int8_t*>(smem + L::kUp));
+            named_bar(1, kTcSoftmax + 32);
+            if (lane == 0 && going) {
+                const int nt = it.t1 - it.t0;
+                going = wait(qfull, item & 1u);
                 tc_fence_after();
-                for (int v = 0; v < nv + 2 && ok; v++) {
-                    const int s = v & 1;
-                    if (v >= 2) {              // O += P V of step v - 2
-                        const int u = v - 2, t = PAIR ? u >> 1 : u;
-                        const uint32_t p = part + 2 * t + 1;
-                        if (!wait(&pfull[s], (steps[s] - 1) & 1u) || !wait(&full[p % L::kRing], p / L::kRing & 1u)) break;
+                // S 0, S 1, P V 0, S 2, P V 1, ...: buffer b = tile & 1 of S is free once P of the tile two before is written
+                for (int v = 0; v < nt + 2 && going; v++) {
+                    const int b = v & 1;
+                    if (v >= 2) {
+                        const uint32_t p = part + 2 * (v - 2) + 1;
+                        going = wait(&pfull[b], (steps[b] - 1) & 1u) && wait(&full[p % L::kRing], p / L::kRing & 1u);
+                        if (!going) break;
                         tc_fence_after();
                         const uint32_t vb = smem_addr(smem + L::kKV + p % L::kRing * L::kHalf);
                         #pragma unroll
                         for (int k = 0; k < kTcKT / 16; k++)
-                            tc_mma_ts(tmem + kTmO + 128 * s, tmem + 128 * s + 8 * k, mn_major_sw128_desc(vb + k * 2048, kTcKT * 128), id_o,
-                                      (u >= 2 || k) ? 1u : 0u);
-                        if (!PAIR || s) mma_commit(&empty[p % L::kRing]);
-                        mma_commit(&pvdone[s]);
+                            tc_mma_ts(tmem + kTmO, tmem + kTmP + 64 * b + 8 * k, mn_major_sw128_desc(vb + k * 2048, kTcKT * 128), id_o,
+                                      (v > 2 || k) ? 1u : 0u);
+                        mma_commit(&empty[p % L::kRing]);
+                        mma_commit(&pvdone[b]);
                     }
-                    if (v < nv) {              // S = Q K^T of step v, over the P that the product above has read
-                        const int t = PAIR ? v >> 1 : v;
-                        const uint32_t p = part + 2 * t;
-                        if (v >= 2 && !wait(&pvdone[s], (steps[s] - 1) & 1u)) break;
-                        if (!wait(&full[p % L::kRing], p / L::kRing & 1u)) break;
+                    if (v < nt) {
+                        const uint32_t p = part + 2 * v;
+                        going = wait(&full[p % L::kRing], p / L::kRing & 1u);
+                        if (!going) break;
                         tc_fence_after();
-                        const uint32_t kb = smem_addr(smem + L::kKV + p % L::kRing * L::kHalf);
-                        const uint32_t qb = smem_addr(smem + L::kQ + (PAIR ? s : 0) * L::kHalf);
+                        const uint32_t kb = smem_addr(smem + L::kKV + p % L::kRing * L::kHalf), qb = smem_addr(smem + L::kQ);
                         #pragma unroll
                         for (int k = 0; k < D / 16; k++)
-                            mma_bf16(tmem + 128 * s, kmajor_sw128_desc(qb + (k >> 2) * (128 * 128) + (k & 3) * 32),
+                            mma_bf16(tmem + 128 * b, kmajor_sw128_desc(qb + (k >> 2) * (kTcRows * 128) + (k & 3) * 32),
                                      kmajor_sw128_desc(kb + (k >> 2) * (kTcKT * 128) + (k & 3) * 32), id_s, k ? 1u : 0u);
-                        if (!PAIR || s) mma_commit(&empty[p % L::kRing]);
-                        mma_commit(&sfull[s]);
-                        steps[s]++;
+                        mma_commit(&empty[p % L::kRing]);
+                        mma_commit(&sfull[b]);
+                        steps[b]++;
                     }
                 }
                 part += 2 * nt;
-                item++;
-            } while (ok && it.next());
+            }
+            __syncwarp();
+            item++;
+        } while (it.next());
+        if (lane == 0) {
             mma_commit(drained);
             if (!mbar_wait(drained, 0, kWaitNs)) *fault = 1;
         }
         __syncwarp();
-    } else if (busy && warp < 8) {
+    } else if (busy && warp < kProducer) {
         // ---------------- softmax ----------------
-        const int s = warp >> 2, rl = 32 * (warp & 3) + lane;              // stream, row of its block
-        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t ts = tmem + lanes + 128 * s, to = tmem + lanes + kTmO;
-        float2* ml = reinterpret_cast<float2*>(smem + L::kMl);
+        const int half = warp >> 2, rl = 32 * (warp & 3) + lane;           // half of the keys, row of the item
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, to = tmem + lanes + kTmO;
+        float* xm = reinterpret_cast<float*>(smem + L::kXm);               // [tile parity][half][row]
         const int M = P.n_nodes * P.group;
         const bool flip = P.scale_log2 < 0.f;                              // a negative scale: its sign goes to the queries
         uint32_t item = 0, steps = 0, tile = 0;
+        uint32_t uses[2] = {0, 0};                                         // tiles of a buffer so far
         bool first_item = true;
         do {
-            it.item<L::kRows>(P);
-            const int nt = it.t1 - it.t0, mine = PAIR ? nt : (nt + 1 - s) >> 1;   // steps of this stream
-            named_bar(1, 256);                                             // the item before is written, its masks and queries are free
-            if (tid == 0) odd[(item - 1) & 7] = 0;
-            if (warp == 0) tree_masks(P, it.seq, it.len, anc, reinterpret_cast<int8_t*>(smem + L::kUp));
-            const int row = it.r_base + (PAIR ? 128 * s : 0) + rl;         // one block: both streams' threads rl share a row
+            it.item(P);
+            const int nt = it.t1 - it.t0;
+            // (the item before's products are done: its queries' place is free)
+            const int row = it.r_base + rl;
+            const int node = row / P.group, hq = it.h * P.group + row - node * P.group;
+            const bool live = row < M;
             float c = fabsf(P.scale_log2);                                 // (kept above 0: -inf * 0 would be NaN)
             {
-                const int node = row / P.group, hq = it.h * P.group + row % P.group;
+                // this thread's half of the row
+                constexpr int kPer = D / 16;
                 const uint4* src = reinterpret_cast<const uint4*>(P.q + (((size_t)it.seq * P.n_nodes + node) * (size_t)P.ldq + (size_t)hq * D) * 2);
-                const bool live = row < M;
+                uint4 w[kPer];
+                #pragma unroll
+                for (int i = 0; i < kPer; i++) w[i] = live ? __ldg(src + half * kPer + i) : make_uint4(0, 0, 0, 0);
                 float down = 1.0f;
                 if constexpr (L::k8 && QT == QWEN_BF16) {                  // into fp16's range, a power of two a row
                     uint32_t m = 0;
+                    auto largest = [&](const uint4& y) {
+                        const uint32_t x[4] = {y.x, y.y, y.z, y.w};
+                        #pragma unroll
+                        for (int e = 0; e < 4; e++) m = max(m, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
+                    };
+                    #pragma unroll
+                    for (int i = 0; i < kPer; i++) largest(w[i]);
                     if (live) {
-                        #pragma unroll 4
-                        for (int i = 0; i < D / 8; i++) {
-                            const uint4 w = __ldg(src + i);
-                            const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-                            #pragma unroll
-                            for (int e = 0; e < 4; e++) m = max(m, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
-                        }
+                        #pragma unroll
+                        for (int i = 0; i < kPer; i++) largest(__ldg(src + (half ^ 1) * kPer + i));
                     }
                     const int e = min(max((int)(m >> 7), 1), 253);
                     down = __uint_as_float((uint32_t)(254 - e) << 23);
                     c *= __uint_as_float((uint32_t)e << 23);
                 }
-                constexpr int kAll = D / 8;
-                const int i0 = PAIR ? 0 : s * (kAll / 2), i1 = PAIR ? kAll : i0 + kAll / 2;
-                uint8_t* dst = smem + L::kQ + (PAIR ? s : 0) * L::kHalf + rl * 128;
-                #pragma unroll 4
-                for (int i = i0; i < i1; i++) {
-                    uint4 w = live ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+                uint8_t* dst = smem + L::kQ + rl * 128;
+                #pragma unroll
+                for (int i = 0; i < kPer; i++) {
                     if constexpr (L::k8 && QT == QWEN_BF16) {
-                        w.x = kv::half2_bits(bf_lo(w.x) * down, bf_hi(w.x) * down);
-                        w.y = kv::half2_bits(bf_lo(w.y) * down, bf_hi(w.y) * down);
-                        w.z = kv::half2_bits(bf_lo(w.z) * down, bf_hi(w.z) * down);
-                        w.w = kv::half2_bits(bf_lo(w.w) * down, bf_hi(w.w) * down);
+                        w[i].x = kv::half2_bits(bf_lo(w[i].x) * down, bf_hi(w[i].x) * down);
+                        w[i].y = kv::half2_bits(bf_lo(w[i].y) * down, bf_hi(w[i].y) * down);
+                        w[i].z = kv::half2_bits(bf_lo(w[i].z) * down, bf_hi(w[i].z) * down);
+                        w[i].w = kv::half2_bits(bf_lo(w[i].w) * down, bf_hi(w[i].w) * down);
                     }
-                    if (flip) { w.x ^= 0x80008000u; w.y ^= 0x80008000u; w.z ^= 0x80008000u; w.w ^= 0x80008000u; }
-                    *reinterpret_cast<uint4*>(dst + (i >> 3) * (128 * 128) + (((i & 7) ^ (rl & 7)) << 4)) = w;
+                    if (flip) { w[i].x ^= 0x80008000u; w[i].y ^= 0x80008000u; w[i].z ^= 0x80008000u; w[i].w ^= 0x80008000u; }
+                    const int ch = half * kPer + i;
+                    *reinterpret_cast<uint4*>(dst + (ch >> 3) * (kTcRows * 128) + (((ch & 7) ^ (rl & 7)) << 4)) = w[i];
                 }
             }
             c = fmaxf(c, 1e-37f);
             fence_async_smem();
-            named_bar(1, 256);                                             // masks
+            tc_fence_before();
+            named_bar(1, kTcSoftmax + 32);                                 // the masks are there; every thread is behind the item before
+            if (tid == 0) odd[(item - 1) & 7] = 0;
+            const uint64_t see = live ? anc[node] : 0;
+            __syncwarp();
             if (lane == 0) mbar_arrive(qfull);
-            const uint64_t see = row < M ? anc[row / P.group] : 0;
-            float top = -INFINITY, base = -INFINITY, l = 0.f;              // running maximum; what exponents are taken from
+            float top = -INFINITY, base = -INFINITY, l = 0.f;              // the row's running maximum; what exponents are taken from; this half's sum
             int ve_run = 37;                                               // 8 bits: largest exponent of a value scale so far, 2^-90 at least
-            for (int i = 0; i < mine; i++, steps++) {
-                const int tl = PAIR ? i : 2 * i + s, k0 = (it.t0 + tl) * kTcKT;
+            for (int i = 0; i < nt; i++, steps++) {
+                const int k0 = (it.t0 + i) * kTcKT + 64 * half;
+                const int b = i & 1;
                 const float *ks = nullptr, *vs = nullptr;
                 if constexpr (L::k8) {
-                    const uint32_t ring = (tile + tl) % kScaleRing;
-                    wait(&scaled[ring], (tile + tl) / kScaleRing & 1u);
-                    ks = reinterpret_cast<const float*>(smem + L::kScales) + ring * 2 * kTcKT;
+                    const uint32_t ring = (tile + i) % kScaleRing;
+                    wait(&scaled[ring], (tile + i) / kScaleRing & 1u);
+                    ks = reinterpret_cast<const float*>(smem + L::kScales) + ring * 2 * kTcKT + 64 * half;
                     vs = ks + kTcKT;
                     const volatile uint32_t* v4 = reinterpret_cast<const volatile uint32_t*>(smem + L::kVe) + ring * 4;
                     ve_run = max(ve_run, (int)max(max(v4[0], v4[1]), max(v4[2], v4[3])));
                 }
-                wait(&sfull[s], steps & 1u);
+                const uint32_t use = uses[b];
+                wait(&sfull[b], use & 1u);
                 tc_fence_after();
-                const bool tail = k0 + kTcKT > it.len;
-                // column x of the tile: whether this row sees it
-                auto sees = [&](int x) {
-                    const int node = k0 + x - it.len;
-                    return node < 0 || (node < kMaxNodes && ((see >> node) & 1));
-                };
+                const bool tail = k0 + 64 > it.len;
+                // bit x: the row sees column x of this half
+                const uint64_t vis = tail ? visible(see, it.len - k0) : ~0ull;
+                // scores of columns c0 .. c0 + 31 of this half (read twice: for the maximum, and for the exponentials)
                 auto scores = [&](int c0, float (&v)[32]) {
-                    tmem_ld32(ts + c0, v);
+                    tmem_ld32(tmem + lanes + 128 * b + 64 * half + c0, v);
                     if constexpr (L::k8) {
                         #pragma unroll
                         for (int x = 0; x < 32; x += 4) {
@@ -463,19 +490,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                         }
                     }
                     if (tail) {
+                        const uint32_t m = (uint32_t)(vis >> c0);
                         #pragma unroll
-                        for (int x = 0; x < 32; x++) if (!sees(c0 + x)) v[x] = -INFINITY;
+                        for (int x = 0; x < 32; x++) if (!(m >> x & 1)) v[x] = -INFINITY;
                     }
                 };
                 float mx = -INFINITY;
                 #pragma unroll 1
-                for (int c0 = 0; c0 < kTcKT; c0 += 32) {
-                    float v[32];
+                for (int c0 = 0; c0 < 64; c0 += 32) {
+                    float v[32], my = -INFINITY;
                     scores(c0, v);
                     #pragma unroll
-                    for (int x = 0; x < 32; x += 2) mx = max3(mx, v[x], v[x + 1]);
+                    for (int x = 0; x < 32; x += 4) { mx = max3(mx, v[x], v[x + 1]); my = max3(my, v[x + 2], v[x + 3]); }
+                    mx = fmaxf(mx, my);
                 }
-                // c = 0 with an infinite score is NaN, as it should be; an all-masked tile stays -inf
+                xm[((steps & 1) * 2 + half) * 128 + rl] = mx;
+                named_bar(2, kTcSoftmax);
+                mx = fmaxf(mx, xm[((steps & 1) * 2 + (half ^ 1)) * 128 + rl]);
+                // an all-masked tile stays -inf
                 top = fmaxf(top, mx == -INFINITY ? mx : mx * c);
                 const float want = L::k8 ? top + (float)(ve_run - 127) : top;
                 float f = 1.0f;
@@ -485,86 +517,68 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                     l *= f;
                     base = want;
                 }
-                if (i > 0 && __any_sync(~0u, move)) {                      // O of the steps before is complete: S was formed after it
+                if (i > 0 && __any_sync(~0u, move)) {
+                    wait(&pvdone[b ^ 1], (uses[b ^ 1] - 1) & 1u);          // O of the tile before
+                    tc_fence_after();
                     #pragma unroll 1
-                    for (int c0 = 0; c0 < D; c0 += 32) {
+                    for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 32) {
                         float o[32];
-                        tmem_ld32(to + 128 * s + c0, o);
+                        tmem_ld32(to + c0, o);
                         #pragma unroll
                         for (int x = 0; x < 32; x++) o[x] *= f;
-                        tc_st32(to + 128 * s + c0, o);
+                        tc_st32(to + c0, o);
                     }
                 }
                 const float from = base == -INFINITY ? 0.f : base;
-                float sum = 0.f;
+                if (i > 1) wait(&pvdone[b], (use - 1) & 1u);               // the P buffer's last product
+                tc_fence_after();
+                float sum0 = 0.f, sum1 = 0.f;
                 #pragma unroll 1
-                for (int c0 = 0; c0 < kTcKT; c0 += 32) {
+                for (int c0 = 0; c0 < 64; c0 += 32) {
                     float v[32];
                     scores(c0, v);
                     uint32_t w[16];
+                    const uint32_t m = (uint32_t)(vis >> c0);
                     #pragma unroll
                     for (int x = 0; x < 32; x += 2) {
-                        float a = exp2_approx(fmaf(v[x], c, -from)), b = exp2_approx(fmaf(v[x + 1], c, -from));
-                        sum += a + b;
+                        float a = exp2_approx(fmaf(v[x], c, -from)), d = exp2_approx(fmaf(v[x + 1], c, -from));
+                        sum0 += a;
+                        sum1 += d;
                         if constexpr (L::k8) {
                             const float2 y = *reinterpret_cast<const float2*>(vs + c0 + x);
-                            a *= !tail || sees(c0 + x) ? y.x : 0.f;
-                            b *= !tail || sees(c0 + x + 1) ? y.y : 0.f;
+                            a *= !tail || (m >> x & 1) ? y.x : 0.f;         // (an unseen row's scale may be NaN)
+                            d *= !tail || (m >> (x + 1) & 1) ? y.y : 0.f;
                         }
-                        w[x / 2] = pack2<BF>(a, b);
+                        w[x / 2] = pack2<BF>(a, d);
                     }
-                    tc_st16(ts + c0 / 2, w);
+                    tc_st16(tmem + lanes + kTmP + 64 * b + 32 * half + c0 / 2, w);
                 }
-                l += sum;
+                l += sum0 + sum1;
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&pfull[s]);
+                if (lane == 0) mbar_arrive(&pfull[b]);
+                uses[b]++;
             }
             tile += nt;
-            // ---- the item's rows ----
-            if (mine) wait(&pvdone[s], (steps - 1) & 1u);
-            tc_fence_after();
-            const bool whole = it.t0 == 0 && it.t1 == it.n;
-            float mm = base, ll = l, f0 = 1.0f, f1 = 0.0f;                 // this row of O is f0 O_s + f1 O_other
-            bool both = false;
-            if constexpr (!PAIR) {
-                ml[s * 128 + rl] = make_float2(mine ? base : -INFINITY, l);
-                tc_fence_before();
-                named_bar(1, 256);
-                tc_fence_after();
-                const float2 other = ml[(s ^ 1) * 128 + rl];
-                both = nt > 1;
-                mm = fmaxf(base, other.x);
-                f0 = base == -INFINITY ? (mm == -INFINITY ? 1.0f : 0.f) : exp2_approx(base - mm);
-                f1 = other.x == -INFINITY ? (mm == -INFINITY && both ? 1.0f : 0.f) : exp2_approx(other.x - mm);
-                ll = l * f0 + other.y * f1;
+            // ---- the item's rows: this thread's half of the dims ----
+            {
+                const int b = (nt - 1) & 1;
+                wait(&pvdone[b], (uses[b] - 1) & 1u);
             }
+            tc_fence_after();
+            xm[((steps & 1) * 2 + half) * 128 + rl] = l;
+            named_bar(2, kTcSoftmax);
+            l += xm[((steps & 1) * 2 + (half ^ 1)) * 128 + rl];
+            steps++;                                                       // (the next tile's maxima go to the other half of xm)
             const bool odd_rows = odd[item & 7] != 0;                      // (every part of the item has been announced)
-            const bool live = row < M, present = see != 0;
-            const float inv = !present || ll == 0.f ? 0.f : 1.0f / ll;
-            const int node = row / P.group, hq = it.h * P.group + row % P.group;
-            uint8_t* dst = P.out + (((size_t)it.seq * P.n_nodes + node) * (size_t)P.ldo + (size_t)hq * D) * 2;
+            const bool whole = it.t0 == 0 && it.t1 == it.n, present = see != 0, failed = *fault != 0;
+            const float inv = !present || l == 0.f ? 0.f : 1.0f / l;
             float* slot = P.work + (size_t)(2 * blockIdx.x + (first_item ? 0 : 1)) * L::kSlot;
-            const int r = row - it.r_base;
-            const int d0 = PAIR ? 0 : s * (D / 2), d1 = PAIR ? D : d0 + D / 2;
             #pragma unroll 1
-            for (int c0 = d0; c0 < d1; c0 += 32) {
+            for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 32) {
                 float o[32];
-                if (PAIR || mine) {
-                    tmem_ld32(to + 128 * s + c0, o);
-                    #pragma unroll
-                    for (int x = 0; x < 32; x++) o[x] *= f0;
-                } else {
-                    #pragma unroll
-                    for (int x = 0; x < 32; x++) o[x] = 0.f;
-                }
-                if (!PAIR && (both || !mine)) {   // the other stream has steps
-                    float b[32];
-                    tmem_ld32(to + 128 * (s ^ 1) + c0, b);
-                    #pragma unroll
-                    for (int x = 0; x < 32; x++) o[x] = fmaf(b[x], f1, o[x]);
-                }
+                tmem_ld32(to + c0, o);
                 if (odd_rows) {                   // infinities and NaN of the tree's V rows, for the rows that see them
                     const size_t head = (size_t)it.seq * P.cache.seq_stride + (size_t)it.h * P.cache.head_stride;
                     for (int j = 0; j < P.n_nodes; j++) {
@@ -582,26 +596,36 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                         }
                     }
                 }
-                if (*fault) {
-                    #pragma unroll
-                    for (int x = 0; x < 32; x++) o[x] = NAN;
-                }
-                if (!live) continue;
+                #pragma unroll
+                for (int x = 0; x < 32; x++) o[x] = failed ? NAN : present ? o[x] : 0.f;
                 if (whole) {
+                    // 16-bit rows into the queries' place, swizzled, and from there whole rows to memory
                     uint32_t w[16];
                     #pragma unroll
-                    for (int x = 0; x < 16; x++) w[x] = present ? pack2<QT == QWEN_BF16>(o[2 * x] * inv, o[2 * x + 1] * inv) : 0u;
+                    for (int x = 0; x < 16; x++) w[x] = pack2<QT == QWEN_BF16>(o[2 * x] * inv, o[2 * x + 1] * inv);
                     #pragma unroll
                     for (int x = 0; x < 4; x++)
-                        *reinterpret_cast<uint4*>(dst + (c0 + 8 * x) * 2) = make_uint4(w[4 * x], w[4 * x + 1], w[4 * x + 2], w[4 * x + 3]);
-                } else {
+                        *reinterpret_cast<uint4*>(smem + L::kQ + swz<D * 2>(rl, c0 / 8 + x)) = make_uint4(w[4 * x], w[4 * x + 1], w[4 * x + 2], w[4 * x + 3]);
+                } else if (live) {
                     #pragma unroll
                     for (int x = 0; x < 32; x += 4)
-                        *reinterpret_cast<float4*>(slot + r * D + c0 + x) = present ? make_float4(o[x], o[x + 1], o[x + 2], o[x + 3])
-                                                                                     : make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (c0 == 0)
-                        *reinterpret_cast<float2*>(slot + L::kRows * D + 2 * r) = present ? make_float2(mm, ll) : make_float2(-INFINITY, 0.f);
+                        *reinterpret_cast<float4*>(slot + (((c0 + x) / 4) * kTcRows + rl) * 4) = make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+                    if (c0 == 0) *reinterpret_cast<float2*>(slot + kTcRows * D + 2 * rl) = present ? make_float2(base, l) : make_float2(-INFINITY, 0.f);
                 }
+            }
+            if (whole) {                          // the same for all
+                named_bar(2, kTcSoftmax);
+                constexpr int kChunks = D / 8, kStep = kTcSoftmax / kChunks;
+                const int ch = tid % kChunks;
+                #pragma unroll 2
+                for (int r = tid / kChunks; r < kTcRows; r += kStep) {
+                    const int orow = it.r_base + r;
+                    if (orow >= M) break;
+                    const int onode = orow / P.group, ohq = it.h * P.group + orow - onode * P.group;
+                    *reinterpret_cast<uint4*>(P.out + (((size_t)it.seq * P.n_nodes + onode) * (size_t)P.ldo + (size_t)ohq * D + ch * 8) * 2) =
+                        *reinterpret_cast<const uint4*>(smem + L::kQ + swz<D * 2>(r, ch));
+                }
+                named_bar(2, kTcSoftmax);         // the queries' place is free again
             }
             tc_fence_before();
             first_item = false;
@@ -610,7 +634,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) tmem_dealloc(tmem, 512);
+    if (warp == kIssuer) tmem_dealloc(tmem, 512);
 }
 
 }  // namespace ta
