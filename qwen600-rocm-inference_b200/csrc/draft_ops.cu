@@ -169,7 +169,7 @@ int check_rows(const qwen_kv_cache_t* c, const void* k, const void* v, int dtype
 int attention_rows(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : 128; }
 
 struct Plan {
-    int rows, row_blocks, shares;
+    int rows, row_blocks, beside, shares;   // shares: CTAs, beside for each share of the line
     size_t bytes;
 };
 int check_tree(const qwen_kv_cache_t* c, int n_nodes, int n_heads) {
@@ -184,18 +184,20 @@ int attention_plan(const qwen_kv_cache_t* c, int n_nodes, int n_heads, int dev, 
     TRY(sm_count(dev, &nsm));
     p->rows = attention_rows((int)m);
     p->row_blocks = (int)((m + p->rows - 1) / p->rows);
-    // two CTAs an SM (the tensor-memory kernel: one), but no more than there can be tiles (64 keys at least, 128)
-    const int keys = p->rows <= 32 ? 64 : 128;
-    const double most = (double)c->n_seqs * c->n_kv_heads * p->row_blocks * ((c->capacity + keys - 1) / keys);
-    p->shares = (int)std::min((double)(p->rows <= 32 ? 2 * nsm : nsm), most);
+    // two CTAs an SM (the tensor-memory kernel: one), shared out over the blocks of rows that walk side by side
+    const int keys = p->rows <= 32 ? 64 : 128, ctas = p->rows <= 32 ? 2 * nsm : nsm;
+    p->beside = p->row_blocks <= ctas ? p->row_blocks : 1;
+    // no more shares than the line can have positions
+    const double most = (double)c->n_seqs * c->n_kv_heads * (p->row_blocks / p->beside) * ((c->capacity + keys - 1) / keys + qb::ta::kTcItemCost);
+    p->shares = (int)std::min((double)(ctas / p->beside), most) * p->beside;
     p->bytes = (size_t)2 * p->shares * p->rows * (c->head_dim + 2) * sizeof(float);
     return QWEN_OK;
 }
 
 // The kernel that joins the shares' partial results, launched so that it may start its set-up early.
-template <int QT, int KT, int D, int ROWS, bool ACROSS>
+template <int QT, int KT, int COST, int D, int ROWS, bool ACROSS>
 int join_launch(const qb::ta::Params& P, const Plan& plan, cudaStream_t st) {
-    if (plan.shares == 1) return QWEN_OK;
+    if (plan.shares == plan.beside) return QWEN_OK;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(plan.shares, qb::ta::join_blocks<D, ROWS, ACROSS>());
     cfg.blockDim = dim3(qb::ta::kJoinThreads);
@@ -205,7 +207,7 @@ int join_launch(const qb::ta::Params& P, const Plan& plan, cudaStream_t st) {
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    CU(cudaLaunchKernelEx(&cfg, qb::ta::combine_kernel<QT, KT, D, ROWS, ACROSS>, P, plan.row_blocks));
+    CU(cudaLaunchKernelEx(&cfg, qb::ta::combine_kernel<QT, KT, COST, D, ROWS, ACROSS>, P));
     return QWEN_OK;
 }
 template <int QT, int STORE, int D, int MT>
@@ -214,9 +216,9 @@ int attention_launch(const qb::ta::Params& P, const Plan& plan, int dev, cudaStr
     static std::atomic<uint64_t> done{0};
     auto kernel = qb::ta::attention_kernel<QT, STORE, D, MT>;
     TRY(smem_limit(kernel, done, dev, L::kSmem));
-    kernel<<<plan.shares, qb::ta::kThreads, L::kSmem, st>>>(P, plan.row_blocks);
+    kernel<<<plan.shares, qb::ta::kThreads, L::kSmem, st>>>(P);
     CU(cudaGetLastError());
-    return join_launch<QT, L::KT, D, L::kRows, false>(P, plan, st);
+    return join_launch<QT, L::KT, qb::ta::kItemCost, D, L::kRows, false>(P, plan, st);
 }
 template <int QT, int STORE, int D>
 int attention_tc_launch(const qb::ta::Params& P, const Plan& plan, int dev, cudaStream_t st) {
@@ -224,9 +226,9 @@ int attention_tc_launch(const qb::ta::Params& P, const Plan& plan, int dev, cuda
     static std::atomic<uint64_t> done{0};
     auto kernel = qb::ta::attention_tc_kernel<QT, STORE, D>;
     TRY(smem_limit(kernel, done, dev, L::kSmem));
-    kernel<<<plan.shares, qb::ta::kTcThreads, L::kSmem, st>>>(P, plan.row_blocks);
+    kernel<<<plan.shares, qb::ta::kTcThreads, L::kSmem, st>>>(P);
     CU(cudaGetLastError());
-    return join_launch<QT, qb::ta::kTcKT, D, qb::ta::kTcRows, true>(P, plan, st);
+    return join_launch<QT, qb::ta::kTcKT, qb::ta::kTcItemCost, D, qb::ta::kTcRows, true>(P, plan, st);
 }
 template <int QT, int STORE, int D>
 int attention_by_rows(const qb::ta::Params& P, const Plan& plan, int dev, cudaStream_t st) {
@@ -365,6 +367,8 @@ extern "C" int qwen_tree_attention(const qwen_kv_cache_t* cache, const void* q, 
     P.n_kv_heads = cache->n_kv_heads;
     P.group = n_heads / cache->n_kv_heads;
     P.n_nodes = n_nodes;
+    P.row_blocks = plan.row_blocks;
+    P.beside = plan.beside;
     P.scale_log2 = scale * 1.4426950408889634f;
     const cudaStream_t st = (cudaStream_t)stream;
     const int dim = cache->head_dim;

@@ -8,13 +8,16 @@
 // the scores); O += P V with P = 2^(score - m), scaled down when m rises.
 //
 // The rows of a work item are the n_nodes * group (query head, node) pairs that
-// share a K/V head, so each K/V byte is read once for all of them.  The items
-// (sequence, K/V head, block of rows) are laid end to end in units of key tiles, and
-// CTA i takes the i-th of G equal shares of that line: ragged lengths balance
-// by themselves, and a single long sequence spreads over all SMs.  An item that
-// crosses a share's border leaves partial (m, l, O) in the workspace, two slots a
-// CTA, and combine_kernel joins them in the order of the keys, so results do not
-// depend on timing.  The shares are computed on the device from lens.
+// share a K/V head, or a block of them, so each K/V byte is read once for all of
+// them.  The items (sequence, K/V head) are laid end to end on a line of key tiles, each
+// with a few positions more for its fixed cost, and the line is cut into equal
+// shares, one a CTA: ragged lengths balance by themselves, and a single long
+// sequence spreads over all SMs.  Where a K/V head's rows take several blocks, as many
+// CTAs as blocks walk the same share side by side, so that the tiles come from
+// the memory once and for the others from the L2.  An item that crosses a border
+// between shares leaves partial (m, l, O) in the workspace, two slots a CTA, and
+// combine_kernel joins them in the order of the keys, so results do not depend on
+// timing.  The shares are computed on the device from lens.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -36,6 +39,7 @@ struct Params {
     float* work;
     long long ldq, ldo;
     int n_seqs, n_kv_heads, group, n_nodes;
+    int row_blocks, beside;   // blocks of rows that a K/V head has; CTAs side by side on a share (row_blocks, or 1 where that is more than the grid)
     float scale_log2;   // scale * log2(e)
 };
 
@@ -47,23 +51,27 @@ __device__ __forceinline__ int seq_end(const Params& P, int len) {
 template <int KT>
 __device__ __forceinline__ int seq_tiles(const Params& P, int len) { return max(1, (seq_end(P, len) + KT - 1) / KT); }
 
-// All lanes of a warp: the number of tiles on the line, units = items per sequence.
-template <int KT>
-__device__ __forceinline__ long long line_tiles(const Params& P, int units) {
+// Positions of an item on the line: its tiles and COST for what every item costs.
+template <int KT, int COST>
+__device__ __forceinline__ int seq_line(const Params& P, int len) { return seq_tiles<KT>(P, len) + COST; }
+
+// All lanes of a warp: the line's length, units = items per sequence.
+template <int KT, int COST>
+__device__ __forceinline__ long long line_length(const Params& P, int units) {
     long long n = 0;
-    for (int s = threadIdx.x & 31; s < P.n_seqs; s += 32) n += seq_tiles<KT>(P, P.lens[s]);
+    for (int s = threadIdx.x & 31; s < P.n_seqs; s += 32) n += seq_line<KT, COST>(P, P.lens[s]);
     #pragma unroll
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(~0u, n, o);
     return n * units;
 }
-// All lanes of a warp: the sequence that tile x of the line belongs to, and the
-// tiles before it.  x is below line_tiles.
-template <int KT>
+// All lanes of a warp: the sequence that position x of the line belongs to, and
+// the positions before it.  x is below line_length.
+template <int KT, int COST>
 __device__ __forceinline__ int line_find(const Params& P, int units, long long x, long long& before) {
     const int lane = threadIdx.x & 31;
     before = 0;
     for (int s0 = 0; s0 < P.n_seqs; s0 += 32) {
-        const long long n = s0 + lane < P.n_seqs ? (long long)seq_tiles<KT>(P, P.lens[s0 + lane]) * units : 0;
+        const long long n = s0 + lane < P.n_seqs ? (long long)seq_line<KT, COST>(P, P.lens[s0 + lane]) * units : 0;
         long long inc = n;
         #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -84,14 +92,66 @@ __device__ __forceinline__ int line_find(const Params& P, int units, long long x
 __device__ __forceinline__ long long quotient(long long a, long long b) {
     return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
 }
-// The line cut into G shares: share i begins at tile i * tiles / G (rounded down).
+// The line cut into G shares: share i begins at position i * n / G (rounded down).
 struct Shares {
-    long long tiles, whole;
+    long long n, whole;
     uint32_t rest, G;
-    __device__ __forceinline__ Shares(long long n, int g) : tiles(n), whole(quotient(n, g)), rest((uint32_t)(n - whole * g)), G((uint32_t)g) {}
+    __device__ __forceinline__ Shares(long long length, int g)
+        : n(length), whole(quotient(length, g)), rest((uint32_t)(length - whole * g)), G((uint32_t)g) {}
     __device__ __forceinline__ long long begin(int i) const { return whole * i + (rest * (uint32_t)i) / G; }   // rest * i < G^2
-    // the share that tile x lies in: the last one that begins at x or before
-    __device__ __forceinline__ int of(long long x) const { return (int)quotient((x + 1) * G - 1, tiles); }
+    // the share that position x lies in: the last one that begins at x or before
+    __device__ __forceinline__ int of(long long x) const { return (int)quotient((x + 1) * G - 1, n); }
+};
+
+// This CTA's share of the line, item after item.
+template <int KT, int COST, int ROWS>
+struct Items {
+    long long at, to, before;
+    int seq, len, end, n, unit_blocks, units, beside, step;
+    int h, r_base, t0, t1;   // the item's K/V head, first row, tiles t0 .. t1-1 of n
+    bool first;              // the share's first item: it holds the share's beginning
+
+    __device__ __forceinline__ void item(const Params& P) {
+        len = P.lens[seq];
+        end = seq_end(P, len);
+        n = seq_tiles<KT>(P, len);
+        const int per = n + COST, unit = (int)quotient(at - before, per), v0 = (int)((at - before) - (long long)unit * per);
+        const int v1 = (int)min((long long)per, v0 + (to - at));
+        step = v1 - v0;
+        t0 = max(0, v0 - COST);
+        t1 = v1 - COST;
+        h = unit_blocks == 1 ? unit : unit / unit_blocks;
+        r_base = (unit - h * unit_blocks + (int)blockIdx.x % beside) * ROWS;
+    }
+    __device__ __forceinline__ bool advance(const Params& P) {
+        at += step;
+        first = false;
+        if (at >= to) return false;
+        if (at - before == (long long)(n + COST) * units) { before = at; seq++; }
+        item(P);
+        return true;
+    }
+    // the next item that has tiles in the share
+    __device__ __forceinline__ bool next(const Params& P) {
+        do {
+            if (!advance(P)) return false;
+        } while (t1 <= t0);
+        return true;
+    }
+    // all lanes of a warp; false: nothing to do
+    __device__ __forceinline__ bool start(const Params& P) {
+        beside = P.beside;
+        unit_blocks = beside == 1 ? P.row_blocks : 1;
+        units = P.n_kv_heads * unit_blocks;
+        const Shares shares(line_length<KT, COST>(P, units), gridDim.x / beside);
+        at = shares.begin(blockIdx.x / beside);
+        to = shares.begin(blockIdx.x / beside + 1);
+        if (at >= to) return false;
+        seq = line_find<KT, COST>(P, units, at, before);
+        first = true;
+        item(P);
+        return t1 > t0 || next(P);
+    }
 };
 
 // ---- the tree --------------------------------------------------------------------
@@ -199,6 +259,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) { return BF ? cvt_
 // fp16.  P is rounded to 16 bits (half a step: 2^-9 or 2^-12 relative) as
 // the product with V takes it; l sums it unrounded.
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kStages = 3;
+constexpr int kItemCost = 2;   // what an item costs beside its tiles, in tiles: set-up, queries, joining the warps
 
 template <int STORE, int D, int MT>
 struct Layout {
@@ -229,10 +290,9 @@ __device__ __forceinline__ int swz(int r, int c) {
     else return r * ROW + ((c ^ ((r >> 1) & 3)) << 4);
 }
 
-// grid G (shares), kThreads threads, Layout::kSmem bytes.  row_blocks: blocks of
-// kRows rows an item's K/V head has.
+// grid: a CTA for each share and block of rows beside it, kThreads threads, Layout::kSmem bytes.
 template <int QT, int STORE, int D, int MT>
-__global__ void __launch_bounds__(kThreads, 2) attention_kernel(const Params P, int row_blocks) {
+__global__ void __launch_bounds__(kThreads, 2) attention_kernel(const Params P) {
     using L = Layout<STORE, D, MT>;
     constexpr bool BF = QT == QWEN_BF16 && !L::k8;       // type of the products
     constexpr int KW = L::KW, NT = KW / 8, DT = D / 8, KS = D / 16;
@@ -244,21 +304,11 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const Params P, 
     pdl_wait();
     pdl_launch_dependents();   // after the wait: what the joining kernel reads early (lens) is then complete
 
-    const int units = P.n_kv_heads * row_blocks, G = gridDim.x;
-    const long long tiles = line_tiles<L::KT>(P, units);
-    const Shares shares(tiles, G);
-    long long at = shares.begin(blockIdx.x);
-    const long long to = shares.begin(blockIdx.x + 1);
-    if (at >= to) return;
-    long long before;
-    int seq = line_find<L::KT>(P, units, at, before);
-    bool first_item = true;
+    Items<L::KT, kItemCost, L::kRows> it;
+    if (!it.start(P)) return;
     const int M = P.n_nodes * P.group;
-    while (at < to) {
-        const int len = P.lens[seq], end = seq_end(P, len), n = seq_tiles<L::KT>(P, len);
-        const int unit = (int)quotient(at - before, n), t0 = (int)((at - before) - (long long)unit * n);
-        const int t1 = (int)min((long long)n, t0 + (to - at));
-        const int h = unit / row_blocks, r_base = (unit - h * row_blocks) * L::kRows;
+    do {
+        const int seq = it.seq, len = it.len, end = it.end, h = it.h, r_base = it.r_base, t0 = it.t0, t1 = it.t1;
         const size_t head = (size_t)seq * P.cache.seq_stride + (size_t)h * P.cache.head_stride;
         const uint8_t *kb = P.cache.k + head * L::kEs, *vb = P.cache.v + head * L::kEs;
         const float *ksb = L::k8 ? P.cache.ks + head / D : nullptr, *vsb = L::k8 ? P.cache.vs + head / D : nullptr;
@@ -592,8 +642,8 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const Params P, 
                 }
         }
         __syncthreads();
-        const bool whole = t0 == 0 && t1 == n;
-        float* slot = P.work + (size_t)(2 * blockIdx.x + (first_item ? 0 : 1)) * L::kSlot;
+        const bool whole = t0 == 0 && t1 == it.n;
+        float* slot = P.work + (size_t)(2 * blockIdx.x + (it.first ? 0 : 1)) * L::kSlot;
         for (int i = tid; i < L::kRows * (D / 4); i += kThreads) {
             const int r = i / (D / 4), d = i % (D / 4) * 4, row = r_base + r;
             if (row >= M) break;
@@ -622,50 +672,46 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const Params P, 
             }
         }
         __syncthreads();
-        first_item = false;
-        at += t1 - t0;
-        if (at < to && at - before == (long long)n * units) { before = at; seq++; }
-    }
+    } while (it.next(P));
 }
 
 // Joins the partial results of the items that cross a border between shares:
-// blocks (i, y) take the item that begins in share i and goes on in share i + 1.
+// blocks (i, y) take the item that begins in CTA i's share and goes on in the next.
 // ACROSS: a slot holds O as [dim / 4][row] (the tensor-memory kernel: a thread a
-// row) and a thread here joins 16 dims of a row, lanes along the rows; otherwise O
+// row) and a thread here joins 8 dims of a row, lanes along the rows; otherwise O
 // is [row][dim] and a thread joins 4 dims, lanes along the dims.
 constexpr int kJoinThreads = 128;
 template <int D, int ROWS, bool ACROSS>
-__host__ __device__ constexpr int join_blocks() { return ROWS * (ACROSS ? D / 16 : D / 4) / kJoinThreads; }
-template <int QT, int KT, int D, int ROWS, bool ACROSS>
-__global__ void __launch_bounds__(kJoinThreads) combine_kernel(const Params P, int row_blocks) {
-    constexpr int kSlot = ROWS * (D + 2), kVec = ACROSS ? 4 : 1, kAhead = ACROSS ? 4 : 8;   // float4s a thread; partial results loaded at once
-    const int i = blockIdx.x, G = gridDim.x, units = P.n_kv_heads * row_blocks;
-    const long long tiles = line_tiles<KT>(P, units);
-    const Shares shares(tiles, G);
+__host__ __device__ constexpr int join_blocks() { return ROWS * (ACROSS ? D / 8 : D / 4) / kJoinThreads; }
+template <int QT, int KT, int COST, int D, int ROWS, bool ACROSS>
+__global__ void __launch_bounds__(kJoinThreads) combine_kernel(const Params P) {
+    constexpr int kSlot = ROWS * (D + 2), kVec = ACROSS ? 2 : 1, kAhead = 8;   // float4s a thread; partial results loaded at once
+    const int beside = P.beside, unit_blocks = beside == 1 ? P.row_blocks : 1, units = P.n_kv_heads * unit_blocks;
+    const int i = blockIdx.x / beside, lane = blockIdx.x - i * beside;
+    const Shares shares(line_length<KT, COST>(P, units), gridDim.x / beside);
     const long long from = shares.begin(i), edge = shares.begin(i + 1);
-    long long before = 0, s = edge, e = edge;   // the item at the border: its tiles
+    long long before = 0, s = edge, e = edge;   // the item at the border: its positions
     int seq = 0, unit = 0;
-    if (edge > from && edge < tiles) {
-        seq = line_find<KT>(P, units, edge, before);
-        const int n = seq_tiles<KT>(P, P.lens[seq]);
-        unit = (int)quotient(edge - before, n);
-        s = before + (long long)unit * n;
-        e = s + n;
+    if (edge > from && edge < shares.n) {
+        seq = line_find<KT, COST>(P, units, edge, before);
+        const int per = seq_line<KT, COST>(P, P.lens[seq]);
+        unit = (int)quotient(edge - before, per);
+        s = before + (long long)unit * per;
+        e = s + per;
     }
     pdl_wait();   // on every path: this kernel may not end before the one that it joins
     if (s >= edge || s < from) return;          // it begins at the border, or before this share
-    const int last = shares.of(e - 1);
+    const int begun = shares.of(s + COST), last = shares.of(e - 1);   // the shares with its tiles
+    if (begun == last) return;                  // one has them all and has written the rows
     const int t = blockIdx.y * kJoinThreads + threadIdx.x;
-    const int h = unit / row_blocks, r = ACROSS ? t % ROWS : t / (D / 4), d = ACROSS ? t / ROWS * 16 : t % (D / 4) * 4;
-    const int row = (unit - h * row_blocks) * ROWS + r;
+    const int h = unit / unit_blocks, r = ACROSS ? t % ROWS : t / (D / 4), d = ACROSS ? t / ROWS * 8 : t % (D / 4) * 4;
+    const int row = (unit - h * unit_blocks + lane) * ROWS + r;
     if (row >= P.n_nodes * P.group) return;
-    // share i holds the item last (its second slot) unless it begins with it
-    const size_t first_slot = 2 * (size_t)i + (from < s ? 1 : 0);
     float mm = -INFINITY, ll = 0.f;
     float4 a[kVec];
     #pragma unroll
     for (int v = 0; v < kVec; v++) a[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k0 = i; k0 <= last; k0 += kAhead) {
+    for (int k0 = begun; k0 <= last; k0 += kAhead) {
         float2 ml[kAhead];
         float4 b[kAhead][kVec];
         #pragma unroll
@@ -674,8 +720,9 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(const Params P, i
             ml[j] = make_float2(-INFINITY, 0.f);
             #pragma unroll
             for (int v = 0; v < kVec; v++) b[j][v] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (k > last || (k > i && shares.whole == 0 && shares.begin(k) == shares.begin(k + 1))) continue;   // (a share without a tile)
-            const float* slot = P.work + (k == i ? first_slot : 2 * (size_t)k) * kSlot;
+            if (k > last || (shares.whole == 0 && shares.begin(k) == shares.begin(k + 1))) continue;   // (an empty share)
+            // a share that begins before the item holds it in its second slot
+            const float* slot = P.work + (2 * ((size_t)k * beside + lane) + (k == i && from < s ? 1 : 0)) * kSlot;
             ml[j] = *reinterpret_cast<const float2*>(slot + ROWS * D + 2 * r);
             #pragma unroll
             for (int v = 0; v < kVec; v++) b[j][v] = *reinterpret_cast<const float4*>(ACROSS ? slot + ((d / 4 + v) * ROWS + r) * 4 : slot + r * D + d);

@@ -113,43 +113,11 @@ __device__ __forceinline__ bool mbar_spin(uint64_t* bar, uint32_t parity, uint64
     }
 }
 
-// A share of the line, item after item; every role walks it alike.
-struct Items {
-    long long at, to, before;
-    int seq, len, end, n, h, r_base, t0, t1, units, row_blocks;
-    // all lanes of a warp; false: nothing to do
-    __device__ __forceinline__ bool start(const Params& P, int blocks) {
-        row_blocks = blocks;
-        units = P.n_kv_heads * blocks;
-        const Shares shares(line_tiles<kTcKT>(P, units), gridDim.x);
-        at = shares.begin(blockIdx.x);
-        to = shares.begin(blockIdx.x + 1);
-        if (at >= to) return false;
-        seq = line_find<kTcKT>(P, units, at, before);
-        return true;
-    }
-    __device__ __forceinline__ void item(const Params& P) {
-        len = P.lens[seq];
-        end = seq_end(P, len);
-        n = seq_tiles<kTcKT>(P, len);
-        const int unit = (int)quotient(at - before, n);
-        t0 = (int)((at - before) - (long long)unit * n);
-        t1 = (int)min((long long)n, t0 + (to - at));
-        h = unit / row_blocks;
-        r_base = (unit - h * row_blocks) * kTcRows;
-    }
-    __device__ __forceinline__ bool next() {
-        at += t1 - t0;
-        if (at >= to) return false;
-        if (at - before == (long long)n * units) { before = at; seq++; }
-        return true;
-    }
-};
+constexpr int kTcItemCost = 3;   // what an item costs beside its tiles, in tiles: queries, first products, rows out
 
-// grid G (shares; one CTA an SM), kTcThreads threads, TcLayout::kSmem bytes.
-// row_blocks: blocks of kTcRows rows that a K/V head has.
+// grid: a CTA (one an SM) for each share and block of rows beside it, kTcThreads threads, TcLayout::kSmem bytes.
 template <int QT, int STORE, int D>
-__global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Params P, int row_blocks) {
+__global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Params P) {
     using L = TcLayout<STORE, D>;
     using namespace qb::tc;
     constexpr bool BF = QT == QWEN_BF16 && !L::k8;
@@ -195,8 +163,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
         if (ok && !mbar_spin(bar, parity, kWaitNs)) { ok = false; *fault = 1; }
         return ok;
     };
-    Items it;
-    const bool busy = it.start(P, row_blocks);   // the same for the whole CTA
+    Items<kTcKT, kTcItemCost, kTcRows> it;       // every role walks it alike
+    const bool busy = it.start(P);   // the same for the whole CTA
     if (busy && warp >= kProducer && warp < kIssuer) {
         // ---------------- producers ----------------
         const int pt = tid - 32 * kProducer;
@@ -209,7 +177,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
             return wait(&empty[p % L::kRing], (p / L::kRing - 1) & 1u);
         };
         do {
-            it.item(P);
             const size_t head = (size_t)it.seq * P.cache.seq_stride + (size_t)it.h * P.cache.head_stride;
             const uint8_t* base[2] = {P.cache.k + head * (L::k8 ? 1 : 2), P.cache.v + head * (L::k8 ? 1 : 2)};
             if constexpr (!L::k8) {
@@ -335,7 +302,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                 tile += it.t1 - it.t0;
             }
             item++;
-        } while (ok && it.next());
+        } while (ok && it.next(P));
         cp_async_wait<0>();
         if (ok) for (; unsaid; unsaid--) say(part - unsaid);
     } else if (busy && warp == kIssuer) {
@@ -345,7 +312,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
         uint32_t steps[2] = {0, 0};   // tiles of a buffer so far
         bool going = true;
         do {
-            it.item(P);
             // every softmax thread has taken what it needs of the item before's masks (it announced that item's queries after)
             tree_masks(P, it.seq, it.len, anc, reinterpret_cast<int8_t*>(smem + L::kUp));
             named_bar(1, kTcSoftmax + 32);
@@ -388,7 +354,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
             }
             __syncwarp();
             item++;
-        } while (it.next());
+        } while (it.next(P));
         if (lane == 0) {
             mma_commit(drained);
             if (!mbar_wait(drained, 0, kWaitNs)) *fault = 1;
@@ -403,9 +369,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
         const bool flip = P.scale_log2 < 0.f;                              // a negative scale: its sign goes to the queries
         uint32_t item = 0, steps = 0, tile = 0;
         uint32_t uses[2] = {0, 0};                                         // tiles of a buffer so far
-        bool first_item = true;
         do {
-            it.item(P);
             const int nt = it.t1 - it.t0;
             // (the item before's products are done: its queries' place is free)
             const int row = it.r_base + rl;
@@ -561,6 +525,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                 uses[b]++;
             }
             tile += nt;
+            {   // the next item's queries on their way while the last products run
+                auto nx = it;
+                if (nx.next(P)) {
+                    const int nrow = nx.r_base + rl, nnode = nrow / P.group;
+                    if (nrow < M)
+                        asm volatile("prefetch.global.L1 [%0];" ::"l"(P.q + (((size_t)nx.seq * P.n_nodes + nnode) * (size_t)P.ldq +
+                                                                             (size_t)(nx.h * P.group + nrow - nnode * P.group) * D + half * (D / 2)) * 2));
+                }
+            }
             // ---- the item's rows: this thread's half of the dims ----
             {
                 const int b = (nt - 1) & 1;
@@ -574,7 +547,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
             const bool odd_rows = odd[item & 7] != 0;                      // (every part of the item has been announced)
             const bool whole = it.t0 == 0 && it.t1 == it.n, present = see != 0, failed = *fault != 0;
             const float inv = !present || l == 0.f ? 0.f : 1.0f / l;
-            float* slot = P.work + (size_t)(2 * blockIdx.x + (first_item ? 0 : 1)) * L::kSlot;
+            float* slot = P.work + (size_t)(2 * blockIdx.x + (it.first ? 0 : 1)) * L::kSlot;
             #pragma unroll 1
             for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 32) {
                 float o[32];
@@ -615,22 +588,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
             }
             if (whole) {                          // the same for all
                 named_bar(2, kTcSoftmax);
-                constexpr int kChunks = D / 8, kStep = kTcSoftmax / kChunks;
-                const int ch = tid % kChunks;
-                #pragma unroll 2
-                for (int r = tid / kChunks; r < kTcRows; r += kStep) {
-                    const int orow = it.r_base + r;
-                    if (orow >= M) break;
-                    const int onode = orow / P.group, ohq = it.h * P.group + orow - onode * P.group;
-                    *reinterpret_cast<uint4*>(P.out + (((size_t)it.seq * P.n_nodes + onode) * (size_t)P.ldo + (size_t)ohq * D + ch * 8) * 2) =
-                        *reinterpret_cast<const uint4*>(smem + L::kQ + swz<D * 2>(r, ch));
+                constexpr int kChunks = D / 8, kStep = kTcSoftmax / kChunks, kPer = kTcRows / kStep;
+                const int ch = tid % kChunks, r0 = tid / kChunks;
+                uint4 w[kPer];
+                #pragma unroll
+                for (int i = 0; i < kPer; i++) w[i] = *reinterpret_cast<const uint4*>(smem + L::kQ + swz<D * 2>(r0 + i * kStep, ch));
+                uint8_t* out = P.out + ((size_t)it.seq * P.n_nodes * (size_t)P.ldo + (size_t)it.h * P.group * D + ch * 8) * 2;
+                #pragma unroll
+                for (int i = 0; i < kPer; i++) {
+                    const int orow = it.r_base + r0 + i * kStep, onode = orow / P.group;
+                    if (orow < M) *reinterpret_cast<uint4*>(out + ((size_t)onode * (size_t)P.ldo + (size_t)(orow - onode * P.group) * D) * 2) = w[i];
                 }
                 named_bar(2, kTcSoftmax);         // the queries' place is free again
             }
             tc_fence_before();
-            first_item = false;
             item++;
-        } while (it.next());
+        } while (it.next(P));
     }
     tc_fence_before();
     __syncthreads();
