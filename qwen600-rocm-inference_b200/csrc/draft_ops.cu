@@ -131,9 +131,13 @@ template <int R, int S, int D>
 struct Append {
     static int go(const qwen_kv_cache_t* c, const void* k, const void* v, long long ld, int n_tokens, const int* start, const int* counts,
                   cudaStream_t st) {
+        // blocks of one head's tokens where a head has as many tokens as a block takes (measured at 16 x 2048 tokens, bf16 to int8:
+        // 38 us against 44 with rows in one order; 3 x 517 tokens: 6.0 us against 5.2)
         const unsigned rows = (unsigned)c->n_kv_heads * (unsigned)n_tokens, per = qb::kv::Place<D>::kRows;
-        qb::kv::append_kernel<R, S, D><<<dim3((rows + per - 1) / per, c->n_seqs, 2), qb::kv::kThreads, 0, st>>>(
-            device_view(c), (const uint8_t*)k, (const uint8_t*)v, ld, c->n_kv_heads, n_tokens, start, counts);
+        const bool two = n_tokens >= 2 * (int)per && (double)rows * c->n_seqs >= 4096.0 * per;   // (and every SM gets several blocks)
+        const dim3 grid(two ? (unsigned)c->n_kv_heads * ((n_tokens + 2 * per - 1) / (2 * per)) : (rows + per - 1) / per, c->n_seqs, 2);
+        const auto kernel = two ? qb::kv::append_kernel<R, S, D, 2> : qb::kv::append_kernel<R, S, D, 1>;
+        kernel<<<grid, qb::kv::kThreads, 0, st>>>(device_view(c), (const uint8_t*)k, (const uint8_t*)v, ld, c->n_kv_heads, n_tokens, start, counts);
         CU(cudaGetLastError());
         return QWEN_OK;
     }
@@ -313,14 +317,14 @@ extern "C" int qwen_kv_keep(const qwen_kv_cache_t* cache, const int* start, cons
     TRY(check_view(cache));
     if (n_nodes < 1 || n_nodes > qb::kv::kMaxNodes) return fail(QWEN_E_ARG, "n_nodes out of [1, 64]");
     TRY(check_ptrs({QB_VIEW_PTRS(cache), {start, "start", 4, true}, {path, "path", 4, true}, {n_path, "n_path", 4, true}}, &dev));
-    const dim3 grid(cache->n_kv_heads, cache->n_seqs);
+    const dim3 grid((cache->n_kv_heads + qb::kv::kKeepHeads - 1) / qb::kv::kKeepHeads, cache->n_seqs);
     const auto c = device_view(cache);
     const cudaStream_t st = (cudaStream_t)stream;
     const bool k8 = is8(cache->dtype), wide = cache->head_dim == 128;
-    if (k8 && wide) qb::kv::keep_kernel<128, true><<<grid, qb::kv::kKeepThreads, 0, st>>>(c, start, path, n_path, n_nodes, 1);
-    else if (k8) qb::kv::keep_kernel<64, true><<<grid, qb::kv::kKeepThreads, 0, st>>>(c, start, path, n_path, n_nodes, 1);
-    else if (wide) qb::kv::keep_kernel<256, false><<<grid, qb::kv::kKeepThreads, 0, st>>>(c, start, path, n_path, n_nodes, 2);
-    else qb::kv::keep_kernel<128, false><<<grid, qb::kv::kKeepThreads, 0, st>>>(c, start, path, n_path, n_nodes, 2);
+    if (k8 && wide) qb::kv::keep_kernel<128, true><<<grid, qb::kv::kKeepThreads, 0, st>>>(c, start, path, n_path, cache->n_kv_heads, n_nodes, 1);
+    else if (k8) qb::kv::keep_kernel<64, true><<<grid, qb::kv::kKeepThreads, 0, st>>>(c, start, path, n_path, cache->n_kv_heads, n_nodes, 1);
+    else if (wide) qb::kv::keep_kernel<256, false><<<grid, qb::kv::kKeepThreads, 0, st>>>(c, start, path, n_path, cache->n_kv_heads, n_nodes, 2);
+    else qb::kv::keep_kernel<128, false><<<grid, qb::kv::kKeepThreads, 0, st>>>(c, start, path, n_path, cache->n_kv_heads, n_nodes, 2);
     CU(cudaGetLastError());
     return QWEN_OK;
 }

@@ -40,33 +40,35 @@ struct Cache {
     int capacity;
 };
 
-// 16 consecutive elements as fp32
-template <int T>
-__device__ __forceinline__ void load16(const uint8_t* p, float (&x)[16]) {
-    if constexpr (T == QWEN_FP32) {
+// 16 consecutive elements as fp32: from 2 (16 bits) or 4 pieces of 16 bytes, from memory
+template <int T, int N>
+__device__ __forceinline__ void unpack16(const uint4 (&raw)[N], float (&x)[16]) {
+    static_assert(N == (T == QWEN_FP32 ? 4 : 2), "16 elements");
+    #pragma unroll
+    for (int i = 0; i < N; i++) {
+        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
         #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(p) + i);
-            x[4 * i] = a.x; x[4 * i + 1] = a.y; x[4 * i + 2] = a.z; x[4 * i + 3] = a.w;
-        }
-    } else {
-        #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint4 a = __ldg(reinterpret_cast<const uint4*>(p) + i);
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-            #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if constexpr (T == QWEN_BF16) {
-                    x[8 * i + 2 * j] = bf_lo(w[j]);
-                    x[8 * i + 2 * j + 1] = bf_hi(w[j]);
-                } else {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-                    x[8 * i + 2 * j] = f.x;
-                    x[8 * i + 2 * j + 1] = f.y;
-                }
+        for (int j = 0; j < 4; j++) {
+            if constexpr (T == QWEN_FP32) {
+                x[4 * i + j] = __uint_as_float(w[j]);
+            } else if constexpr (T == QWEN_BF16) {
+                x[8 * i + 2 * j] = bf_lo(w[j]);
+                x[8 * i + 2 * j + 1] = bf_hi(w[j]);
+            } else {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+                x[8 * i + 2 * j] = f.x;
+                x[8 * i + 2 * j + 1] = f.y;
             }
         }
     }
+}
+template <int T>
+__device__ __forceinline__ void load16(const uint8_t* p, float (&x)[16]) {
+    constexpr int kN = T == QWEN_FP32 ? 4 : 2;
+    uint4 raw[kN];
+    #pragma unroll
+    for (int i = 0; i < kN; i++) raw[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    unpack16<T>(raw, x);
 }
 __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
@@ -173,15 +175,20 @@ __device__ __forceinline__ uint4 encode16(const float (&x)[16], float a) {
 }
 
 // A thread's place: rows of one sequence in the order (head, token), 16 elements
-// of one row a thread.  grid (row blocks, n_seqs, 2: K and V).
+// of a row a thread.  grid (row blocks, n_seqs, 2: K and V).
 template <int D>
 struct Place {
     static constexpr int kLanes = D / 16;                  // threads a row
-    static constexpr int kRows = kThreads / kLanes;        // rows a block
+    static constexpr int kRows = kThreads / kLanes;        // rows that a block's threads cover at once
 };
 
-// grid (ceil(rows / kRows), n_seqs, 2); SRC rows -> STORE cache.
-template <int SRC, int STORE, int D>
+// SRC rows -> STORE cache.  A quantised row costs its thread's arithmetic more
+// issue slots than its bytes cost the memory, so the number of other
+// instructions counts.  U = 1: any number of tokens, threads over the rows in the
+// order (head, token), a division a row; grid (ceil(rows / kRows), n_seqs, 2).  U = 2:
+// a block takes 2 kRows tokens of one head, two a thread; grid (heads * ceil(tokens
+// / (2 kRows)), n_seqs, 2).
+template <int SRC, int STORE, int D, int U>
 __global__ void __launch_bounds__(kThreads) append_kernel(Cache c, const uint8_t* __restrict__ k, const uint8_t* __restrict__ v, long long ld,
                                                           int n_heads, int n_tokens, const int* __restrict__ start,
                                                           const int* __restrict__ counts) {
@@ -189,35 +196,68 @@ __global__ void __launch_bounds__(kThreads) append_kernel(Cache c, const uint8_t
     const int seq = blockIdx.y, first = start[seq];
     const int live = counts ? min(counts[seq], n_tokens) : n_tokens;
     if (first < 0 || live <= 0) return;
-    const unsigned row = blockIdx.x * P::kRows + threadIdx.x / P::kLanes, part = threadIdx.x % P::kLanes;
-    const unsigned h = row / (unsigned)n_tokens, t = row - h * (unsigned)n_tokens;
-    const bool mine = h < (unsigned)n_heads && t < (unsigned)live && (long long)first + t < c.capacity;
+    const unsigned part = threadIdx.x % P::kLanes;
     constexpr int kSrc = SRC == QWEN_FP32 ? 4 : 2;
-    float x[16];
-    if (mine) {
-        const uint8_t* src = (blockIdx.z ? v : k) + (((size_t)seq * n_tokens + t) * (size_t)ld + (size_t)h * D + part * 16) * kSrc;
-        load16<SRC>(src, x);
-    }
-    const size_t at = (size_t)seq * c.seq_stride + (size_t)h * c.head_stride + ((size_t)first + t) * D;
-    uint8_t* base = blockIdx.z ? c.v : c.k;
-    if constexpr (STORE == QWEN_E4M3 || STORE == QWEN_INT8) {
-        // magnitudes as bit patterns: NaN above infinity above every number
-        uint32_t m = 0;
-        if (mine) {
-            #pragma unroll
-            for (int i = 0; i < 16; i++) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
-        }
-        #pragma unroll
-        for (int o = 1; o < P::kLanes; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (!mine) return;
-        const bool finite = m < 0x7f800000u;
-        const float a = fmaxf(__uint_as_float(m), kMinAmax);
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (finite) w = encode16<SRC, STORE>(x, a);
-        *reinterpret_cast<uint4*>(base + at + part * 16) = w;
-        if (part == 0) (blockIdx.z ? c.vs : c.ks)[at / D] = finite ? a / top_of<STORE>() : __uint_as_float(0x7fffffffu);
+    unsigned h, t;
+    if constexpr (U == 1) {
+        const unsigned row = blockIdx.x * P::kRows + threadIdx.x / P::kLanes;
+        h = row / (unsigned)n_tokens;
+        t = row - h * (unsigned)n_tokens;
     } else {
-        if (mine) store16<STORE>(base + (at + part * 16) * 2, x);
+        const unsigned blocks = ((unsigned)n_tokens + U * P::kRows - 1) / (U * P::kRows);
+        h = blockIdx.x / blocks;
+        t = (blockIdx.x - h * blocks) * (U * P::kRows) + threadIdx.x / P::kLanes;
+    }
+    const uint8_t* src = (blockIdx.z ? v : k) + (((size_t)seq * n_tokens + t) * (size_t)ld + (size_t)h * D + part * 16) * kSrc;
+    const size_t at0 = (size_t)seq * c.seq_stride + (size_t)h * c.head_stride + ((size_t)first + t) * D;
+    uint8_t* base = blockIdx.z ? c.v : c.k;
+    uint4 raw[U][kSrc];
+    bool mine[U];
+    #pragma unroll
+    for (int u = 0; u < U; u++) {
+        const unsigned tu = t + u * P::kRows;
+        mine[u] = h < (unsigned)n_heads && tu < (unsigned)live && (long long)first + tu < c.capacity;
+        if (mine[u]) {
+            #pragma unroll
+            for (int i = 0; i < kSrc; i++) raw[u][i] = __ldg(reinterpret_cast<const uint4*>(src + (size_t)u * P::kRows * (size_t)ld * kSrc) + i);
+        }
+    }
+    #pragma unroll
+    for (int u = 0; u < U; u++) {
+        const size_t at = at0 + (size_t)u * P::kRows * D;
+        float x[16];
+        if (mine[u]) unpack16<SRC>(raw[u], x);
+        if constexpr (STORE == QWEN_E4M3 || STORE == QWEN_INT8) {
+            // magnitudes as bit patterns: NaN above infinity above every number
+            uint32_t m = 0;
+            if (mine[u]) {
+                if constexpr (SRC == QWEN_FP32) {
+                    #pragma unroll
+                    for (int i = 0; i < 16; i++) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+                } else {
+                    #pragma unroll
+                    for (int i = 0; i < kSrc; i++)
+                        m = __vmaxu2(__vmaxu2(__vmaxu2(m, raw[u][i].x & 0x7fff7fffu), __vmaxu2(raw[u][i].y & 0x7fff7fffu, raw[u][i].z & 0x7fff7fffu)),
+                                     raw[u][i].w & 0x7fff7fffu);
+                    m = max(m & 0xffffu, m >> 16);
+                }
+            }
+            #pragma unroll
+            for (int o = 1; o < P::kLanes; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            if (!mine[u]) continue;
+            float a;
+            bool finite;
+            if constexpr (SRC == QWEN_FP32) { a = __uint_as_float(m); finite = m < 0x7f800000u; }
+            else if constexpr (SRC == QWEN_BF16) { a = __uint_as_float(m << 16); finite = m < 0x7f80u; }
+            else { a = __half2float(__ushort_as_half((uint16_t)m)); finite = m < 0x7c00u; }
+            a = fmaxf(a, kMinAmax);
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (finite) w = encode16<SRC, STORE>(x, a);
+            *reinterpret_cast<uint4*>(base + at + part * 16) = w;
+            if (part == 0) (blockIdx.z ? c.vs : c.ks)[at / D] = finite ? a / top_of<STORE>() : __uint_as_float(0x7fffffffu);
+        } else {
+            if (mine[u]) store16<STORE>(base + (at + part * 16) * 2, x);
+        }
     }
 }
 
@@ -257,51 +297,83 @@ __global__ void __launch_bounds__(kThreads) read_kernel(Cache c, uint8_t* __rest
     store16<DST>((blockIdx.z ? v : k) + (((size_t)seq * n_tokens + t) * (size_t)ld + (size_t)h * D + part * 16) * kDst, x);
 }
 
-// Moves the rows of a kept branch: one block per (head, sequence), all source
-// rows of K and V read before any is written, so paths may be in any order.
-// kChunks: 16-byte pieces of a row.  grid (n_heads, n_seqs).
-constexpr int kKeepThreads = 128;
+// Moves the rows of a kept branch.  A block takes kKeepHeads heads of a sequence:
+// finding the rows that move is a chain of loads that all of them share.  Of as many
+// heads as its threads hold in registers (kKeepPer pieces of 16 bytes each) all
+// source rows of K and V are read before any is written, so paths may be in any
+// order.  grid (ceil(n_heads / kKeepHeads), n_seqs).
+constexpr int kKeepThreads = 256, kKeepHeads = 8, kKeepPer = 8;
 constexpr int kMaxNodes = 64;
 template <int ROW_BYTES, bool SCALED>
 __global__ void __launch_bounds__(kKeepThreads) keep_kernel(Cache c, const int* __restrict__ start, const int* __restrict__ path,
-                                                            const int* __restrict__ n_path, int n_nodes, int elem_bytes) {
-    constexpr int kChunks = ROW_BYTES / 16, kPer = kMaxNodes * kChunks / kKeepThreads;
-    __shared__ int from[kMaxNodes];
-    const int h = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, first = start[seq];
+                                                            const int* __restrict__ n_path, int n_heads, int n_nodes, int elem_bytes) {
+    constexpr int kChunks = ROW_BYTES / 16;
+    static_assert(kMaxNodes * kChunks * 2 <= kKeepThreads * kKeepPer && kKeepPer <= 2 * kChunks, "a head's rows (and scales) fit the block's registers");
+    __shared__ int from[kMaxNodes], to[kMaxNodes], moves;
+    const int seq = blockIdx.y, tid = threadIdx.x, first = start[seq];
     const int n = min(n_path[seq], n_nodes);
     if (first < 0 || n <= 0) return;
-    if (tid < n) {
-        const int p = path[(size_t)seq * n_nodes + tid];
-        const bool fine = p >= 0 && p < n_nodes && p != tid && (long long)first + p < c.capacity && (long long)first + tid < c.capacity;
-        from[tid] = fine ? p : -1;   // a row that stays where it is moves nothing
+    if (tid < 32) {   // the rows that move, in a list (a row that stays where it is does not)
+        int have = 0;
+        #pragma unroll
+        for (int k = 0; k < kMaxNodes; k += 32) {
+            const int r = k + tid, p = r < n ? path[(size_t)seq * n_nodes + r] : -1;
+            const bool fine = p >= 0 && p < n_nodes && p != r && (long long)first + p < c.capacity && (long long)first + r < c.capacity;
+            const uint32_t some = __ballot_sync(~0u, fine);
+            if (fine) {
+                const int i = have + __popc(some & ((1u << tid) - 1));
+                from[i] = p;
+                to[i] = r;
+            }
+            have += __popc(some);
+        }
+        if (tid == 0) moves = have;
     }
     __syncthreads();
-    const size_t elem = (size_t)seq * c.seq_stride + (size_t)h * c.head_stride;   // position 0
-    const size_t row0 = elem * elem_bytes + (size_t)first * ROW_BYTES;
-    uint4 kk[kPer], vv[kPer];
-    #pragma unroll
-    for (int i = 0; i < kPer; i++) {
-        const int p = tid + i * kKeepThreads, r = p / kChunks;
-        if (r < n && from[r] >= 0) {
-            const size_t at = row0 + (size_t)from[r] * ROW_BYTES + (p % kChunks) * 16;
-            kk[i] = *reinterpret_cast<const uint4*>(c.k + at);
-            vv[i] = *reinterpret_cast<const uint4*>(c.v + at);
+    const int m = moves;
+    if (m == 0) return;
+    const int h1 = min(n_heads, (int)(blockIdx.x + 1) * kKeepHeads), per_head = 2 * kChunks * m;   // pieces of a head
+    const int batch = kKeepThreads * kKeepPer / per_head;                                          // heads at a time
+    const size_t seq0 = (size_t)seq * c.seq_stride;
+    for (int h0 = blockIdx.x * kKeepHeads; h0 < h1; h0 += batch) {
+        const int heads = min(batch, h1 - h0), pieces = heads * per_head;
+        uint4 w[kKeepPer];
+        uint8_t* dst[kKeepPer];
+        #pragma unroll
+        for (int i = 0; i < kKeepPer; i++) {
+            const int x = tid + i * kKeepThreads;
+            dst[i] = nullptr;
+            if (x < pieces) {
+                const int ch = x % kChunks, y = x / kChunks, kv = y & 1, z = y >> 1, h = z / m, r = z - h * m;
+                uint8_t* row0 = (kv ? c.v : c.k) + (seq0 + (size_t)(h0 + h) * c.head_stride) * elem_bytes + (size_t)first * ROW_BYTES + ch * 16;
+                w[i] = *reinterpret_cast<const uint4*>(row0 + (size_t)from[r] * ROW_BYTES);
+                dst[i] = row0 + (size_t)to[r] * ROW_BYTES;
+            }
+        }
+        float s[2];
+        float* sdst[2] = {nullptr, nullptr};
+        if constexpr (SCALED) {
+            // (a batch has at most kKeepThreads kKeepPer / kChunks <= 2 kKeepThreads rows)
+            #pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int x = tid + i * kKeepThreads;
+                if (x < heads * m * 2) {
+                    const int kv = x & 1, z = x >> 1, h = z / m, r = z - h * m;
+                    float* row0 = (kv ? c.vs : c.ks) + (seq0 + (size_t)(h0 + h) * c.head_stride) / (ROW_BYTES / elem_bytes) + first;
+                    s[i] = row0[from[r]];
+                    sdst[i] = row0 + to[r];
+                }
+            }
+        }
+        __syncthreads();
+        #pragma unroll
+        for (int i = 0; i < kKeepPer; i++)
+            if (dst[i]) *reinterpret_cast<uint4*>(dst[i]) = w[i];
+        if constexpr (SCALED) {
+            #pragma unroll
+            for (int i = 0; i < 2; i++) if (sdst[i]) *sdst[i] = s[i];
         }
     }
-    float ks = 0.f, vs = 0.f;
-    const size_t srow = SCALED ? elem / (ROW_BYTES / elem_bytes) + first : 0;
-    if (SCALED && tid < n && from[tid] >= 0) { ks = c.ks[srow + from[tid]]; vs = c.vs[srow + from[tid]]; }
-    __syncthreads();
-    #pragma unroll
-    for (int i = 0; i < kPer; i++) {
-        const int p = tid + i * kKeepThreads, r = p / kChunks;
-        if (r < n && from[r] >= 0) {
-            const size_t at = row0 + (size_t)r * ROW_BYTES + (p % kChunks) * 16;
-            *reinterpret_cast<uint4*>(c.k + at) = kk[i];
-            *reinterpret_cast<uint4*>(c.v + at) = vv[i];
-        }
-    }
-    if (SCALED && tid < n && from[tid] >= 0) { c.ks[srow + tid] = ks; c.vs[srow + tid] = vs; }
 }
 
 }  // namespace kv
