@@ -188,8 +188,8 @@ int attention_plan(const qwen_kv_cache_t* c, int n_nodes, int n_heads, int dev, 
     TRY(sm_count(dev, &nsm));
     p->rows = attention_rows((int)m);
     p->row_blocks = (int)((m + p->rows - 1) / p->rows);
-    // two CTAs an SM (the tensor-memory kernel: one), shared out over the blocks of rows that walk side by side
-    const int keys = p->rows <= 32 ? 64 : 128, ctas = p->rows <= 32 ? 2 * nsm : nsm;
+    // as many CTAs as the SMs hold (the tensor-memory kernel: one each), shared out over the blocks of rows that walk side by side
+    const int keys = p->rows <= 32 ? 64 : 128, ctas = p->rows <= 32 ? qb::ta::attention_ctas(p->rows) * nsm : nsm;
     p->beside = p->row_blocks <= ctas ? p->row_blocks : 1;
     // no more shares than the line can have positions
     const double most = (double)c->n_seqs * c->n_kv_heads * (p->row_blocks / p->beside) * ((c->capacity + keys - 1) / keys + qb::ta::kTcItemCost);

@@ -204,6 +204,9 @@ __device__ __forceinline__ uint64_t visible(uint64_t see, int before) {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool live) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
 }
@@ -224,18 +227,24 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
 }
-// Two 8-bit codes to an fp16 pair (exact).  The pair is bytes (B0, B1) of w.
-template <int STORE, int B0, int B1>
-__device__ __forceinline__ uint32_t codes_f16x2(uint32_t w) {
+// Four 8-bit codes to two fp16 pairs (exact): bytes (0, 1) and (2, 3) of w, or, ODD_EVEN, (0, 2) and (1, 3).
+template <int STORE, bool ODD_EVEN>
+__device__ __forceinline__ void codes_f16x2(uint32_t w, uint32_t& p, uint32_t& q) {
     if constexpr (STORE == QWEN_INT8) {
         // 0x6400 | u is 1024 + u; u = code + 128
-        const uint32_t h = __byte_perm(w ^ 0x80808080u, 0x64646464u, 0x4040u | B0 | (B1 << 8));
-        const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
-        return *reinterpret_cast<const uint32_t*>(&r);
+        const uint32_t u = w ^ 0x80808080u;
+        const __half2 k = __half2half2(__ushort_as_half(0x6480));
+        const uint32_t a = __byte_perm(u, 0x64646464u, ODD_EVEN ? 0x4240u : 0x4140u), b = __byte_perm(u, 0x64646464u, ODD_EVEN ? 0x4341u : 0x4342u);
+        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), k), y = __hsub2(*reinterpret_cast<const __half2*>(&b), k);
+        p = *reinterpret_cast<const uint32_t*>(&x);
+        q = *reinterpret_cast<const uint32_t*>(&y);
     } else {
-        uint32_t h;
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)__byte_perm(w, 0, B0 | (B1 << 4))));
-        return h;
+        const uint32_t u = ODD_EVEN ? __byte_perm(w, 0, 0x3120) : w;
+        asm("{\n\t.reg .b16 lo, hi;\n\t"
+            "mov.b32 {lo, hi}, %2;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %0, lo;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+            : "=r"(p), "=r"(q) : "r"(u));
     }
 }
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -258,9 +267,11 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) { return BF ? cvt_
 // two that is at least the largest scale so far, so the weights stay within
 // fp16.  P is rounded to 16 bits (half a step: 2^-9 or 2^-12 relative) as
 // the product with V takes it; l sums it unrounded.
-constexpr int kWarps = 4, kThreads = 32 * kWarps, kStages = 3;
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kItemCost = 2;   // what an item costs beside its tiles, in tiles: set-up, queries, joining the warps
 
+// CTAs on an SM: with 16 rows three (168 registers a thread, two stages), with 32 two (255 and three).
+__host__ __device__ constexpr int attention_ctas(int rows) { return rows <= 16 ? 3 : 2; }
 template <int STORE, int D, int MT>
 struct Layout {
     static constexpr int kEs = STORE == QWEN_E4M3 || STORE == QWEN_INT8 ? 1 : 2;
@@ -269,6 +280,8 @@ struct Layout {
     static constexpr int KW = kRow == 256 ? 16 : 32;           // keys of a warp's part of a tile
     static constexpr int KT = kWarps * KW;                     // keys of a tile
     static constexpr int kRows = 16 * MT;                      // query rows of an item
+    static constexpr int kCtas = attention_ctas(kRows);        // on an SM
+    static constexpr int kStages = kCtas == 3 ? 2 : 3;
     static constexpr int kPart = KW * kRow;                    // bytes of K (or V) of a warp's stage
     static constexpr int kScale = k8 ? 2 * KW * 4 : 0;         // its scales
     static constexpr int kStage = 2 * kPart + kScale;
@@ -281,7 +294,7 @@ struct Layout {
     static constexpr int kSmem = kQf + kRows * 4;
     static constexpr int kSlot = kRows * (D + 2);              // floats of a workspace slot: O, then (m, l) pairs
     static_assert(kRing % 16 == 0 && kJoin % 16 == 0 && kStage % 16 == 0, "rows of 16-byte pieces");
-    static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two CTAs an SM");
+    static_assert(kCtas * (kSmem + 1024) <= 228 * 1024, "kCtas CTAs an SM");
 };
 // Byte of 16-byte piece c of row r, so that 8 rows of one piece (or 8 pieces) meet no bank twice.
 template <int ROW>
@@ -292,10 +305,10 @@ __device__ __forceinline__ int swz(int r, int c) {
 
 // grid: a CTA for each share and block of rows beside it, kThreads threads, Layout::kSmem bytes.
 template <int QT, int STORE, int D, int MT>
-__global__ void __launch_bounds__(kThreads, 2) attention_kernel(const Params P) {
+__global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT)) attention_kernel(const Params P) {
     using L = Layout<STORE, D, MT>;
     constexpr bool BF = QT == QWEN_BF16 && !L::k8;       // type of the products
-    constexpr int KW = L::KW, NT = KW / 8, DT = D / 8, KS = D / 16;
+    constexpr int KW = L::KW, NT = KW / 8, DT = D / 8, KS = D / 16, kStages = L::kStages;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j = lane & 3;
     uint8_t* ring = smem + warp * kStages * L::kStage;
@@ -314,23 +327,35 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const Params P) 
         const float *ksb = L::k8 ? P.cache.ks + head / D : nullptr, *vsb = L::k8 ? P.cache.vs + head / D : nullptr;
 
         auto load = [&](int t, int s) {   // this warp's part of tile t into stage s; positions >= end as zeros
-            uint8_t* st = ring + s * L::kStage;
+            const uint32_t st = smem_addr(ring + s * L::kStage);
             const int k0 = t * L::KT + warp * KW;
-            constexpr int kChunks = L::kRow / 16, kPer = KW * kChunks / 32;
-            #pragma unroll
-            for (int i = 0; i < kPer; i++) {
-                const int c = lane + 32 * i, r = c / kChunks, p = c % kChunks;
-                const bool live = k0 + r < end;
-                const size_t off = live ? (size_t)(k0 + r) * L::kRow + p * 16 : 0;
-                cp_async16(smem_addr(st + swz<L::kRow>(r, p)), kb + off, live);
-                cp_async16(smem_addr(st + L::kPart + swz<L::kRow>(r, p)), vb + off, live);
+            // the part is KW * kRow bytes in a row: lane's piece i lies 512 i bytes on, in row r0 + kStep i; with r0 < kStep the
+            // swizzle's row bits of the two add up without a carry
+            constexpr int kChunks = L::kRow / 16, kPer = KW * kChunks / 32, kStep = 32 / kChunks;
+            const uint32_t off0 = swz<L::kRow>(lane / kChunks, lane % kChunks);
+            const uint8_t *ksrc = kb + (size_t)k0 * L::kRow + lane * 16, *vsrc = vb + (size_t)k0 * L::kRow + lane * 16;
+            if (k0 + KW <= end) {
+                #pragma unroll
+                for (int i = 0; i < kPer; i++) {
+                    const uint32_t off = (off0 ^ (L::kRow >= 128 ? ((kStep * i) & 7) << 4 : 0)) + 512 * i;
+                    cp_async16(st + off, ksrc + 512 * i);
+                    cp_async16(st + L::kPart + off, vsrc + 512 * i);
+                }
+            } else {
+                #pragma unroll
+                for (int i = 0; i < kPer; i++) {
+                    const uint32_t off = (off0 ^ (L::kRow >= 128 ? ((kStep * i) & 7) << 4 : 0)) + 512 * i;
+                    const bool live = k0 + lane / kChunks + kStep * i < end;
+                    cp_async16(st + off, live ? ksrc + 512 * i : kb, live);
+                    cp_async16(st + L::kPart + off, live ? vsrc + 512 * i : vb, live);
+                }
             }
             if constexpr (L::k8) {
                 static_assert(KW == 32, "one scale a lane");
                 const bool live = k0 + lane < end;
                 const size_t off = live ? k0 + lane : 0;
-                cp_async4(smem_addr(st + 2 * L::kPart + 4 * lane), ksb + off, live);
-                cp_async4(smem_addr(st + 2 * L::kPart + 4 * KW + 4 * lane), vsb + off, live);
+                cp_async4(st + 2 * L::kPart + 4 * lane, ksb + off, live);
+                cp_async4(st + 2 * L::kPart + 4 * KW + 4 * lane, vsb + off, live);
             }
         };
         #pragma unroll
@@ -450,7 +475,8 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const Params P) 
                         ldsm_x4(smem_addr(st + swz<L::kRow>(lane, ks)), b[0], b[1], b[2], b[3]);
                         #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            const uint32_t b0 = codes_f16x2<STORE, 0, 1>(b[i]), b1 = codes_f16x2<STORE, 2, 3>(b[i]);
+                            uint32_t b0, b1;
+                            codes_f16x2<STORE, false>(b[i], b0, b1);
                             #pragma unroll
                             for (int mt = 0; mt < MT; mt++) mma16816<BF>(s[mt][i], a[mt], b0, b1);
                         }
@@ -600,16 +626,22 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const Params P) 
                     for (int p = 0; p < L::kRow / 16; p += 2) {   // two 16-byte pieces of the 16 keys' rows
                         uint32_t b[4];
                         ldsm_x4_t(smem_addr(sv + swz<L::kRow>(16 * kk + (lane & 15), p + (lane >> 4))), b[0], b[1], b[2], b[3]);
-                        #pragma unroll
-                        for (int mt = 0; mt < MT; mt++) {
-                            if constexpr (!L::k8) {
+                        if constexpr (!L::k8) {
+                            #pragma unroll
+                            for (int mt = 0; mt < MT; mt++) {
                                 mma16816<BF>(o[mt][p], a[mt], b[0], b[1]);
                                 mma16816<BF>(o[mt][p + 1], a[mt], b[2], b[3]);
-                            } else {
+                            }
+                        } else {
+                            #pragma unroll
+                            for (int q = 0; q < 2; q++) {
+                                uint32_t e0, e1, d0, d1;   // even and odd dims of the piece, keys 0-7 and 8-15
+                                codes_f16x2<STORE, true>(b[2 * q], e0, d0);
+                                codes_f16x2<STORE, true>(b[2 * q + 1], e1, d1);
                                 #pragma unroll
-                                for (int q = 0; q < 2; q++) {
-                                    mma16816<BF>(o[mt][2 * (p + q)], a[mt], codes_f16x2<STORE, 0, 2>(b[2 * q]), codes_f16x2<STORE, 0, 2>(b[2 * q + 1]));
-                                    mma16816<BF>(o[mt][2 * (p + q) + 1], a[mt], codes_f16x2<STORE, 1, 3>(b[2 * q]), codes_f16x2<STORE, 1, 3>(b[2 * q + 1]));
+                                for (int mt = 0; mt < MT; mt++) {
+                                    mma16816<BF>(o[mt][2 * (p + q)], a[mt], e0, e1);
+                                    mma16816<BF>(o[mt][2 * (p + q) + 1], a[mt], d0, d1);
                                 }
                             }
                         }

@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                         }
                         uint32_t o[8];
                         #pragma unroll
-                        for (int e = 0; e < 4; e++) { o[2 * e] = codes_f16x2<STORE, 0, 1>(q[e]); o[2 * e + 1] = codes_f16x2<STORE, 2, 3>(q[e]); }
+                        for (int e = 0; e < 4; e++) codes_f16x2<STORE, false>(q[e], o[2 * e], o[2 * e + 1]);
                         const int ch = (2 * c) & 7;
                         *reinterpret_cast<uint4*>(dst + r * 128 + ((ch ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
                         *reinterpret_cast<uint4*>(dst + r * 128 + (((ch + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
