@@ -189,11 +189,12 @@ int attention_plan(const qwen_kv_cache_t* c, int n_nodes, int n_heads, int dev, 
     p->rows = attention_rows((int)m);
     p->row_blocks = (int)((m + p->rows - 1) / p->rows);
     // as many CTAs as the SMs hold (the tensor-memory kernel: one each), shared out over the blocks of rows that walk side by side
-    const int keys = p->rows <= 32 ? 64 : 128, ctas = p->rows <= 32 ? qb::ta::attention_ctas(p->rows) * nsm : nsm;
+    const int keys = p->rows <= 32 ? 64 : 128, ctas = p->rows <= 32 ? qb::ta::attention_ctas(p->rows, c->head_dim) * nsm : nsm;
     p->beside = p->row_blocks <= ctas ? p->row_blocks : 1;
     // no more shares than the line can have positions
     const double most = (double)c->n_seqs * c->n_kv_heads * (p->row_blocks / p->beside) * ((c->capacity + keys - 1) / keys + qb::ta::kTcItemCost);
     p->shares = (int)std::min((double)(ctas / p->beside), most) * p->beside;
+    if (most >= 2147483648.0) return fail(QWEN_E_UNSUPPORTED, "too many sequences, heads and positions for one call");
     p->bytes = (size_t)2 * p->shares * p->rows * (c->head_dim + 2) * sizeof(float);
     return QWEN_OK;
 }

@@ -51,72 +51,93 @@ __device__ __forceinline__ int seq_end(const Params& P, int len) {
 template <int KT>
 __device__ __forceinline__ int seq_tiles(const Params& P, int len) { return max(1, (seq_end(P, len) + KT - 1) / KT); }
 
-// Positions of an item on the line: its tiles and COST for what every item costs.
-template <int KT, int COST>
-__device__ __forceinline__ int seq_line(const Params& P, int len) { return seq_tiles<KT>(P, len) + COST; }
-
-// All lanes of a warp: the line's length, units = items per sequence.
-template <int KT, int COST>
-__device__ __forceinline__ long long line_length(const Params& P, int units) {
-    long long n = 0;
-    for (int s = threadIdx.x & 31; s < P.n_seqs; s += 32) n += seq_line<KT, COST>(P, P.lens[s]);
-    #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(~0u, n, o);
-    return n * units;
-}
-// All lanes of a warp: the sequence that position x of the line belongs to, and
-// the positions before it.  x is below line_length.
-template <int KT, int COST>
-__device__ __forceinline__ int line_find(const Params& P, int units, long long x, long long& before) {
-    const int lane = threadIdx.x & 31;
-    before = 0;
-    for (int s0 = 0; s0 < P.n_seqs; s0 += 32) {
-        const long long n = s0 + lane < P.n_seqs ? (long long)seq_line<KT, COST>(P, P.lens[s0 + lane]) * units : 0;
-        long long inc = n;
-        #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(~0u, inc, o);
-            if (lane >= o) inc += y;
-        }
-        const uint32_t hit = __ballot_sync(~0u, n > 0 && before + inc > x);
-        if (hit) {
-            const int l = __ffs(hit) - 1;
-            before += __shfl_sync(~0u, inc - n, l);
-            return s0 + l;
-        }
-        before += __shfl_sync(~0u, inc, 31);
-    }
-    return P.n_seqs - 1;
-}
-// a / b for a >= 0, b > 0: by 32 bits where they do (a 64-bit division takes some hundred instructions)
-__device__ __forceinline__ long long quotient(long long a, long long b) {
-    return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
-}
-// The line cut into G shares: share i begins at position i * n / G (rounded down).
+// The line cut into G shares (as many as positions at most, so that none is
+// empty): share i begins at position i * n / G (rounded down).  Positions are below
+// 2^31 (the host sees to it).
 struct Shares {
-    long long n, whole;
-    uint32_t rest, G;
-    __device__ __forceinline__ Shares(long long length, int g)
-        : n(length), whole(quotient(length, g)), rest((uint32_t)(length - whole * g)), G((uint32_t)g) {}
-    __device__ __forceinline__ long long begin(int i) const { return whole * i + (rest * (uint32_t)i) / G; }   // rest * i < G^2
+    int n, whole, rest, G;
+    __device__ __forceinline__ Shares() {}
+    __device__ __forceinline__ Shares(int length, int g) : n(length), G(min(g, length)) {
+        whole = (int)((unsigned)n / (unsigned)G);
+        rest = n - whole * G;
+    }
+    __device__ __forceinline__ int begin(int i) const { return i >= G ? n : whole * i + (int)((unsigned)(rest * i) / (unsigned)G); }   // rest * i < G^2
     // the share that position x lies in: the last one that begins at x or before
-    __device__ __forceinline__ int of(long long x) const { return (int)quotient((x + 1) * G - 1, n); }
+    __device__ __forceinline__ int of(int x) const {
+        int i = min((int)(((float)x + 0.5f) * (float)G / (float)n), G - 1);   // a guess
+        while (i + 1 < G && begin(i + 1) <= x) i++;
+        while (begin(i) > x) i--;
+        return i;
+    }
+};
+
+// The line of all items, units a sequence, by all lanes of a warp: every length
+// is loaded once, up to kHeld sequences' with one wait.
+template <int KT, int COST>
+struct Line {
+    static constexpr int kHeld = 128;
+    int len[kHeld / 32];     // sequences lane, lane + 32, ... (all of them where there are no more)
+    int units;
+    Shares shares;
+    __device__ __forceinline__ int positions(const Params& P, int s, int l) const {
+        return s < P.n_seqs ? (seq_tiles<KT>(P, l) + COST) * units : 0;
+    }
+    __device__ __forceinline__ Line(const Params& P, int items, int groups) : units(items) {
+        const int lane = threadIdx.x & 31;
+        #pragma unroll
+        for (int k = 0; k < kHeld / 32; k++) len[k] = lane + 32 * k < P.n_seqs ? P.lens[lane + 32 * k] : -1;
+        int n = 0;
+        #pragma unroll
+        for (int k = 0; k < kHeld / 32; k++) n += positions(P, lane + 32 * k, len[k]);
+        for (int s = kHeld + lane; s < P.n_seqs; s += 32) n += positions(P, s, P.lens[s]);
+        shares = Shares(__reduce_add_sync(~0u, n), groups);
+    }
+    // The sequence that position x (below shares.n) belongs to, the positions before it, its length.
+    __device__ __forceinline__ int find(const Params& P, int x, int& before, int& length) const {
+        const int lane = threadIdx.x & 31;
+        before = 0;
+        int s = P.n_seqs - 1;
+        length = -1;
+        bool found = false;
+        auto look = [&](int s0, int l) {
+            const int n = positions(P, s0 + lane, l);
+            int inc = n;
+            #pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(~0u, inc, o);
+                if (lane >= o) inc += y;
+            }
+            const uint32_t hit = __ballot_sync(~0u, n > 0 && before + inc > x);
+            if (hit) {
+                const int f = __ffs(hit) - 1;
+                before += __shfl_sync(~0u, inc - n, f);
+                length = __shfl_sync(~0u, l, f);
+                s = s0 + f;
+                found = true;
+            } else {
+                before += __shfl_sync(~0u, inc, 31);
+            }
+        };
+        #pragma unroll
+        for (int k = 0; k < kHeld / 32; k++) if (!found && 32 * k < P.n_seqs) look(32 * k, len[k]);
+        for (int s0 = kHeld; s0 < P.n_seqs && !found; s0 += 32) look(s0, s0 + lane < P.n_seqs ? P.lens[s0 + lane] : -1);
+        return s;
+    }
 };
 
 // This CTA's share of the line, item after item.
 template <int KT, int COST, int ROWS>
 struct Items {
-    long long at, to, before;
+    int at, to, before;      // positions of the line
     int seq, len, end, n, unit_blocks, units, beside, step;
     int h, r_base, t0, t1;   // the item's K/V head, first row, tiles t0 .. t1-1 of n
     bool first;              // the share's first item: it holds the share's beginning
 
     __device__ __forceinline__ void item(const Params& P) {
-        len = P.lens[seq];
         end = seq_end(P, len);
         n = seq_tiles<KT>(P, len);
-        const int per = n + COST, unit = (int)quotient(at - before, per), v0 = (int)((at - before) - (long long)unit * per);
-        const int v1 = (int)min((long long)per, v0 + (to - at));
+        const int per = n + COST, unit = (int)((unsigned)(at - before) / (unsigned)per), v0 = at - before - unit * per;
+        const int v1 = min(per, v0 + (to - at));
         step = v1 - v0;
         t0 = max(0, v0 - COST);
         t1 = v1 - COST;
@@ -127,7 +148,10 @@ struct Items {
         at += step;
         first = false;
         if (at >= to) return false;
-        if (at - before == (long long)(n + COST) * units) { before = at; seq++; }
+        if (at - before == (n + COST) * units) {
+            before = at;
+            len = P.lens[++seq];
+        }
         item(P);
         return true;
     }
@@ -143,11 +167,11 @@ struct Items {
         beside = P.beside;
         unit_blocks = beside == 1 ? P.row_blocks : 1;
         units = P.n_kv_heads * unit_blocks;
-        const Shares shares(line_length<KT, COST>(P, units), gridDim.x / beside);
-        at = shares.begin(blockIdx.x / beside);
-        to = shares.begin(blockIdx.x / beside + 1);
+        const Line<KT, COST> line(P, units, gridDim.x / beside);
+        at = line.shares.begin(blockIdx.x / beside);
+        to = line.shares.begin(blockIdx.x / beside + 1);
         if (at >= to) return false;
-        seq = line_find<KT, COST>(P, units, at, before);
+        seq = line.find(P, at, before, len);
         first = true;
         item(P);
         return t1 > t0 || next(P);
@@ -190,6 +214,49 @@ __device__ __forceinline__ void tree_masks(const Params& P, int seq, int len, ui
     for (int k = 0; k < 2; k++)
         if (up[lane + 32 * k] != kNone) anc[lane + 32 * k] = 0;
     __syncwarp();
+}
+
+// The same with the nodes' parents in registers (nodes lane and lane + 32 of a
+// warp; load_parents) and shuffles in place of shared memory.
+__device__ __forceinline__ void load_parents(const Params& P, int seq, int (&up)[2]) {
+    const int lane = threadIdx.x & 31;
+    #pragma unroll
+    for (int k = 0; k < 2; k++) up[k] = lane + 32 * k < P.n_nodes ? P.parents[(size_t)seq * P.n_nodes + lane + 32 * k] : -2;
+}
+__device__ __forceinline__ void tree_masks(const Params& P, int len, int (&up)[2], uint64_t (&see)[2]) {
+    const int lane = threadIdx.x & 31, N = P.n_nodes;
+    #pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int i = lane + 32 * k;
+        if (up[k] < -1 || up[k] >= i || len < 0 || (long long)len + i >= P.cache.capacity) up[k] = -2;
+        see[k] = 1ull << i;
+    }
+    for (int step = 1; step < N; step <<= 1) {
+        uint64_t a[2];
+        int u[2];
+        #pragma unroll
+        for (int k = 0; k < 2; k++) {
+            if (k == 1 && N <= 32) break;
+            const int p = max(up[k], 0);   // (every lane takes part in the shuffles)
+            uint64_t x = __shfl_sync(~0u, see[0], p & 31);
+            int y = __shfl_sync(~0u, up[0], p & 31);
+            if (N > 32) {
+                const uint64_t x1 = __shfl_sync(~0u, see[1], p & 31);
+                const int y1 = __shfl_sync(~0u, up[1], p & 31);
+                if (p >= 32) { x = x1; y = y1; }
+            }
+            a[k] = up[k] >= 0 ? see[k] | x : see[k];
+            u[k] = up[k] >= 0 ? y : up[k];
+        }
+        #pragma unroll
+        for (int k = 0; k < 2; k++) {
+            if (k == 1 && N <= 32) break;
+            see[k] = a[k];
+            up[k] = u[k];
+        }
+    }
+    #pragma unroll
+    for (int k = 0; k < 2; k++) if (up[k] != -1) see[k] = 0;
 }
 
 // Of the 64 positions len - before .. that begin `before` positions in front of the tree's first: bit x is set where a node that
@@ -270,8 +337,8 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) { return BF ? cvt_
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kItemCost = 2;   // what an item costs beside its tiles, in tiles: set-up, queries, joining the warps
 
-// CTAs on an SM: with 16 rows three (168 registers a thread, two stages), with 32 two (255 and three).
-__host__ __device__ constexpr int attention_ctas(int rows) { return rows <= 16 ? 3 : 2; }
+// CTAs on an SM: where O takes 64 registers a thread three (168 in all, two stages), with 32 rows of 128 dims two (255 and three).
+__host__ __device__ constexpr int attention_ctas(int rows, int dim) { return rows * dim <= 16 * 128 ? 3 : 2; }
 template <int STORE, int D, int MT>
 struct Layout {
     static constexpr int kEs = STORE == QWEN_E4M3 || STORE == QWEN_INT8 ? 1 : 2;
@@ -280,7 +347,7 @@ struct Layout {
     static constexpr int KW = kRow == 256 ? 16 : 32;           // keys of a warp's part of a tile
     static constexpr int KT = kWarps * KW;                     // keys of a tile
     static constexpr int kRows = 16 * MT;                      // query rows of an item
-    static constexpr int kCtas = attention_ctas(kRows);        // on an SM
+    static constexpr int kCtas = attention_ctas(kRows, D);        // on an SM
     static constexpr int kStages = kCtas == 3 ? 2 : 3;
     static constexpr int kPart = KW * kRow;                    // bytes of K (or V) of a warp's stage
     static constexpr int kScale = k8 ? 2 * KW * 4 : 0;         // its scales
@@ -289,8 +356,7 @@ struct Layout {
     static constexpr int kJoin = kWarps * kRows * (D + 2) * 4; // the warps' (O, m, l) at the end of an item (over the ring)
     static constexpr int kQ = kRing > kJoin ? kRing : kJoin;   // query rows, 16 bits
     static constexpr int kAnc = kQ + kRows * D * 2;            // tree masks
-    static constexpr int kUp = kAnc + kMaxNodes * 8;
-    static constexpr int kQf = kUp + kMaxNodes;                // the rows' powers of two
+    static constexpr int kQf = kAnc + kMaxNodes * 8;           // the rows' powers of two
     static constexpr int kSmem = kQf + kRows * 4;
     static constexpr int kSlot = kRows * (D + 2);              // floats of a workspace slot: O, then (m, l) pairs
     static_assert(kRing % 16 == 0 && kJoin % 16 == 0 && kStage % 16 == 0, "rows of 16-byte pieces");
@@ -305,7 +371,7 @@ __device__ __forceinline__ int swz(int r, int c) {
 
 // grid: a CTA for each share and block of rows beside it, kThreads threads, Layout::kSmem bytes.
 template <int QT, int STORE, int D, int MT>
-__global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT)) attention_kernel(const Params P) {
+__global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attention_kernel(const Params P) {
     using L = Layout<STORE, D, MT>;
     constexpr bool BF = QT == QWEN_BF16 && !L::k8;       // type of the products
     constexpr int KW = L::KW, NT = KW / 8, DT = D / 8, KS = D / 16, kStages = L::kStages;
@@ -365,51 +431,70 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT)) attention_k
         }
         // queries to shared memory, 16 bits; for 8-bit caches fp16 with the dims of each 16 in
         // the order in which the K codes come out of ldmatrix: 4j, 4j+1 at 2j, 4j+2, 4j+3 at 8 + 2j
-        if (warp == 0) tree_masks(P, seq, len, anc, reinterpret_cast<int8_t*>(smem + L::kUp));
-        {
-            constexpr int kLanes = D / 8;   // 8 elements a thread
-            const int part = tid % kLanes;
-            for (int r = tid / kLanes; r < L::kRows; r += kThreads / kLanes) {
-                const int row = r_base + r, node = row / P.group, hq = h * P.group + row % P.group;
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (row < M) w = *reinterpret_cast<const uint4*>(P.q + (((size_t)seq * P.n_nodes + node) * (size_t)P.ldq + (size_t)hq * D + part * 8) * 2);
-                if constexpr (!L::k8) {
-                    *reinterpret_cast<uint4*>(smem + L::kQ + swz<D * 2>(r, part)) = w;
-                } else {
-                    uint32_t x[4] = {w.x, w.y, w.z, w.w};
-                    if constexpr (QT == QWEN_BF16) {
-                        uint32_t m = 0;
-                        #pragma unroll
-                        for (int i = 0; i < 4; i++) m = max(m, max(x[i] & 0x7fffu, (x[i] >> 16) & 0x7fffu));
-                        #pragma unroll
-                        for (int o = 1; o < kLanes; o <<= 1) m = max(m, __shfl_xor_sync(~0u, m, o));
-                        // 2^e <= the row's largest magnitude < 2^(e+1); infinities and NaN go through as they are
-                        const int e = min(max((int)(m >> 7), 1), 253);
-                        const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-                        #pragma unroll
-                        for (int i = 0; i < 4; i++) x[i] = kv::half2_bits(bf_lo(x[i]) * down, bf_hi(x[i]) * down);
-                        if (part == 0) qf[r] = __uint_as_float((uint32_t)e << 23);
-                    } else if (part == 0) {
-                        qf[r] = 1.0f;
-                    }
-                    // this thread's 8 dims are the first or second half of a 16: pairs p = 0..3 (dims 2p, 2p+1) of it
-                    const int half = part & 1, chunk = part & ~1;
+        constexpr int kLanes = D / 8, kQStep = kThreads / kLanes, kQPer = L::kRows / kQStep;   // 8 elements a thread
+        const int part = tid % kLanes, rq = tid / kLanes;
+        int up[2];
+        uint64_t nodes[2];        // what nodes lane and lane + 32 see
+        load_parents(P, seq, up);
+        uint4 qv[kQPer];
+        #pragma unroll
+        for (int i = 0; i < kQPer; i++) {
+            const int row = r_base + rq + i * kQStep, node = row / P.group;
+            qv[i] = make_uint4(0, 0, 0, 0);
+            if (row < M)
+                qv[i] = *reinterpret_cast<const uint4*>(P.q + (((size_t)seq * P.n_nodes + node) * (size_t)P.ldq +
+                                                               (size_t)(h * P.group + row - node * P.group) * D + part * 8) * 2);
+        }
+        tree_masks(P, len, up, nodes);
+        uint64_t see[2 * MT];     // what this lane's rows see of the tree
+        #pragma unroll
+        for (int i = 0; i < 2 * MT; i++) {
+            const int row = r_base + 16 * (i >> 1) + g + 8 * (i & 1), node = min(row / P.group, kMaxNodes - 1);
+            const uint64_t a = __shfl_sync(~0u, nodes[0], node & 31), b = __shfl_sync(~0u, nodes[1], node & 31);
+            see[i] = row < M ? (node < 32 ? a : b) : 0;
+        }
+        if (warp == 0) {
+            anc[lane] = nodes[0];
+            anc[lane + 32] = nodes[1];
+        }
+        const uint32_t flip = P.scale_log2 < 0.f ? 0x80008000u : 0u;   // a negative scale: its sign goes to the queries
+        #pragma unroll
+        for (int i = 0; i < kQPer; i++) {
+            const int r = rq + i * kQStep;
+            uint32_t x[4] = {qv[i].x ^ flip, qv[i].y ^ flip, qv[i].z ^ flip, qv[i].w ^ flip};
+            if constexpr (!L::k8) {
+                *reinterpret_cast<uint4*>(smem + L::kQ + swz<D * 2>(r, part)) = make_uint4(x[0], x[1], x[2], x[3]);
+            } else {
+                if constexpr (QT == QWEN_BF16) {
+                    uint32_t m = 0;
                     #pragma unroll
-                    for (int p = 0; p < 4; p++) {
-                        const int d = 8 * half + 2 * p, jj = d >> 2, k = (d & 2) ? 8 + 2 * jj : 2 * jj;
-                        *reinterpret_cast<uint32_t*>(smem + L::kQ + swz<D * 2>(r, chunk + (k >> 3)) + (k & 7) * 2) = x[p];
-                    }
+                    for (int e = 0; e < 4; e++) m = max(m, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
+                    #pragma unroll
+                    for (int o = 1; o < kLanes; o <<= 1) m = max(m, __shfl_xor_sync(~0u, m, o));
+                    // 2^e <= the row's largest magnitude < 2^(e+1); infinities and NaN go through as they are
+                    const int e = min(max((int)(m >> 7), 1), 253);
+                    const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+                    #pragma unroll
+                    for (int e2 = 0; e2 < 4; e2++) x[e2] = kv::half2_bits(bf_lo(x[e2]) * down, bf_hi(x[e2]) * down);
+                    if (part == 0) qf[r] = __uint_as_float((uint32_t)e << 23);
+                } else if (part == 0) {
+                    qf[r] = 1.0f;
+                }
+                // this thread's 8 dims are the first or second half of a 16: pairs p = 0..3 (dims 2p, 2p+1) of it
+                const int half = part & 1, chunk = part & ~1;
+                #pragma unroll
+                for (int p = 0; p < 4; p++) {
+                    const int d = 8 * half + 2 * p, jj = d >> 2, k = (d & 2) ? 8 + 2 * jj : 2 * jj;
+                    *reinterpret_cast<uint32_t*>(smem + L::kQ + swz<D * 2>(r, chunk + (k >> 3)) + (k & 7) * 2) = x[p];
                 }
             }
         }
         __syncthreads();
-        uint64_t see[2 * MT];     // what this lane's rows see of the tree
-        float c[2 * MT];          // their score factors
+        float c[2 * MT];          // these rows' score factors (kept above 0: -inf * 0 would be NaN)
         #pragma unroll
         for (int i = 0; i < 2 * MT; i++) {
-            const int r = 16 * (i >> 1) + g + 8 * (i & 1), row = r_base + r;
-            see[i] = row < M ? anc[row / P.group] : 0;
-            c[i] = L::k8 ? P.scale_log2 * qf[r] : P.scale_log2;
+            const float a = fabsf(P.scale_log2);
+            c[i] = fmaxf(L::k8 ? a * qf[16 * (i >> 1) + g + 8 * (i & 1)] : a, 1e-37f);
         }
         uint32_t qa[MT == 1 ? KS : 1][4];   // one block of rows: its fragments stay in registers
         auto q_frag = [&](int mt, int ks, uint32_t (&a)[4]) {
@@ -494,18 +579,10 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT)) attention_k
                         vs[i][1] = vs2.y;
                         #pragma unroll
                         for (int mt = 0; mt < MT; mt++) {
-                            s[mt][i][0] *= c[2 * mt] * ks2.x; s[mt][i][1] *= c[2 * mt] * ks2.y;
-                            s[mt][i][2] *= c[2 * mt + 1] * ks2.x; s[mt][i][3] *= c[2 * mt + 1] * ks2.y;
+                            s[mt][i][0] *= ks2.x; s[mt][i][1] *= ks2.y;
+                            s[mt][i][2] *= ks2.x; s[mt][i][3] *= ks2.y;
                         }
                     }
-                } else {
-                    #pragma unroll
-                    for (int i = 0; i < NT; i++)
-                        #pragma unroll
-                        for (int mt = 0; mt < MT; mt++) {
-                            s[mt][i][0] *= c[2 * mt]; s[mt][i][1] *= c[2 * mt];
-                            s[mt][i][2] *= c[2 * mt + 1]; s[mt][i][3] *= c[2 * mt + 1];
-                        }
                 }
                 uint32_t vis[2 * MT];   // bit x: the row sees position k0 + x (KW <= 32)
                 if (tail) {
@@ -530,7 +607,11 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT)) attention_k
                     e = __reduce_max_sync(~0u, e);
                     if (e > ve) { up = e - ve; ve = e; }
                 }
-                const float vinv = L::k8 ? __uint_as_float((254u - ve) << 23) : 1.0f;
+                if constexpr (L::k8) {
+                    const float vinv = __uint_as_float((254u - ve) << 23);
+                    #pragma unroll
+                    for (int i = 0; i < NT; i++) { vs[i][0] *= vinv; vs[i][1] *= vinv; }
+                }
                 float f[2 * MT];
                 bool moved = up != 0;
                 #pragma unroll
@@ -540,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT)) attention_k
                     for (int i = 0; i < NT; i++) mx = fmaxf(mx, fmaxf(s[r >> 1][i][2 * (r & 1)], s[r >> 1][i][2 * (r & 1) + 1]));
                     mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
-                    const float mn = fmaxf(m[r], mx);
+                    const float mn = fmaxf(m[r], mx == -INFINITY ? mx : mx * c[r]);
                     const float base = mn == -INFINITY ? 0.f : mn;
                     f[r] = exp2_approx(m[r] - base);
                     moved |= mn > m[r];
@@ -551,9 +632,9 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT)) attention_k
                         #pragma unroll
                         for (int e = 0; e < 2; e++) {
                             float& x = s[r >> 1][i][2 * (r & 1) + e];
-                            x = exp2_approx(x - base);
+                            x = exp2_approx(fmaf(x, c[r], -base));
                             sum += x;
-                            if constexpr (L::k8) x *= !tail || sees(r, 8 * i + 2 * j + e) ? vs[i][e] * vinv : 0.f;
+                            if constexpr (L::k8) x *= !tail || sees(r, 8 * i + 2 * j + e) ? vs[i][e] : 0.f;
                         }
                     l[r] = l[r] * f[r] + sum;
                 }
@@ -716,19 +797,21 @@ constexpr int kJoinThreads = 128;
 template <int D, int ROWS, bool ACROSS>
 __host__ __device__ constexpr int join_blocks() { return ROWS * (ACROSS ? D / 8 : D / 4) / kJoinThreads; }
 template <int QT, int KT, int COST, int D, int ROWS, bool ACROSS>
-__global__ void __launch_bounds__(kJoinThreads) combine_kernel(const Params P) {
-    constexpr int kSlot = ROWS * (D + 2), kVec = ACROSS ? 2 : 1, kAhead = 8;   // float4s a thread; partial results loaded at once
+__global__ void __launch_bounds__(kJoinThreads, 6) combine_kernel(const Params P) {
+    constexpr int kSlot = ROWS * (D + 2), kVec = ACROSS ? 2 : 1, kAhead = ACROSS ? 5 : 8;   // float4s a thread; partial results loaded at once
     const int beside = P.beside, unit_blocks = beside == 1 ? P.row_blocks : 1, units = P.n_kv_heads * unit_blocks;
     const int i = blockIdx.x / beside, lane = blockIdx.x - i * beside;
-    const Shares shares(line_length<KT, COST>(P, units), gridDim.x / beside);
-    const long long from = shares.begin(i), edge = shares.begin(i + 1);
-    long long before = 0, s = edge, e = edge;   // the item at the border: its positions
+    const Line<KT, COST> line(P, units, gridDim.x / beside);
+    const Shares& shares = line.shares;
+    const int from = shares.begin(i), edge = shares.begin(i + 1);
+    int before = 0, s = edge, e = edge;   // the item at the border: its positions
     int seq = 0, unit = 0;
     if (edge > from && edge < shares.n) {
-        seq = line_find<KT, COST>(P, units, edge, before);
-        const int per = seq_line<KT, COST>(P, P.lens[seq]);
-        unit = (int)quotient(edge - before, per);
-        s = before + (long long)unit * per;
+        int len;
+        seq = line.find(P, edge, before, len);
+        const int per = seq_tiles<KT>(P, len) + COST;
+        unit = (int)((unsigned)(edge - before) / (unsigned)per);
+        s = before + unit * per;
         e = s + per;
     }
     pdl_wait();   // on every path: this kernel may not end before the one that it joins
@@ -752,7 +835,7 @@ __global__ void __launch_bounds__(kJoinThreads) combine_kernel(const Params P) {
             ml[j] = make_float2(-INFINITY, 0.f);
             #pragma unroll
             for (int v = 0; v < kVec; v++) b[j][v] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (k > last || (shares.whole == 0 && shares.begin(k) == shares.begin(k + 1))) continue;   // (an empty share)
+            if (k > last) continue;
             // a share that begins before the item holds it in its second slot
             const float* slot = P.work + (2 * ((size_t)k * beside + lane) + (k == i && from < s ? 1 : 0)) * kSlot;
             ml[j] = *reinterpret_cast<const float2*>(slot + ROWS * D + 2 * r);
