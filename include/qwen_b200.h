@@ -455,7 +455,7 @@ int qwen_kv_read(const qwen_kv_cache_t* cache, void* k, void* v, int dst_dtype, 
  * then holds start[s] + n_path[s] positions. */
 int qwen_kv_keep(const qwen_kv_cache_t* cache, const int* start, const int* path, const int* n_path, int n_nodes, void* stream);
 
-/* Bytes of workspace that qwen_tree_attention needs for these sizes. */
+/* Bytes of workspace that qwen_tree_attention needs for these sizes (0 for caches of a few hundred positions). */
 int qwen_tree_attention_workspace(const qwen_kv_cache_t* cache, int n_nodes, int n_heads, size_t* bytes);
 
 /* Attention of a tree of drafted tokens over a cache whose positions lens[s] +
@@ -471,8 +471,9 @@ int qwen_tree_attention_workspace(const qwen_kv_cache_t* cache, int n_nodes, int
  * are absent.  What positions that a node does not see hold (NaN included) has
  * no influence on it.  Scores, softmax statistics and sums are fp32; the
  * weights enter the product with V in 16 bits.  workspace: as many bytes as
- * qwen_tree_attention_workspace says, contents free, 16-byte aligned; calls
- * that may overlap need one each. */
+ * qwen_tree_attention_workspace says, contents free, 16-byte aligned (may be
+ * NULL where it says 0); calls that may overlap need one each.  The rows of a
+ * call whose device-side waits ran out (they are bounded) are NaN. */
 int qwen_tree_attention(const qwen_kv_cache_t* cache, const void* q, void* out, int dtype, long long ldq, long long ldo, int n_nodes,
                         int n_heads, const int* lens, const int* parents, float scale, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -174,6 +174,7 @@ int attention_rows(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : 128; }
 
 struct Plan {
     int rows, row_blocks, beside, shares;   // shares: CTAs, beside for each share of the line
+    bool whole;                             // a CTA for each item, no joining
     size_t bytes;
 };
 int check_tree(const qwen_kv_cache_t* c, int n_nodes, int n_heads) {
@@ -182,17 +183,33 @@ int check_tree(const qwen_kv_cache_t* c, int n_nodes, int n_heads) {
     if (n_heads / c->n_kv_heads > 1 << 14) return fail(QWEN_E_UNSUPPORTED, "more than 2^14 query heads for each K/V head");
     return QWEN_OK;
 }
+// What the plan has without the device: rows, row_blocks, whole.
+void attention_shape(const qwen_kv_cache_t* c, int n_nodes, int n_heads, Plan* p) {
+    const int m = n_nodes * (n_heads / c->n_kv_heads);
+    p->rows = attention_rows(m);
+    p->row_blocks = (m + p->rows - 1) / p->rows;
+    // A few tiles: a CTA for each item.  Spreading them over several CTAs saves at most the time of all but one (about 0.5 us
+    // each, 1.3 us in the tensor-memory kernel), joining costs a second launch (5 us in all).
+    const int keys = p->rows <= 32 ? 64 : 128;
+    const long long tiles = (c->capacity + keys - 1) / keys, items = (long long)c->n_seqs * c->n_kv_heads * p->row_blocks;
+    p->whole = tiles <= (p->rows <= 32 ? 8 : 4) && items < 1 << 30;
+}
 int attention_plan(const qwen_kv_cache_t* c, int n_nodes, int n_heads, int dev, Plan* p) {
-    const long long m = (long long)n_nodes * (n_heads / c->n_kv_heads);
+    attention_shape(c, n_nodes, n_heads, p);
+    if (p->whole) {
+        p->beside = p->row_blocks;
+        p->shares = c->n_seqs * c->n_kv_heads * p->row_blocks;
+        p->bytes = 0;
+        return QWEN_OK;
+    }
     int nsm = 0;
     TRY(sm_count(dev, &nsm));
-    p->rows = attention_rows((int)m);
-    p->row_blocks = (int)((m + p->rows - 1) / p->rows);
     // as many CTAs as the SMs hold (the tensor-memory kernel: one each), shared out over the blocks of rows that walk side by side
     const int keys = p->rows <= 32 ? 64 : 128, ctas = p->rows <= 32 ? qb::ta::attention_ctas(p->rows, c->head_dim) * nsm : nsm;
     p->beside = p->row_blocks <= ctas ? p->row_blocks : 1;
     // no more shares than the line can have positions
-    const double most = (double)c->n_seqs * c->n_kv_heads * (p->row_blocks / p->beside) * ((c->capacity + keys - 1) / keys + qb::ta::kTcItemCost);
+    const double most = (double)c->n_seqs * c->n_kv_heads * (p->row_blocks / p->beside) *
+                        ((c->capacity + keys - 1) / keys + qb::ta::kTcItemCost);
     p->shares = (int)std::min((double)(ctas / p->beside), most) * p->beside;
     if (most >= 2147483648.0) return fail(QWEN_E_UNSUPPORTED, "too many sequences, heads and positions for one call");
     p->bytes = (size_t)2 * p->shares * p->rows * (c->head_dim + 2) * sizeof(float);
@@ -202,7 +219,7 @@ int attention_plan(const qwen_kv_cache_t* c, int n_nodes, int n_heads, int dev, 
 // The kernel that joins the shares' partial results, launched so that it may start its set-up early.
 template <int QT, int KT, int COST, int D, int ROWS, bool ACROSS>
 int join_launch(const qb::ta::Params& P, const Plan& plan, cudaStream_t st) {
-    if (plan.shares == plan.beside) return QWEN_OK;
+    if (plan.whole || plan.shares == plan.beside) return QWEN_OK;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(plan.shares, qb::ta::join_blocks<D, ROWS, ACROSS>());
     cfg.blockDim = dim3(qb::ta::kJoinThreads);
@@ -334,9 +351,10 @@ extern "C" int qwen_tree_attention_workspace(const qwen_kv_cache_t* cache, int n
     if (!bytes) return fail(QWEN_E_ARG, "NULL argument");
     TRY(check_view(cache));
     TRY(check_tree(cache, n_nodes, n_heads));
-    int dev = 0;
-    CU(cudaGetDevice(&dev));
     Plan p;
+    attention_shape(cache, n_nodes, n_heads, &p);
+    int dev = 0;
+    if (!p.whole) CU(cudaGetDevice(&dev));
     TRY(attention_plan(cache, n_nodes, n_heads, dev, &p));
     *bytes = p.bytes;
     return QWEN_OK;
@@ -354,9 +372,10 @@ extern "C" int qwen_tree_attention(const qwen_kv_cache_t* cache, const void* q, 
     if (!std::isfinite(scale)) return fail(QWEN_E_ARG, "scale must be finite");
     if (q == out) return fail(QWEN_E_ARG, "out must not be q");
     int dev = 0;
-    TRY(check_ptrs({QB_VIEW_PTRS(cache), {q, "q", 16, true}, {out, "out", 16, true}, {lens, "lens", 4, true}, {parents, "parents", 4, true},
-                    {workspace, "workspace", 16, true}}, &dev));
     Plan plan;
+    attention_shape(cache, n_nodes, n_heads, &plan);
+    TRY(check_ptrs({QB_VIEW_PTRS(cache), {q, "q", 16, true}, {out, "out", 16, true}, {lens, "lens", 4, true}, {parents, "parents", 4, true},
+                    {workspace, "workspace", 16, workspace || !plan.whole}}, &dev));
     TRY(attention_plan(cache, n_nodes, n_heads, dev, &plan));
     if (workspace_bytes < plan.bytes) return fail(QWEN_E_ARG, "workspace is smaller than qwen_tree_attention_workspace says");
     qb::ta::Params P;
@@ -372,6 +391,7 @@ extern "C" int qwen_tree_attention(const qwen_kv_cache_t* cache, const void* q, 
     P.n_kv_heads = cache->n_kv_heads;
     P.group = n_heads / cache->n_kv_heads;
     P.n_nodes = n_nodes;
+    P.whole = plan.whole;
     P.row_blocks = plan.row_blocks;
     P.beside = plan.beside;
     P.scale_log2 = scale * 1.4426950408889634f;

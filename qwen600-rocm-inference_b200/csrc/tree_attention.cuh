@@ -17,7 +17,8 @@
 // the memory once and for the others from the L2.  An item that crosses a border
 // between shares leaves partial (m, l, O) in the workspace, two slots a CTA, and
 // combine_kernel joins them in the order of the keys, so results do not depend on
-// timing.  The shares are computed on the device from lens.
+// timing.  The shares are computed on the device from lens.  Where the cache's
+// capacity is a few tiles, a CTA takes a whole item and nothing is joined.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -39,6 +40,7 @@ struct Params {
     float* work;
     long long ldq, ldo;
     int n_seqs, n_kv_heads, group, n_nodes;
+    int whole;                // a CTA for each item: CTA (sequence * n_kv_heads + head) * row_blocks + block
     int row_blocks, beside;   // blocks of rows that a K/V head has; CTAs side by side on a share (row_blocks, or 1 where that is more than the grid)
     float scale_log2;   // scale * log2(e)
 };
@@ -164,6 +166,21 @@ struct Items {
     }
     // all lanes of a warp; false: nothing to do
     __device__ __forceinline__ bool start(const Params& P) {
+        if (P.whole) {
+            const int item_i = blockIdx.x / P.row_blocks;
+            beside = P.row_blocks;
+            seq = item_i / P.n_kv_heads;
+            h = item_i - seq * P.n_kv_heads;
+            r_base = (blockIdx.x - item_i * P.row_blocks) * ROWS;
+            len = P.lens[seq];
+            end = seq_end(P, len);
+            n = t1 = seq_tiles<KT>(P, len);
+            at = before = t0 = 0;
+            to = step = 1;
+            units = unit_blocks = 1;
+            first = true;
+            return true;
+        }
         beside = P.beside;
         unit_blocks = beside == 1 ? P.row_blocks : 1;
         units = P.n_kv_heads * unit_blocks;

@@ -65,7 +65,13 @@ GOOD = dict(q=OK_PTR, out=OK_PTR + 16, dtype=0, ldq=512, ldo=512, n_nodes=4, n_h
     dict(n_nodes=0), dict(n_nodes=65), dict(n_heads=0), dict(n_heads=3), dict(lens=0), dict(parents=OK_PTR + 1), dict(scale=float("nan")),
     dict(scale=float("inf")), dict(work=0), dict(work=OK_PTR + 4)])
 def test_bad_attention(qb, over):
-    _raises(qb, -1, qb.tree_attention, _view(qb), *{**GOOD, **over}.values())
+    big = _view(qb, capacity=4096, head_stride=4096 * 128, seq_stride=2 * 4096 * 128)
+    _raises(qb, -1, qb.tree_attention, big, *{**GOOD, **over}.values())
+
+
+def test_small_caches_need_no_workspace(qb):
+    assert qb.tree_attention_workspace(_view(qb), 4, 4) == 0
+    _raises(qb, -1, qb.tree_attention, _view(qb), *{**GOOD, "work": OK_PTR + 4}.values())
 
 
 def test_bad_workspace_queries(qb):

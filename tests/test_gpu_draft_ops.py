@@ -832,7 +832,8 @@ def test_two_streams_and_repeats(qb):
 def test_refusals_on_the_device(qb):
     """Host memory, too small a workspace: refused with a message, and the next call works."""
     import torch
-    s = _step_buffers(qb, "bf16", 5)
+    s = _step_buffers(qb, "bf16", 5, length=1500)      # (long enough to need a workspace)
+    assert s["work"].numel() > 0
     host = torch.zeros(4096, dtype=torch.int32)
     pinned = torch.zeros(4096, dtype=torch.int32).pin_memory()
     c = s["c"]
