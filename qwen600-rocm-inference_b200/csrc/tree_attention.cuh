@@ -196,45 +196,9 @@ struct Items {
 };
 
 // ---- the tree --------------------------------------------------------------------
-// One warp: anc[i] = the nodes that node i sees (itself and its ancestors), 0 if it
-// is absent.  Six rounds of doubling the step; two nodes a lane.
-__device__ __forceinline__ void tree_masks(const Params& P, int seq, int len, uint64_t* anc, int8_t* up) {
-    const int lane = threadIdx.x & 31, N = P.n_nodes;
-    constexpr int8_t kNone = -1, kAbsent = -2;
-    #pragma unroll
-    for (int k = 0; k < 2; k++) {
-        const int i = lane + 32 * k;
-        int p = kAbsent;
-        if (i < N) {
-            p = P.parents[(size_t)seq * N + i];
-            if (p < -1 || p >= i || len < 0 || (long long)len + i >= P.cache.capacity) p = kAbsent;
-        }
-        up[i] = (int8_t)p;
-        anc[i] = 1ull << i;
-    }
-    __syncwarp();
-    for (int step = 1; step < N; step <<= 1) {
-        uint64_t a[2];
-        int8_t u[2];
-        #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int i = lane + 32 * k, p = up[i];
-            a[k] = anc[i] | (p >= 0 ? anc[p] : 0);
-            u[k] = p >= 0 ? up[p] : (int8_t)p;
-        }
-        __syncwarp();
-        #pragma unroll
-        for (int k = 0; k < 2; k++) { anc[lane + 32 * k] = a[k]; up[lane + 32 * k] = u[k]; }
-        __syncwarp();
-    }
-    #pragma unroll
-    for (int k = 0; k < 2; k++)
-        if (up[lane + 32 * k] != kNone) anc[lane + 32 * k] = 0;
-    __syncwarp();
-}
-
-// The same with the nodes' parents in registers (nodes lane and lane + 32 of a
-// warp; load_parents) and shuffles in place of shared memory.
+// What each node sees (itself and its ancestors; 0: absent), nodes lane and lane +
+// 32 of a warp, from their parents (load_parents): up to six rounds of doubling the
+// step, by shuffles.
 __device__ __forceinline__ void load_parents(const Params& P, int seq, int (&up)[2]) {
     const int lane = threadIdx.x & 31;
     #pragma unroll

@@ -47,8 +47,8 @@ struct TcLayout {
     static constexpr int kScales = kRaw + kRawRing * kRawHalf;                        // [ring][ks 128, vs 128]
     static constexpr int kXm = kScales + (k8 ? kScaleRing * 2 * kTcKT * 4 : 0);       // [tile parity][half][row] maxima, then sums
     static constexpr int kAnc = kXm + 2 * 2 * kTcRows * 4;
-    static constexpr int kUp = kAnc + kMaxNodes * 8;
-    static constexpr int kVe = kUp + kMaxNodes;                                       // [ring][producer warp] largest exponent of vs
+    static constexpr int kQf = kAnc + kMaxNodes * 8;                                  // the rows' powers of two
+    static constexpr int kVe = kQf + kTcRows * 4;                                       // [ring][producer warp] largest exponent of vs
     static constexpr int kBar = kVe + kScaleRing * 4 * 4;
     static constexpr int kBars = 2 * kRing + kScaleRing + 8;
     static constexpr int kMisc = kBar + kBars * 8;                                    // tensor-memory address, fault, odd[8]
@@ -138,6 +138,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
     uint64_t* anc = reinterpret_cast<uint64_t*>(smem + L::kAnc);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+    pdl_wait();
+    pdl_launch_dependents();         // after the wait: what the joining kernel reads early (lens) is then complete
+    Items<kTcKT, kTcItemCost, kTcRows> it;       // every role walks it alike
+    const bool busy = it.start(P);               // the same for the whole CTA
     if (tid == 0) {
         for (int i = 0; i < L::kRing; i++) { mbar_init(&full[i], kTcProducers); mbar_init(&empty[i], 1); }
         for (int i = 0; i < kScaleRing; i++) mbar_init(&scaled[i], kTcProducers);
@@ -155,16 +159,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     constexpr uint32_t kTmO = 256, kTmP = 384;   // columns: S buffers 0 and 128, O 256, P buffers 384 and 448
-    pdl_wait();
-    pdl_launch_dependents();         // after the wait: what the joining kernel reads early (lens) is then complete
-
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
         if (ok && !mbar_spin(bar, parity, kWaitNs)) { ok = false; *fault = 1; }
         return ok;
     };
-    Items<kTcKT, kTcItemCost, kTcRows> it;       // every role walks it alike
-    const bool busy = it.start(P);   // the same for the whole CTA
     if (busy && warp >= kProducer && warp < kIssuer) {
         // ---------------- producers ----------------
         const int pt = tid - 32 * kProducer;
@@ -312,8 +311,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
         uint32_t steps[2] = {0, 0};   // tiles of a buffer so far
         bool going = true;
         do {
+            int up[2];
+            uint64_t nodes[2];
+            load_parents(P, it.seq, up);
+            tree_masks(P, it.len, up, nodes);
             // every softmax thread has taken what it needs of the item before's masks (it announced that item's queries after)
-            tree_masks(P, it.seq, it.len, anc, reinterpret_cast<int8_t*>(smem + L::kUp));
+            anc[lane] = nodes[0];
+            anc[lane + 32] = nodes[1];
             named_bar(1, kTcSoftmax + 32);
             if (lane == 0 && going) {
                 const int nt = it.t1 - it.t0;
@@ -373,53 +377,47 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
             const int nt = it.t1 - it.t0;
             // (the item before's products are done: its queries' place is free)
             const int row = it.r_base + rl;
-            const int node = row / P.group, hq = it.h * P.group + row - node * P.group;
+            const int node = row / P.group;
             const bool live = row < M;
-            float c = fabsf(P.scale_log2);                                 // (kept above 0: -inf * 0 would be NaN)
-            {
-                // this thread's half of the row
-                constexpr int kPer = D / 16;
-                const uint4* src = reinterpret_cast<const uint4*>(P.q + (((size_t)it.seq * P.n_nodes + node) * (size_t)P.ldq + (size_t)hq * D) * 2);
+            float* qf = reinterpret_cast<float*>(smem + L::kQf);
+            {   // the item's queries: D / 8 neighbouring threads a row
+                constexpr int kLanes = D / 8, kStep = kTcSoftmax / kLanes, kPer = kTcRows / kStep;
+                const int part = tid % kLanes, r0 = tid / kLanes;
                 uint4 w[kPer];
                 #pragma unroll
-                for (int i = 0; i < kPer; i++) w[i] = live ? __ldg(src + half * kPer + i) : make_uint4(0, 0, 0, 0);
-                float down = 1.0f;
-                if constexpr (L::k8 && QT == QWEN_BF16) {                  // into fp16's range, a power of two a row
-                    uint32_t m = 0;
-                    auto largest = [&](const uint4& y) {
-                        const uint32_t x[4] = {y.x, y.y, y.z, y.w};
-                        #pragma unroll
-                        for (int e = 0; e < 4; e++) m = max(m, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
-                    };
-                    #pragma unroll
-                    for (int i = 0; i < kPer; i++) largest(w[i]);
-                    if (live) {
-                        #pragma unroll
-                        for (int i = 0; i < kPer; i++) largest(__ldg(src + (half ^ 1) * kPer + i));
-                    }
-                    const int e = min(max((int)(m >> 7), 1), 253);
-                    down = __uint_as_float((uint32_t)(254 - e) << 23);
-                    c *= __uint_as_float((uint32_t)e << 23);
+                for (int i = 0; i < kPer; i++) {
+                    const int qrow = it.r_base + r0 + i * kStep, qnode = qrow / P.group;
+                    w[i] = make_uint4(0, 0, 0, 0);
+                    if (qrow < M)
+                        w[i] = __ldg(reinterpret_cast<const uint4*>(P.q + (((size_t)it.seq * P.n_nodes + qnode) * (size_t)P.ldq +
+                                                                          (size_t)(it.h * P.group + qrow - qnode * P.group) * D + part * 8) * 2));
                 }
-                uint8_t* dst = smem + L::kQ + rl * 128;
+                const uint32_t sign = flip ? 0x80008000u : 0u;
                 #pragma unroll
                 for (int i = 0; i < kPer; i++) {
-                    if constexpr (L::k8 && QT == QWEN_BF16) {
-                        w[i].x = kv::half2_bits(bf_lo(w[i].x) * down, bf_hi(w[i].x) * down);
-                        w[i].y = kv::half2_bits(bf_lo(w[i].y) * down, bf_hi(w[i].y) * down);
-                        w[i].z = kv::half2_bits(bf_lo(w[i].z) * down, bf_hi(w[i].z) * down);
-                        w[i].w = kv::half2_bits(bf_lo(w[i].w) * down, bf_hi(w[i].w) * down);
+                    const int r = r0 + i * kStep;
+                    uint32_t x[4] = {w[i].x ^ sign, w[i].y ^ sign, w[i].z ^ sign, w[i].w ^ sign};
+                    if constexpr (L::k8 && QT == QWEN_BF16) {              // into fp16's range, a power of two a row
+                        uint32_t m = 0;
+                        #pragma unroll
+                        for (int e = 0; e < 4; e++) m = max(m, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
+                        #pragma unroll
+                        for (int o = 1; o < kLanes; o <<= 1) m = max(m, __shfl_xor_sync(~0u, m, o));
+                        const int e = min(max((int)(m >> 7), 1), 253);
+                        const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+                        #pragma unroll
+                        for (int j = 0; j < 4; j++) x[j] = kv::half2_bits(bf_lo(x[j]) * down, bf_hi(x[j]) * down);
+                        if (part == 0) qf[r] = __uint_as_float((uint32_t)e << 23);
                     }
-                    if (flip) { w[i].x ^= 0x80008000u; w[i].y ^= 0x80008000u; w[i].z ^= 0x80008000u; w[i].w ^= 0x80008000u; }
-                    const int ch = half * kPer + i;
-                    *reinterpret_cast<uint4*>(dst + (ch >> 3) * (kTcRows * 128) + (((ch & 7) ^ (rl & 7)) << 4)) = w[i];
+                    *reinterpret_cast<uint4*>(smem + L::kQ + (part >> 3) * (kTcRows * 128) + r * 128 + (((part & 7) ^ (r & 7)) << 4)) =
+                        make_uint4(x[0], x[1], x[2], x[3]);
                 }
             }
-            c = fmaxf(c, 1e-37f);
             fence_async_smem();
             tc_fence_before();
             named_bar(1, kTcSoftmax + 32);                                 // the masks are there; every thread is behind the item before
             if (tid == 0) odd[(item - 1) & 7] = 0;
+            const float c = fmaxf(fabsf(P.scale_log2) * (L::k8 && QT == QWEN_BF16 ? qf[rl] : 1.0f), 1e-37f);   // (above 0: -inf * 0 would be NaN)
             const uint64_t see = live ? anc[node] : 0;
             __syncwarp();
             if (lane == 0) mbar_arrive(qfull);
