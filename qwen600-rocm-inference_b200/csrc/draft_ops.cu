@@ -390,6 +390,7 @@ extern "C" int qwen_tree_attention(const qwen_kv_cache_t* cache, const void* q, 
     P.n_seqs = cache->n_seqs;
     P.n_kv_heads = cache->n_kv_heads;
     P.group = n_heads / cache->n_kv_heads;
+    P.per_group = 1.0f / (float)P.group;
     P.n_nodes = n_nodes;
     P.whole = plan.whole;
     P.row_blocks = plan.row_blocks;

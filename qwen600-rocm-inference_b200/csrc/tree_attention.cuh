@@ -43,6 +43,10 @@ struct Params {
     int whole;                // a CTA for each item: CTA (sequence * n_kv_heads + head) * row_blocks + block
     int row_blocks, beside;   // blocks of rows that a K/V head has; CTAs side by side on a share (row_blocks, or 1 where that is more than the grid)
     float scale_log2;   // scale * log2(e)
+    float per_group;    // 1 / group
+    // The node of a row (row < 64 * group, group <= 2^14): (row + 1/2) / group lies at least 2^-15 from a whole number below 64,
+    // and the product's two roundings move it by less than 2^-17.
+    __device__ __forceinline__ int node_of(int row) const { return (int)(((float)row + 0.5f) * per_group); }
 };
 
 // ---- the line of key tiles -----------------------------------------------------
@@ -420,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attentio
         uint4 qv[kQPer];
         #pragma unroll
         for (int i = 0; i < kQPer; i++) {
-            const int row = r_base + rq + i * kQStep, node = row / P.group;
+            const int row = r_base + rq + i * kQStep, node = P.node_of(row);
             qv[i] = make_uint4(0, 0, 0, 0);
             if (row < M)
                 qv[i] = *reinterpret_cast<const uint4*>(P.q + (((size_t)seq * P.n_nodes + node) * (size_t)P.ldq +
@@ -430,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attentio
         uint64_t see[2 * MT];     // what this lane's rows see of the tree
         #pragma unroll
         for (int i = 0; i < 2 * MT; i++) {
-            const int row = r_base + 16 * (i >> 1) + g + 8 * (i & 1), node = min(row / P.group, kMaxNodes - 1);
+            const int row = r_base + 16 * (i >> 1) + g + 8 * (i & 1), node = min(P.node_of(row), kMaxNodes - 1);
             const uint64_t a = __shfl_sync(~0u, nodes[0], node & 31), b = __shfl_sync(~0u, nodes[1], node & 31);
             see[i] = row < M ? (node < 32 ? a : b) : 0;
         }
@@ -615,9 +619,18 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attentio
                             float& x = s[r >> 1][i][2 * (r & 1) + e];
                             x = exp2_approx(fmaf(x, c[r], -base));
                             sum += x;
-                            if constexpr (L::k8) x *= !tail || sees(r, 8 * i + 2 * j + e) ? vs[i][e] : 0.f;
+                            if constexpr (L::k8) x *= vs[i][e];
                         }
                     l[r] = l[r] * f[r] + sum;
+                }
+                if (L::k8 && tail) {   // (a scale that a row does not see may be NaN)
+                    #pragma unroll
+                    for (int r = 0; r < 2 * MT; r++)
+                        #pragma unroll
+                        for (int i = 0; i < NT; i++)
+                            #pragma unroll
+                            for (int e = 0; e < 2; e++)
+                                if (!sees(r, 8 * i + 2 * j + e)) s[r >> 1][i][2 * (r & 1) + e] = 0.f;
                 }
                 if (__any_sync(~0u, moved)) {
                     const float w = L::k8 ? (up < 127u ? __uint_as_float((127u - up) << 23) : 0.f) : 1.0f;
@@ -741,7 +754,7 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attentio
         for (int i = tid; i < L::kRows * (D / 4); i += kThreads) {
             const int r = i / (D / 4), d = i % (D / 4) * 4, row = r_base + r;
             if (row >= M) break;
-            const bool present = anc[row / P.group] != 0;
+            const bool present = anc[P.node_of(row)] != 0;
             float mm = -INFINITY, ll = 0.f;
             #pragma unroll
             for (int w = 0; w < kWarps; w++) mm = fmaxf(mm, join_ml[(w * L::kRows + r) * 2]);
@@ -757,7 +770,7 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attentio
             if (!present) { mm = -INFINITY; ll = 0.f; a = make_float4(0.f, 0.f, 0.f, 0.f); }
             if (whole) {
                 const float inv = ll == 0.f ? 0.f : 1.0f / ll;
-                const int node = row / P.group, hq = h * P.group + row % P.group;
+                const int node = P.node_of(row), hq = h * P.group + row - node * P.group;
                 uint8_t* dst = P.out + (((size_t)seq * P.n_nodes + node) * (size_t)P.ldo + (size_t)hq * D + d) * 2;
                 *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<QT == QWEN_BF16>(a.x * inv, a.y * inv), pack2<QT == QWEN_BF16>(a.z * inv, a.w * inv));
             } else {
@@ -842,7 +855,7 @@ __global__ void __launch_bounds__(kJoinThreads, 6) combine_kernel(const Params P
         mm = mn;
     }
     const float inv = ll == 0.f ? 0.f : 1.0f / ll;
-    const int node = row / P.group, hq = h * P.group + row % P.group;
+    const int node = P.node_of(row), hq = h * P.group + row - node * P.group;
     uint8_t* dst = P.out + (((size_t)seq * P.n_nodes + node) * (size_t)P.ldo + (size_t)hq * D + d) * 2;
     #pragma unroll
     for (int v = 0; v < kVec; v++)

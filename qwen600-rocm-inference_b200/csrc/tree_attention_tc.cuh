@@ -377,40 +377,63 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
             const int nt = it.t1 - it.t0;
             // (the item before's products are done: its queries' place is free)
             const int row = it.r_base + rl;
-            const int node = row / P.group;
+            const int node = P.node_of(row);
             const bool live = row < M;
             float* qf = reinterpret_cast<float*>(smem + L::kQf);
             {   // the item's queries: D / 8 neighbouring threads a row
                 constexpr int kLanes = D / 8, kStep = kTcSoftmax / kLanes, kPer = kTcRows / kStep;
                 const int part = tid % kLanes, r0 = tid / kLanes;
-                uint4 w[kPer];
-                #pragma unroll
-                for (int i = 0; i < kPer; i++) {
-                    const int qrow = it.r_base + r0 + i * kStep, qnode = qrow / P.group;
-                    w[i] = make_uint4(0, 0, 0, 0);
-                    if (qrow < M)
-                        w[i] = __ldg(reinterpret_cast<const uint4*>(P.q + (((size_t)it.seq * P.n_nodes + qnode) * (size_t)P.ldq +
-                                                                          (size_t)(it.h * P.group + qrow - qnode * P.group) * D + part * 8) * 2));
-                }
                 const uint32_t sign = flip ? 0x80008000u : 0u;
-                #pragma unroll
-                for (int i = 0; i < kPer; i++) {
-                    const int r = r0 + i * kStep;
-                    uint32_t x[4] = {w[i].x ^ sign, w[i].y ^ sign, w[i].z ^ sign, w[i].w ^ sign};
-                    if constexpr (L::k8 && QT == QWEN_BF16) {              // into fp16's range, a power of two a row
-                        uint32_t m = 0;
-                        #pragma unroll
-                        for (int e = 0; e < 4; e++) m = max(m, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
-                        #pragma unroll
-                        for (int o = 1; o < kLanes; o <<= 1) m = max(m, __shfl_xor_sync(~0u, m, o));
-                        const int e = min(max((int)(m >> 7), 1), 253);
-                        const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-                        #pragma unroll
-                        for (int j = 0; j < 4; j++) x[j] = kv::half2_bits(bf_lo(x[j]) * down, bf_hi(x[j]) * down);
-                        if (part == 0) qf[r] = __uint_as_float((uint32_t)e << 23);
+                const uint8_t* qbase = P.q + ((size_t)it.seq * P.n_nodes * (size_t)P.ldq + (size_t)it.h * P.group * D + part * 8) * 2;
+                uint8_t* dst = smem + L::kQ + (part >> 3) * (kTcRows * 128);
+                auto src = [&](int r, bool& in) {
+                    const int qrow = it.r_base + r, qnode = P.node_of(qrow);
+                    in = qrow < M;
+                    return in ? qbase + ((size_t)qnode * (size_t)P.ldq + (size_t)(qrow - qnode * P.group) * D) * 2 : P.q;
+                };
+                if constexpr (!L::k8) {
+                    #pragma unroll 2
+                    for (int i = 0; i < kPer; i++) {
+                        const int r = r0 + i * kStep;
+                        bool in;
+                        const uint8_t* from = src(r, in);
+                        cp_async16(smem_addr(dst + r * 128 + (((part & 7) ^ (r & 7)) << 4)), from, in);
                     }
-                    *reinterpret_cast<uint4*>(smem + L::kQ + (part >> 3) * (kTcRows * 128) + r * 128 + (((part & 7) ^ (r & 7)) << 4)) =
-                        make_uint4(x[0], x[1], x[2], x[3]);
+                    cp_async_commit();
+                    cp_async_wait<0>();
+                    if (flip) {
+                        for (int i = 0; i < kPer; i++) {
+                            const int r = r0 + i * kStep;
+                            uint4* p = reinterpret_cast<uint4*>(dst + r * 128 + (((part & 7) ^ (r & 7)) << 4));
+                            const uint4 w = *p;
+                            *p = make_uint4(w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign);
+                        }
+                    }
+                } else {
+                    uint4 w[kPer];
+                    #pragma unroll
+                    for (int i = 0; i < kPer; i++) {
+                        bool in;
+                        const uint8_t* from = src(r0 + i * kStep, in);
+                        w[i] = in ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0, 0, 0, 0);
+                    }
+                    #pragma unroll
+                    for (int i = 0; i < kPer; i++) {
+                        const int r = r0 + i * kStep;
+                        uint32_t x[4] = {w[i].x ^ sign, w[i].y ^ sign, w[i].z ^ sign, w[i].w ^ sign};
+                        if constexpr (QT == QWEN_BF16) {                   // into fp16's range, a power of two a row
+                            const uint32_t y = __vmaxu2(__vmaxu2(x[0] & 0x7fff7fffu, x[1] & 0x7fff7fffu), __vmaxu2(x[2] & 0x7fff7fffu, x[3] & 0x7fff7fffu));
+                            uint32_t m = max(y & 0xffffu, y >> 16);
+                            #pragma unroll
+                            for (int o = 1; o < kLanes; o <<= 1) m = max(m, __shfl_xor_sync(~0u, m, o));
+                            const int e = min(max((int)(m >> 7), 1), 253);
+                            const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+                            #pragma unroll
+                            for (int j = 0; j < 4; j++) x[j] = kv::half2_bits(bf_lo(x[j]) * down, bf_hi(x[j]) * down);
+                            if (part == 0) qf[r] = __uint_as_float((uint32_t)e << 23);
+                        }
+                        *reinterpret_cast<uint4*>(dst + r * 128 + (((part & 7) ^ (r & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+                    }
                 }
             }
             fence_async_smem();
@@ -508,10 +531,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                         sum1 += d;
                         if constexpr (L::k8) {
                             const float2 y = *reinterpret_cast<const float2*>(vs + c0 + x);
-                            a *= !tail || (m >> x & 1) ? y.x : 0.f;         // (an unseen row's scale may be NaN)
-                            d *= !tail || (m >> (x + 1) & 1) ? y.y : 0.f;
+                            a *= y.x;
+                            d *= y.y;
                         }
                         w[x / 2] = pack2<BF>(a, d);
+                    }
+                    if (L::k8 && tail) {   // (a scale that the row does not see may be NaN)
+                        #pragma unroll
+                        for (int x = 0; x < 32; x += 2)
+                            w[x / 2] &= (m >> x & 1 ? 0xffffu : 0u) | (m >> (x + 1) & 1 ? 0xffff0000u : 0u);
                     }
                     tc_st16(tmem + lanes + kTmP + 64 * b + 32 * half + c0 / 2, w);
                 }
@@ -526,7 +554,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
             {   // the next item's queries on their way while the last products run
                 auto nx = it;
                 if (nx.next(P)) {
-                    const int nrow = nx.r_base + rl, nnode = nrow / P.group;
+                    const int nrow = nx.r_base + rl, nnode = P.node_of(nrow);
                     if (nrow < M)
                         asm volatile("prefetch.global.L1 [%0];" ::"l"(P.q + (((size_t)nx.seq * P.n_nodes + nnode) * (size_t)P.ldq +
                                                                              (size_t)(nx.h * P.group + nrow - nnode * P.group) * D + half * (D / 2)) * 2));
@@ -594,7 +622,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                 uint8_t* out = P.out + ((size_t)it.seq * P.n_nodes * (size_t)P.ldo + (size_t)it.h * P.group * D + ch * 8) * 2;
                 #pragma unroll
                 for (int i = 0; i < kPer; i++) {
-                    const int orow = it.r_base + r0 + i * kStep, onode = orow / P.group;
+                    const int orow = it.r_base + r0 + i * kStep, onode = P.node_of(orow);
                     if (orow < M) *reinterpret_cast<uint4*>(out + ((size_t)onode * (size_t)P.ldo + (size_t)(orow - onode * P.group) * D) * 2) = w[i];
                 }
                 named_bar(2, kTcSoftmax);         // the queries' place is free again
