@@ -77,7 +77,6 @@ struct Shared {
     double run_sum[kWarps];          // the owner's second look: its runs' sums, last weighted tokens, the token
     int run_last[kWarps], found;
     uint64_t arrived[2][kWarps];     // a row buffer's bulk copies, per warp
-    int late;                        // a wait for them ran out
     float lx[kMaxNodes], qx[kMaxNodes], u[kMaxNodes];
     int par[kMaxNodes], tok[kMaxNodes], gone[kMaxNodes];   // gone: refused tokens at this node (chosen drafts)
 };
@@ -180,10 +179,11 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Params P) {
             else reinterpret_cast<uint16_t*>(dst)[k - lo] = __ldg((const uint16_t*)row + k);
         }
     };
-    // Waits for buffer b's part; a wait that runs out marks the sequence (next = -1) and goes on.
+    // Waits for buffer b's part; a wait that runs out marks the warp, whose word to the others then is NaN or +inf (next = -1).
+    bool late = false;
     auto landed = [&](int b) {
         if (coming >> b & 1) {
-            if (!mbar_wait(&sh.arrived[b][warp], phase >> b & 1, kWaitNs)) sh.late = 1;
+            if (!mbar_wait(&sh.arrived[b][warp], phase >> b & 1, kWaitNs)) late = true;
             phase ^= 1u << b;
             coming &= ~(1u << b);
         }
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Params P) {
         sh.tok[tid] = N > 1 ? P.tokens[(size_t)seq * N + tid] : 0;
         sh.u[tid] = greedy ? 0.f : P.uniforms[(size_t)seq * N + tid];
     }
-    if (tid == 0) { sh.found = INT_MAX; sh.late = 0; }
+    if (tid == 0) sh.found = INT_MAX;
     int* path = P.path + (size_t)seq * N;
     if (rank == 0 && tid < N) path[tid] = -1;
     __syncthreads();         // (path's -1 come before its entries)
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Params P) {
         if (HELD && next_row && P.buffers == 1) inside = child;
         if (!greedy) bad = z != z;
         // the warp's, then the cluster's: the largest first, then the sums on its scale.  A warp that met a NaN says +inf.
-        float M = max_lanes(__any_sync(~0u, bad) ? INFINITY : m);
+        float M = max_lanes(__any_sync(~0u, bad || late) ? INFINITY : m);
         {
             uint64_t* box = sh.box[turn & 1];
             turn++;
@@ -401,7 +401,10 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Params P) {
             for (int g = 0; g < n_gone; g++) if (sh.gone[g] == i) return true;
             return false;
         };
-        const uint64_t* sums = nullptr;   // the parts' sums of rest, of the last sum pass
+        // of the last sum pass: the parts' sums of rest, lane * per .. of them this lane's; their sum and the running sum
+        const uint64_t* sums = nullptr;
+        const int per = (parts + 31) / 32;
+        double lane_sum = 0.0, lane_run = 0.0;
         auto sum_pass = [&]() {
             if (HELD && P.buffers == 1 && inside != at) {
                 landed(0);
@@ -412,14 +415,15 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Params P) {
             double sum[8] = {};
             bool any = false;
             for (int g = 0; g < n_gone; g++) any |= sh.gone[g] >= lo && sh.gone[g] < hi;
-            for (int i0 = lo; i0 < hi; i0 += 2 * kRun) {
-                float x[8], q[8];
-                double e[8];
-                bool in[8];
+            auto add = [&](int i0, auto& x) {   // the step of sizeof(x) / 16 runs
+                constexpr int kN = sizeof(x) / 4;
+                float q[kN];
+                double e[kN];
+                bool in[kN];
                 step(i0, x);
                 if (S > 0.0) {
                     #pragma unroll
-                    for (int k = 0; k < 2; k++) {
+                    for (int k = 0; k < kN / 4; k++) {
                         float y[4];
                         load4<QWEN_FP32>(qrow, i0 + kRun * k + 4 * lane, hi, vec, 0.f, y);
                         #pragma unroll
@@ -429,24 +433,37 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Params P) {
                 weights(x, q, e, in);
                 if (any) {
                     #pragma unroll
-                    for (int j = 0; j < 8; j++) if (is_gone(i0 + kRun * (j >> 2) + 4 * lane + (j & 3))) in[j] = false;
+                    for (int j = 0; j < kN; j++) if (is_gone(i0 + kRun * (j >> 2) + 4 * lane + (j & 3))) in[j] = false;
                 }
                 #pragma unroll
-                for (int j = 0; j < 8; j++) if (in[j]) sum[j] += e[j];
-            }
+                for (int j = 0; j < kN; j++) if (in[j]) sum[j] += e[j];
+            };
+            int i0 = lo;
+            for (; i0 + kRun < hi; i0 += 2 * kRun) { float x[8]; add(i0, x); }
+            if (i0 < hi) { float x[4]; add(i0, x); }
             double s = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
             #pragma unroll
             for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
             uint64_t* box = sh.box[turn & 1];
             turn++;
-            if (lane < size) st_cluster(box + mine, lane, (uint64_t)__double_as_longlong(s));
+            if (lane < size) st_cluster(box + mine, lane, (uint64_t)__double_as_longlong(late ? NAN : s));
             cluster_sync();
-            double t = 0.0;
-            for (int i = lane; i < parts; i += 32) t += __longlong_as_double((long long)box[i]);
+            double t[kMaxParts / 32];
             #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
+            for (int k = 0; k < kMaxParts / 32; k++)
+                t[k] = k < per && lane * per + k < parts ? __longlong_as_double((long long)box[lane * per + k]) : 0.0;
+            #pragma unroll
+            for (int o = kMaxParts / 64; o > 0; o >>= 1)
+                #pragma unroll
+                for (int k = 0; k < o; k++) t[k] += t[k + o];
+            lane_sum = lane_run = t[0];
+            #pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double y = __shfl_up_sync(~0u, lane_run, o);
+                if (lane >= o) lane_run += y;
+            }
             sums = box;
-            return t;
+            return __shfl_sync(~0u, lane_run, 31);
         };
         for (; children && kept < 0 && !none; children &= children - 1) {
             const int i = __ffsll((long long)children) - 1, x = sh.tok[i];
@@ -497,42 +514,31 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Params P) {
             n_gone = 0;
             total = sum_pass();
         }
+        if (!(total > 0.0)) {   // (a wait that ran out)
+            if (rank == 0 && tid == 0) P.next[seq] = -1;
+            break;
+        }
         // the part in which the running sum crosses the target, or else the last one with any weight
         const double target = (double)sh.u[0] * total;
-        double run;              // the sum before the owner's part
-        int owner;
-        bool over;               // nothing crosses: the last token with any weight
-        {
-            double part_sum[kMaxParts / 32], mine_sum = 0.0;
-            const int per = (parts + 31) / 32;
-            int last = -1;
-            #pragma unroll
-            for (int k = 0; k < kMaxParts / 32; k++) {
-                const int p = lane * per + k;
-                part_sum[k] = k < per && p < parts ? __longlong_as_double((long long)sums[p]) : 0.0;
-                mine_sum += part_sum[k];
-                if (part_sum[k] > 0.0) last = p;
+        const uint32_t some = __ballot_sync(~0u, lane_sum > 0.0), cross = __ballot_sync(~0u, lane_sum > 0.0 && lane_run > target);
+        const bool over = cross == 0;              // nothing crosses: the last token with any weight
+        const int at_lane = over ? 31 - __clz(some) : __ffs(cross) - 1;
+        int owner = -1;
+        double run = lane_run - lane_sum;          // the sum before the owner's part
+        if (lane == at_lane) {
+            double before = run;
+            for (int k = 0; k < per && lane * per + k < parts; k++) {
+                const double w = __longlong_as_double((long long)sums[lane * per + k]);
+                if (w > 0.0) {
+                    owner = lane * per + k;
+                    run = before;
+                    if (!over && before + w > target) break;
+                }
+                before += w;
             }
-            double inc = mine_sum;
-            #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double y = __shfl_up_sync(~0u, inc, o);
-                if (lane >= o) inc += y;
-            }
-            double before = inc - mine_sum;
-            int first = INT_MAX;
-            double first_run = 0.0;
-            #pragma unroll
-            for (int k = 0; k < kMaxParts / 32; k++) {
-                if (first == INT_MAX && part_sum[k] > 0.0 && before + part_sum[k] > target) { first = lane * per + k; first_run = before; }
-                before += part_sum[k];
-            }
-            owner = __reduce_min_sync(~0u, first);
-            last = __reduce_max_sync(~0u, last);
-            over = owner == INT_MAX;
-            if (over) owner = last;
-            run = __shfl_sync(~0u, first_run, min(owner / per, 31));
         }
+        owner = __shfl_sync(~0u, owner, at_lane);
+        run = __shfl_sync(~0u, run, at_lane);
         if (owner / kWarps == rank) {
             // the CTA's warps share the owner's part: run k of each round of kWarps runs
             const int o0 = (int)((long long)runs * owner / parts) * kRun, o1 = min((int)((long long)runs * (owner + 1) / parts) * kRun, V);
@@ -609,8 +615,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Params P) {
         landed(0);
         landed(1);
     }
-    cluster_sync();   // no CTA leaves while another may still write to its box
-    if (tid == 0 && sh.late) P.next[seq] = -1;
+    // (a CTA's last writes to another's box came before a cluster barrier that both have passed)
 }
 
 }  // namespace tv
