@@ -137,6 +137,33 @@ def test_append_codes_are_the_nearest(qb, store, src, kind, b, t, kv, dim):
         assert torch.equal(after[2 + i], before[2 + i])
 
 
+@pytest.mark.parametrize("store,src,dim,t", [("e4m3", "bf16", 128, 5501), ("int8", "fp16", 128, 5469), ("int8", "bf16", 64, 10977), ("e4m3", "fp32", 64, 10923),
+                                             ("bf16", "bf16", 128, 5501)])
+def test_append_many_rows(qb, store, src, dim, t):
+    """Prompts of several sequences, none of a whole number of blocks: every row, and nothing beside them."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(t)
+    kind_src, dtype = _types(qb)[src]
+    b, kv = 3, 8
+    c = Cache(qb, b, kv, t + 2, dim, store, room=1)
+    x = [_rows(g, (b, t, kv * dim), dtype, "ties" if store == "e4m3" else "normal") for _ in range(2)]
+    start, counts = np.array([2, 0, 5], np.int32), np.array([t, t - 1001, t], np.int32)     # the last sequence runs out of the cache
+    st, ct = _dev(start), _dev(counts)
+    qb.kv_append(c.view, x[0].data_ptr(), x[1].data_ptr(), kind_src, kv * dim, t, st.data_ptr(), ct.data_ptr(), _stream())
+    for rows, got, all_, scale, sc_all in ((x[0], c.k, c.k_all, c.ks, c.ks_all), (x[1], c.v, c.v_all, c.vs, c.vs_all)):
+        for r in range(b):
+            s, n = int(start[r]), min(int(counts[r]), c.cap - int(start[r]))
+            y = rows[r, :n].view(n, kv, dim).transpose(0, 1)
+            if scale is None:
+                assert torch.equal(got[r, :, s:s + n], y.to(c.dtype))
+            else:
+                want, a = _codes64(y.double(), store)
+                assert torch.equal(got[r, :, s:s + n].float(), want.float()) and torch.equal(scale[r, :, s:s + n], a[..., 0].float())
+                sc_all[r, :kv, s:s + n] = -7.0
+            all_.view(torch.uint8)[r, :kv, s:s + n] = DIRTY
+        assert bool((all_.view(torch.uint8) == DIRTY).all()) and (scale is None or bool((sc_all == -7.0).all()))
+
+
 @pytest.mark.parametrize("store", ["e4m3", "int8", "bf16", "fp16"])
 @pytest.mark.parametrize("dst", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("b,t,kv,dim", [(3, 41, 2, 128), (4, 1, 3, 64)])
@@ -428,6 +455,39 @@ def test_attention_many_sequences(qb):
     q = torch.randn(b, t, 6, 64, generator=g, device="cuda").to(torch.bfloat16)
     rng = np.random.RandomState(8)
     lens = np.where(rng.rand(b) < 0.2, rng.randint(0, 138, b), rng.randint(-1, 3, b))
+    _check_attention(qb, c, q, lens, _tree(rng, b, t, absent=True), 0.125)
+
+
+@pytest.mark.parametrize("store", ["16", "e4m3", "int8"])
+@pytest.mark.parametrize("t,group,dim,qt", [(1, 1, 64, "bf16"), (1, 2, 128, "fp16"), (5, 3, 64, "bf16"), (16, 2, 128, "bf16"), (11, 4, 128, "fp16"), (64, 2, 128, "bf16"),
+                                            (64, 1, 64, "fp16"), (64, 7, 128, "bf16"), (33, 16, 64, "fp16")])
+def test_attention_shared_out(qb, store, t, group, dim, qt):
+    """Caches long enough that the sequences' tiles are shared out over all SMs: idle, empty, short and long sequences among each
+    other, lengths on both sides of a tile's end, several blocks of rows, absent nodes, nodes past the capacity."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(t * 7 + group)
+    cap = 1400
+    lens = [0, 1400 - t, -1, 1, 511, 512, 513, cap + 5, 640, 1100, 127, 128, 129, cap - 1, 3, 1024 - t]
+    c = Cache(qb, len(lens), 2, cap, dim, qt if store == "16" else store, room=5).fill(g)
+    assert qb.tree_attention_workspace(c.view, t, 2 * group) > 0
+    q = torch.randn(len(lens), t, 2 * group, dim, generator=g, device="cuda").to(_types(qb)[qt][1])
+    par = _tree(np.random.RandomState(t), len(lens), t, absent=t > 4)
+    _check_attention(qb, c, q, lens, par, 1 / math.sqrt(dim), ldq=2 * group * dim + 24, ldo=2 * group * dim + 8)
+
+
+@pytest.mark.parametrize("b,t,group,cap,dim,store", [(333, 3, 3, 700, 64, "bf16"), (129, 1, 2, 600, 128, "e4m3"), (150, 40, 1, 600, 64, "int8"),
+                                                     (131, 9, 4, 520, 128, "bf16"), (1, 64, 300, 600, 64, "bf16"), (2, 64, 301, 520, 64, "e4m3")])
+def test_attention_shared_out_widely(qb, b, t, group, cap, dim, store):
+    """More sequences than a block keeps the lengths of, most of them short; more blocks of rows than SMs."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(4)
+    c = Cache(qb, b, 1, cap, dim, store).fill(g)
+    assert qb.tree_attention_workspace(c.view, t, group) > 0
+    q = torch.randn(b, t, group, dim, generator=g, device="cuda").to(torch.bfloat16)
+    rng = np.random.RandomState(8)
+    lens = np.where(rng.rand(b) < 0.2, rng.randint(0, cap - 1, b), rng.randint(-1, 3, b))
+    if b < 3:
+        lens[:] = cap - t - 3
     _check_attention(qb, c, q, lens, _tree(rng, b, t, absent=True), 0.125)
 
 
@@ -783,16 +843,17 @@ def _result(s):
     return [x.clone() for x in (s["out"], s["path"], s["n_path"], s["next"], *s["back"])]
 
 
+@pytest.mark.parametrize("length,t", [(150, 8), (1500, 8), (1500, 40)])
 @pytest.mark.parametrize("store", ["bf16", "e4m3"])
-def test_captured_step_follows_its_inputs(qb, store):
+def test_captured_step_follows_its_inputs(qb, store, length, t):
     """The step captured into a CUDA graph and replayed on other inputs, lengths and trees equals the eager step bit for bit."""
     import torch
-    a, other = _step_buffers(qb, store, 1), _step_buffers(qb, store, 2)
+    a, other = _step_buffers(qb, store, 1, t=t, length=length), _step_buffers(qb, store, 2, t=t, length=length)
     _step(qb, a, _stream())                                        # (also: kernels are loaded before the capture)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         _step(qb, a, _stream())
-    other["lens"] = _dev(np.array([17, 149, 0], np.int32))
+    other["lens"] = _dev(np.array([17, length - 1, 0], np.int32))
     for n in ("k", "v", "q", "lens", "logits", "tokens", "parents", "u"):
         a[n].copy_(other[n])
     for x, y in ((a["c"].k, other["c"].k), (a["c"].v, other["c"].v), (a["c"].ks, other["c"].ks), (a["c"].vs, other["c"].vs)):
@@ -809,17 +870,18 @@ def test_captured_step_follows_its_inputs(qb, store):
     graph.reset()
 
 
-def test_two_streams_and_repeats(qb):
+@pytest.mark.parametrize("length,t", [(150, 8), (1500, 8), (1500, 40)])
+def test_two_streams_and_repeats(qb, length, t):
     """Steps on two streams at once, each with its own workspace, give what they give alone, every time."""
     import torch
     alone = []
     for seed in (3, 4):
-        s = _step_buffers(qb, "int8", seed)
+        s = _step_buffers(qb, "int8", seed, t=t, length=length)
         _step(qb, s, _stream())
         torch.cuda.synchronize()
         alone.append(_result(s))
     for _ in range(5):
-        states, streams = [_step_buffers(qb, "int8", seed) for seed in (3, 4)], [torch.cuda.Stream() for _ in range(2)]
+        states, streams = [_step_buffers(qb, "int8", seed, t=t, length=length) for seed in (3, 4)], [torch.cuda.Stream() for _ in range(2)]
         torch.cuda.synchronize()
         for s, st in zip(states, streams):
             _step(qb, s, st.cuda_stream)
