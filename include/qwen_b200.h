@@ -396,6 +396,7 @@ int qwen_row_topk(const float* logits, int rows, int n, int ld, int k, float* va
  * nothing, copy nothing from or to the host and may be captured.  Lengths,
  * trees and counts are read on the device, so a captured call follows them;
  * whatever they hold, nothing outside the described buffers is touched.
+ * What a call writes overlaps nothing else that it takes.
  * Sequences are the rows 0 .. n_seqs - 1 of the view (at most 65535).
  *
  * A tree of n_nodes drafted tokens (1 .. 64) is given by parents[seq][node]:
@@ -429,7 +430,7 @@ int qwen_batch_cache(qwen_t* ctx, int layer, qwen_kv_cache_t* out);
 /* Rows into the cache: token t (0 .. n_tokens-1) of sequence s, at k + (s *
  * n_tokens + t) * ld elements (head h at + h * head_dim; ld a multiple of 8,
  * at least n_kv_heads * head_dim), becomes position start[s] + t, for t <
- * counts[s] (counts NULL: all).  src_dtype QWEN_BF16, QWEN_FP16 or QWEN_FP32.
+ * counts[s] (counts NULL: all; n_tokens at most the capacity).  src_dtype QWEN_BF16, QWEN_FP16 or QWEN_FP32.
  * A row of an 8-bit cache with largest magnitude a (at least 2^-60) gets the
  * scale a / 448 (QWEN_E4M3) or a / 127 (QWEN_INT8), rounded once to fp32, and
  * each code is the nearest one to x * 448 / a (x * 127 / a), ties to even; a
@@ -462,7 +463,7 @@ int qwen_tree_attention_workspace(const qwen_kv_cache_t* cache, int n_nodes, int
  * i already hold the nodes' own K and V (qwen_kv_append): node i of sequence s
  * attends to positions 0 .. lens[s]-1, to its ancestors and to itself,
  * o = sum_j softmax_j(scale * q . k_j) v_j, and query head h to K/V head
- * h / (n_heads / n_kv_heads).  One root and no other node is an ordinary decode
+ * h / (n_heads / n_kv_heads), at most 2^14 for each.  One root and no other node is an ordinary decode
  * step; a chain of nodes is a causal step of several tokens.  q and out are
  * [n_seqs][n_nodes][n_heads][head_dim] with ldq and ldo elements between nodes
  * (multiples of 8, at least n_heads * head_dim), dtype QWEN_BF16 or QWEN_FP16, that of
@@ -470,7 +471,9 @@ int qwen_tree_attention_workspace(const qwen_kv_cache_t* cache, int n_nodes, int
  * position lies outside the cache, and all nodes of sequences with lens[s] < 0,
  * are absent.  What positions that a node does not see hold (NaN included) has
  * no influence on it.  Scores, softmax statistics and sums are fp32; the
- * weights enter the product with V in 16 bits.  workspace: as many bytes as
+ * weights enter the product with V in 16 bits (8-bit caches: weight * scale, as
+ * fp16 relative to the row's largest scale so far, or to 2^-90 where all are
+ * smaller; qwen_kv_append makes none below 2^-69).  workspace: as many bytes as
  * qwen_tree_attention_workspace says, contents free, 16-byte aligned (may be
  * NULL where it says 0); calls that may overlap need one each.  The rows of a
  * call whose device-side waits ran out (they are bounded) are NaN. */
@@ -499,7 +502,7 @@ int qwen_tree_attention(const qwen_kv_cache_t* cache, const void* q, void* out, 
  * smaller token), draft and uniforms are not read and may be NULL.  Tokens cut
  * by top-k or top-p enter with logits of -inf.  A row with a NaN, a +inf or
  * nothing above -inf has no distribution: no child is kept there and next[s] =
- * -1.  Outputs: path[s][n_nodes] the kept nodes from node 0 on, then -1;
+ * -1 (also where a device-side wait, which is bounded, ran out).  Outputs: path[s][n_nodes] the kept nodes from node 0 on, then -1;
  * n_path[s] their number (0, and next -1, if node 0 is not a root); next[s].
  * temperature is 0 or within 1e-6 .. 1e6. */
 int qwen_tree_verify(const void* logits, int logits_dtype, long long ld, const float* draft, long long ld_draft, const int* tokens,

@@ -317,7 +317,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) { return BF ? cvt_
 // fp16's range (bf16 queries; the factor returns with the score), a key's scale
 // multiplies its scores, a value row's scale its weights, divided by a power of
 // two that is at least the largest scale so far, so the weights stay within
-// fp16.  P is rounded to 16 bits (half a step: 2^-9 or 2^-12 relative) as
+// fp16.  P is rounded to 16 bits (off by half a step: 2^-8 or 2^-11 relative) as
 // the product with V takes it; l sums it unrounded.
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kItemCost = 2;   // what an item costs beside its tiles, in tiles: set-up, queries, joining the warps
