@@ -41,6 +41,7 @@ struct Params {
     long long ldq, ldo;
     int n_seqs, n_kv_heads, group, n_nodes;
     int whole;                // a CTA for each item: CTA (sequence * n_kv_heads + head) * row_blocks + block
+    int groups, by_item;      // shares of the line; combine_kernel's blocks are for the items (else: for the shares)
     int row_blocks, beside;   // blocks of rows that a K/V head has; CTAs side by side on a share (row_blocks, or 1 where that is more than the grid)
     float scale_log2;   // scale * log2(e)
     float per_group;    // 1 / group
@@ -97,6 +98,15 @@ struct Line {
         for (int k = 0; k < kHeld / 32; k++) n += positions(P, lane + 32 * k, len[k]);
         for (int s = kHeld + lane; s < P.n_seqs; s += 32) n += positions(P, s, P.lens[s]);
         shares = Shares(__reduce_add_sync(~0u, n), groups);
+    }
+    // The positions before sequence s.
+    __device__ __forceinline__ int before(const Params& P, int s) const {
+        const int lane = threadIdx.x & 31;
+        int n = 0;
+        #pragma unroll
+        for (int k = 0; k < kHeld / 32; k++) n += lane + 32 * k < s ? positions(P, lane + 32 * k, len[k]) : 0;
+        for (int i = kHeld + lane; i < s; i += 32) n += positions(P, i, P.lens[i]);
+        return __reduce_add_sync(~0u, n);
     }
     // The sequence that position x (below shares.n) belongs to, the positions before it, its length.
     __device__ __forceinline__ int find(const Params& P, int x, int& before, int& length) const {
@@ -783,7 +793,8 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attentio
 }
 
 // Joins the partial results of the items that cross a border between shares:
-// blocks (i, y) take the item that begins in CTA i's share and goes on in the next.
+// blocks (x, y) take item x, or where there are more items than shares the one that
+// begins in share x and goes on in the next.
 // ACROSS: a slot holds O as [dim / 4][row] (the tensor-memory kernel: a thread a
 // row) and a thread here joins 8 dims of a row, lanes along the rows; otherwise O
 // is [row][dim] and a thread joins 4 dims, lanes along the dims.
@@ -795,23 +806,33 @@ __global__ void __launch_bounds__(kJoinThreads, 6) combine_kernel(const Params P
     constexpr int kSlot = ROWS * (D + 2), kVec = ACROSS ? 2 : 1, kAhead = ACROSS ? 5 : 8;   // float4s a thread; partial results loaded at once
     const int beside = P.beside, unit_blocks = beside == 1 ? P.row_blocks : 1, units = P.n_kv_heads * unit_blocks;
     const int i = blockIdx.x / beside, lane = blockIdx.x - i * beside;
-    const Line<KT, COST> line(P, units, gridDim.x / beside);
+    int s = 0, e = 0, seq, unit = 0;            // the item: its positions
+    const Line<KT, COST> line(P, units, P.groups);
     const Shares& shares = line.shares;
-    const int from = shares.begin(i), edge = shares.begin(i + 1);
-    int before = 0, s = edge, e = edge;   // the item at the border: its positions
-    int seq = 0, unit = 0;
-    if (edge > from && edge < shares.n) {
-        int len;
-        seq = line.find(P, edge, before, len);
-        const int per = seq_tiles<KT>(P, len) + COST;
-        unit = (int)((unsigned)(edge - before) / (unsigned)per);
-        s = before + unit * per;
+    if (P.by_item) {
+        seq = i / units;
+        unit = i - seq * units;
+        const int per = seq_tiles<KT>(P, P.lens[seq]) + COST;
+        s = line.before(P, seq) + unit * per;
         e = s + per;
+    } else {
+        const int from = shares.begin(i), edge = shares.begin(i + 1);
+        seq = 0;
+        if (edge > from && edge < shares.n) {
+            int before, len;
+            seq = line.find(P, edge, before, len);
+            const int per = seq_tiles<KT>(P, len) + COST;
+            unit = (int)((unsigned)(edge - before) / (unsigned)per);
+            s = before + unit * per;
+            e = s + per;
+            if (s >= edge || s < from) e = s;   // it begins at the border, or before this share
+        }
     }
     pdl_wait();   // on every path: this kernel may not end before the one that it joins
-    if (s >= edge || s < from) return;          // it begins at the border, or before this share
+    if (s >= e) return;
     const int begun = shares.of(s + COST), last = shares.of(e - 1);   // the shares with its tiles
     if (begun == last) return;                  // one has them all and has written the rows
+    const bool second = shares.begin(begun) < s;   // a share that begins before the item holds it in its second slot
     const int t = blockIdx.y * kJoinThreads + threadIdx.x;
     const int h = unit / unit_blocks, r = ACROSS ? t % ROWS : t / (D / 4), d = ACROSS ? t / ROWS * 8 : t % (D / 4) * 4;
     const int row = (unit - h * unit_blocks + lane) * ROWS + r;
@@ -830,8 +851,7 @@ __global__ void __launch_bounds__(kJoinThreads, 6) combine_kernel(const Params P
             #pragma unroll
             for (int v = 0; v < kVec; v++) b[j][v] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (k > last) continue;
-            // a share that begins before the item holds it in its second slot
-            const float* slot = P.work + (2 * ((size_t)k * beside + lane) + (k == i && from < s ? 1 : 0)) * kSlot;
+            const float* slot = P.work + (2 * ((size_t)k * beside + lane) + (k == begun && second ? 1 : 0)) * kSlot;
             ml[j] = *reinterpret_cast<const float2*>(slot + ROWS * D + 2 * r);
             #pragma unroll
             for (int v = 0; v < kVec; v++) b[j][v] = *reinterpret_cast<const float4*>(ACROSS ? slot + ((d / 4 + v) * ROWS + r) * 4 : slot + r * D + d);
