@@ -464,7 +464,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                 const bool tail = k0 + 64 > it.len;
                 // bit x: the row sees column x of this half
                 const uint64_t vis = tail ? visible(see, it.len - k0) : ~0ull;
-                // scores of columns c0 .. c0 + 31 of this half (read twice: for the maximum, and for the exponentials)
+                // scores of columns c0 .. c0 + 31 of this half (of the first 32 read twice: for the maximum, and for the exponentials)
                 auto scores = [&](int c0, float (&v)[32]) {
                     tmem_ld32(tmem + lanes + 128 * b + 64 * half + c0, v);
                     if constexpr (L::k8) {
@@ -480,10 +480,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                         for (int x = 0; x < 32; x++) if (!(m >> x & 1)) v[x] = -INFINITY;
                     }
                 };
-                float mx = -INFINITY;
+                float mx = -INFINITY, v[32];                               // v stays: columns 32 .. 63
                 #pragma unroll 1
                 for (int c0 = 0; c0 < 64; c0 += 32) {
-                    float v[32], my = -INFINITY;
+                    float my = -INFINITY;
                     scores(c0, v);
                     #pragma unroll
                     for (int x = 0; x < 32; x += 4) { mx = max3(mx, v[x], v[x + 1]); my = max3(my, v[x + 2], v[x + 3]); }
@@ -519,9 +519,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                 tc_fence_after();
                 float sum0 = 0.f, sum1 = 0.f;
                 #pragma unroll 1
-                for (int c0 = 0; c0 < 64; c0 += 32) {
-                    float v[32];
-                    scores(c0, v);
+                for (int c0 = 32; c0 >= 0; c0 -= 32) {
+                    if (c0 == 0) scores(0, v);
                     uint32_t w[16];
                     const uint32_t m = (uint32_t)(vis >> c0);
                     #pragma unroll
