@@ -456,7 +456,7 @@ int qwen_kv_read(const qwen_kv_cache_t* cache, void* k, void* v, int dst_dtype, 
  * then holds start[s] + n_path[s] positions. */
 int qwen_kv_keep(const qwen_kv_cache_t* cache, const int* start, const int* path, const int* n_path, int n_nodes, void* stream);
 
-/* Bytes of workspace that qwen_tree_attention needs for these sizes (0 for caches of a few hundred positions). */
+/* Bytes of workspace that qwen_tree_attention needs for these sizes (0 for short caches). */
 int qwen_tree_attention_workspace(const qwen_kv_cache_t* cache, int n_nodes, int n_heads, size_t* bytes);
 
 /* Attention of a tree of drafted tokens over a cache whose positions lens[s] +

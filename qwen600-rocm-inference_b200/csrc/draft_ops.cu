@@ -174,7 +174,10 @@ int attention_rows(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : 128; }
 
 struct Plan {
     int rows, row_blocks, beside, shares;   // shares: CTAs, beside for each share of the line
-    bool whole;                             // a CTA for each item, no joining
+    int tiles;                              // of a cache's capacity
+    long long items;                        // sequences, K/V heads and blocks of rows
+    float spare;
+    bool whole, may_be_whole;               // a CTA for each item, no joining
     size_t bytes;
 };
 int check_tree(const qwen_kv_cache_t* c, int n_nodes, int n_heads) {
@@ -183,33 +186,41 @@ int check_tree(const qwen_kv_cache_t* c, int n_nodes, int n_heads) {
     if (n_heads / c->n_kv_heads > 1 << 14) return fail(QWEN_E_UNSUPPORTED, "more than 2^14 query heads for each K/V head");
     return QWEN_OK;
 }
-// What the plan has without the device: rows, row_blocks, whole.
+// What the plan has without the device.  Caches of a few tiles have a CTA for each item: sharing the tiles out would spare a
+// CTA all but items * tiles / CTAs of them, about 0.5 us each (1.3 us in the tensor-memory kernel), and joining costs 3.5 to 4.5
+// us.  Measured, a CTA for each item against shares (bf16, 8 K/V heads): 1 sequence of 500 8.5 / 7.1 us, 8 of 500 8.7 / 10.8,
+// 8 of 1000 14.4 / 12.5, 32 of 1000 19.2 / 21.4; 64 nodes: 1 sequence of 440 12.7 / 11.7, 4 of 440 13.0 / 14.7, 4 of 900
+// 19.3 / 16.5.  Longer caches are shared out in any case, so that ragged lengths balance.
 void attention_shape(const qwen_kv_cache_t* c, int n_nodes, int n_heads, Plan* p) {
     const int m = n_nodes * (n_heads / c->n_kv_heads);
     p->rows = attention_rows(m);
     p->row_blocks = (m + p->rows - 1) / p->rows;
-    // A few tiles: a CTA for each item.  Spreading them over several CTAs saves at most the time of all but one (about 0.5 us
-    // each, 1.3 us in the tensor-memory kernel), joining costs a second launch (5 us in all).
-    const int keys = p->rows <= 32 ? 64 : 128;
-    const long long tiles = (c->capacity + keys - 1) / keys, items = (long long)c->n_seqs * c->n_kv_heads * p->row_blocks;
-    p->whole = tiles <= (p->rows <= 32 ? 8 : 4) && items < 1 << 30;
+    const bool tc = p->rows > 32;
+    p->tiles = (c->capacity + (tc ? 127 : 63)) / (tc ? 128 : 64);
+    p->items = (long long)c->n_seqs * c->n_kv_heads * p->row_blocks;
+    p->spare = tc ? 3.4f : 7.0f;      // so many tiles are worth the joining
+    p->whole = p->tiles <= p->spare && p->items < 1 << 30;
+    p->may_be_whole = p->tiles <= (tc ? 8 : 16) && p->items < 1 << 30;
 }
 int attention_plan(const qwen_kv_cache_t* c, int n_nodes, int n_heads, int dev, Plan* p) {
     attention_shape(c, n_nodes, n_heads, p);
+    int nsm = 0, ctas = 0;
+    if (!p->whole) {
+        TRY(sm_count(dev, &nsm));
+        ctas = p->rows <= 32 ? qb::ta::attention_ctas(p->rows, c->head_dim) * nsm : nsm;
+        p->whole = p->may_be_whole && (double)p->tiles * std::max(0ll, ctas - p->items) <= (double)p->spare * ctas;
+    }
     if (p->whole) {
         p->beside = p->row_blocks;
-        p->shares = c->n_seqs * c->n_kv_heads * p->row_blocks;
+        p->shares = (int)p->items;
         p->bytes = 0;
         return QWEN_OK;
     }
-    int nsm = 0;
-    TRY(sm_count(dev, &nsm));
     // as many CTAs as the SMs hold (the tensor-memory kernel: one each), shared out over the blocks of rows that walk side by side
-    const int keys = p->rows <= 32 ? 64 : 128, ctas = p->rows <= 32 ? qb::ta::attention_ctas(p->rows, c->head_dim) * nsm : nsm;
     p->beside = p->row_blocks <= ctas ? p->row_blocks : 1;
     // no more shares than the line can have positions
     const double most = (double)c->n_seqs * c->n_kv_heads * (p->row_blocks / p->beside) *
-                        ((c->capacity + keys - 1) / keys + qb::ta::kTcItemCost);
+                        (p->tiles + qb::ta::kTcItemCost);
     p->shares = (int)std::min((double)(ctas / p->beside), most) * p->beside;
     if (most >= 2147483648.0) return fail(QWEN_E_UNSUPPORTED, "too many sequences, heads and positions for one call");
     p->bytes = (size_t)2 * p->shares * p->rows * (c->head_dim + 2) * sizeof(float);
@@ -386,8 +397,9 @@ extern "C" int qwen_tree_attention(const qwen_kv_cache_t* cache, const void* q, 
     Plan plan;
     attention_shape(cache, n_nodes, n_heads, &plan);
     TRY(check_ptrs({QB_VIEW_PTRS(cache), {q, "q", 16, true}, {out, "out", 16, true}, {lens, "lens", 4, true}, {parents, "parents", 4, true},
-                    {workspace, "workspace", 16, workspace || !plan.whole}}, &dev));
+                    {workspace, "workspace", 16, workspace || !plan.may_be_whole}}, &dev));
     TRY(attention_plan(cache, n_nodes, n_heads, dev, &plan));
+    if (plan.bytes && !workspace) return fail(QWEN_E_ARG, "workspace is NULL");
     if (workspace_bytes < plan.bytes) return fail(QWEN_E_ARG, "workspace is smaller than qwen_tree_attention_workspace says");
     qb::ta::Params P;
     P.cache = device_view(cache);

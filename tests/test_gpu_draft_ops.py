@@ -475,8 +475,8 @@ def test_attention_shared_out(qb, store, t, group, dim, qt):
     _check_attention(qb, c, q, lens, par, 1 / math.sqrt(dim), ldq=2 * group * dim + 24, ldo=2 * group * dim + 8)
 
 
-@pytest.mark.parametrize("b,t,group,cap,dim,store", [(333, 3, 3, 700, 64, "bf16"), (129, 1, 2, 600, 128, "e4m3"), (150, 40, 1, 600, 64, "int8"),
-                                                     (131, 9, 4, 520, 128, "bf16"), (1, 64, 300, 600, 64, "bf16"), (2, 64, 301, 520, 64, "e4m3")])
+@pytest.mark.parametrize("b,t,group,cap,dim,store", [(333, 3, 3, 1100, 64, "bf16"), (129, 1, 2, 1090, 128, "e4m3"), (150, 40, 1, 1030, 64, "int8"),
+                                                     (131, 9, 4, 1025, 128, "bf16"), (1, 64, 300, 1100, 64, "bf16"), (2, 64, 301, 1030, 64, "e4m3")])
 def test_attention_shared_out_widely(qb, b, t, group, cap, dim, store):
     """More sequences than a block keeps the lengths of, most of them short; more blocks of rows than SMs."""
     import torch
@@ -488,6 +488,21 @@ def test_attention_shared_out_widely(qb, b, t, group, cap, dim, store):
     lens = np.where(rng.rand(b) < 0.2, rng.randint(0, cap - 1, b), rng.randint(-1, 3, b))
     if b < 3:
         lens[:] = cap - t - 3
+    _check_attention(qb, c, q, lens, _tree(rng, b, t, absent=True), 0.125)
+
+
+@pytest.mark.parametrize("b,t,group,cap,dim,store", [(460, 1, 2, 1024, 64, "bf16"), (450, 3, 2, 1000, 128, "int8"), (310, 4, 8, 1024, 128, "e4m3"), (150, 33, 1, 1024, 128, "bf16"),
+                                                     (150, 20, 2, 1000, 64, "e4m3")])
+def test_attention_without_workspace(qb, b, t, group, cap, dim, store):
+    """As many short caches as there are blocks: each is attended to by one, and no workspace is needed."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(4)
+    c = Cache(qb, b, 1, cap, dim, store).fill(g)
+    assert qb.tree_attention_workspace(c.view, t, group) == 0
+    q = torch.randn(b, t, group, dim, generator=g, device="cuda").to(torch.bfloat16)
+    rng = np.random.RandomState(8)
+    lens = np.where(rng.rand(b) < 0.2, rng.randint(0, cap - 1, b), rng.randint(-1, 3, b))
+    lens[0] = cap - t
     _check_attention(qb, c, q, lens, _tree(rng, b, t, absent=True), 0.125)
 
 
