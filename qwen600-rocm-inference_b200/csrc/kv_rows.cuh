@@ -3,7 +3,10 @@
 // counterpart (the reference's cache is bf16 and written by its RoPE kernel,
 // qwen_model.cuh:321-347).
 //
-// All three are bound by memory traffic: a row is read once and written once.
+// All three are bound by memory traffic where there is enough of it, a row being
+// read once and written once (prompts of 16 x 2048 tokens to int8 and back: 69 us,
+// 53 us at the copy rate), and by their chains of loads where there is not (128
+// tokens in and out 3.7 us, the kept rows of one sequence in 28 layers 2.8 us).
 // A thread owns 16 elements of a row (one 16-byte store of 8-bit codes), 4 or 8
 // neighbouring threads the row, so the row's largest magnitude needs 2 or 3
 // shuffles and every access is a full 32-byte sector.

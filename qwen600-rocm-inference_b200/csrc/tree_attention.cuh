@@ -318,8 +318,11 @@ template <bool BF>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) { return BF ? cvt_bf16x2(lo, hi) : kv::half2_bits(lo, hi); }
 
 // ---- few rows: warp-level tensor cores ------------------------------------------------
-// Bound by the cache's bytes (a row of 128 bf16 values is worth 22 cycles of an SM's
-// share of the memory bandwidth, its products with 16 query rows about 4).  Four
+// Bound by the cache's bytes where it is long (128 sequences of 8 nodes over 1.1 GB of
+// e4m3 cache: 200 us, 5.6 TB/s; what the instructions around the conversions need is
+// close behind), by the chain of plan, first loads and joining where it is short (one
+// token at 1024: 9.4 us), and by instruction issue with 32 rows of 64 dims (32
+// sequences of 7 nodes over 37 MB of int8 cache: 23.6 us, 3,000 cycles a tile).  Four
 // warps; each owns KW keys of a tile, its own ring of kStages cp.async stages and its own (m, l, O) over all
 // rows, so the loop has no block barrier; the four are joined at the end of an
 // item.  16-bit caches multiply in the cache's type.  8-bit codes become fp16
@@ -792,6 +795,7 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attentio
     } while (it.next(P));
 }
 
+// Bound by latency: the plan, two rounds of loads from the L2.
 // Joins the partial results of the items that cross a border between shares:
 // blocks (x, y) take item x, or where there are more items than shares the one that
 // begins in share x and goes on in the next.

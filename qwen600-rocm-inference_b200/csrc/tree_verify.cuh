@@ -28,7 +28,7 @@
 // 256 roots with three operations took as long, on bank conflicts).
 //
 // Measured on a vocabulary of 151,936 in fp32: a chain of 8 nodes of one
-// sequence 22 us, 32 sequences with drafted probabilities 59 us (the rows that are
+// sequence 21 us, 32 sequences with drafted probabilities 58 us (the rows that are
 // reached and the last drafted rows are 13 us of memory traffic; the longest of
 // the 32 walks is eight levels of 4.5 us: 2.6 us for a row's 38,000 tokens an SM,
 // 1.3 us for the exchange).
