@@ -314,6 +314,20 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Pairs of fp32 values, one instruction for both (each rounded as alone).
+__device__ __forceinline__ void mul2(float& a, float& b, float x, float y) {
+    asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmul.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
+        : "+f"(a), "+f"(b) : "f"(x), "f"(y));
+}
+__device__ __forceinline__ void add2(float& a, float& b, float x, float y) {
+    asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tadd.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
+        : "+f"(a), "+f"(b) : "f"(x), "f"(y));
+}
+// (a, b) * m + s
+__device__ __forceinline__ void fma2(float& a, float& b, float m, float s) {
+    asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %2};\n\tmov.b64 r, {%3, %3};\n\tfma.rn.f32x2 p, p, q, r;\n\tmov.b64 {%0, %1}, p;\n\t}"
+        : "+f"(a), "+f"(b) : "f"(m), "f"(s));
+}
 template <bool BF>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) { return BF ? cvt_bf16x2(lo, hi) : kv::half2_bits(lo, hi); }
 
@@ -577,8 +591,8 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attentio
                         vs[i][1] = vs2.y;
                         #pragma unroll
                         for (int mt = 0; mt < MT; mt++) {
-                            s[mt][i][0] *= ks2.x; s[mt][i][1] *= ks2.y;
-                            s[mt][i][2] *= ks2.x; s[mt][i][3] *= ks2.y;
+                            mul2(s[mt][i][0], s[mt][i][1], ks2.x, ks2.y);
+                            mul2(s[mt][i][2], s[mt][i][3], ks2.x, ks2.y);
                         }
                     }
                 }
@@ -608,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attentio
                 if constexpr (L::k8) {
                     const float vinv = __uint_as_float((254u - ve) << 23);
                     #pragma unroll
-                    for (int i = 0; i < NT; i++) { vs[i][0] *= vinv; vs[i][1] *= vinv; }
+                    for (int i = 0; i < NT; i++) mul2(vs[i][0], vs[i][1], vinv, vinv);
                 }
                 float f[2 * MT];
                 bool moved = up != 0;
@@ -624,17 +638,17 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attentio
                     f[r] = exp2_approx(m[r] - base);
                     moved |= mn > m[r];
                     m[r] = mn;
-                    float sum = 0.f;
+                    float sum0 = 0.f, sum1 = 0.f;
                     #pragma unroll
-                    for (int i = 0; i < NT; i++)
-                        #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            float& x = s[r >> 1][i][2 * (r & 1) + e];
-                            x = exp2_approx(fmaf(x, c[r], -base));
-                            sum += x;
-                            if constexpr (L::k8) x *= vs[i][e];
-                        }
-                    l[r] = l[r] * f[r] + sum;
+                    for (int i = 0; i < NT; i++) {
+                        float &x = s[r >> 1][i][2 * (r & 1)], &y = s[r >> 1][i][2 * (r & 1) + 1];
+                        fma2(x, y, c[r], -base);
+                        x = exp2_approx(x);
+                        y = exp2_approx(y);
+                        add2(sum0, sum1, x, y);
+                        if constexpr (L::k8) mul2(x, y, vs[i][0], vs[i][1]);
+                    }
+                    l[r] = l[r] * f[r] + (sum0 + sum1);
                 }
                 if (L::k8 && tail) {   // (a scale that a row does not see may be NaN)
                     #pragma unroll
@@ -652,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attentio
                         #pragma unroll
                         for (int d = 0; d < DT; d++)
                             #pragma unroll
-                            for (int e = 0; e < 4; e++) o[mt][d][e] *= f[2 * mt + (e >> 1)] * w;
+                            for (int e = 0; e < 4; e += 2) mul2(o[mt][d][e], o[mt][d][e + 1], f[2 * mt + (e >> 1)] * w, f[2 * mt + (e >> 1)] * w);
                 }
                 uint8_t* sv = st + L::kPart;
                 // the dim of column e (0, 1) of this lane in column tile d

@@ -480,7 +480,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                         #pragma unroll
                         for (int x = 0; x < 32; x += 4) {
                             const float4 a = *reinterpret_cast<const float4*>(ks + c0 + x);
-                            v[x] *= a.x; v[x + 1] *= a.y; v[x + 2] *= a.z; v[x + 3] *= a.w;
+                            mul2(v[x], v[x + 1], a.x, a.y);
+                            mul2(v[x + 2], v[x + 3], a.z, a.w);
                         }
                     }
                     if (tail) {
@@ -519,7 +520,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                         float o[32];
                         tmem_ld32(to + c0, o);
                         #pragma unroll
-                        for (int x = 0; x < 32; x++) o[x] *= f;
+                        for (int x = 0; x < 32; x += 2) mul2(o[x], o[x + 1], f, f);
                         tc_st32(to + c0, o);
                     }
                 }
@@ -534,13 +535,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                     const uint32_t m = (uint32_t)(vis >> c0);
                     #pragma unroll
                     for (int x = 0; x < 32; x += 2) {
-                        float a = exp2_approx(fmaf(v[x], c, -from)), d = exp2_approx(fmaf(v[x + 1], c, -from));
-                        sum0 += a;
-                        sum1 += d;
+                        fma2(v[x], v[x + 1], c, -from);
+                        float a = exp2_approx(v[x]), d = exp2_approx(v[x + 1]);
+                        add2(sum0, sum1, a, d);
                         if constexpr (L::k8) {
                             const float2 y = *reinterpret_cast<const float2*>(vs + c0 + x);
-                            a *= y.x;
-                            d *= y.y;
+                            mul2(a, d, y.x, y.y);
                         }
                         w[x / 2] = pack2<BF>(a, d);
                     }
