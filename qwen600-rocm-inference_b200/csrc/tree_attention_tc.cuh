@@ -17,11 +17,12 @@
 //
 // Measured, bf16: one sequence of 64 nodes at 8128 19.9 us with the joining (5.2 us of
 // memory traffic; 3,000 cycles each for the plan and the first products), 8 ragged
-// sequences of 64 nodes and 8 query heads a K/V head 129 us (42 us of products at the
+// sequences of 64 nodes and 8 query heads a K/V head 128 us (42 us of products at the
 // rate of a large matrix product: a tile takes 1,300 cycles, the exponentials and what
 // moves them).
-// 8-bit caches: 16 x 20 nodes at 2048 58 us against bf16's 43, bound by the softmax
-// threads, which apply two scales a key, and the conversions beside them.
+// 8-bit caches: 16 x 20 nodes at 2048 57 us against bf16's 43, bound by the four producer
+// warps (2,200 cycles a part of a tile: copies in, codes read, fp16 written, beside the
+// scales' and the products' reads of shared memory).
 //
 // Warps: 0-7 softmax (warp w reads the tensor-memory lanes 32 (w % 4) .., its
 // rows; w / 4 picks the keys' half), 8-11 producers, 12 issues the products.  S = Q
@@ -250,12 +251,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                 auto copy = [&](int x) {
                     if (x < parts) {
                         const int k0 = (it.t0 + (x >> 1)) * kTcKT;
-                        uint8_t* dst = smem + L::kRaw + x % L::kRawRing * L::kRawHalf + pt * 16;
-                        #pragma unroll
-                        for (int i = 0; i < kPer; i++) {
-                            const int r = r0 + i * kStep;
-                            const bool live = k0 + r < it.end;
-                            cp_async16(smem_addr(dst + i * kTcProducers * 16), base[x & 1] + (live ? (size_t)(k0 + r) * L::kRow + c * 16 : 0), live);
+                        const uint32_t dst = smem_addr(smem + L::kRaw + x % L::kRawRing * L::kRawHalf + pt * 16);
+                        const uint8_t* src = base[x & 1] + (size_t)k0 * L::kRow + pt * 16;   // (a head's rows lie one behind the other)
+                        if (k0 + kTcKT <= it.end) {
+                            #pragma unroll
+                            for (int i = 0; i < kPer; i++) cp_async16(dst + i * kTcProducers * 16, src + i * kTcProducers * 16);
+                        } else {
+                            #pragma unroll 1
+                            for (int i = 0; i < kPer; i++) {
+                                const bool live = k0 + r0 + i * kStep < it.end;
+                                cp_async16(dst + i * kTcProducers * 16, live ? src + i * kTcProducers * 16 : base[x & 1], live);
+                            }
                         }
                         if (!(x & 1)) {   // the tile's scales come with K
                             const bool live = k0 + pt < it.end;
@@ -534,15 +540,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                     uint32_t w[16];
                     const uint32_t m = (uint32_t)(vis >> c0);
                     #pragma unroll
-                    for (int x = 0; x < 32; x += 2) {
+                    for (int x = 0; x < 32; x += 4) {
+                        float4 y;
+                        if constexpr (L::k8) y = *reinterpret_cast<const float4*>(vs + c0 + x);
                         fma2(v[x], v[x + 1], c, -from);
-                        float a = exp2_approx(v[x]), d = exp2_approx(v[x + 1]);
-                        add2(sum0, sum1, a, d);
+                        fma2(v[x + 2], v[x + 3], c, -from);
+                        float a[4];
+                        #pragma unroll
+                        for (int j = 0; j < 4; j++) a[j] = exp2_approx(v[x + j]);
+                        add2(sum0, sum1, a[0], a[1]);
+                        add2(sum0, sum1, a[2], a[3]);
                         if constexpr (L::k8) {
-                            const float2 y = *reinterpret_cast<const float2*>(vs + c0 + x);
-                            mul2(a, d, y.x, y.y);
+                            mul2(a[0], a[1], y.x, y.y);
+                            mul2(a[2], a[3], y.z, y.w);
                         }
-                        w[x / 2] = pack2<BF>(a, d);
+                        w[x / 2] = pack2<BF>(a[0], a[1]);
+                        w[x / 2 + 1] = pack2<BF>(a[2], a[3]);
                     }
                     if (L::k8 && tail) {   // (a scale that the row does not see may be NaN)
                         #pragma unroll
