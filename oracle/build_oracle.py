@@ -50,7 +50,7 @@ def build(force=False):
         _run(["g++", "-O3", "-std=c++17", "-mavx2", "-mfma", "-ffp-contract=off", "-fopenmp", "-fPIC", "-shared",
               src, "-o", OUT + ".tmp"])
         os.replace(OUT + ".tmp", OUT)
-    if not os.path.isdir(REF):
+    if not os.path.exists(os.path.join(REF, "sampler.h")):   # (no tree, or an empty directory in its place)
         return
     os.makedirs(REF_OUT, exist_ok=True)
     samp = os.path.join(REF_OUT, "libref_sampler.so")
