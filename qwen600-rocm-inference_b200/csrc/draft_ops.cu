@@ -170,7 +170,7 @@ int check_rows(const qwen_kv_cache_t* c, const void* k, const void* v, int dtype
 // up to 16 and up to 32 the warp-level kernel, in one block of rows; above, where it
 // would read the cache once for every 32 rows, the tensor-memory kernel in blocks
 // of 128.  Both sides measured, 8 K/V heads of 128, warp-level / tensor memory: 24 rows, 16
-// sequences at 2048 38 / 43 us (e4m3 35 / 57), one at 8128 22 / 19; 40 rows 60 / 43 us (e4m3
+// sequences at 2048 38 / 43 us (e4m3 35 / 57), one at 8128 22 / 19; 40 rows 60 / 41 us (e4m3
 // 53 / 57), one at 8128 25 / 19.
 int attention_rows(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : 128; }
 
@@ -240,7 +240,7 @@ int join_launch(const qb::ta::Params& P, const Plan& plan, int dev, cudaStream_t
     cfg.gridDim = dim3(wide, qb::ta::join_blocks<D, ROWS, ACROSS>());
     if (P.by_item) {
         // Shared memory, so that no SM holds more blocks than an even spread over the SMs gives: the first SMs to finish their
-        // share would take six and read those items' partial results alone (one sequence of 64 nodes at 8128: 24.3 us, so 19.9).
+        // share would take six and read those items' partial results alone (one sequence of 64 nodes at 8128: 24.3 us, against 19.9).
         const int each = std::max(1, ((int)cfg.gridDim.y * wide + nsm - 1) / nsm);
         cfg.dynamicSmemBytes = each <= 4 ? (220 * 1024 / each - 1024) / 1024 * 1024 : 0;
         static std::atomic<uint64_t> done{0};

@@ -5,7 +5,7 @@
 //
 // With 33 and more rows (nodes times query heads a K/V head) the warp-level
 // products no longer fit under the cache's bytes, and blocks of 32 rows would
-// read them several times (40 rows, 16 sequences at 2048: 43 us here, 60 us there;
+// read them several times (40 rows, 16 sequences at 2048: 41 us here, 60 us there;
 // 24 rows: 43 us here, 38 us there).  Here an item has 128 rows, tiles have 128 keys, and
 // 256 softmax threads serve them, two a row (64 keys each; they agree on the row's
 // maximum through shared memory).  A tile's two products take 512 cycles each
@@ -15,12 +15,12 @@
 // (Two blocks of rows over shared tiles leave tensor memory for one S each: a
 // chain of products and exponentials without overlap, 2,800 cycles a block and tile.)
 //
-// Measured, bf16: one sequence of 64 nodes at 8128 19.9 us with the joining (5.2 us of
+// Measured, bf16: one sequence of 64 nodes at 8128 19.4 us with the joining (5.2 us of
 // memory traffic; 3,000 cycles each for the plan and the first products), 8 ragged
-// sequences of 64 nodes and 8 query heads a K/V head 128 us (42 us of products at the
-// rate of a large matrix product: a tile takes 1,300 cycles, the exponentials and what
-// moves them).
-// 8-bit caches: 16 x 20 nodes at 2048 57 us against bf16's 43, bound by the four producer
+// sequences of 64 nodes and 8 query heads a K/V head 120 us (42 us of products at the
+// rate of a large matrix product): bound by the chain of a tile, 2,100 cycles from its
+// scores over the maximum and the exponentials to P (the pipes of both are a third busy).
+// 8-bit caches: 16 x 20 nodes at 2048 57 us against bf16's 41, bound by the four producer
 // warps (2,200 cycles a part of a tile: copies in, codes read, fp16 written, beside the
 // scales' and the products' reads of shared memory).
 //
@@ -123,6 +123,15 @@ __device__ __forceinline__ bool mbar_spin(uint64_t* bar, uint32_t parity, uint64
     }
 }
 
+// An item's K and V parts in the order in which the products take them: K 0, K 1, V 0, K 2, V 1, ..., K n-1, V n-2, V n-1.  (In
+// the order K 0, V 0, K 1, ... a K part would wait for the slot of a V part that is taken a tile later.)
+__device__ __forceinline__ uint32_t k_part(int t) { return t == 0 ? 0u : 2u * t - 1u; }
+__device__ __forceinline__ uint32_t v_part(int t, int n) { return (uint32_t)min(2 * t + 2, 2 * n - 1); }
+__device__ __forceinline__ int part_tile(int x, int n, int& kv) {   // part x's tile; kv: 0 K, 1 V
+    kv = x > 0 && (!(x & 1) || x == 2 * n - 1);
+    return x == 2 * n - 1 ? n - 1 : kv ? x / 2 - 1 : (x + 1) / 2;
+}
+
 constexpr int kTcItemCost = 3;   // what an item costs beside its tiles, in tiles: queries, first products, rows out
 
 // grid: a CTA (one an SM) for each share and block of rows beside it, kTcThreads threads, TcLayout::kSmem bytes.
@@ -191,68 +200,69 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
             if constexpr (!L::k8) {
                 constexpr int kChunks = D / 8, kPer = kTcKT * kChunks / kTcProducers, kStep = kTcProducers / kChunks;
                 const int c = pt % kChunks, r0 = pt / kChunks;
-                for (int t = it.t0; t < it.t1 && ok; t++) {
-                    const int k0 = t * kTcKT;
-                    #pragma unroll 1
-                    for (int kv = 0; kv < 2 && ok; kv++, part++) {
-                        if (part >= (uint32_t)L::kRing && unsaid && !mbar_try_wait(&empty[part % L::kRing], (part / L::kRing - 1) & 1u)) {
-                            cp_async_wait<0>();   // the ring is full: announce all that is coming before the wait for a slot
-                            for (; unsaid; unsaid--) say(part - unsaid);
+                const int n = it.t1 - it.t0;
+                #pragma unroll 1
+                for (int x = 0; x < 2 * n && ok; x++, part++) {
+                    int kv;
+                    const int k0 = (it.t0 + part_tile(x, n, kv)) * kTcKT;
+                    if (part >= (uint32_t)L::kRing && unsaid && !mbar_try_wait(&empty[part % L::kRing], (part / L::kRing - 1) & 1u)) {
+                        cp_async_wait<0>();   // the ring is full: announce all that is coming before the wait for a slot
+                        for (; unsaid; unsaid--) say(part - unsaid);
+                    }
+                    if (!free_slot(part)) break;
+                    uint8_t* dst = smem + L::kKV + part % L::kRing * L::kHalf + (c >> 3) * (kTcKT * 128);
+                    #pragma unroll
+                    for (int i = 0; i < kPer; i++) {
+                        const int r = r0 + i * kStep;
+                        const bool live = k0 + r < it.end;
+                        const size_t off = live ? (size_t)(k0 + r) * L::kRow + c * 16 : 0;
+                        cp_async16(smem_addr(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)), base[kv] + off, live);
+                    }
+                    cp_async_commit();
+                    unsaid++;
+                    if (kv == 1 && k0 + kTcKT > it.len) {
+                        // rows of the tree: infinities and NaN would reach nodes that do not see them (0 * NaN): they go to the
+                        // softmax threads by another way (odd), and are zero in the product.  Every thread looks at its own copies.
+                        if (unsaid > 1) {
+                            cp_async_wait<1>();
+                            for (; unsaid > 1; unsaid--) say(part + 1 - unsaid);
                         }
-                        if (!free_slot(part)) break;
-                        uint8_t* dst = smem + L::kKV + part % L::kRing * L::kHalf + (c >> 3) * (kTcKT * 128);
-                        #pragma unroll
+                        cp_async_wait<0>();
+                        constexpr uint32_t kExp = QT == QWEN_BF16 ? 0x7f807f80u : 0x7c007c00u;
+                        bool any = false;
+                        #pragma unroll 4
                         for (int i = 0; i < kPer; i++) {
                             const int r = r0 + i * kStep;
-                            const bool live = k0 + r < it.end;
-                            const size_t off = live ? (size_t)(k0 + r) * L::kRow + c * 16 : 0;
-                            cp_async16(smem_addr(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)), base[kv] + off, live);
-                        }
-                        cp_async_commit();
-                        unsaid++;
-                        if (kv == 1 && k0 + kTcKT > it.len) {
-                            // rows of the tree: infinities and NaN would reach nodes that do not see them (0 * NaN): they go to the
-                            // softmax threads by another way (odd), and are zero in the product.  Every thread looks at its own copies.
-                            if (unsaid > 1) {
-                                cp_async_wait<1>();
-                                for (; unsaid > 1; unsaid--) say(part + 1 - unsaid);
+                            uint4* p = reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+                            const uint4 w = *p;
+                            // all ones where a 16-bit half is not finite
+                            uint4 m = make_uint4(__vcmpeq2(w.x & kExp, kExp), __vcmpeq2(w.y & kExp, kExp), __vcmpeq2(w.z & kExp, kExp),
+                                                 __vcmpeq2(w.w & kExp, kExp));
+                            if ((m.x | m.y | m.z | m.w) && k0 + r >= it.len) {
+                                *p = make_uint4(w.x & ~m.x, w.y & ~m.y, w.z & ~m.z, w.w & ~m.w);
+                                any = true;
                             }
-                            cp_async_wait<0>();
-                            constexpr uint32_t kExp = QT == QWEN_BF16 ? 0x7f807f80u : 0x7c007c00u;
-                            bool any = false;
-                            #pragma unroll 4
-                            for (int i = 0; i < kPer; i++) {
-                                const int r = r0 + i * kStep;
-                                uint4* p = reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-                                const uint4 w = *p;
-                                // all ones where a 16-bit half is not finite
-                                uint4 m = make_uint4(__vcmpeq2(w.x & kExp, kExp), __vcmpeq2(w.y & kExp, kExp), __vcmpeq2(w.z & kExp, kExp),
-                                                     __vcmpeq2(w.w & kExp, kExp));
-                                if ((m.x | m.y | m.z | m.w) && k0 + r >= it.len) {
-                                    *p = make_uint4(w.x & ~m.x, w.y & ~m.y, w.z & ~m.z, w.w & ~m.w);
-                                    any = true;
-                                }
-                            }
-                            if (any) odd[item & 7] = 1;
-                            say(part);
-                            unsaid = 0;
                         }
-                        if (unsaid > 2) {
-                            cp_async_wait<2>();
-                            say(part + 1 - unsaid);
-                            unsaid--;
-                        }
+                        if (any) odd[item & 7] = 1;
+                        say(part);
+                        unsaid = 0;
+                    }
+                    if (unsaid > 2) {
+                        cp_async_wait<2>();
+                        say(part + 1 - unsaid);
+                        unsaid--;
                     }
                 }
             } else {
-                // raw part x (K and V in turn) of this item sits in staging slot x % kRawRing, copied by the thread that converts it
+                // raw part x of this item sits in staging slot x % kRawRing, copied by the thread that converts it
                 constexpr int kChunks = D / 16, kPer = kTcKT * kChunks / kTcProducers, kStep = kTcProducers / kChunks;
-                const int c = pt % kChunks, r0 = pt / kChunks, parts = 2 * (it.t1 - it.t0);
+                const int c = pt % kChunks, r0 = pt / kChunks, n = it.t1 - it.t0, parts = 2 * n;
                 auto copy = [&](int x) {
                     if (x < parts) {
-                        const int k0 = (it.t0 + (x >> 1)) * kTcKT;
+                        int kv;
+                        const int t = part_tile(x, n, kv), k0 = (it.t0 + t) * kTcKT;
                         const uint32_t dst = smem_addr(smem + L::kRaw + x % L::kRawRing * L::kRawHalf + pt * 16);
-                        const uint8_t* src = base[x & 1] + (size_t)k0 * L::kRow + pt * 16;   // (a head's rows lie one behind the other)
+                        const uint8_t* src = base[kv] + (size_t)k0 * L::kRow + pt * 16;   // (a head's rows lie one behind the other)
                         if (k0 + kTcKT <= it.end) {
                             #pragma unroll
                             for (int i = 0; i < kPer; i++) cp_async16(dst + i * kTcProducers * 16, src + i * kTcProducers * 16);
@@ -260,12 +270,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                             #pragma unroll 1
                             for (int i = 0; i < kPer; i++) {
                                 const bool live = k0 + r0 + i * kStep < it.end;
-                                cp_async16(dst + i * kTcProducers * 16, live ? src + i * kTcProducers * 16 : base[x & 1], live);
+                                cp_async16(dst + i * kTcProducers * 16, live ? src + i * kTcProducers * 16 : base[kv], live);
                             }
                         }
-                        if (!(x & 1)) {   // the tile's scales come with K
+                        if (!kv) {        // the tile's scales come with K
                             const bool live = k0 + pt < it.end;
-                            float* sc = reinterpret_cast<float*>(smem + L::kScales) + (tile + (x >> 1)) % kScaleRing * 2 * kTcKT + pt;
+                            float* sc = reinterpret_cast<float*>(smem + L::kScales) + (tile + t) % kScaleRing * 2 * kTcKT + pt;
                             cp_async4(smem_addr(sc), P.cache.ks + head / D + (live ? k0 + pt : 0), live);
                             cp_async4(smem_addr(sc + kTcKT), P.cache.vs + head / D + (live ? k0 + pt : 0), live);
                         }
@@ -278,8 +288,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                     copy(x + L::kRawRing - 1);
                     cp_async_wait<L::kRawRing - 1>();
                     if (!free_slot(part)) break;
-                    const int k0 = (it.t0 + (x >> 1)) * kTcKT;
-                    const bool tail = STORE == QWEN_E4M3 && (x & 1) && k0 + kTcKT > it.len;
+                    int kv;
+                    const int t = part_tile(x, n, kv), k0 = (it.t0 + t) * kTcKT;
+                    const bool tail = STORE == QWEN_E4M3 && kv && k0 + kTcKT > it.len;
                     const uint8_t* src = smem + L::kRaw + x % L::kRawRing * L::kRawHalf + pt * 16;
                     uint8_t* dst = smem + L::kKV + part % L::kRing * L::kHalf + (c >> 2) * (kTcKT * 128);
                     #pragma unroll 4
@@ -302,8 +313,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                         *reinterpret_cast<uint4*>(dst + r * 128 + (((ch + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
                     }
                     say(part);
-                    if (!(x & 1)) {   // the largest exponent of the value scales, a warp's 32 keys
-                        const uint32_t ring = (tile + (x >> 1)) % kScaleRing;
+                    if (!kv) {        // the largest exponent of the value scales, a warp's 32 keys
+                        const uint32_t ring = (tile + t) % kScaleRing;
                         const float vs = reinterpret_cast<const float*>(smem + L::kScales)[ring * 2 * kTcKT + kTcKT + pt];
                         uint32_t e = __float_as_uint(vs) >> 23 & 0xffu;
                         e = __reduce_max_sync(~0u, e == 255u ? 0u : min(e + 1, 253u));
@@ -342,7 +353,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                 for (int v = 0; v < nt + 2 && going; v++) {
                     const int b = v & 1;
                     if (v >= 2) {
-                        const uint32_t p = part + 2 * (v - 2) + 1;
+                        const uint32_t p = part + v_part(v - 2, nt);
                         going = wait(&pfull[b], (steps[b] - 1) & 1u) && wait(&full[p % L::kRing], p / L::kRing & 1u);
                         if (!going) break;
                         tc_fence_after();
@@ -355,7 +366,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                         mma_commit(&pvdone[b]);
                     }
                     if (v < nt) {
-                        const uint32_t p = part + 2 * v;
+                        const uint32_t p = part + k_part(v);
                         going = wait(&full[p % L::kRing], p / L::kRing & 1u);
                         if (!going) break;
                         tc_fence_after();
