@@ -170,7 +170,7 @@ int check_rows(const qwen_kv_cache_t* c, const void* k, const void* v, int dtype
 // up to 16 and up to 32 the warp-level kernel, in one block of rows; above, where it
 // would read the cache once for every 32 rows, the tensor-memory kernel in blocks
 // of 128.  Both sides measured, 8 K/V heads of 128, warp-level / tensor memory: 24 rows, 16
-// sequences at 2048 38 / 43 us (e4m3 35 / 57), one at 8128 22 / 19; 40 rows 60 / 41 us (e4m3
+// sequences at 2048 38 / 43 us (e4m3 35 / 57), one at 8128 22 / 19; 40 rows 60 / 40 us (e4m3
 // 53 / 57), one at 8128 25 / 19.
 int attention_rows(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : 128; }
 

@@ -5,7 +5,7 @@
 //
 // With 33 and more rows (nodes times query heads a K/V head) the warp-level
 // products no longer fit under the cache's bytes, and blocks of 32 rows would
-// read them several times (40 rows, 16 sequences at 2048: 41 us here, 60 us there;
+// read them several times (40 rows, 16 sequences at 2048: 40 us here, 60 us there;
 // 24 rows: 43 us here, 38 us there).  Here an item has 128 rows, tiles have 128 keys, and
 // 256 softmax threads serve them, two a row (64 keys each; they agree on the row's
 // maximum through shared memory).  A tile's two products take 512 cycles each
@@ -17,10 +17,10 @@
 //
 // Measured, bf16: one sequence of 64 nodes at 8128 19.4 us with the joining (5.2 us of
 // memory traffic; 3,000 cycles each for the plan and the first products), 8 ragged
-// sequences of 64 nodes and 8 query heads a K/V head 120 us (42 us of products at the
+// sequences of 64 nodes and 8 query heads a K/V head 119 us (42 us of products at the
 // rate of a large matrix product): bound by the chain of a tile, 2,100 cycles from its
 // scores over the maximum and the exponentials to P (the pipes of both are a third busy).
-// 8-bit caches: 16 x 20 nodes at 2048 57 us against bf16's 41, bound by the four producer
+// 8-bit caches: 16 x 20 nodes at 2048 57 us against bf16's 40, bound by the four producer
 // warps (2,200 cycles a part of a tile: copies in, codes read, fp16 written, beside the
 // scales' and the products' reads of shared memory).
 //
@@ -211,12 +211,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                     }
                     if (!free_slot(part)) break;
                     uint8_t* dst = smem + L::kKV + part % L::kRing * L::kHalf + (c >> 3) * (kTcKT * 128);
-                    #pragma unroll
-                    for (int i = 0; i < kPer; i++) {
-                        const int r = r0 + i * kStep;
-                        const bool live = k0 + r < it.end;
-                        const size_t off = live ? (size_t)(k0 + r) * L::kRow + c * 16 : 0;
-                        cp_async16(smem_addr(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)), base[kv] + off, live);
+                    static_assert(kStep % 8 == 0, "the rows of a thread share their swizzle");
+                    const uint32_t to = smem_addr(dst + r0 * 128 + (((c & 7) ^ (r0 & 7)) << 4));
+                    const uint8_t* src = base[kv] + (size_t)(k0 + r0) * L::kRow + c * 16;
+                    if (k0 + kTcKT <= it.end) {
+                        #pragma unroll
+                        for (int i = 0; i < kPer; i++) cp_async16(to + i * kStep * 128, src + i * kStep * L::kRow);
+                    } else {
+                        #pragma unroll 1
+                        for (int i = 0; i < kPer; i++) {
+                            const bool live = k0 + r0 + i * kStep < it.end;
+                            cp_async16(to + i * kStep * 128, live ? src + i * kStep * L::kRow : base[kv], live);
+                        }
                     }
                     cp_async_commit();
                     unsaid++;
