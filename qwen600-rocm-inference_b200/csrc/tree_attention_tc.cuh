@@ -319,11 +319,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                         *reinterpret_cast<uint4*>(dst + r * 128 + (((ch + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
                     }
                     say(part);
-                    if (!kv) {        // the largest exponent of the value scales, a warp's 32 keys
+                    if (!kv) {        // the largest exponent of the context's value scales, a warp's 32 keys
                         const uint32_t ring = (tile + t) % kScaleRing;
                         const float vs = reinterpret_cast<const float*>(smem + L::kScales)[ring * 2 * kTcKT + kTcKT + pt];
-                        uint32_t e = __float_as_uint(vs) >> 23 & 0xffu;
-                        e = __reduce_max_sync(~0u, e == 255u ? 0u : min(e + 1, 253u));
+                        const uint32_t e = __reduce_max_sync(~0u, k0 + pt < it.len ? scale_exponent(vs) : 0u);
                         if (lane == 0) reinterpret_cast<volatile uint32_t*>(smem + L::kVe)[ring * 4 + (warp - kProducer)] = e;
                         __syncwarp();
                         mbar_arrive(&scaled[ring]);
@@ -477,7 +476,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
             __syncwarp();
             if (lane == 0) mbar_arrive(qfull);
             float top = -INFINITY, base = -INFINITY, l = 0.f;              // the row's running maximum; what exponents are taken from; this half's sum
-            int ve_run = 37;                                               // 8 bits: largest exponent of a value scale so far, 2^-90 at least
+            int ve_run = 37;                                               // 8 bits: largest exponent of a seen value scale so far, 2^-90 at least
             for (int i = 0; i < nt; i++, steps++) {
                 const int k0 = (it.t0 + i) * kTcKT + 64 * half;
                 const int b = i & 1;
@@ -489,6 +488,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
                     vs = ks + kTcKT;
                     const volatile uint32_t* v4 = reinterpret_cast<const volatile uint32_t*>(smem + L::kVe) + ring * 4;
                     ve_run = max(ve_run, (int)max(max(v4[0], v4[1]), max(v4[2], v4[3])));
+                    const int t0 = k0 - 64 * half, first = it.len - t0;    // the tile's first key; its key that is node 0 (or beyond its ends)
+                    if (first < kTcKT) {   // and of the tree's keys in the tile those that this row sees: the others' scales may be any
+                        uint64_t own = see;
+                        if (first < 0) own &= ~0ull << -first;
+                        else if (first > kTcKT - 64) own &= (1ull << (kTcKT - first)) - 1;
+                        const float* tree = vs - 64 * half + first;
+                        for (; own; own &= own - 1) ve_run = max(ve_run, (int)scale_exponent(tree[__ffsll((long long)own) - 1]));
+                        __syncwarp();
+                    }
                 }
                 const uint32_t use = uses[b];
                 wait(&sfull[b], use & 1u);

@@ -411,6 +411,60 @@ def test_attention_unseen_values_do_not_matter(qb, store, t, length):
         assert not bool(got[:, i].isfinite().all())
 
 
+@pytest.mark.parametrize("store", ["e4m3", "int8"])
+@pytest.mark.parametrize("t,group,dim,length,cap", [(6, 2, 128, 20, 60), (6, 2, 64, 0, 60), (12, 2, 64, 117, 300), (24, 1, 128, 50, 150), (40, 1, 128, 100, 300),
+                                                    (64, 2, 64, 33, 200), (64, 8, 128, 90, 160), (6, 2, 128, 1270, 1400), (28, 1, 64, 1273, 1400), (64, 1, 128, 1215, 1400),
+                                                    (64, 3, 64, 1280, 1400)])
+def test_attention_unseen_scales_do_not_matter(qb, store, t, group, dim, length, cap):
+    """Scales of any size at positions that a node does not see (another branch's, an absent node's, those behind a short count)
+    leave its result as it is, bit for bit; the nodes that see such rows are right as well."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(t + length)
+    b, kv = 3, 2
+    clean = Cache(qb, b, kv, cap, dim, store).fill(g)
+    q = torch.randn(b, t, kv * group, dim, generator=g, device="cuda").to(torch.bfloat16)
+    here = t - t // 4                            # nodes from here on are absent
+    par = np.full((b, t), -2, np.int32)
+    par[:, 0] = -1
+    for i in range(1, here):                     # two branches: 0, 1, 3, 5, .. and 0, 2, 4, ..
+        par[:, i] = max(0, i - 2)
+    lens = [length, max(length - 9, 0), length // 2]
+    want = _attend(qb, clean, q, lens, par, dim ** -0.5)
+    assert bool(want[:, :here].isfinite().all()) and bool((want[:, :here] != 0).any(-1).all())
+
+    def poisoned(nodes, value, behind):
+        c = Cache(qb, b, kv, cap, dim, store)
+        for x, y in ((c.k, clean.k), (c.v, clean.v)):
+            x.view(torch.uint8).copy_(y.view(torch.uint8))
+        for x, y in ((c.ks, clean.ks), (c.vs, clean.vs)):
+            x.copy_(y)
+            for r in range(b):
+                at = [lens[r] + i for i in nodes if lens[r] + i < cap]
+                x[r, :, at] = value
+                if behind:
+                    x[r, :, lens[r] + t:] = value
+        return c
+
+    for value in (1e-30, 1e5, -1e9, 1e30, torch.finfo(torch.float32).max):
+        got = _attend(qb, poisoned(range(here, t), value, True), q, lens, par, dim ** -0.5)
+        assert torch.equal(got, want), value
+        got = _attend(qb, poisoned(range(2, t, 2), value, False), q, lens, par, dim ** -0.5)
+        odd = [0] + list(range(1, here, 2))
+        assert torch.equal(got[:, odd], want[:, odd]), value
+    for value in (1e-20, 3e3, 1e18):             # rows that see them: large values, but an ordinary score
+        c = poisoned(range(2, t, 2), value, True)
+        c.ks.copy_(clean.ks)
+        got = _attend(qb, c, q, lens, par, dim ** -0.5).double()
+        want64, tol = _attention64(c, q, lens, par, dim ** -0.5)
+        codes = c.v.float().double().abs()
+        for r in range(b):                       # Weight times scale is fp16 in a unit of at most twice the largest seen scale: half of its
+            for i in range(here):                # smallest step is 2^-25 of that, for each key's code; the sum of the weights is at least 1.
+                at = list(range(lens[r])) + [lens[r] + j for j in sorted(_sees(par[r].tolist(), lens[r], cap)[i])]
+                low = 2.0 ** -24 * c.vs[r][:, at].double().amax(1)[:, None] * codes[r][:, at].sum(1)
+                tol[r, i] += low.repeat_interleave(group, 0)
+        assert bool(((got - want64).abs() <= tol).all()), value
+
+
 def test_attention_infinity_in_a_seen_branch(qb):
     """A V row with one infinity: that dim of the nodes that see it becomes infinite, nothing else changes."""
     import torch
