@@ -20,8 +20,9 @@
 // straight to every CTA through distributed shared memory: one cluster barrier a
 // pass.
 //
-// Statistics that decide a comparison (largest logit, sum) are fp32 while nothing
-// is refused.  Sums that the drawn token's position depends on are fp64: the
+// Statistics that decide a comparison (largest logit, sum) are fp32 until a token
+// with drafted probabilities, or most of the row's weight, is refused; then what is
+// left is summed in fp64.  Sums that the drawn token's position depends on are fp64: the
 // running sum crosses a border for each of up to 10^5 tokens, so 24 bits would
 // misplace about one draw in a hundred.  Their powers of two are a polynomial of
 // degree 8 in fp64 (relative error 2^-39, 13 fp64 operations a token; a table of
@@ -347,9 +348,9 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Params P) {
 
         // ---- children in index order ----
         int kept = -1, n_gone = 0;
-        // Z: the sum; left, S and rest are Z times those of the walk's definition
+        // Z: the last sum; left, S and rest are the row's sum times those of the walk's definition
         double Z = z, left = Z, S = 0.0;
-        bool summed = false;
+        bool summed = false;     // left is the last sum pass's
         const double M64 = M;
         // weights 2^(c (x - M)) = 2^n 2^f, |f| <= 1/2, of K tokens; in[j]: the weight counts (not below 2^-1000).  The steps go
         // over all K in turn, so that each fp64 operation finds the others' in the pipe
@@ -487,6 +488,13 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Params P) {
                 if (tid == 0) sh.gone[n_gone] = x;
                 __syncthreads();
                 n_gone++;
+                summed = false;
+                // Little is left of the last sum: the next child is compared with a sum of what is left, in 64 bits, not with a
+                // difference of fp32 sums (off by about 2^-21 of Z: 2^-18 of an eighth of it).
+                if ((children & (children - 1)) && left < 0.125 * Z) {
+                    left = Z = sum_pass();
+                    summed = true;
+                }
             }
         }
         if (kept >= 0) {

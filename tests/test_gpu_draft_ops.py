@@ -727,6 +727,39 @@ def test_verify_edges_of_the_uniforms(qb, with_draft):
         _check_verify(qb, logits, draft, tokens, par, u, 0.8)
 
 
+@pytest.mark.parametrize("vocab,dtype", [(151936, "fp32"), (151936, "bf16"), (1000, "fp32")])
+@pytest.mark.parametrize("top", [0.8, 0.95, 0.999, 0.99999])
+def test_verify_after_a_likely_token_is_refused(qb, vocab, dtype, top):
+    """Chosen drafts: a refused token that had nearly all of the weight leaves little, and the next children are compared with
+    exactly that: uniforms at either side of each border decide as in 64 bits."""
+    import torch
+    b = 48
+    g = torch.Generator(device="cuda").manual_seed(vocab + int(top * 1e5))
+    logits = torch.randn(b, 5, vocab, generator=g, device="cuda")
+    rest = logits[:, 0, 4:].double().exp().sum(-1)
+    for i, share in enumerate((0.3, 0.25, 0.2)):                   # of what is left behind token 0
+        logits[:, 0, 1 + i] = (rest * share / 0.25).log().float()
+    logits[:, 0, 0] = (logits[:, 0, 1:].double().exp().sum(-1) * top / (1 - top)).log().float()
+    logits = logits.to(_types(qb)[dtype][1])
+    p = torch.softmax(logits[:, 0].double(), -1).cpu().numpy()
+    par = np.tile(np.array([-1, 0, 0, 0, 0], np.int32), (b, 1))
+    tokens = np.tile(np.array([0, 0, 1, 2, 3], np.int32), (b, 1))
+    u = np.random.RandomState(5).rand(b, 5)
+    # fp32 sums of the row are off by about 2^-21; what is left behind the first child by 2^-18 at most, or it is summed in 64 bits
+    edge = 1e-5
+    for r in range(b):
+        left = 1 - p[r, 0]
+        u[r, 1] = p[r, 0] + 0.5 * left                             # refused
+        u[r, 2] = p[r, 1] / left * (1 + (edge if r & 1 else -edge))
+        left -= p[r, 1]
+        u[r, 3] = p[r, 2] / left * (1 + (edge if r & 2 else -edge))
+        left -= p[r, 2]
+        u[r, 4] = p[r, 3] / left * (1 + (edge if r & 4 else -edge))
+    got = _check_verify(qb, logits, None, tokens, par, u.astype(np.float32), 1.0)
+    want = [2 if not r & 1 else 3 if not r & 2 else 4 if not r & 4 else -1 for r in range(b)]
+    assert got[0][:, 1].tolist() == want
+
+
 @pytest.mark.parametrize("temp", [0.0, 1.0])
 def test_verify_rows_without_a_distribution(qb, temp):
     import torch
