@@ -509,6 +509,15 @@ int qwen_tree_verify(const void* logits, int logits_dtype, long long ld, const f
                      const int* parents, const float* uniforms, int n_seqs, int n_nodes, int vocab, float temperature, int* path,
                      int* n_path, int* next, void* stream);
 
+/* Failure testing of the two calls above without a GPU fault: every later call
+ * of the process waits at most wait_ns (>= 1 ms; 0 restores the default 1 s) on
+ * the device, and, with part >= 0, one wait can only run out:
+ * qwen_tree_attention's for slot `part` of the ring that K and V come through (a
+ * call with more than 32 query rows a K/V head), qwen_tree_verify's for the row of
+ * node `part` (where rows start on 16 bytes and are held in shared memory).
+ * qwen_debug_draft_wait(0, -1) restores normal operation. */
+int qwen_debug_draft_wait(unsigned long long wait_ns, int part);
+
 #ifdef __cplusplus
 }
 #endif

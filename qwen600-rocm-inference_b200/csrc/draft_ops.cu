@@ -33,6 +33,11 @@ int fail(int code, const std::string& msg) { return qwen_internal_fail(code, msg
         if (rc_ != QWEN_OK) return rc_;    \
     } while (0)
 
+// ---- waits (qwen_debug_draft_wait) ---------------------------------------------
+constexpr unsigned long long kWaitNs = 1000000000ull;   // for copies and products on this GPU: they take microseconds
+std::atomic<unsigned long long> g_wait_ns{kWaitNs};
+std::atomic<int> g_withheld{-1};
+
 // ---- argument checks -----------------------------------------------------------
 struct Ptr {
     const void* p;
@@ -342,6 +347,14 @@ int verify_launch(qb::tv::Params& P, int n_seqs, int nsm, int dev, cudaStream_t 
 
 }  // namespace
 
+extern "C" int qwen_debug_draft_wait(unsigned long long wait_ns, int part) {
+    if (part < -1 || part >= qb::tv::kMaxNodes) return fail(QWEN_E_ARG, "part out of [-1, 63]");
+    if (wait_ns != 0 && wait_ns < 1000000ull) return fail(QWEN_E_ARG, "wait limit below 1 ms");
+    g_wait_ns.store(wait_ns ? wait_ns : kWaitNs);
+    g_withheld.store(part);
+    return QWEN_OK;
+}
+
 extern "C" int qwen_kv_append(const qwen_kv_cache_t* cache, const void* k, const void* v, int src_dtype, long long ld, int n_tokens,
                               const int* start, const int* counts, void* stream) {
     TRY(check_rows(cache, k, v, src_dtype, ld, n_tokens, start, counts));
@@ -423,6 +436,8 @@ extern "C" int qwen_tree_attention(const qwen_kv_cache_t* cache, const void* q, 
     P.groups = plan.shares / plan.beside;
     P.by_item = !plan.whole && (long long)P.n_seqs * P.n_kv_heads * (P.row_blocks / P.beside) <= P.groups;
     P.scale_log2 = scale * 1.4426950408889634f;
+    P.wait_ns = g_wait_ns.load();
+    P.withheld = g_withheld.load();
     const cudaStream_t st = (cudaStream_t)stream;
     const int dim = cache->head_dim;
     const bool bf = dtype == QWEN_BF16;
@@ -465,6 +480,8 @@ extern "C" int qwen_tree_verify(const void* logits, int logits_dtype, long long 
     const bool rows16 = ((uintptr_t)logits | (size_t)ld * elem) % 16 == 0;
     P.vec = rows16 && (!P.draft || ((uintptr_t)draft | (size_t)ld_draft * 4) % 16 == 0);
     P.temperature = temperature;
+    P.wait_ns = g_wait_ns.load();
+    P.withheld = g_withheld.load();
     const cudaStream_t st = (cudaStream_t)stream;
     switch (logits_dtype) {
         case QWEN_BF16: return verify_launch<QWEN_BF16>(P, n_seqs, nsm, dev, st);

@@ -42,6 +42,8 @@ struct Params {
     int n_seqs, n_kv_heads, group, n_nodes;
     int whole;                // a CTA for each item: CTA (sequence * n_kv_heads + head) * row_blocks + block
     int groups, by_item;      // shares of the line; combine_kernel's blocks are for the items (else: for the shares)
+    int withheld;             // -1, or for failure tests: this part of the ring that K and V come through is never announced
+    unsigned long long wait_ns;   // longest wait of the tensor-memory kernel
     int row_blocks, beside;   // blocks of rows that a K/V head has; CTAs side by side on a share (row_blocks, or 1 where that is more than the grid)
     float scale_log2;   // scale * log2(e)
     float per_group;    // 1 / group

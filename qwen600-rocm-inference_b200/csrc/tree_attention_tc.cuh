@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
     Items<kTcKT, kTcItemCost, kTcRows> it;       // every role walks it alike
     const bool busy = it.start(P);               // the same for the whole CTA
     if (tid == 0) {
-        for (int i = 0; i < L::kRing; i++) { mbar_init(&full[i], kTcProducers); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < L::kRing; i++) { mbar_init(&full[i], kTcProducers + (i == P.withheld)); mbar_init(&empty[i], 1); }
         for (int i = 0; i < kScaleRing; i++) mbar_init(&scaled[i], kTcProducers);
         for (int i = 0; i < 2; i++) { mbar_init(&sfull[i], 1); mbar_init(&pfull[i], 8); mbar_init(&pvdone[i], 1); }
         mbar_init(qfull, 8);
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
     constexpr uint32_t kTmO = 256, kTmP = 384;   // columns: S buffers 0 and 128, O 256, P buffers 384 and 448
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (ok && !mbar_spin(bar, parity, kWaitNs)) { ok = false; *fault = 1; }
+        if (ok && !mbar_spin(bar, parity, P.wait_ns)) { ok = false; *fault = 1; }
         return ok;
     };
     if (busy && warp >= kProducer && warp < kIssuer) {
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
         } while (it.next(P));
         if (lane == 0) {
             mma_commit(drained);
-            if (!mbar_wait(drained, 0, kWaitNs)) *fault = 1;
+            if (!mbar_wait(drained, 0, P.wait_ns)) *fault = 1;
         }
         __syncwarp();
     } else if (busy && warp < kProducer) {

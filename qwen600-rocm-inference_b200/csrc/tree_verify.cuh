@@ -44,7 +44,6 @@ namespace qb {
 namespace tv {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32, kRun = 128;
-constexpr uint64_t kWaitNs = 1000000000ull;   // longest wait for a copy from this GPU's own memory
 constexpr int kMaxNodes = 64, kMaxCluster = 16, kMaxParts = kMaxCluster * kWarps;
 
 struct Params {
@@ -56,6 +55,8 @@ struct Params {
     long long ld, ld_draft;
     int n_nodes, vocab, vec;   // vec: rows of logits and draft start on 16 bytes
     int buffers, part_bytes;   // row buffers in shared memory (0: parts do not fit), bytes of a warp's part (whole steps)
+    int withheld;              // -1, or for failure tests a node: the last warp waits for 16 bytes of its row that never come
+    unsigned long long wait_ns;   // longest wait for a copy from this GPU's own memory
     float temperature;
 };
 
@@ -162,14 +163,16 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Params P) {
     // issue slots from the arithmetic, where rows start on 16 bytes.  first: the first piece of the part.
     uint32_t phase = 0;      // bit b: the parity that buffer b's next part completes
     uint32_t coming = 0;     // bit b: a part is on its way
+    bool late = false;       // a wait ran out (the same for the warp): nothing is copied from then on
     auto fetch = [&](int node, int b, int from, int to, bool first) {
+        if (late) return;
         uint8_t* dst = parts_mem + (size_t)(b * kWarps + warp) * P.part_bytes;
         const uint8_t* row = row_of(node);
         int k = from;        // tokens from here on are copied one by one
         if (vec) {
             const uint32_t n = (uint32_t)((to - from) * kEs) & ~15u, all = (uint32_t)((hi - lo) * kEs) & ~15u;
             if (lane == 0) {
-                if (first && all) mbar_arrive_expect_tx(&sh.arrived[b][warp], all);
+                if (first && all) mbar_arrive_expect_tx(&sh.arrived[b][warp], all + (node == P.withheld && mine == parts - 1 ? 16u : 0u));
                 if (n) bulk_g2s(dst + (size_t)(from - lo) * kEs, row + (size_t)from * kEs, n, &sh.arrived[b][warp], policy_evict_last());
             }
             if (all) coming |= 1u << b;
@@ -181,12 +184,15 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Params P) {
         }
     };
     // Waits for buffer b's part; a wait that runs out marks the warp, whose word to the others then is NaN or +inf (next = -1).
-    bool late = false;
+    // The part stays on its way: the kernel's end waits for it once more, and no other copy goes into its buffer.
     auto landed = [&](int b) {
         if (coming >> b & 1) {
-            if (!mbar_wait(&sh.arrived[b][warp], phase >> b & 1, kWaitNs)) late = true;
-            phase ^= 1u << b;
-            coming &= ~(1u << b);
+            if (__all_sync(~0u, mbar_wait(&sh.arrived[b][warp], phase >> b & 1, P.wait_ns))) {
+                phase ^= 1u << b;
+                coming &= ~(1u << b);
+            } else {
+                late = true;
+            }
         }
         __syncwarp();
     };

@@ -96,6 +96,7 @@ _SIGS = {
                                        _c.c_size_t, _P]),
     "qwen_tree_verify": (_c.c_int, [_P, _c.c_int, _c.c_longlong, _P, _c.c_longlong, _P, _P, _P, _c.c_int, _c.c_int, _c.c_int, _c.c_float,
                                     _P, _P, _P, _P]),
+    "qwen_debug_draft_wait": (_c.c_int, [_c.c_ulonglong, _c.c_int]),
     "qwen_tokenizer_load": (_c.c_int, [_c.c_char_p, _c.c_int, _c.POINTER(_P)]),
     "qwen_tokenizer_free": (None, [_P]),
     "qwen_tokenizer_info": (_c.c_int, [_P, _c.POINTER(_c.c_int), _c.POINTER(_c.c_int), _c.POINTER(_c.c_int), _c.POINTER(_c.c_int)]),
@@ -290,6 +291,12 @@ def tree_verify(logits_ptr, dtype, ld, draft_ptr, ld_draft, tokens_ptr, parents_
     """Which drafted nodes the target's logits keep (path, n_path) and the token after them (next)."""
     _check(load_library().qwen_tree_verify(logits_ptr, dtype, ld, draft_ptr, ld_draft, tokens_ptr, parents_ptr, uniforms_ptr, n_seqs, n_nodes,
                                            vocab, temperature, path_ptr, n_path_ptr, next_ptr, stream))
+
+
+def debug_draft_wait(wait_ns=0, part=-1):
+    """Failure testing of tree_attention and tree_verify: wait limit of later calls (0 = default) and a ring slot or
+    node whose wait runs out (-1 = none)."""
+    _check(load_library().qwen_debug_draft_wait(int(wait_ns), int(part)))
 
 
 class Engine:

@@ -95,3 +95,9 @@ def test_bad_verify(qb, over):
 
 def test_batch_cache_needs_a_handle(qb):
     assert qb.load_library().qwen_batch_cache(None, 0, ctypes.byref(qb.KVCache())) == -1
+
+
+@pytest.mark.parametrize("args", [(999_999, 0), (1, -1), (0, -2), (0, 64)])
+def test_bad_debug_wait(qb, args):
+    _raises(qb, -1, qb.debug_draft_wait, *args)
+    qb.debug_draft_wait()

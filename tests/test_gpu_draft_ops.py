@@ -1019,6 +1019,47 @@ def test_refusals_on_the_device(qb):
     assert bool(s["out"].isfinite().all())
 
 
+@pytest.mark.parametrize("b,with_draft,temp,node", [(1, False, 0.0, 0), (1, True, 1.0, 0), (1, False, 1.0, 1), (6, True, 1.0, 1), (37, True, 0.7, 0), (37, True, 0.7, 1)])
+def test_verify_reports_a_wait_that_ran_out(qb, b, with_draft, temp, node):
+    """A row's copy that never completes: the bounded wait ends, the call returns -1 for the next token of every sequence that waits
+    for it, and the next call is right."""
+    import torch
+    case = _drafted(b, b, 3, 151936, torch.float32, with_draft, temp)
+    case[3][:] = np.array([-1, 0, 1])                              # node 1's row is copied while node 0's is read
+    qb.debug_draft_wait(5_000_000, node)
+    try:
+        path, n_path, nxt = _verify(qb, *case, temp)
+    finally:
+        qb.debug_draft_wait()
+    if node == 0:
+        assert (nxt == -1).all() and (n_path == 1).all() and (path[:, 0] == 0).all() and (path[:, 1:] == -1).all()
+    else:                                                          # those that reached node 1 have no token; the others did not need its row
+        want = _check_verify(qb, *case, temp)
+        reached = want[1] > 1
+        assert (nxt[reached] == -1).all() and (n_path[reached] == 2).all()
+        assert ((nxt == want[2]) | (nxt == -1)).all()
+    _check_verify(qb, *case, temp)
+
+
+@pytest.mark.parametrize("store", ["bf16", "e4m3"])
+@pytest.mark.parametrize("cap", [200, 1500])
+def test_attention_reports_a_wait_that_ran_out(qb, store, cap):
+    """K and V that are never announced: the bounded waits end, the call's rows are NaN, and the next call is right."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(3)
+    t = 40
+    c = Cache(qb, 2, 2, cap, 128, store).fill(g)
+    q = torch.randn(2, t, 2, 128, generator=g, device="cuda").to(torch.bfloat16)
+    par, lens = _tree(np.random.RandomState(1), 2, t), [cap - t, 3]
+    qb.debug_draft_wait(5_000_000, 0)
+    try:
+        got = _attend(qb, c, q, lens, par, 0.1)
+    finally:
+        qb.debug_draft_wait()
+    assert bool(got.isnan().all())
+    _check_attention(qb, c, q, lens, par, 0.1)
+
+
 def test_batch_cache_views_the_slots(qb, checkpoint):
     """qwen_batch_cache: the K/V that the batched prompt pass wrote, read through the view, match between the one-layer and the
     all-layers view, and attention over a slot's layer runs on them."""
