@@ -147,7 +147,7 @@ struct Line {
 template <int KT, int COST, int ROWS>
 struct Items {
     int at, to, before;      // positions of the line
-    int seq, len, end, n, unit_blocks, units, beside, step;
+    int seq, len, end, n, unit_blocks, units, beside, step;   // len: -1 for every negative length (differences to it are taken)
     int h, r_base, t0, t1;   // the item's K/V head, first row, tiles t0 .. t1-1 of n
     bool first;              // the share's first item: it holds the share's beginning
 
@@ -168,7 +168,7 @@ struct Items {
         if (at >= to) return false;
         if (at - before == (n + COST) * units) {
             before = at;
-            len = P.lens[++seq];
+            len = max(P.lens[++seq], -1);
         }
         item(P);
         return true;
@@ -188,7 +188,7 @@ struct Items {
             seq = item_i / P.n_kv_heads;
             h = item_i - seq * P.n_kv_heads;
             r_base = (blockIdx.x - item_i * P.row_blocks) * ROWS;
-            len = P.lens[seq];
+            len = max(P.lens[seq], -1);
             end = seq_end(P, len);
             n = t1 = seq_tiles<KT>(P, len);
             at = before = t0 = 0;
@@ -205,6 +205,7 @@ struct Items {
         to = line.shares.begin(blockIdx.x / beside + 1);
         if (at >= to) return false;
         seq = line.find(P, at, before, len);
+        len = max(len, -1);
         first = true;
         item(P);
         return t1 > t0 || next(P);

@@ -411,6 +411,19 @@ def test_attention_unseen_values_do_not_matter(qb, store, t, length):
         assert not bool(got[:, i].isfinite().all())
 
 
+@pytest.mark.parametrize("store", ["bf16", "int8"])
+@pytest.mark.parametrize("t,cap", [(6, 200), (6, 1500), (40, 300), (40, 1500)])
+def test_attention_any_negative_length_is_idle(qb, store, t, cap):
+    """Lengths down to the smallest number: their sequences' rows are 0, the others right."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(t)
+    lens = [cap - t, -1, -2 ** 31, -2 ** 31 + 1, -2 ** 31 + 70, 33]
+    c = Cache(qb, len(lens), 2, cap, 128, store).fill(g)
+    q = torch.randn(len(lens), t, 4, 128, generator=g, device="cuda").to(torch.bfloat16)
+    got = _check_attention(qb, c, q, lens, _tree(np.random.RandomState(t), len(lens), t), 0.1)
+    assert bool((got[1:5] == 0).all()) and bool((got[[0, 5]] != 0).any())
+
+
 @pytest.mark.parametrize("store", ["e4m3", "int8"])
 @pytest.mark.parametrize("t,group,dim,length,cap", [(6, 2, 128, 20, 60), (6, 2, 64, 0, 60), (12, 2, 64, 117, 300), (24, 1, 128, 50, 150), (40, 1, 128, 100, 300),
                                                     (64, 2, 64, 33, 200), (64, 8, 128, 90, 160), (6, 2, 128, 1270, 1400), (28, 1, 64, 1273, 1400), (64, 1, 128, 1215, 1400),
