@@ -406,7 +406,7 @@ extern "C" int qwen_tree_attention(const qwen_kv_cache_t* cache, const void* q, 
     TRY(check_tree(cache, n_nodes, n_heads));
     const long long width = (long long)n_heads * cache->head_dim;
     if (ldq % 8 || ldo % 8 || ldq < width || ldo < width) return fail(QWEN_E_ARG, "ldq and ldo must be multiples of 8 and hold every head");
-    if (!std::isfinite(scale)) return fail(QWEN_E_ARG, "scale must be finite");
+    if (!(std::fabs(scale) < 0x1p127f)) return fail(QWEN_E_ARG, "scale must be finite and below 2^127 in magnitude");   // (times log2 e)
     if (q == out) return fail(QWEN_E_ARG, "out must not be q");
     int dev = 0;
     Plan plan;

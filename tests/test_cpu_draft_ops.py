@@ -69,6 +69,14 @@ def test_bad_attention(qb, over):
     _raises(qb, -1, qb.tree_attention, big, *{**GOOD, **over}.values())
 
 
+@pytest.mark.parametrize("scale", [2.0 ** 127, -2.4e38, 3.4e38])
+def test_attention_scales_whose_base_2_form_overflows(qb, scale):
+    big = _view(qb, capacity=4096, head_stride=4096 * 128, seq_stride=2 * 4096 * 128)
+    _raises(qb, -1, qb.tree_attention, big, *{**GOOD, "scale": scale, "parents": 0}.values())
+    with pytest.raises(qb.QwenError, match="scale"):
+        qb.tree_attention(big, *{**GOOD, "scale": scale, "parents": 0}.values())
+
+
 def test_small_caches_need_no_workspace(qb):
     assert qb.tree_attention_workspace(_view(qb), 4, 4) == 0
     _raises(qb, -1, qb.tree_attention, _view(qb), *{**GOOD, "work": OK_PTR + 4}.values())
