@@ -181,7 +181,7 @@ int attention_rows(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : 128; }
 
 struct Plan {
     int rows, row_blocks, beside, shares;   // shares: CTAs, beside for each share of the line
-    int tiles;                              // of a cache's capacity
+    int tiles, blocks;                      // of a cache's capacity: the kernel's tiles; blocks of 64 keys (tensor-memory kernel: 128)
     long long items;                        // sequences, K/V heads and blocks of rows
     float spare;
     bool whole, may_be_whole;               // a CTA for each item, no joining
@@ -193,21 +193,26 @@ int check_tree(const qwen_kv_cache_t* c, int n_nodes, int n_heads) {
     if (n_heads / c->n_kv_heads > 1 << 14) return fail(QWEN_E_UNSUPPORTED, "more than 2^14 query heads for each K/V head");
     return QWEN_OK;
 }
-// What the plan has without the device.  Caches of a few tiles have a CTA for each item: sharing the tiles out would spare a
-// CTA all but items * tiles / CTAs of them, about 0.5 us each (1.3 us in the tensor-memory kernel), and joining costs 3.5 to 4.5
-// us.  Measured, a CTA for each item against shares (bf16, 8 K/V heads): 1 sequence of 500 8.5 / 7.1 us, 8 of 500 8.7 / 10.8,
-// 8 of 1000 14.4 / 12.5, 32 of 1000 19.2 / 21.4; 64 nodes: 1 sequence of 440 12.7 / 11.7, 4 of 440 13.0 / 14.7, 4 of 900
-// 19.3 / 16.5.  Longer caches are shared out in any case, so that ragged lengths balance.
+// What the plan has without the device.  Caches of a few blocks of 64 keys have a CTA for each item: sharing the blocks out would
+// spare a CTA all but items * blocks / CTAs of them, about 0.5 us each (1.3 us for 128 in the tensor-memory kernel), and joining
+// costs 3.5 to 4.5 us.  Measured, a CTA for each item against shares, one query token and 8 K/V heads of 128, bf16: 1 sequence of
+// 500 8.4 / 6.9 us, 8 of 500 8.5 / 10.7, 8 of 1000 14.5 / 12.5, 32 of 1000 24.6 / 29.7; e4m3: 1 of 500 8.4 / 7.7, 8 of 500 8.5 /
+// 9.9, 8 of 1000 13.4 / 12.6, 32 of 1000 18.7 / 23.2.  Heads of 64, int8: 1 of 500 6.2 / 6.4, 8 of 1000 9.5 / 9.7; bf16: 1 of 500
+// 5.7 / 6.4, 8 of 1000 8.2 / 9.6 (there the blocks cost less, and the rule shares out too soon).  64 nodes, bf16: 1 sequence of
+// 440 12.7 / 12.0, 4 of 440 12.8 / 14.8, 4 of 900 18.2 / 16.3; e4m3: 1 of 240 21.0 / 17.3 (which the rule gives to one CTA), 4 of
+// 440 22.6 / 23.1, 4 of 900 31.5 / 25.7.  Longer caches are shared out in any case, so that ragged lengths balance.
 void attention_shape(const qwen_kv_cache_t* c, int n_nodes, int n_heads, Plan* p) {
     const int m = n_nodes * (n_heads / c->n_kv_heads);
     p->rows = attention_rows(m);
     p->row_blocks = (m + p->rows - 1) / p->rows;
     const bool tc = p->rows > 32;
-    p->tiles = (c->capacity + (tc ? 127 : 63)) / (tc ? 128 : 64);
+    const int keys = tc ? qb::ta::kTcKT : qb::ta::tile_keys(is8(c->dtype) ? c->head_dim : 2 * c->head_dim);
+    p->tiles = (c->capacity + keys - 1) / keys;
+    p->blocks = (c->capacity + (tc ? 127 : 63)) / (tc ? 128 : 64);
     p->items = (long long)c->n_seqs * c->n_kv_heads * p->row_blocks;
-    p->spare = tc ? 3.4f : 7.0f;      // so many tiles are worth the joining
-    p->whole = p->tiles <= p->spare && p->items < 1 << 30;
-    p->may_be_whole = p->tiles <= (tc ? 8 : 16) && p->items < 1 << 30;
+    p->spare = tc ? 3.4f : 7.0f;      // so many blocks are worth the joining
+    p->whole = p->blocks <= p->spare && p->items < 1 << 30;
+    p->may_be_whole = p->blocks <= (tc ? 8 : 16) && p->items < 1 << 30;
 }
 int attention_plan(const qwen_kv_cache_t* c, int n_nodes, int n_heads, int dev, Plan* p) {
     attention_shape(c, n_nodes, n_heads, p);
@@ -215,7 +220,7 @@ int attention_plan(const qwen_kv_cache_t* c, int n_nodes, int n_heads, int dev, 
     if (!p->whole) {
         TRY(sm_count(dev, &nsm));
         ctas = p->rows <= 32 ? qb::ta::attention_ctas(p->rows, c->head_dim) * nsm : nsm;
-        p->whole = p->may_be_whole && (double)p->tiles * std::max(0ll, ctas - p->items) <= (double)p->spare * ctas;
+        p->whole = p->may_be_whole && (double)p->blocks * std::max(0ll, ctas - p->items) <= (double)p->spare * ctas;
     }
     if (p->whole) {
         p->beside = p->row_blocks;

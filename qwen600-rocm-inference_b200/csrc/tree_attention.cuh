@@ -379,13 +379,15 @@ constexpr int kItemCost = 2;   // what an item costs beside its tiles, in tiles:
 
 // CTAs on an SM: where O takes 64 registers a thread three (168 in all, two stages), with 32 rows of 128 dims two (255 and three).
 __host__ __device__ constexpr int attention_ctas(int rows, int dim) { return rows * dim <= 16 * 128 ? 3 : 2; }
+// Keys of a tile, by the bytes of a cache row: 16 or 32 for each warp.
+__host__ __device__ constexpr int tile_keys(int row_bytes) { return kWarps * (row_bytes == 256 ? 16 : 32); }
 template <int STORE, int D, int MT>
 struct Layout {
     static constexpr int kEs = STORE == QWEN_E4M3 || STORE == QWEN_INT8 ? 1 : 2;
     static constexpr bool k8 = kEs == 1;
     static constexpr int kRow = D * kEs;                       // bytes of a cache row
-    static constexpr int KW = kRow == 256 ? 16 : 32;           // keys of a warp's part of a tile
-    static constexpr int KT = kWarps * KW;                     // keys of a tile
+    static constexpr int KT = tile_keys(kRow);                 // keys of a tile
+    static constexpr int KW = KT / kWarps;                     // keys of a warp's part of it
     static constexpr int kRows = 16 * MT;                      // query rows of an item
     static constexpr int kCtas = attention_ctas(kRows, D);        // on an SM
     static constexpr int kStages = kCtas == 3 ? 2 : 3;
