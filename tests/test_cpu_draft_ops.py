@@ -2,8 +2,13 @@
 stride, NULL and misaligned pointer is turned down with a status and a message
 before the device is touched."""
 import ctypes
+import os
+import re
+from decimal import Decimal, getcontext
 
 import pytest
+
+from conftest import PKG
 
 OK_PTR = 1 << 20    # 16-byte aligned, never followed: the calls below end before
 
@@ -109,3 +114,33 @@ def test_batch_cache_needs_a_handle(qb):
 def test_bad_debug_wait(qb, args):
     _raises(qb, -1, qb.debug_draft_wait, *args)
     qb.debug_draft_wait()
+
+
+def test_power_of_two_polynomial():
+    """The verification's fp64 powers of two: its coefficients interpolate 2^f at the nine Chebyshev nodes of [-1/2, 1/2], and are
+    within 2^-39 of it."""
+    src = open(os.path.join(PKG, "csrc", "tree_verify.cuh")).read()
+    low = [float(x) for x in re.search(r"kC\[8\] = \{([^}]*)\}", src).group(1).split(",")]
+    c = [float(re.search(r"fma\(f\[j\], ([0-9.e-]+), kC\[0\]\)", src).group(1))] + low      # highest power first
+    getcontext().prec = 50
+    ln2 = Decimal(2).ln()
+    cosines = [Decimal("0.98480775301220805936674302458952"), Decimal("0.86602540378443864676372317075294"),
+               Decimal("0.64278760968653932632264340990726"), Decimal("0.34202014332566873304409961468226")]
+    nodes = [x / 2 for x in cosines] + [Decimal(0)] + [-x / 2 for x in cosines]                # cos((2 k + 1) 10 degrees) / 2
+    table, newton = [(x * ln2).exp() for x in nodes], []
+    for i in range(9):                                                                         # divided differences
+        newton.append(table[0])
+        table = [(table[k + 1] - table[k]) / (nodes[k + 1 + i] - nodes[k]) for k in range(len(table) - 1)]
+    want = [newton[8]]
+    for i in range(7, -1, -1):                                                                 # (...) (f - node) + difference, expanded
+        want = [a - b * nodes[i] for a, b in zip(want + [Decimal(0)], [Decimal(0)] + want)]
+        want[-1] += newton[i]
+    for a, b in zip(c, want):
+        assert abs(Decimal(a) - b) <= Decimal(2) ** -48 * abs(b), (a, b)      # (the stored numbers have 16 or 17 digits of a 64-bit solution)
+    worst = 0.0
+    for k in range(-500, 501):
+        f, y = k / 1000, 0.0
+        for a in c:
+            y = y * f + a
+        worst = max(worst, abs(float(Decimal(y) / (Decimal(k) / 1000 * ln2).exp() - 1)))
+    assert worst <= 2.0 ** -39, worst
