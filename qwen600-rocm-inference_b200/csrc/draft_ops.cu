@@ -175,8 +175,10 @@ int check_rows(const qwen_kv_cache_t* c, const void* k, const void* v, int dtype
 // up to 16 and up to 32 the warp-level kernel, in one block of rows; above, where it
 // would read the cache once for every 32 rows, the tensor-memory kernel in blocks
 // of 128.  Both sides measured, 8 K/V heads of 128, warp-level / tensor memory: 24 rows, 16
-// sequences at 2048 38 / 43 us (e4m3 35 / 57), one at 8128 22 / 19; 40 rows 60 / 40 us (e4m3
-// 53 / 57), one at 8128 25 / 19.
+// sequences at 2048 37.5 / 39.7 us (e4m3 34.0 / 57.9), one at 8128 21.4 / 18.1 (e4m3 17.1 /
+// 22.1); 40 rows 57 / 40 us (e4m3 53.4 / 58.5), one at 8128 24.9 / 18.3 (e4m3 19.7 / 22.4).
+// So the rule by rows alone costs up to 15 % in two places: one long sequence of 17 to
+// 32 rows in 16 bits, and 33 to 64 rows over 8-bit caches.
 int attention_rows(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : 128; }
 
 struct Plan {

@@ -360,10 +360,11 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) { return BF ? cvt_
 
 // ---- few rows: warp-level tensor cores ------------------------------------------------
 // Bound by the cache's bytes where it is long (128 sequences of 8 nodes over 1.1 GB of
-// e4m3 cache: 200 us, 5.6 TB/s; what the instructions around the conversions need is
+// e4m3 cache: 202 us, 5.5 TB/s; what the instructions around the conversions need is
 // close behind), by the chain of plan, first loads and joining where it is short (one
-// token at 1024: 9.4 us), and by instruction issue with 32 rows of 64 dims (32
-// sequences of 7 nodes over 37 MB of int8 cache: 23.6 us, 3,000 cycles a tile).  Four
+// token at 1024: 9.4 us), and with 32 rows of 64 dims by the fixed latencies of its own
+// instructions, three warps a scheduler filling 53 % of the issue slots (32 sequences
+// of 7 nodes over 37 MB of int8 cache: 23.7 us, 3,000 cycles a tile).  Four
 // warps; each owns KW keys of a tile, its own ring of kStages cp.async stages and its own (m, l, O) over all
 // rows, so the loop has no block barrier; the four are joined at the end of an
 // item.  16-bit caches multiply in the cache's type.  8-bit codes become fp16

@@ -5,8 +5,8 @@
 //
 // With 33 and more rows (nodes times query heads a K/V head) the warp-level
 // products no longer fit under the cache's bytes, and blocks of 32 rows would
-// read them several times (40 rows, 16 sequences at 2048: 40 us here, 60 us there;
-// 24 rows: 43 us here, 38 us there).  Here an item has 128 rows, tiles have 128 keys, and
+// read them several times (bf16, 40 rows, 16 sequences at 2048: 40 us here, 57 us
+// there; 24 rows: 40 us here, 37 us there).  Here an item has 128 rows, tiles have 128 keys, and
 // 256 softmax threads serve them, two a row (64 keys each; they agree on the row's
 // maximum through shared memory).  A tile's two products take 512 cycles each
 // (4,096 multiply-adds a cycle), its 16,384 exponentials 1,024 (16 a cycle), its bytes
@@ -17,10 +17,11 @@
 //
 // Measured, bf16: one sequence of 64 nodes at 8128 19.4 us with the joining (5.2 us of
 // memory traffic; 3,000 cycles each for the plan and the first products), 8 ragged
-// sequences of 64 nodes and 8 query heads a K/V head 119 us (42 us of products at the
-// rate of a large matrix product): bound by the chain of a tile, 2,100 cycles from its
+// sequences of 64 nodes and 8 query heads a K/V head 119 to 153 us by the lengths that
+// are drawn (42 us of products at the rate of a large matrix product, for lengths of
+// the mean): bound by the chain of a tile, 2,100 cycles from its
 // scores over the maximum and the exponentials to P (the pipes of both are a third busy).
-// 8-bit caches: 16 x 20 nodes at 2048 57 us against bf16's 40, bound by the four producer
+// 8-bit caches: 16 x 20 nodes at 2048 59 us against bf16's 40, bound by the four producer
 // warps (2,200 cycles a part of a tile: copies in, codes read, fp16 written, beside the
 // scales' and the products' reads of shared memory).
 //

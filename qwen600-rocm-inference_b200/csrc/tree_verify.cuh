@@ -31,10 +31,12 @@
 // conflicts).
 //
 // Measured on a vocabulary of 151,936 in fp32: a chain of 8 nodes of one
-// sequence 21 us, 32 sequences with drafted probabilities 58 us (the rows that are
-// reached and the last drafted rows are 13 us of memory traffic; the longest of
-// the 32 walks is eight levels of 4.5 us: 2.6 us for a row's 38,000 tokens an SM,
-// 1.3 us for the exchange).
+// sequence 21 us (greedy 7.6), 32 sequences with drafted probabilities 59 us (the
+// rows that are reached and the last drafted rows are 13 us of memory traffic; the
+// longest of the 32 walks is eight levels of 4.5 us: 2.6 us for a row's 38,000 tokens
+// an SM, 1.3 us for the exchange).  Batches whose rows do not fit shared memory: 75
+// sequences of 4 nodes 109 us of 18, 150 181 us of 37, a row's parts being read from
+// the memory by one or two CTAs.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
