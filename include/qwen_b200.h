@@ -467,7 +467,8 @@ int qwen_tree_attention_workspace(const qwen_kv_cache_t* cache, int n_nodes, int
  * step; a chain of nodes is a causal step of several tokens.  q and out are
  * [n_seqs][n_nodes][n_heads][head_dim] with ldq and ldo elements between nodes
  * (multiples of 8, at least n_heads * head_dim), dtype QWEN_BF16 or QWEN_FP16, that of
- * a 16-bit cache; out is not q.  scale is finite, below 2^127 in magnitude.  Rows of absent nodes become 0; nodes whose
+ * a 16-bit cache; out is not q.  scale is finite, below 2^127 in magnitude.
+ * Rows of absent nodes become 0; nodes whose
  * position lies outside the cache, and all nodes of sequences with lens[s] < 0,
  * are absent.  What positions that a node does not see hold (NaN included) has
  * no influence on it.  Scores, softmax statistics and sums are fp32; the

@@ -3,14 +3,14 @@
 // counterpart (the reference's cache is bf16 and written by its RoPE kernel,
 // qwen_model.cuh:321-347).
 //
-// All three are bound by memory traffic where there is enough of it, a row being
-// read once and written once (prompts of 16 x 2048 tokens to int8 and back: 70 us,
-// 53 us at the copy rate; without short counts an append of all rows 41 us and a read
-// 36 us of 31, in 16 bits 42 us each of 41), and by their chains of loads where there is not (128
-// tokens in and out 3.7 us, the kept rows of one sequence in 28 layers 2.8 us).
-// A thread owns 16 elements of a row (one 16-byte store of 8-bit codes), 4 or 8
-// neighbouring threads the row, so the row's largest magnitude needs 2 or 3
-// shuffles and every access is a full 32-byte sector.
+// All three are bound by memory traffic where there is enough of it, a row being read
+// once and written once (prompts of 16 x 2048 tokens to int8 and back: 70 us, 53 us at
+// the copy rate; without short counts an append of all rows 41 us and a read 36 us of
+// 31, in 16 bits 42 us each of 41), and by their chains of loads where there is not
+// (128 tokens in and out 3.7 us, the kept rows of one sequence in 28 layers 2.8 us). A
+// thread owns 16 elements of a row (one 16-byte store of 8-bit codes), 4 or 8
+// neighbouring threads the row, so the row's largest magnitude needs 2 or 3 shuffles
+// and every access is a full 32-byte sector.
 //
 // Quantising.  The code of x in a row of largest magnitude a is the nearest
 // representable value to the real number x * top / a (top = 448 or 127), ties
@@ -186,12 +186,12 @@ struct Place {
     static constexpr int kRows = kThreads / kLanes;        // rows that a block's threads cover at once
 };
 
-// SRC rows -> STORE cache.  A quantised element takes 16 instructions (16 x 2048 tokens,
-// bf16 to int8: 71 % of the issue slots, the memory at 54 % of the copy rate), so the
-// number of those around the arithmetic counts.  U = 1: any number of tokens, threads over the rows in the
-// order (head, token), a division a row; grid (ceil(rows / kRows), n_seqs, 2).  U = 2:
-// a block takes 2 kRows tokens of one head, two a thread; grid (heads * ceil(tokens
-// / (2 kRows)), n_seqs, 2).
+// SRC rows -> STORE cache.  A quantised element takes 16 instructions (16 x 2048
+// tokens, bf16 to int8: 71 % of the issue slots, the memory at 54 % of the copy rate),
+// so the number of those around the arithmetic counts.  U = 1: any number of tokens,
+// threads over the rows in the order (head, token), a division a row; grid (ceil(rows /
+// kRows), n_seqs, 2).  U = 2: a block takes 2 kRows tokens of one head, two a thread;
+// grid (heads * ceil(tokens / (2 kRows)), n_seqs, 2).
 template <int SRC, int STORE, int D, int U>
 __global__ void __launch_bounds__(kThreads) append_kernel(Cache c, const uint8_t* __restrict__ k, const uint8_t* __restrict__ v, long long ld,
                                                           int n_heads, int n_tokens, const int* __restrict__ start,

@@ -364,17 +364,17 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) { return BF ? cvt_
 // close behind), by the chain of plan, first loads and joining where it is short (one
 // token at 1024: 9.4 us), and with 32 rows of 64 dims by the fixed latencies of its own
 // instructions, three warps a scheduler filling 53 % of the issue slots (32 sequences
-// of 7 nodes over 37 MB of int8 cache: 23.7 us, 3,000 cycles a tile).  Four
-// warps; each owns KW keys of a tile, its own ring of kStages cp.async stages and its own (m, l, O) over all
-// rows, so the loop has no block barrier; the four are joined at the end of an
-// item.  16-bit caches multiply in the cache's type.  8-bit codes become fp16
-// (exact for both types): queries are scaled by a power of two per row into
-// fp16's range (bf16 queries; the factor returns with the score), a key's scale
-// multiplies its scores, a value row's scale its weights; m is the running maximum
-// times a power of two that is at least the largest scale so far of the keys that
-// the row sees (within 2^14 for the tree's), so the weights stay within fp16 and
-// unseen scales have no part in them.  P is rounded to 16 bits (off by half a step:
-// 2^-8 or 2^-11 relative) as the product with V takes it; l sums it unrounded.
+// of 7 nodes over 37 MB of int8 cache: 23.7 us, 3,000 cycles a tile).  Four warps; each
+// owns KW keys of a tile, its own ring of kStages cp.async stages and its own (m, l, O)
+// over all rows, so the loop has no block barrier; the four are joined at the end of an
+// item.  16-bit caches multiply in the cache's type.  8-bit codes become fp16 (exact
+// for both types): queries are scaled by a power of two per row into fp16's range (bf16
+// queries; the factor returns with the score), a key's scale multiplies its scores, a
+// value row's scale its weights; m is the running maximum times a power of two that is
+// at least the largest scale so far of the keys that the row sees (within 2^14 for the
+// tree's), so the weights stay within fp16 and unseen scales have no part in them.  P
+// is rounded to 16 bits (off by half a step: 2^-8 or 2^-11 relative) as the product
+// with V takes it; l sums it unrounded.
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kItemCost = 2;   // what an item costs beside its tiles, in tiles: set-up, queries, joining the warps
 

@@ -3,17 +3,17 @@
 // mathematics and the division of the work are tree_attention.cuh's.  No
 // reference counterpart.
 //
-// With 33 and more rows (nodes times query heads a K/V head) the warp-level
-// products no longer fit under the cache's bytes, and blocks of 32 rows would
-// read them several times (bf16, 40 rows, 16 sequences at 2048: 40 us here, 57 us
-// there; 24 rows: 40 us here, 37 us there).  Here an item has 128 rows, tiles have 128 keys, and
-// 256 softmax threads serve them, two a row (64 keys each; they agree on the row's
-// maximum through shared memory).  A tile's two products take 512 cycles each
-// (4,096 multiply-adds a cycle), its 16,384 exponentials 1,024 (16 a cycle), its bytes
-// (bf16, 128 dims) 2,800 of an SM's share of the memory bandwidth.  S and P have two
-// buffers each, so that the next tile's S is formed during a tile's exponentials.
-// (Two blocks of rows over shared tiles leave tensor memory for one S each: a
-// chain of products and exponentials without overlap, 2,800 cycles a block and tile.)
+// With 33 and more rows (nodes times query heads a K/V head) the warp-level products no
+// longer fit under the cache's bytes, and blocks of 32 rows would read them several
+// times (bf16, 40 rows, 16 sequences at 2048: 40 us here, 57 us there; 24 rows: 40 us
+// here, 37 us there).  Here an item has 128 rows, tiles have 128 keys, and 256 softmax
+// threads serve them, two a row (64 keys each; they agree on the row's maximum through
+// shared memory).  A tile's two products take 512 cycles each (4,096 multiply-adds a
+// cycle), its 16,384 exponentials 1,024 (16 a cycle), its bytes (bf16, 128 dims) 2,800
+// of an SM's share of the memory bandwidth.  S and P have two buffers each, so that the
+// next tile's S is formed during a tile's exponentials. (Two blocks of rows over shared
+// tiles leave tensor memory for one S each: a chain of products and exponentials
+// without overlap, 2,800 cycles a block and tile.)
 //
 // Measured, bf16: one sequence of 64 nodes at 8128 19.4 us with the joining (5.2 us of
 // memory traffic; 3,000 cycles each for the plan and the first products), 8 ragged

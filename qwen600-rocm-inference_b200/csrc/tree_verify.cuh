@@ -20,15 +20,14 @@
 // straight to every CTA through distributed shared memory: one cluster barrier a
 // pass.
 //
-// Statistics that decide a comparison (largest logit, sum) are fp32 until a token
-// with drafted probabilities, or most of the row's weight, is refused; then what is
-// left is summed in fp64.  Sums that the drawn token's position depends on are fp64: the
-// running sum crosses a border for each of up to 10^5 tokens, so 24 bits would
-// misplace about one draw in a hundred.  Their powers of two are a polynomial of
-// degree 8 in fp64, which interpolates 2^f at the nine Chebyshev nodes
-// cos((2 k + 1) pi / 18) / 2 of [-1/2, 1/2] (relative error 2^-39, 13 fp64 operations
-// a token; a table of 256 roots with three operations took as long, on bank
-// conflicts).
+// Statistics that decide a comparison (largest logit, sum) are fp32 until a token with
+// drafted probabilities, or most of the row's weight, is refused; then what is left is
+// summed in fp64.  Sums that the drawn token's position depends on are fp64: the
+// running sum crosses a border for each of up to 10^5 tokens, so 24 bits would misplace
+// about one draw in a hundred.  Their powers of two are a polynomial of degree 8 in
+// fp64, which interpolates 2^f at the nine Chebyshev nodes cos((2 k + 1) pi / 18) / 2
+// of [-1/2, 1/2] (relative error 2^-39, 13 fp64 operations a token; a table of 256
+// roots with three operations took as long, on bank conflicts).
 //
 // Measured on a vocabulary of 151,936 in fp32: a chain of 8 nodes of one
 // sequence 21 us (greedy 7.6), 32 sequences with drafted probabilities 59 us (the

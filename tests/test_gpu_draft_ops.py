@@ -464,7 +464,7 @@ def test_attention_unseen_scales_do_not_matter(qb, store, t, group, dim, length,
         got = _attend(qb, poisoned(range(2, t, 2), value, False), q, lens, par, dim ** -0.5)
         odd = [0] + list(range(1, here, 2))
         assert torch.equal(got[:, odd], want[:, odd]), value
-    for value in (1e-20, 3e3, 1e18):             # rows that see them: large values, but an ordinary score
+    for value in (1e-20, 10.0, 60.0, 3e3, 1e18): # rows that see them: large values, but an ordinary score
         c = poisoned(range(2, t, 2), value, True)
         c.ks.copy_(clean.ks)
         got = _attend(qb, c, q, lens, par, dim ** -0.5).double()
