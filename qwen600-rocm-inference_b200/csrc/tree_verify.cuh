@@ -359,8 +359,8 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Params P) {
 
         // ---- children in index order ----
         int kept = -1, n_gone = 0;
-        // Z: the last sum; left, S and rest are the row's sum times those of the walk's definition
-        double Z = z, left = Z, S = 0.0;
+        // left, S and rest are the row's sum times those of the walk's definition; low: where what is left must be summed anew
+        double left = z, low = 0.0625 * left, S = 0.0;
         bool summed = false;     // left is the last sum pass's
         const double M64 = M;
         // weights 2^(c (x - M)) = 2^n 2^f, |f| <= 1/2, of K tokens; in[j]: the weight counts (not below 2^-1000).  The steps go
@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Params P) {
             if ((double)sh.u[i] * left * q < rest) {
                 kept = i;
             } else if (qrow) {
-                if (!summed) left = Z = sum_pass();   // to 64 bits from here on
+                if (!summed) left = sum_pass();   // to 64 bits from here on
                 S += left;
                 left = sum_pass();
                 summed = true;
@@ -500,10 +500,11 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Params P) {
                 __syncthreads();
                 n_gone++;
                 summed = false;
-                // Little is left of the last sum: the next child is compared with a sum of what is left, in 64 bits, not with a
-                // difference of fp32 sums (off by about 2^-21 of Z: 2^-18 of an eighth of it).
-                if ((children & (children - 1)) && left < 0.125 * Z) {
-                    left = Z = sum_pass();
+                // Little is left, and the next child is compared with it: not with a difference of an fp32 sum, which is off by about
+                // 2^-21 (2^-17 of a sixteenth of it), but with a sum in fp64.  (That is off by 2^-39: differences of it last longer.)
+                if ((children & (children - 1)) && left < low) {
+                    left = sum_pass();
+                    low = 0x1p-16 * left;
                     summed = true;
                 }
             }

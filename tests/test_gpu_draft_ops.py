@@ -771,7 +771,7 @@ def test_verify_after_a_likely_token_is_refused(qb, vocab, dtype, top):
     par = np.tile(np.array([-1, 0, 0, 0, 0], np.int32), (b, 1))
     tokens = np.tile(np.array([0, 0, 1, 2, 3], np.int32), (b, 1))
     u = np.random.RandomState(5).rand(b, 5)
-    # fp32 sums of the row are off by about 2^-21; what is left behind the first child by 2^-18 at most, or it is summed in 64 bits
+    # fp32 sums of the row are off by about 2^-21; what is left behind the first child by 2^-17 at most, or it is summed in 64 bits
     edge = 1e-5
     for r in range(b):
         left = 1 - p[r, 0]
