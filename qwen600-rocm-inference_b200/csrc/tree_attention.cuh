@@ -646,8 +646,9 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attentio
                 uint32_t rows_ve = 0;   // 8-bit, where a scale of the tree lies far above the context's: a byte for each of this lane's rows
                 if constexpr (L::k8) {
                     const uint32_t own = scale_exponent(reinterpret_cast<const float*>(st + 2 * L::kPart)[KW + lane]);
-                    ve = max(ve, __reduce_max_sync(~0u, k0 + lane < len ? own : 0u));
-                    if (tail && __any_sync(~0u, k0 + lane >= len && own > ve + kTreeRise))
+                    const bool all_see = k0 + lane < len + (P.n_nodes == 1);   // (a single node's row sees itself, or is dropped)
+                    ve = max(ve, __reduce_max_sync(~0u, all_see ? own : 0u));
+                    if (tail && __any_sync(~0u, !all_see && own > ve + kTreeRise))
                         rows_ve = tree_exponents<2 * MT>(own, ve, vis[0], vis[1], vis[2 * MT - 2], vis[2 * MT - 1], max(len - k0, 0), min(KW, end - k0));
                 }
                 const float unit = L::k8 ? (float)((int)ve - 127) : 0.f;
