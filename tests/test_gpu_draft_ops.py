@@ -574,13 +574,13 @@ def test_attention_without_workspace(qb, b, t, group, cap, dim, store):
 
 
 def test_attention_workspace_of_the_longest_lines(qb):
-    """65,535 sequences of 16 heads over 131,072 positions are 1.07 * 10^9 tiles of 128 keys: a plan below 2^31. Twice as long is not."""
+    """65,535 sequences of 16 heads over 131,200 positions are 1.08 * 10^9 tiles of 128 keys: a plan below 2^31. Twice as long is not."""
     def view(cap, store):
         scale = 1 << 20 if store == "e4m3" else None
         return qb.KVCache(1 << 20, 1 << 20, scale, scale, 16 * cap * 128, cap * 128, _types(qb)[store][0], 65535, 16, 128, cap)
 
-    assert qb.tree_attention_workspace(view(131072, "e4m3"), 1, 16) > 0
-    for cap, store in ((262144, "e4m3"), (131072, "bf16")):
+    assert qb.tree_attention_workspace(view(131200, "e4m3"), 1, 16) > 0
+    for cap, store in ((262400, "e4m3"), (131200, "bf16")):
         with pytest.raises(qb.QwenError) as e:
             qb.tree_attention_workspace(view(cap, store), 1, 16)
         assert e.value.code == -6
