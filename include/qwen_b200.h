@@ -474,10 +474,11 @@ int qwen_tree_attention_workspace(const qwen_kv_cache_t* cache, int n_nodes, int
  * no influence on it.  Scores, softmax statistics and sums are fp32; the
  * weights enter the product with V in 16 bits.  8-bit caches: weight * scale, as
  * fp16 relative to the largest scale so far that the row sees, or to 2^-90 where
- * all are smaller (qwen_kv_append makes none below 2^-69); with scales above 2^100
- * (values above 5 * 10^32) weights below 2^-26 of the largest may be left out; bf16
- * queries become fp16 relative to the largest element of their row and head, so
- * elements below 2^-17 of it lose bits.  workspace: as many bytes as
+ * all are smaller (qwen_kv_append makes none below 2^-69).  A call of more than 32
+ * query rows a K/V head may leave out of the sums weights below 2^-26 of the largest
+ * where scales exceed 2^100 (values 5 * 10^32), and keys whose scales lie 2^126 below
+ * another's.  bf16 queries become fp16 relative to the largest element of their row
+ * and head, so elements below 2^-17 of it lose bits.  workspace: as many bytes as
  * qwen_tree_attention_workspace says, contents free, 16-byte aligned (may be
  * NULL where it says 0); calls that may overlap need one each.  The rows of a
  * call whose device-side waits ran out (they are bounded) are NaN. */

@@ -337,12 +337,12 @@ __device__ __forceinline__ uint32_t scale_exponent(float vs) {
     return e == 255u ? 0u : min(e + 1, 253u);
 }
 // Scales of the tree may lie up to 2^14 above the context's in the same units: weight times scale is then below 2^14, within fp16.
-// Beyond that a row takes the largest exponent of the tree's keys that it sees (own: lane x's is key x's; bit x of v: the row sees
-// it), and ve where none of those is as large: a byte for each of this lane's rows.  Out of line: seldom, and inline it costs the
-// loop around it 1 to 3 %.
+// Beyond that rows have units of their own: the largest exponent of the tree's keys that the row sees (own: lane x's is key x's; bit
+// x of v: the row sees it), or was, where none of those is 2^14 above it; a byte for each of this lane's rows.  Out of line: seldom,
+// and inline it costs the loop around it 1 to 3 %.
 constexpr uint32_t kTreeRise = 14;
 template <int ROWS>
-__device__ __noinline__ uint32_t tree_exponents(uint32_t own, uint32_t ve, uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3, int from, int to) {
+__device__ __noinline__ uint32_t tree_exponents(uint32_t own, uint32_t was, uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3, int from, int to) {
     const uint32_t v[4] = {v0, v1, v2, v3};
     uint32_t most = 0;
     for (int x = from; x < to; x++) {
@@ -352,8 +352,8 @@ __device__ __noinline__ uint32_t tree_exponents(uint32_t own, uint32_t ve, uint3
         for (int r = 0; r < ROWS; r++) seen |= (v[r] >> x & 1 ? e : 0u) << (8 * r);
         most = __vmaxu4(most, seen);
     }
-    const uint32_t above = __vcmpgtu4(most, min(ve + kTreeRise, 255u) * 0x01010101u);
-    return (most & above) | (ve * 0x01010101u & ~above);
+    const uint32_t above = __vcmpgtu4(most, __vaddus4(was, kTreeRise * 0x01010101u));
+    return (most & above) | (was & ~above);
 }
 template <bool BF>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) { return BF ? cvt_bf16x2(lo, hi) : kv::half2_bits(lo, hi); }
@@ -370,10 +370,10 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) { return BF ? cvt_
 // item.  16-bit caches multiply in the cache's type.  8-bit codes become fp16 (exact
 // for both types): queries are scaled by a power of two per row into fp16's range (bf16
 // queries; the factor returns with the score), a key's scale multiplies its scores, a
-// value row's scale its weights; m is the running maximum times a power of two that is
-// at least the largest scale so far of the keys that the row sees (within 2^14 for the
-// tree's), so the weights stay within fp16 and unseen scales have no part in them.  P
-// is rounded to 16 bits (off by half a step: 2^-8 or 2^-11 relative) as the product
+// value row's scale its weights, divided by a power of two that is at least the
+// largest scale so far of the keys that the row sees (within 2^14 for the tree's), so
+// the weights stay within fp16 and unseen scales have no part in them.  P is rounded
+// to 16 bits (off by half a step: 2^-8 or 2^-11 relative) as the product
 // with V takes it; l sums it unrounded.
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kItemCost = 2;   // what an item costs beside its tiles, in tiles: set-up, queries, joining the warps
@@ -558,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attentio
                 for (int e = 0; e < 4; e++) o[mt][d][e] = 0.f;
         #pragma unroll
         for (int i = 0; i < 2 * MT; i++) { m[i] = -INFINITY; l[i] = 0.f; }
-        uint32_t ve = 37;  // 8-bit caches: the exponent of the context's largest value scale so far, 2^-90 at least; m holds it as well
+        uint32_t ve = 1;   // 8-bit caches: O is in units of 2^(ve - 127); above 255 a byte for each of this lane's rows
 
         for (int t = t0; t < t1; t++) {
             {
@@ -643,17 +643,27 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attentio
                                 if (!sees(2 * mt + (e >> 1), 8 * i + 2 * j + (e & 1))) s[mt][i][e] = -INFINITY;
                 }
                 // ---- softmax ----
-                uint32_t rows_ve = 0;   // 8-bit, where a scale of the tree lies far above the context's: a byte for each of this lane's rows
+                uint32_t up = 0;        // 8-bit: the rise of ve, or of its bytes
+                bool apart = false;     // rows have units of their own (the same for the warp)
                 if constexpr (L::k8) {
                     const uint32_t own = scale_exponent(reinterpret_cast<const float*>(st + 2 * L::kPart)[KW + lane]);
                     const bool all_see = k0 + lane < len + (P.n_nodes == 1);   // (a single node's row sees itself, or is dropped)
-                    ve = max(ve, __reduce_max_sync(~0u, all_see ? own : 0u));
-                    if (tail && __any_sync(~0u, !all_see && own > ve + kTreeRise))
-                        rows_ve = tree_exponents<2 * MT>(own, ve, vis[0], vis[1], vis[2 * MT - 2], vis[2 * MT - 1], max(len - k0, 0), min(KW, end - k0));
+                    const uint32_t e = __reduce_max_sync(~0u, all_see ? own : 0u);
+                    apart = ve > 255u || (tail && __any_sync(~0u, !all_see && own > max(e, ve) + kTreeRise));
+                    if (!apart) {
+                        if (e > ve) { up = e - ve; ve = e; }
+                        const float vinv = __uint_as_float((254u - ve) << 23);
+                        #pragma unroll
+                        for (int i = 0; i < NT; i++) mul2(vs[i][0], vs[i][1], vinv, vinv);
+                    } else {
+                        const uint32_t was = ve > 255u ? ve : ve * 0x01010101u;
+                        ve = tree_exponents<2 * MT>(own, __vmaxu4(was, e * 0x01010101u), vis[0], vis[1], vis[2 * MT - 2], vis[2 * MT - 1], max(len - k0, 0),
+                                                    min(KW, end - k0));
+                        up = ve - was;   // (no byte falls)
+                    }
                 }
-                const float unit = L::k8 ? (float)((int)ve - 127) : 0.f;
                 float f[2 * MT];
-                bool moved = false;
+                bool moved = up != 0;
                 #pragma unroll
                 for (int r = 0; r < 2 * MT; r++) {
                     float mx = -INFINITY;
@@ -661,9 +671,7 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attentio
                     for (int i = 0; i < NT; i++) mx = fmaxf(mx, fmaxf(s[r >> 1][i][2 * (r & 1)], s[r >> 1][i][2 * (r & 1) + 1]));
                     mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
-                    float mn = mx == -INFINITY ? mx : L::k8 ? fmaf(mx, c[r], unit) : mx * c[r];
-                    if (L::k8 && rows_ve) mn += (float)((int)(rows_ve >> (8 * r) & 0xffu) - (int)ve);
-                    mn = fmaxf(m[r], mn);
+                    const float mn = fmaxf(m[r], mx == -INFINITY ? mx : mx * c[r]);
                     const float base = mn == -INFINITY ? 0.f : mn;
                     f[r] = exp2_approx(m[r] - base);
                     moved |= mn > m[r];
@@ -688,8 +696,29 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attentio
                             #pragma unroll
                             for (int e = 0; e < 2; e++)
                                 if (!sees(r, 8 * i + 2 * j + e)) s[r >> 1][i][2 * (r & 1) + e] = 0.f;
+                    if (apart) {
+                        #pragma unroll
+                        for (int r = 0; r < 2 * MT; r++) {
+                            const float vinv = __uint_as_float((254u - (ve >> (8 * r) & 0xffu)) << 23);
+                            #pragma unroll
+                            for (int i = 0; i < NT; i++) mul2(s[r >> 1][i][2 * (r & 1)], s[r >> 1][i][2 * (r & 1) + 1], vinv, vinv);
+                        }
+                    }
                 }
                 if (__any_sync(~0u, moved)) {
+                    if constexpr (L::k8) {
+                        if (!apart) {
+                            const float w = up < 127u ? __uint_as_float((127u - up) << 23) : 0.f;
+                            #pragma unroll
+                            for (int r = 0; r < 2 * MT; r++) f[r] *= w;
+                        } else {
+                            #pragma unroll
+                            for (int r = 0; r < 2 * MT; r++) {
+                                const uint32_t u = up >> (8 * r) & 0xffu;
+                                f[r] *= u < 127u ? __uint_as_float((127u - u) << 23) : 0.f;
+                            }
+                        }
+                    }
                     #pragma unroll
                     for (int mt = 0; mt < MT; mt++)
                         #pragma unroll
@@ -787,6 +816,7 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attentio
         float* join_ml = join + kWarps * L::kRows * D;
         #pragma unroll
         for (int r = 0; r < 2 * MT; r++) {
+            const float unit_v = L::k8 ? __uint_as_float((ve > 255u ? ve >> (8 * r) & 0xffu : ve) << 23) : 1.0f;
             float sum = l[r];
             sum += __shfl_xor_sync(~0u, sum, 1);
             sum += __shfl_xor_sync(~0u, sum, 2);
@@ -800,7 +830,7 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attentio
                 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     const int dim = L::k8 ? (d >> 1) * 16 + 4 * j + 2 * e + (d & 1) : 8 * d + 2 * j + e;
-                    join[(warp * L::kRows + row) * D + dim] = o[r >> 1][d][2 * (r & 1) + e];
+                    join[(warp * L::kRows + row) * D + dim] = o[r >> 1][d][2 * (r & 1) + e] * unit_v;
                 }
         }
         __syncthreads();

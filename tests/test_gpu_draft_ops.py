@@ -478,6 +478,29 @@ def test_attention_unseen_scales_do_not_matter(qb, store, t, group, dim, length,
         assert bool(((got - want64).abs() <= tol).all()), value
 
 
+@pytest.mark.parametrize("store", ["e4m3", "int8"])
+@pytest.mark.parametrize("t,group,dim,cap,low,high", [(3, 2, 128, 300, -60, 115), (3, 2, 128, 1400, -60, 115), (7, 4, 64, 300, 90, 115), (12, 2, 128, 1400, -60, 60),
+                                                      (40, 1, 128, 300, -30, 90), (40, 2, 64, 1400, 60, 90)])
+def test_attention_value_scales_of_any_size(qb, store, t, group, dim, cap, low, high):
+    """Value rows between 2^low and 2^high: the small ones vanish beside the large, and every key counts in the sum of the weights."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(t + high)
+    c = Cache(qb, 2, 2, cap, dim, store).fill(g)
+    c.vs *= torch.exp2(torch.randint(low, high + 1, c.vs.shape, generator=g, device="cuda").float())
+    q = torch.randn(2, t, 2 * group, dim, generator=g, device="cuda").to(torch.bfloat16)
+    lens, par = [cap - t, cap // 3], _tree(np.random.RandomState(t), 2, t)
+    got = _attend(qb, c, q, lens, par, dim ** -0.5).double()
+    want, tol = _attention64(c, q, lens, par, dim ** -0.5)
+    codes = c.v.float().double().abs()
+    for r in range(2):                           # fp16's smallest steps, as above: 2^-24 of the largest seen scale for each key's code
+        for i, up in enumerate(_sees(par[r].tolist(), lens[r], cap)):
+            if up is not None:
+                at = list(range(lens[r])) + [lens[r] + j for j in sorted(up)]
+                low_bits = 2.0 ** -24 * c.vs[r][:, at].double().amax(1)[:, None] * codes[r][:, at].sum(1)
+                tol[r, i] += low_bits.repeat_interleave(group, 0)
+    assert bool(((got - want).abs() <= tol).all())
+
+
 def test_attention_infinity_in_a_seen_branch(qb):
     """A V row with one infinity: that dim of the nodes that see it becomes infinite, nothing else changes."""
     import torch
