@@ -523,6 +523,98 @@ int qwen_tree_verify(const void* logits, int logits_dtype, long long ld, const f
  * qwen_debug_draft_wait(0, -1) restores normal operation. */
 int qwen_debug_draft_wait(unsigned long long wait_ns, int part);
 
+/* ---- serving over a K/V cache in pages (no reference counterpart) ---------- */
+/* The operators of a server that packs its prompts and keeps its cache in pages:
+ * new rows are normalised, rotated and put into their pages, whole prompts attend
+ * to themselves, single tokens attend to their pages, and given tokens are
+ * scored.  The common rules of the operators above hold for these too (device
+ * memory of the current device, rows 16-byte aligned and the rest 4-byte,
+ * asynchronous on `stream`, nothing allocated, capturable; lengths, positions and
+ * page numbers are read on the device, and whatever they hold, nothing outside the
+ * described buffers is touched; what a call writes overlaps nothing else that it
+ * takes). */
+
+/* A cache in pages: n_pages pages of page_size positions each (a power of two up
+ * to 2^16).  Position p of head h of sequence s is row p % page_size of page table[s *
+ * max_pages + p / page_size]: the head_dim elements at k + page * page_stride + h *
+ * head_stride + (p % page_size) * head_dim (elements; strides are multiples of
+ * head_dim, at least page_size * head_dim, and no two rows that the table names share memory).  A page
+ * number outside 0 .. n_pages-1 marks a page that is not there.  dtype, head_dim and
+ * the 8-bit types' scales are as for qwen_kv_cache_t, the scale of a row at k_scale
+ * + (page * page_stride + h * head_stride) / head_dim + p % page_size.  A page may
+ * serve several sequences.  max_pages * page_size is at most 2^30. */
+typedef struct {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    const int* table;
+    long long page_stride, head_stride;
+    int dtype, n_pages, n_seqs, n_kv_heads, head_dim, page_size, max_pages;
+} qwen_kv_pages_t;
+
+/* The norms of queries and keys, their rotation, and the way into the cache, in
+ * one pass over n_rows tokens' projections.  Row r of q (n_heads heads), k and v
+ * (n_kv_heads heads; head_dim 64 or 128; dtype QWEN_BF16, QWEN_FP16 or QWEN_FP32; rows
+ * ldq, ldk, ldv elements apart, multiples of 8 that hold every head) is a token at position
+ * positions[r] (of sequence seqs[r]).  Each head x of q and k becomes
+ *     y = x / sqrt(mean(x^2) + eps) * gain   (gain: head_dim values of gain_dtype, which is
+ *         QWEN_BF16, QWEN_FP16 or QWEN_FP32; q_gain and k_gain may both be NULL: y = x),
+ *     y_j cos a_j - y_(j+head_dim/2) sin a_j  and  y_(j+head_dim/2) cos a_j + y_j sin a_j,
+ *     a_j = positions[r] * base^(-2 j / head_dim),   j < head_dim / 2,
+ * computed in fp32 (angles modulo a turn in 64-bit whole numbers, so far positions
+ * are as exact as near ones) and rounded once.  q goes to q_out, k to k_out (out_dtype
+ * QWEN_BF16, QWEN_FP16 or QWEN_FP32, rows ldqo and ldko apart; k_out may be NULL), and,
+ * with pages not NULL, k and v to their pages, 8-bit ones quantised by qwen_kv_append's rule
+ * (k from its fp32 values).  Without pages v and seqs are not read and may be NULL.  Tokens
+ * whose sequence, position or page is not there reach no page; rows with a negative
+ * position are left out altogether.  No two rows may have the same place in the pages.
+ * eps is finite and not negative, base finite and at least 1. */
+int qwen_qk_rope(const void* q, const void* k, const void* v, int dtype, long long ldq, long long ldk, long long ldv, int n_rows,
+                 int n_heads, int n_kv_heads, int head_dim, const void* q_gain, const void* k_gain, int gain_dtype, float eps, double base,
+                 const int* positions, void* q_out, void* k_out, int out_dtype, long long ldqo, long long ldko,
+                 const qwen_kv_pages_t* pages, const int* seqs, void* stream);
+
+/* Attention of whole prompts, packed one behind the other.  Sequence s has the query
+ * rows starts[s] .. starts[s+1]-1 and the keys k_starts[s] .. k_starts[s+1]-1 (k_starts
+ * NULL: the same as the queries); its last query sees all of its keys and each query
+ * before it one key fewer: query i of n sees keys 0 .. m - n + i of m, so keys may begin
+ * with a context.  A query that sees no key gets zeros.  q and out are [n_rows][n_heads][head_dim],
+ * k and v [n_keys][n_kv_heads][head_dim] (rows ldq, ldo, ldk, ldv elements apart, multiples of 8),
+ * dtype QWEN_BF16 or QWEN_FP16, head_dim 64 or 128, query head h uses K/V head h / (n_heads /
+ * n_kv_heads), at most 128 for each.  starts and k_starts ([n_seqs + 1], not falling, within 0 ..
+ * n_rows and 0 .. n_keys; what lies beyond counts as the nearest end, and a sequence whose
+ * start lies behind its end has no rows or keys).  Rows that belong to no sequence stay as they
+ * were.  o = sum_j softmax_j(scale * q . k_j) v_j with scores, softmax statistics and sums in fp32; the
+ * weights enter the product with V in 16 bits.  What a query does not see (NaN included) has
+ * no influence on it.  scale is finite, below 2^127 in magnitude.  The rows of a call whose
+ * device-side waits ran out (they are bounded) are NaN. */
+int qwen_prompt_attention(const void* q, const void* k, const void* v, void* out, int dtype, long long ldq, long long ldk, long long ldv,
+                          long long ldo, const int* starts, const int* k_starts, int n_seqs, int n_rows, int n_keys, int n_heads,
+                          int n_kv_heads, int head_dim, float scale, void* stream);
+
+/* Bytes of workspace that qwen_paged_attention needs for these sizes (0 for short caches). */
+int qwen_paged_attention_workspace(const qwen_kv_pages_t* pages, int n_heads, size_t* bytes);
+
+/* Attention of one new token a sequence over its pages: the token at position lens[s],
+ * whose own K and V are already there, attends to positions 0 .. lens[s].  q and out are
+ * [n_seqs][n_heads][head_dim], rows ldq and ldo elements apart; types, head layout, scale,
+ * roundings and workspace are as for qwen_tree_attention with a single node, 8-bit caches
+ * included.  Positions whose page is not there are left out.  lens[s] < 0 or beyond the
+ * table, and sequences without any page, give zeros. */
+int qwen_paged_attention(const qwen_kv_pages_t* pages, const void* q, void* out, int dtype, long long ldq, long long ldo, int n_heads,
+                         const int* lens, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Log probabilities under p = softmax(logits / temperature) of each of n_rows rows of logits
+ * (dtype QWEN_FP32, QWEN_BF16 or QWEN_FP16; vocab columns, rows ld elements apart):
+ * logprob[r] = log p(tokens[r]) (tokens and logprob may both be NULL; a token outside 0 ..
+ * vocab-1 gives NaN), entropy[r] = -sum p log p (may be NULL), and the n_top likeliest tokens
+ * (0 .. 64) with their log probabilities, likeliest first, equal logits by the smaller id:
+ * top_ids and top_logprobs, [n_rows][n_top]; places beyond the vocabulary hold -1 and -inf.  Logits of
+ * -inf are tokens that cannot come.  A row with a NaN, a +inf or nothing above -inf has no
+ * distribution: NaN, ids -1.  temperature is within 1e-6 .. 1e6.  Differences between
+ * logits below -1e30 count as none in the sums. */
+int qwen_token_logprobs(const void* logits, int dtype, long long ld, int n_rows, int vocab, const int* tokens, float temperature, int n_top,
+                        float* logprob, float* entropy, int* top_ids, float* top_logprobs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

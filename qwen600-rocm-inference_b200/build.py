@@ -17,10 +17,11 @@ LIB = os.path.join(HERE, "lib")
 OUT = os.path.join(LIB, "libqwen_b200.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
-CUDA_SOURCES = ["engine.cu", "draft_ops.cu"]
+CUDA_SOURCES = ["engine.cu", "draft_ops.cu", "serve_ops.cu"]
 HOST_SOURCES = ["model_format.cpp", "host_sampler.cpp", "tokenizer.cpp"]
 HEADERS = ["decode_kernel.cuh", "attention_tc5.cuh", "gemv_kernel.cuh", "gemm_tc.cuh", "prefill_kernels.cuh", "ptx.cuh", "model_format.h",
-           "kv_rows.cuh", "tree_attention.cuh", "tree_attention_tc.cuh", "tree_verify.cuh"]
+           "kv_rows.cuh", "tree_attention.cuh", "tree_attention_tc.cuh", "tree_verify.cuh", "op_checks.cuh", "attention_plan.cuh", "kv_pages.cuh",
+           "paged_attention.cuh", "prompt_attention.cuh", "token_logprobs.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-std=c++17", "-Xcompiler", "-fPIC,-fopenmp", "-I", os.path.join(HERE, "..", "include")]
 

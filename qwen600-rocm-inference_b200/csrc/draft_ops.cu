@@ -8,66 +8,31 @@
 #include <atomic>
 #include <climits>
 #include <cmath>
-#include <initializer_list>
 #include <string>
 
 #include "../../include/qwen_b200.h"
+#include "attention_plan.cuh"
 #include "kv_rows.cuh"
+#include "op_checks.cuh"
 #include "tree_attention.cuh"
 #include "tree_attention_tc.cuh"
 #include "tree_verify.cuh"
 
-int qwen_internal_fail(int code, const std::string& msg);
-
 namespace {
-
-int fail(int code, const std::string& msg) { return qwen_internal_fail(code, msg); }
-#define CU(call)                                                                                        \
-    do {                                                                                                \
-        cudaError_t e_ = (call);                                                                        \
-        if (e_ != cudaSuccess) return fail(QWEN_E_CUDA, std::string(#call) + ": " + cudaGetErrorString(e_)); \
-    } while (0)
-#define TRY(call)                          \
-    do {                                   \
-        int rc_ = (call);                  \
-        if (rc_ != QWEN_OK) return rc_;    \
-    } while (0)
 
 // ---- waits (qwen_debug_draft_wait) ---------------------------------------------
 constexpr unsigned long long kWaitNs = 1000000000ull;   // for copies and products on this GPU: they take microseconds
 std::atomic<unsigned long long> g_wait_ns{kWaitNs};
 std::atomic<int> g_withheld{-1};
 
-// ---- argument checks -----------------------------------------------------------
-struct Ptr {
-    const void* p;
-    const char* name;
-    size_t align;
-    bool used;   // false: may be anything
-};
-// NULL and alignment first (no GPU needed), then: device memory of the current device, *dev.
-int check_ptrs(std::initializer_list<Ptr> ptrs, int* dev) {
-    for (const Ptr& a : ptrs) {
-        if (!a.used) continue;
-        if (!a.p) return fail(QWEN_E_ARG, std::string(a.name) + " is NULL");
-        if ((uintptr_t)a.p % a.align) return fail(QWEN_E_ARG, std::string(a.name) + " must be " + std::to_string(a.align) + "-byte aligned");
-    }
-    CU(cudaGetDevice(dev));
-    for (const Ptr& a : ptrs) {
-        if (!a.used) continue;
-        cudaPointerAttributes at;
-        const cudaError_t e = cudaPointerGetAttributes(&at, a.p);
-        if (e != cudaSuccess) cudaGetLastError();   // not left behind for the caller's next query
-        if (e != cudaSuccess || (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged))
-            return fail(QWEN_E_ARG, std::string(a.name) + " is not device memory");
-        if (at.type == cudaMemoryTypeDevice && at.device != *dev)
-            return fail(QWEN_E_ARG, std::string(a.name) + " lies on another device than the current one");
-    }
-    return QWEN_OK;
-}
-bool is16(int t) { return t == QWEN_BF16 || t == QWEN_FP16; }
-bool is8(int t) { return t == QWEN_E4M3 || t == QWEN_INT8; }
+}  // namespace
 
+unsigned long long qwen_internal_wait_ns() { return g_wait_ns.load(); }
+int qwen_internal_withheld() { return g_withheld.load(); }
+
+namespace {
+
+// ---- argument checks -----------------------------------------------------------
 int check_view(const qwen_kv_cache_t* c) {
     if (!c) return fail(QWEN_E_ARG, "NULL cache view");
     if (!is16(c->dtype) && !is8(c->dtype)) return fail(QWEN_E_ARG, "cache dtype must be QWEN_BF16, QWEN_FP16, QWEN_E4M3 or QWEN_INT8");
@@ -88,26 +53,6 @@ int check_view(const qwen_kv_cache_t* c) {
         Ptr{(c)->v_scale, "cache v_scale", 4, is8((c)->dtype)}
 qb::kv::Cache device_view(const qwen_kv_cache_t* c) {
     return qb::kv::Cache{(uint8_t*)c->k, (uint8_t*)c->v, c->k_scale, c->v_scale, c->seq_stride, c->head_stride, c->capacity};
-}
-int sm_count(int dev, int* n) {
-    static std::atomic<int> known[64];
-    if (dev < 0 || dev >= 64) return fail(QWEN_E_ARG, "device index beyond 63");
-    int v = known[dev].load();
-    if (!v) {
-        CU(cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev));
-        known[dev].store(v);
-    }
-    *n = v;
-    return QWEN_OK;
-}
-// Sets a kernel's shared-memory limit once per device (not a stream operation: allowed during capture).
-template <typename K>
-int smem_limit(K kernel, std::atomic<uint64_t>& done, int dev, int bytes) {
-    if (!((done.load() >> dev) & 1)) {
-        CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-        done.fetch_or(1ull << dev);
-    }
-    return QWEN_OK;
 }
 
 // ---- cache rows -------------------------------------------------------------------
@@ -181,14 +126,6 @@ int check_rows(const qwen_kv_cache_t* c, const void* k, const void* v, int dtype
 // 32 rows in 16 bits, and 33 to 64 rows over 8-bit caches.
 int attention_rows(int m) { return m <= 16 ? 16 : m <= 32 ? 32 : 128; }
 
-struct Plan {
-    int rows, row_blocks, beside, shares;   // shares: CTAs, beside for each share of the line
-    int tiles, blocks;                      // of a cache's capacity: the kernel's tiles; blocks of 64 keys (tensor-memory kernel: 128)
-    long long items;                        // sequences, K/V heads and blocks of rows
-    float spare;
-    bool whole, may_be_whole;               // a CTA for each item, no joining
-    size_t bytes;
-};
 int check_tree(const qwen_kv_cache_t* c, int n_nodes, int n_heads) {
     if (n_nodes < 1 || n_nodes > qb::ta::kMaxNodes) return fail(QWEN_E_ARG, "n_nodes out of [1, 64]");
     if (n_heads < 1 || n_heads % c->n_kv_heads) return fail(QWEN_E_ARG, "n_heads must be a positive multiple of n_kv_heads");
@@ -221,53 +158,13 @@ int attention_plan(const qwen_kv_cache_t* c, int n_nodes, int n_heads, int dev, 
     int nsm = 0, ctas = 0;
     if (!p->whole) {
         TRY(sm_count(dev, &nsm));
+        // as many CTAs as the SMs hold (the tensor-memory kernel: one each)
         ctas = p->rows <= 32 ? qb::ta::attention_ctas(p->rows, c->head_dim) * nsm : nsm;
         p->whole = p->may_be_whole && (double)p->blocks * std::max(0ll, ctas - p->items) <= (double)p->spare * ctas;
     }
-    if (p->whole) {
-        p->beside = p->row_blocks;
-        p->shares = (int)p->items;
-        p->bytes = 0;
-        return QWEN_OK;
-    }
-    // as many CTAs as the SMs hold (the tensor-memory kernel: one each), shared out over the blocks of rows that walk side by side
-    p->beside = p->row_blocks <= ctas ? p->row_blocks : 1;
-    // no more shares than the line can have positions
-    const double most = (double)c->n_seqs * c->n_kv_heads * (p->row_blocks / p->beside) *
-                        (p->tiles + qb::ta::kTcItemCost);
-    p->shares = (int)std::min((double)(ctas / p->beside), most) * p->beside;
-    if (most >= 2147483648.0) return fail(QWEN_E_UNSUPPORTED, "too many sequences, heads and positions for one call");
-    p->bytes = (size_t)2 * p->shares * p->rows * (c->head_dim + 2) * sizeof(float);
-    return QWEN_OK;
+    return plan_shares(p, ctas, c->head_dim);
 }
 
-// The kernel that joins the shares' partial results, launched so that it may start its set-up early.
-template <int QT, int KT, int COST, int D, int ROWS, bool ACROSS>
-int join_launch(const qb::ta::Params& P, const Plan& plan, int dev, cudaStream_t st) {
-    int nsm = 0;
-    TRY(sm_count(dev, &nsm));
-    if (plan.whole || plan.shares == plan.beside) return QWEN_OK;
-    cudaLaunchConfig_t cfg = {};
-    const int wide = P.by_item ? P.n_seqs * P.n_kv_heads * P.row_blocks : plan.shares;
-    cfg.gridDim = dim3(wide, qb::ta::join_blocks<D, ROWS, ACROSS>());
-    if (P.by_item) {
-        // Shared memory, so that no SM holds more blocks than an even spread over the SMs gives: the first SMs to finish their
-        // share would take six and read those items' partial results alone (one sequence of 64 nodes at 8128: 24.3 us, against 19.9).
-        const int each = std::max(1, ((int)cfg.gridDim.y * wide + nsm - 1) / nsm);
-        cfg.dynamicSmemBytes = each <= 4 ? (220 * 1024 / each - 1024) / 1024 * 1024 : 0;
-        static std::atomic<uint64_t> done{0};
-        TRY(smem_limit(qb::ta::combine_kernel<QT, KT, COST, D, ROWS, ACROSS>, done, dev, 219 * 1024));
-    }
-    cfg.blockDim = dim3(qb::ta::kJoinThreads);
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    CU(cudaLaunchKernelEx(&cfg, qb::ta::combine_kernel<QT, KT, COST, D, ROWS, ACROSS>, P));
-    return QWEN_OK;
-}
 template <int QT, int STORE, int D, int MT>
 int attention_launch(const qb::ta::Params& P, const Plan& plan, int dev, cudaStream_t st) {
     using L = qb::ta::Layout<STORE, D, MT>;

@@ -96,6 +96,13 @@ _SIGS = {
                                        _c.c_size_t, _P]),
     "qwen_tree_verify": (_c.c_int, [_P, _c.c_int, _c.c_longlong, _P, _c.c_longlong, _P, _P, _P, _c.c_int, _c.c_int, _c.c_int, _c.c_float,
                                     _P, _P, _P, _P]),
+    "qwen_qk_rope": (_c.c_int, [_P, _P, _P, _c.c_int, _c.c_longlong, _c.c_longlong, _c.c_longlong, _c.c_int, _c.c_int, _c.c_int, _c.c_int, _P, _P,
+                                _c.c_int, _c.c_float, _c.c_double, _P, _P, _P, _c.c_int, _c.c_longlong, _c.c_longlong, _P, _P, _P]),
+    "qwen_prompt_attention": (_c.c_int, [_P, _P, _P, _P, _c.c_int, _c.c_longlong, _c.c_longlong, _c.c_longlong, _c.c_longlong, _P, _P, _c.c_int,
+                                         _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_float, _P]),
+    "qwen_paged_attention_workspace": (_c.c_int, [_P, _c.c_int, _c.POINTER(_c.c_size_t)]),
+    "qwen_paged_attention": (_c.c_int, [_P, _P, _P, _c.c_int, _c.c_longlong, _c.c_longlong, _c.c_int, _P, _c.c_float, _P, _c.c_size_t, _P]),
+    "qwen_token_logprobs": (_c.c_int, [_P, _c.c_int, _c.c_longlong, _c.c_int, _c.c_int, _P, _c.c_float, _c.c_int, _P, _P, _P, _P, _P]),
     "qwen_debug_draft_wait": (_c.c_int, [_c.c_ulonglong, _c.c_int]),
     "qwen_tokenizer_load": (_c.c_int, [_c.c_char_p, _c.c_int, _c.POINTER(_P)]),
     "qwen_tokenizer_free": (None, [_P]),
@@ -130,6 +137,15 @@ class KVCache(ctypes.Structure):
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
                 ("seq_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong), ("dtype", ctypes.c_int), ("n_seqs", ctypes.c_int),
                 ("n_kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("capacity", ctypes.c_int)]
+
+
+class KVPages(ctypes.Structure):
+    """qwen_kv_pages_t: a view of K/V rows in pages of device memory (pointers as ints, None for
+    absent scales; strides in elements)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("table", ctypes.c_void_p), ("page_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong), ("dtype", ctypes.c_int),
+                ("n_pages", ctypes.c_int), ("n_seqs", ctypes.c_int), ("n_kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("max_pages", ctypes.c_int)]
 
 
 def load_library(path=None):
@@ -291,6 +307,42 @@ def tree_verify(logits_ptr, dtype, ld, draft_ptr, ld_draft, tokens_ptr, parents_
     """Which drafted nodes the target's logits keep (path, n_path) and the token after them (next)."""
     _check(load_library().qwen_tree_verify(logits_ptr, dtype, ld, draft_ptr, ld_draft, tokens_ptr, parents_ptr, uniforms_ptr, n_seqs, n_nodes,
                                            vocab, temperature, path_ptr, n_path_ptr, next_ptr, stream))
+
+
+# ---- serving over a K/V cache in pages (device pointers, ints) ----
+def qk_rope(q_ptr, k_ptr, v_ptr, dtype, ldq, ldk, ldv, n_rows, n_heads, n_kv_heads, head_dim, q_gain_ptr, k_gain_ptr, gain_dtype, eps, base,
+            positions_ptr, q_out_ptr, k_out_ptr, out_dtype, ldqo, ldko, pages=None, seqs_ptr=0, stream=0):
+    """Norms and rotation of Q and K rows: q -> q_out, k -> k_out (0: nowhere) and, with v, their places in the pages."""
+    _check(load_library().qwen_qk_rope(q_ptr, k_ptr, v_ptr, dtype, ldq, ldk, ldv, n_rows, n_heads, n_kv_heads, head_dim, q_gain_ptr, k_gain_ptr,
+                                       gain_dtype, eps, base, positions_ptr, q_out_ptr, k_out_ptr, out_dtype, ldqo, ldko,
+                                       None if pages is None else ctypes.byref(pages), seqs_ptr, stream))
+
+
+def prompt_attention(q_ptr, k_ptr, v_ptr, out_ptr, dtype, ldq, ldk, ldv, ldo, starts_ptr, k_starts_ptr, n_seqs, n_rows, n_keys, n_heads, n_kv_heads,
+                     head_dim, scale, stream=0):
+    """Causal attention of packed prompts: sequence s has queries starts[s] .. starts[s+1]-1 and keys k_starts[s] .. (0: as the queries)."""
+    _check(load_library().qwen_prompt_attention(q_ptr, k_ptr, v_ptr, out_ptr, dtype, ldq, ldk, ldv, ldo, starts_ptr, k_starts_ptr, n_seqs, n_rows,
+                                                n_keys, n_heads, n_kv_heads, head_dim, scale, stream))
+
+
+def paged_attention_workspace(pages, n_heads):
+    """Bytes of workspace of paged_attention."""
+    n = ctypes.c_size_t()
+    _check(load_library().qwen_paged_attention_workspace(ctypes.byref(pages), n_heads, ctypes.byref(n)))
+    return n.value
+
+
+def paged_attention(pages, q_ptr, out_ptr, dtype, ldq, ldo, n_heads, lens_ptr, scale, workspace_ptr, workspace_bytes, stream=0):
+    """Attention of the token at position lens[s] of each sequence over positions 0 .. lens[s] of its pages."""
+    _check(load_library().qwen_paged_attention(ctypes.byref(pages), q_ptr, out_ptr, dtype, ldq, ldo, n_heads, lens_ptr, scale, workspace_ptr,
+                                               workspace_bytes, stream))
+
+
+def token_logprobs(logits_ptr, dtype, ld, n_rows, vocab, tokens_ptr, temperature, n_top, logprob_ptr, entropy_ptr, top_ids_ptr, top_logprobs_ptr,
+                   stream=0):
+    """Log probability of each row's token, the row's entropy, and its n_top likeliest tokens (ids, log probabilities)."""
+    _check(load_library().qwen_token_logprobs(logits_ptr, dtype, ld, n_rows, vocab, tokens_ptr, temperature, n_top, logprob_ptr, entropy_ptr,
+                                              top_ids_ptr, top_logprobs_ptr, stream))
 
 
 def debug_draft_wait(wait_ns=0, part=-1):
