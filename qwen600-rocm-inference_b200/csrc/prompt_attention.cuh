@@ -433,6 +433,8 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             const int n = max(it.n[0], it.n[1]);
             for (int i = 0; i < n && !*fault; i++) {
                 const uint32_t pv = part + 2 * i + 1;
+                // (K parts too: a slot of an odd ring holds K and V in turn, and a wait that skips a phase may take the one before for it)
+                wait(&full[(pv - 1) % L::kRing], (pv - 1) / L::kRing & 1u);
                 wait(&full[pv % L::kRing], pv / L::kRing & 1u);
                 if (i * kKT + kKT - 1 > it.off) {
                     constexpr uint32_t kExp = BF ? 0x7f807f80u : 0x7c007c00u;
