@@ -37,7 +37,8 @@ using ta::mul2;
 using ta::pack2;
 
 constexpr int kKT = 128;                  // keys of a tile
-constexpr int kThreads = 384, kLoader = 8, kIssuer = 9, kFinder = 10, kLooker = 11;
+constexpr int kSoftmax = 16;              // warps: two threads a row, 64 keys of a tile each
+constexpr int kThreads = 640, kLoader = 16, kIssuer = 17, kLooker = 18;
 constexpr int kItems = 4;                 // items between the finder and the slowest warp
 constexpr int kClean = 4;                 // V parts that the looker may be ahead
 
@@ -67,13 +68,14 @@ struct Item {
 template <int D>
 struct Layout {
     static constexpr int kPart = kKT * D * 2;                 // K or V of a tile, or the rows of a row tile
-    static constexpr int kRing = D == 64 ? 8 : 5;             // K / V parts in flight: K 0, V 0, K 1, V 1, ...
+    static constexpr int kRing = D == 64 ? 8 : 4;             // K / V parts in flight, in the order in which they are used: K 0, K 1, V 0, K 2, V 1, ...
     static constexpr int kQ = 0;
     static constexpr int kKV = 2 * kPart;
     static constexpr int kBar = kKV + kRing * kPart;
-    static constexpr int kBars = 2 * kRing + kClean + 2 * kItems + 11;
+    static constexpr int kBars = 2 * kRing + kClean + 2 * kItems + 14;
     static constexpr int kItem = kBar + (kBars * 8 + 15) / 16 * 16;
-    static constexpr int kMisc = kItem + kItems * (int)sizeof(Item);
+    static constexpr int kXm = kItem + kItems * (int)sizeof(Item);       // [row tile][parity][half][row] maxima, then sums
+    static constexpr int kMisc = kXm + 2 * 2 * 2 * 128 * 4;
     static constexpr int kSmem = kMisc + 16 + 1024;
     static_assert(kRing / 2 + kRing % 2 <= kClean, "V parts in flight");
     static_assert(kSmem <= 227 * 1024, "one CTA's shared memory");
@@ -86,43 +88,19 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
         ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
         : "memory");
 }
-// 128 consecutive fp32 columns of this warp's 32 tensor-memory lanes (one row per lane).
-__device__ __forceinline__ void tmem_ld128(uint32_t taddr, float (&v)[128]) {
-    uint32_t r[128];
+// 32 consecutive fp32 columns of this warp's 32 tensor-memory lanes (one row per lane); the values are there after tmem_wait_ld.
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, float* v) {
     asm volatile(
-        "{\n\t"
-        "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
-        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
-        "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
-        "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63, "
-        "%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, "
-        "%80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, "
-        "%96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, "
-        "%112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}, [%128];\n\t"
-        "tcgen05.wait::ld.sync.aligned;\n\t}"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
-          "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
-          "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
-          "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
-          "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
-          "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
-          "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
-          "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
-          "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+          "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+          "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+          "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
         : "r"(taddr)
         : "memory");
-    #pragma unroll
-    for (int i = 0; i < 128; i++) v[i] = __uint_as_float(r[i]);
 }
-
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
     uint32_t r[16];
     asm volatile(
@@ -135,6 +113,59 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
         : "memory");
     #pragma unroll
     for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
+}
+
+// A place in a ring of barriers, and the parity of its use.
+template <int N>
+struct Ring {
+    uint32_t slot = 0, phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++slot == N) { slot = 0; phase ^= 1u; }
+    }
+};
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+// 8 columns of this warp's lanes times f; complete after tc_wait_st.
+__device__ __forceinline__ void scale8(uint32_t taddr, float f) {
+    float o[8];
+    asm volatile(
+        "{\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
+        "tcgen05.wait::ld.sync.aligned;\n\t}"
+        : "=f"(o[0]), "=f"(o[1]), "=f"(o[2]), "=f"(o[3]), "=f"(o[4]), "=f"(o[5]), "=f"(o[6]), "=f"(o[7]) : "r"(taddr) : "memory");
+    #pragma unroll
+    for (int x = 0; x < 8; x += 2) mul2(o[x], o[x + 1], f, f);
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(taddr), "f"(o[0]), "f"(o[1]), "f"(o[2]), "f"(o[3]), "f"(o[4]), "f"(o[5]), "f"(o[6]), "f"(o[7]) : "memory");
+}
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+// 2^a and 2^b on the fused multiply-add pipe, for part of the weights, whose exponentials are what the softmax warps wait for:
+// a = n + f with the whole number n nearest to a (adding 1.5 * 2^23 rounds to it), 2^f by the polynomial of degree 4 that
+// interpolates it at the five Chebyshev nodes of [-1/2, 1/2] (within 2^-17), times 2^n from n's bits.  NaN stays NaN; below -125 it
+// is 2^-125.
+constexpr int kByHand = 1;     // of every four pairs
+__device__ __forceinline__ void fma2(float& a, float& b, float x, float y, float s, float t) {   // (a, b) * (x, y) + (s, t)
+    asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmov.b64 r, {%4, %5};\n\tfma.rn.f32x2 p, p, q, r;\n\tmov.b64 {%0, %1}, p;\n\t}"
+        : "+f"(a), "+f"(b) : "f"(x), "f"(y), "f"(s), "f"(t));
+}
+__device__ __forceinline__ void exp2_by_hand(float& a, float& b) {
+    constexpr float kC[5] = {1.0f, 0.6931210160255432f, 0.2402234971523285f, 0.055921975523233414f, 0.00966636836528778f};
+    const float x = max_nan(a, -125.0f), y = max_nan(b, -125.0f);
+    float s = x, t = y;
+    add2(s, t, 12582912.0f, 12582912.0f);
+    const uint32_t ns = __float_as_uint(s), nt = __float_as_uint(t);
+    add2(s, t, -12582912.0f, -12582912.0f);
+    fma2(s, t, -1.0f, -1.0f, x, y);
+    float p = kC[4], q = kC[4];
+    #pragma unroll
+    for (int i = 3; i >= 0; i--) fma2(p, q, s, t, kC[i], kC[i]);
+    mul2(p, q, __uint_as_float((ns << 23) + 0x3f800000u), __uint_as_float((nt << 23) + 0x3f800000u));
+    a = p;
+    b = q;
 }
 
 // The sequences, by all lanes of a warp: where each one's rows and keys lie, and its items.
@@ -242,9 +273,10 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     uint64_t* qfull = taken + kItems;                               // the item's rows have arrived
     uint64_t* qempty = qfull + 2;                                   // their last S is formed
     uint64_t* sfull = qfull + 4;                                    // S formed
-    uint64_t* pfull = qfull + 6;                                    // P written, O scaled (4 warps)
-    uint64_t* odone = qfull + 8;                                    // P V added
-    uint64_t* drained = qfull + 10;                                 // all products are done, at the end
+    uint64_t* odone = qfull + 6;                                    // P V added
+    uint64_t* pfull = qfull + 8;                                    // [2][2] a half of P written, O scaled (4 warps)
+    uint64_t* sread = qfull + 12;                                   // S is in registers (8 warps)
+    uint64_t* drained = qfull + 13;                                 // all products are done, at the end
     Item* items = reinterpret_cast<Item*>(smem + L::kItem);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
     volatile int* fault = reinterpret_cast<int*>(smem + L::kMisc + 4);
@@ -252,14 +284,16 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     if (tid == 0) {
         for (int i = 0; i < L::kRing; i++) { mbar_init(&full[i], 1 + (i == P.withheld)); mbar_init(&empty[i], 1); }
         for (int i = 0; i < kClean; i++) mbar_init(&clean[i], 1);
-        for (int i = 0; i < kItems; i++) { mbar_init(&given[i], 1); mbar_init(&taken[i], 11); }   // 8 softmax warps, loads, products, looker
+        for (int i = 0; i < kItems; i++) { mbar_init(&given[i], 1); mbar_init(&taken[i], kSoftmax + 2); }   // softmax, products, looker
         for (int w = 0; w < 2; w++) {
             mbar_init(&qfull[w], 1);
             mbar_init(&qempty[w], 1);
             mbar_init(&sfull[w], 1);
-            mbar_init(&pfull[w], 4);
+            mbar_init(&pfull[2 * w], 4);
+            mbar_init(&pfull[2 * w + 1], 4);
             mbar_init(&odone[w], 1);
         }
+        mbar_init(sread, 8);
         mbar_init(drained, 1);
         fence_barrier_init();
         *fault = 0;
@@ -289,8 +323,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     auto next_item = [&]() {                  // all lanes of a warp; false: no more
         const int slot = seen % kItems;
         if (!ta::mbar_spin(&given[slot], seen / kItems & 1u, 8 * P.wait_ns)) { *fault = 1; return false; }
-        it = items[slot];
-        return !it.stop;
+        return !items[slot].stop;
     };
     auto item_done = [&]() {
         __syncwarp();
@@ -298,43 +331,39 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         seen++;
     };
 
-    if (warp == kFinder) {
-        // ---------------- items ----------------
+    // The block's 640 x 96 registers, shared out anew: 104 for a softmax thread, 64 for the others (512 x 104 + 128 x 64 = 640 x 96).
+    auto fewer = [] { asm volatile("setmaxnreg.dec.sync.aligned.u32 64;"); };
+    if (warp == kLoader) {
+        // ---------------- items and loads ----------------
+        fewer();
         const Finder finder(P);
         const int G = gridDim.x;
+        uint32_t part = 0, used[2] = {0, 0};   // K / V parts so far; items so far that have the row tile
         bool more = true;
         for (int k = 0; more; k++) {
             const long long at = (long long)k * G + (k & 1 ? G - 1 - (int)blockIdx.x : (int)blockIdx.x);   // forwards and backwards
             int seq = 0, tile = 0;
             more = at / P.n_kv_heads < 0x7fffffff && finder.find(P, (int)(at / P.n_kv_heads), seq, tile);
-            Item x = {};
-            x.stop = !more;
+            it = {};
+            it.stop = !more;
             if (more) {
                 int q0, nq, k0, nk;
                 finder.bounds(P, seq, q0, nq, k0, nk);
-                x.h = (int)(at % P.n_kv_heads);
-                x.q0 = q0 + tile * finder.per;
-                x.nq = min(nq - tile * finder.per, finder.per);
-                x.k0 = k0;
-                x.off = nk - nq + tile * finder.per;
+                it.h = (int)(at % P.n_kv_heads);
+                it.q0 = q0 + tile * finder.per;
+                it.nq = min(nq - tile * finder.per, finder.per);
+                it.k0 = k0;
+                it.off = nk - nq + tile * finder.per;
                 for (int w = 0; w < 2; w++) {
-                    const int count = min(x.nq - w * P.tokens, P.tokens), last = x.off + w * P.tokens + count - 1;
-                    x.n[w] = count <= 0 || last < 0 ? 0 : last / kKT + 1;
+                    const int count = min(it.nq - w * P.tokens, P.tokens), last = it.off + w * P.tokens + count - 1;
+                    it.n[w] = count <= 0 || last < 0 ? 0 : last / kKT + 1;
                 }
             }
             const int slot = k % kItems;
             if (k >= kItems && !ta::mbar_spin(&taken[slot], (k / kItems - 1) & 1u, 8 * P.wait_ns)) { *fault = 1; break; }
             if (lane == 0) {
-                items[slot] = x;
+                items[slot] = it;
                 mbar_arrive(&given[slot]);
-            }
-            __syncwarp();
-        }
-    } else if (warp == kLoader) {
-        // ---------------- loads ----------------
-        uint32_t part = 0, used[2] = {0, 0};   // K / V parts so far; items so far that have the row tile
-        while (next_item()) {
-            if (lane == 0) {
                 const int n = max(it.n[0], it.n[1]);
                 auto rows = [&](int w) {
                     if (!it.n[w]) return;
@@ -360,10 +389,11 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                 for (int i = 0; i < n && !*fault; i++) {
                     keys(&map_k, i);
                     if (i == 0) rows(1);
-                    keys(&map_v, i);
+                    else keys(&map_v, i - 1);
                 }
+                if (n) keys(&map_v, n - 1);
             }
-            item_done();
+            __syncwarp();
         }
         if (*fault && lane == 0) {             // nothing may still be on its way when the CTA ends
             for (uint32_t p = part > (uint32_t)L::kRing ? part - L::kRing : 0; p < part; p++) mbar_wait(&full[p % L::kRing], p / L::kRing & 1u, 10000000ull);
@@ -372,73 +402,102 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         __syncwarp();
     } else if (warp == kIssuer) {
         // ---------------- products ----------------
+        fewer();
+        // The whole warp walks, one lane issues: what a product takes is then the same for the warp and stays in uniform registers (with a
+        // lane alone, a product cost 110 cycles of address arithmetic, twice what it computes).
         constexpr uint32_t id_s = ta::tc_idesc<BF>(kKT, false), id_o = ta::tc_idesc<BF>(D, true);
-        uint32_t part = 0, used[2] = {0, 0}, steps[2] = {0, 0};   // steps: key tiles of a row tile so far
+        const bool leader = elect_one();
+        const uint64_t qd = kmajor_sw128_desc(smem_addr(smem + L::kQ)), kd = kmajor_sw128_desc(smem_addr(smem + L::kKV)),
+                       vd = ta::mn_major_sw128_desc(smem_addr(smem + L::kKV), kKT * 128);
+        uint32_t parts = 0, looks = 0;         // K / V parts, V parts of the items so far
+        uint32_t used[2] = {0, 0}, steps[2] = {0, 0}, formed = 0;   // items, key tiles of a row tile so far; S so far
         while (next_item()) {
-            if (lane == 0) {
-                const int n = max(it.n[0], it.n[1]);
-                auto form_s = [&](int w, int i) {
-                    if (i >= it.n[w]) return;
-                    if (i == 0) { wait(&qfull[w], used[w] & 1u); used[w]++; tc_fence_after(); }
-                    const uint32_t kb = smem_addr(smem + L::kKV + (part + 2 * i) % L::kRing * L::kPart), qb = smem_addr(smem + L::kQ + w * L::kPart);
+            it = items[seen % kItems];
+            const int n[2] = {__shfl_sync(~0u, it.n[0], 0), __shfl_sync(~0u, it.n[1], 0)}, most = max(n[0], n[1]);
+            auto form_s = [&](int w, int i) {
+                if (i >= n[w]) return;
+                if (i == 0) { wait(&qfull[w], used[w] & 1u); used[w]++; }
+                if (formed) wait(sread, (formed - 1) & 1u);
+                formed++;
+                tc_fence_after();
+                const uint32_t slot = (parts + ta::k_part(i)) % L::kRing;
+                const uint64_t a = qd + (uint64_t)(w * (L::kPart >> 4)), b = kd + (uint64_t)(slot * (uint32_t)(L::kPart >> 4));
+                if (leader) {
                     #pragma unroll
                     for (int k = 0; k < D / 16; k++)
-                        mma_bf16(tmem + 128 * w, kmajor_sw128_desc(qb + (k >> 2) * (128 * 128) + (k & 3) * 32),
-                                 kmajor_sw128_desc(kb + (k >> 2) * (kKT * 128) + (k & 3) * 32), id_s, k ? 1u : 0u);
+                        mma_bf16(tmem, a + (((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4), b + (((k >> 2) * (kKT * 128) + (k & 3) * 32) >> 4), id_s, k ? 1u : 0u);
                     mma_commit(&sfull[w]);
-                    if (i + 1 == it.n[w]) mma_commit(&qempty[w]);
-                };
-                auto add_pv = [&](int w, int i) {
-                    if (i >= it.n[w]) return;
-                    wait(&pfull[w], steps[w] & 1u);
-                    steps[w]++;
+                    if (i + 1 == n[w]) mma_commit(&qempty[w]);
+                }
+                __syncwarp();
+            };
+            auto add_pv = [&](int w, int i) {
+                if (i < 0 || i >= n[w]) return;
+                const uint32_t slot = (parts + ta::v_part(i, most)) % L::kRing;
+                const uint64_t b = vd + (uint64_t)(slot * (uint32_t)(L::kPart >> 4));
+                #pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    wait(&pfull[2 * w + half], steps[w] & 1u);
                     tc_fence_after();
-                    const uint32_t vb = smem_addr(smem + L::kKV + (part + 2 * i + 1) % L::kRing * L::kPart);
-                    #pragma unroll
-                    for (int k = 0; k < kKT / 16; k++)
-                        ta::tc_mma_ts(tmem + 256 + 128 * w, tmem + 128 * w + 8 * k, ta::mn_major_sw128_desc(vb + k * 2048, kKT * 128), id_o, (i | k) ? 1u : 0u);
-                    mma_commit(&odone[w]);
-                };
-                auto arrived = [&](uint64_t* bar, uint32_t parity) { wait(bar, parity); tc_fence_after(); };
-                if (n) {
-                    arrived(&full[part % L::kRing], part / L::kRing & 1u);
-                    form_s(0, 0);
-                    form_s(1, 0);
-                    mma_commit(&empty[part % L::kRing]);
+                    if (leader) {
+                        #pragma unroll
+                        for (int k = 4 * half; k < 4 * half + 4; k++)
+                            ta::tc_mma_ts(tmem + 256 + 128 * w, tmem + 128 + 64 * w + 8 * k, b + (k * 2048 >> 4), id_o, (i | k) ? 1u : 0u);
+                        if (half) mma_commit(&odone[w]);
+                    }
+                    __syncwarp();
                 }
-                for (int i = 0; i < n && !*fault; i++) {
-                    const uint32_t pv = part + 2 * i + 1, pk = part + 2 * i + 2;
-                    arrived(&clean[(pv >> 1) % kClean], (pv >> 1) / kClean & 1u);
-                    add_pv(0, i);
-                    if (i + 1 < n) arrived(&full[pk % L::kRing], pk / L::kRing & 1u);
-                    form_s(0, i + 1);
-                    add_pv(1, i);
-                    mma_commit(&empty[pv % L::kRing]);
-                    form_s(1, i + 1);
-                    if (i + 1 < n) mma_commit(&empty[pk % L::kRing]);
+                steps[w]++;
+            };
+            auto done_with = [&](uint32_t part) {
+                if (leader) mma_commit(&empty[(parts + part) % L::kRing]);
+                __syncwarp();
+            };
+            // S_A(i), P_A(i-1) V, S_B(i), P_B(i-1) V: the order in which the softmax warps come to wait for them
+            for (int i = 0; i <= most && !*fault; i++) {
+                if (i < most) {
+                    const uint32_t p = parts + ta::k_part(i);
+                    wait(&full[p % L::kRing], p / L::kRing & 1u);
+                    form_s(0, i);
                 }
-                part += 2 * n;
+                if (i >= 1) {
+                    const uint32_t x = looks + i - 1;
+                    wait(&clean[x % kClean], x / kClean & 1u);
+                    add_pv(0, i - 1);
+                }
+                if (i < most) {
+                    form_s(1, i);
+                    done_with(ta::k_part(i));
+                }
+                if (i >= 1) {
+                    add_pv(1, i - 1);
+                    done_with(ta::v_part(i - 1, most));
+                }
             }
+            parts += 2 * most;
+            looks += most;
             item_done();
         }
-        if (lane == 0) {
+        if (leader) {
             mma_commit(drained);
             if (!mbar_wait(drained, 0, P.wait_ns)) *fault = 1;
         }
         __syncwarp();
     } else if (warp == kLooker) {
         // ---------------- infinities and NaN among V rows that not all rows see ----------------
-        uint32_t part = 0;
+        fewer();
+        uint32_t part = 0, looks = 0;
         while (next_item()) {
+            it = items[seen % kItems];
             const int n = max(it.n[0], it.n[1]);
-            for (int i = 0; i < n && !*fault; i++) {
-                const uint32_t pv = part + 2 * i + 1;
-                // (K parts too: a slot of an odd ring holds K and V in turn, and a wait that skips a phase may take the one before for it)
-                wait(&full[(pv - 1) % L::kRing], (pv - 1) / L::kRing & 1u);
-                wait(&full[pv % L::kRing], pv / L::kRing & 1u);
+            for (int x = 0; x < 2 * n && !*fault; x++, part++) {
+                int value;
+                const int i = ta::part_tile(x, n, value);
+                wait(&full[part % L::kRing], part / L::kRing & 1u);        // (K parts too: a wait that skips a phase may take the one before for it)
+                if (!value) continue;
                 if (i * kKT + kKT - 1 > it.off) {
                     constexpr uint32_t kExp = BF ? 0x7f807f80u : 0x7c007c00u;
-                    uint4* rows = reinterpret_cast<uint4*>(smem + L::kKV + pv % L::kRing * L::kPart);
+                    uint4* rows = reinterpret_cast<uint4*>(smem + L::kKV + part % L::kRing * L::kPart);
                     bool any = false;
                     #pragma unroll 8
                     for (int x = lane; x < L::kPart / 16; x += 32) {
@@ -457,44 +516,60 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                     }
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&clean[(pv >> 1) % kClean]);
+                if (lane == 0) mbar_arrive(&clean[looks % kClean]);
+                looks++;
             }
-            part += 2 * n;
             item_done();
         }
+    } else if (warp > kLooker) {
+        fewer();
     } else {
         // ---------------- softmax and output ----------------
-        const int w = warp >> 2, rl = 32 * (warp & 3) + lane;              // row tile, row of it
-        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, ts = tmem + lanes + 128 * w, to = tmem + lanes + 256 + 128 * w;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        const int w = warp >> 3, half = warp >> 2 & 1, rl = 32 * (warp & 3) + lane;   // row tile, half of the keys, row
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, ts = tmem + lanes + 64 * half, tp = tmem + lanes + 128 + 64 * w + 32 * half, to = tmem + lanes + 256 + 128 * w + half * (D / 2);
         const int token = w * P.tokens + rl / P.group, head = rl % P.group;
         const bool placed = rl < P.tokens * P.group;
         const float c = fmaxf(fabsf(P.scale_log2), 1e-37f);                // (above 0: -inf * 0 would be NaN)
-        const float sign = P.scale_log2 < 0.f ? -1.0f : 1.0f;
-        uint32_t steps = 0;                                                // key tiles so far
+        const bool flip = P.scale_log2 < 0.f;
+        float* mine = reinterpret_cast<float*>(smem + L::kXm) + w * 512 + half * 128 + rl;   // + 256 for odd steps
+        const float* other = reinterpret_cast<const float*>(smem + L::kXm) + w * 512 + (half ^ 1) * 128 + rl;
+        uint32_t steps = 0, swaps = 0;                                     // key tiles, exchanges so far
         while (next_item()) {
-            const bool live = placed && token < it.nq;
-            const int n = it.n[w], sees = live ? it.off + token : 1 << 30;   // the last key that the row sees (rows that are none: any)
+            const Item* item = &items[seen % kItems];                      // (read where it is needed: registers are scarce)
+            const int n = item->n[w], sees = placed && token < item->nq ? item->off + token : 1 << 30;   // the last key that the row sees (rows that are none: any)
             float base = -INFINITY, l = 0.f;
-            for (int i = 0; i < n; i++, steps++) {
+            for (int i = 0; i < n; i++, steps++, swaps++) {
+                const int last = sees - i * kKT - 64 * half;               // columns 0 .. last are seen
+                const bool part = __any_sync(~0u, last < 63);
                 wait(&sfull[w], steps & 1u);
                 tc_fence_after();
-                float v[128];
-                tmem_ld128(ts, v);
-                if (sign < 0.f) {
+                float v[64];
+                tmem_ld32_async(ts, v);
+                tmem_ld32_async(ts + 32, v + 32);
+                tmem_wait_ld();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(sread);
+                if (flip) {
                     #pragma unroll
-                    for (int x = 0; x < 128; x++) v[x] = -v[x];
+                    for (int x = 0; x < 64; x++) v[x] = -v[x];
                 }
-                const int last = sees - i * kKT;                           // columns 0 .. last are seen
-                if (__any_sync(~0u, last < kKT - 1)) {
+                if (part) {
                     #pragma unroll
-                    for (int x = 0; x < 128; x++) if (x > last) v[x] = -INFINITY;
+                    for (int x = 0; x < 64; x++) if (x > last) v[x] = -INFINITY;
                 }
                 float mx[4] = {v[0], v[1], v[2], v[3]};
                 #pragma unroll
-                for (int x = 4; x < 124; x += 8)
+                for (int x = 4; x < 60; x += 8)
                     #pragma unroll
                     for (int y = 0; y < 4; y++) mx[y] = max3(mx[y], v[x + y], v[x + y + 4]);
-                const float top = fmaxf(max3(max3(mx[0], v[124], v[125]), mx[1], mx[2]), max3(mx[3], v[126], v[127]));
+                #pragma unroll
+                for (int y = 0; y < 4; y++) mx[y] = fmaxf(mx[y], v[60 + y]);
+                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                mine[swaps % 2 * 256] = top;
+                named_bar(2 + w, 256);
+                top = fmaxf(top, other[swaps % 2 * 256]);
                 const float want = top == -INFINITY ? top : top * c;       // an all-masked tile stays -inf
                 const bool move = want > base + 8.0f;                      // (from -inf: the first tile that has a key)
                 float f = 1.0f;
@@ -507,78 +582,83 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                     wait(&odone[w], (steps - 1) & 1u);                     // O of the tile before
                     tc_fence_after();
                     #pragma unroll 1
-                    for (int c0 = 0; c0 < D; c0 += 16) {
-                        float o[16];
-                        tmem_ld16(to + c0, o);
-                        #pragma unroll
-                        for (int x = 0; x < 16; x += 2) mul2(o[x], o[x + 1], f, f);
-                        uint32_t b[16];
-                        #pragma unroll
-                        for (int x = 0; x < 16; x++) b[x] = __float_as_uint(o[x]);
-                        ta::tc_st16(to + c0, b);
-                    }
+                    for (int c0 = 0; c0 < D / 2; c0 += 8) scale8(to + c0, f);
                 }
                 const float from = base == -INFINITY ? 0.f : base;
                 float sum0 = 0.f, sum1 = 0.f;
-                #pragma unroll
-                for (int c0 = 0; c0 < 128; c0 += 32) {
-                    uint32_t p[16];
+                uint32_t p[16];
+                auto weights = [&](int c0, auto mixed) {
                     #pragma unroll
                     for (int x = 0; x < 32; x += 2) {
-                        float &a = v[c0 + x], &b = v[c0 + x + 1];
+                        float a = v[c0 + x], b = v[c0 + x + 1];
                         fma2(a, b, c, -from);
-                        a = exp2_approx(a);
-                        b = exp2_approx(b);
+                        if (decltype(mixed)::value && x % 8 >= 8 - 2 * kByHand) {
+                            exp2_by_hand(a, b);
+                        } else {
+                            a = exp2_approx(a);
+                            b = exp2_approx(b);
+                        }
                         add2(sum0, sum1, a, b);
                         p[x / 2] = pack2<BF>(a, b);
                     }
-                    ta::tc_st16(ts + c0 / 2, p);
-                }
-                l += sum0 + sum1;
+                };
+                // (a column that is not seen has to weigh nothing, which the polynomial cannot say)
+                if (part) weights(0, No());
+                else weights(0, Yes());
+                if (i > 0) wait(&odone[w], (steps - 1) & 1u);              // P of the tile before has been taken
+                tc_fence_after();
+                ta::tc_st16(tp, p);
+                if (part) weights(32, No());
+                else weights(32, Yes());
+                ta::tc_st16(tp + 16, p);
                 ta::tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&pfull[w]);
+                if (lane == 0) mbar_arrive(&pfull[2 * w + half]);
+                l += sum0 + sum1;
             }
-            // ---- the row ----
+            // ---- the row: this thread's half of the dims ----
             if (n) {
+                mine[swaps % 2 * 256] = l;
+                named_bar(2 + w, 256);
+                l += other[swaps % 2 * 256];
+                swaps++;
                 wait(&odone[w], (steps - 1) & 1u);
                 tc_fence_after();
             }
-            const bool failed = *fault != 0;
-            const bool odd = live && *(volatile int*)&items[seen % kItems].odd != 0;
+            it = *item;
+            const bool failed = *fault != 0, live = placed && token < it.nq;
+            const bool odd = live && *(const volatile int*)&item->odd != 0;
             const float inv = l == 0.f ? 0.f : 1.0f / l;
-            uint8_t* dst = P.out + ((size_t)(it.q0 + token) * P.ldo + (size_t)(it.h * P.group + head) * D) * 2;
+            uint8_t* dst = P.out + ((size_t)(it.q0 + token) * P.ldo + (size_t)(it.h * P.group + head) * D + half * (D / 2)) * 2;
             #pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 32) {
-                float o[32];
-                if (n) tmem_ld32(to + c0, o);
+            for (int c0 = 0; c0 < D / 2; c0 += 16) {
+                float o[16];
+                if (n) tmem_ld16(to + c0, o);
                 if (odd) {
                     for (int key = (max(it.off, -1) + 1) / kKT * kKT; key <= sees; key++) {
-                        const uint16_t* row = reinterpret_cast<const uint16_t*>(P.v) + (size_t)(it.k0 + key) * P.ldv + (size_t)it.h * D + c0;
+                        const uint16_t* row = reinterpret_cast<const uint16_t*>(P.v) + (size_t)(it.k0 + key) * P.ldv + (size_t)it.h * D + half * (D / 2) + c0;
                         constexpr uint32_t kExp = BF ? 0x7f80u : 0x7c00u;
                         #pragma unroll
-                        for (int x = 0; x < 32; x++) {
+                        for (int x = 0; x < 16; x++) {
                             const uint16_t b = row[x];
                             if ((b & kExp) == kExp) o[x] += BF ? bf2f(b) : __half2float(__ushort_as_half(b));
                         }
                     }
                 }
-                uint32_t b[16];
+                uint32_t b[8];
                 #pragma unroll
-                for (int x = 0; x < 16; x++) {
+                for (int x = 0; x < 8; x++) {
                     const float y = failed ? NAN : sees < 0 ? 0.f : o[2 * x] * inv, z = failed ? NAN : sees < 0 ? 0.f : o[2 * x + 1] * inv;
                     b[x] = pack2<BF>(y, z);
                 }
                 if (live) {
                     if (P.out32) {
-                        #pragma unroll
-                        for (int x = 0; x < 16; x += 8)
-                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + c0 * 2 + x * 4), "r"(b[x]), "r"(b[x + 1]), "r"(b[x + 2]),
-                                         "r"(b[x + 3]), "r"(b[x + 4]), "r"(b[x + 5]), "r"(b[x + 6]), "r"(b[x + 7]) : "memory");
+                        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + c0 * 2), "r"(b[0]), "r"(b[1]), "r"(b[2]), "r"(b[3]),
+                                     "r"(b[4]), "r"(b[5]), "r"(b[6]), "r"(b[7]) : "memory");
                     } else {
-                        #pragma unroll
-                        for (int x = 0; x < 16; x += 4) *reinterpret_cast<uint4*>(dst + c0 * 2 + x * 4) = make_uint4(b[x], b[x + 1], b[x + 2], b[x + 3]);
+                        *reinterpret_cast<uint4*>(dst + c0 * 2) = make_uint4(b[0], b[1], b[2], b[3]);
+                        *reinterpret_cast<uint4*>(dst + c0 * 2 + 16) = make_uint4(b[4], b[5], b[6], b[7]);
                     }
                 }
             }

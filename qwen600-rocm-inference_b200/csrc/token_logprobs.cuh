@@ -43,11 +43,6 @@ struct Params {
     int* top_ids;
 };
 
-__device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
