@@ -38,7 +38,7 @@ using ta::pack2;
 
 constexpr int kKT = 128;                  // keys of a tile
 constexpr int kSoftmax = 16;              // warps: two threads a row, 64 keys of a tile each
-constexpr int kThreads = 640, kLoader = 16, kIssuer = 17, kLooker = 18;
+constexpr int kThreads = 640, kLoader = 16, kScores = 17, kValues = 18, kLooker = 19;
 constexpr int kItems = 4;                 // items between the finder and the slowest warp
 constexpr int kClean = 4;                 // V parts that the looker may be ahead
 
@@ -72,7 +72,7 @@ struct Layout {
     static constexpr int kQ = 0;
     static constexpr int kKV = 2 * kPart;
     static constexpr int kBar = kKV + kRing * kPart;
-    static constexpr int kBars = 2 * kRing + kClean + 2 * kItems + 14;
+    static constexpr int kBars = 2 * kRing + kClean + 2 * kItems + 15;
     static constexpr int kItem = kBar + (kBars * 8 + 15) / 16 * 16;
     static constexpr int kXm = kItem + kItems * (int)sizeof(Item);       // [row tile][parity][half][row] maxima, then sums
     static constexpr int kMisc = kXm + 2 * 2 * 2 * 128 * 4;
@@ -276,7 +276,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     uint64_t* odone = qfull + 6;                                    // P V added
     uint64_t* pfull = qfull + 8;                                    // [2][2] a half of P written, O scaled (4 warps)
     uint64_t* sread = qfull + 12;                                   // S is in registers (8 warps)
-    uint64_t* drained = qfull + 13;                                 // all products are done, at the end
+    uint64_t* drained = qfull + 13;                                 // [2] all products of a warp are done, at the end
     Item* items = reinterpret_cast<Item*>(smem + L::kItem);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
     volatile int* fault = reinterpret_cast<int*>(smem + L::kMisc + 4);
@@ -284,7 +284,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     if (tid == 0) {
         for (int i = 0; i < L::kRing; i++) { mbar_init(&full[i], 1 + (i == P.withheld)); mbar_init(&empty[i], 1); }
         for (int i = 0; i < kClean; i++) mbar_init(&clean[i], 1);
-        for (int i = 0; i < kItems; i++) { mbar_init(&given[i], 1); mbar_init(&taken[i], kSoftmax + 2); }   // softmax, products, looker
+        for (int i = 0; i < kItems; i++) { mbar_init(&given[i], 1); mbar_init(&taken[i], kSoftmax + 3); }   // softmax, products, looker
         for (int w = 0; w < 2; w++) {
             mbar_init(&qfull[w], 1);
             mbar_init(&qempty[w], 1);
@@ -294,14 +294,14 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             mbar_init(&odone[w], 1);
         }
         mbar_init(sread, 8);
-        mbar_init(drained, 1);
+        for (int i = 0; i < 2; i++) mbar_init(&drained[i], 1);
         fence_barrier_init();
         *fault = 0;
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
     }
-    if (warp == kIssuer) tmem_alloc(tmem_slot, 512);
+    if (warp == kScores) tmem_alloc(tmem_slot, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -400,11 +400,12 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             for (int w = 0; w < 2; w++) if (used[w]) mbar_wait(&qfull[w], (used[w] - 1) & 1u, 10000000ull);
         }
         __syncwarp();
-    } else if (warp == kIssuer) {
+    } else if (warp == kScores || warp == kValues) {
         // ---------------- products ----------------
+        // A warp for S and one for P V, so that the waits of one pass under the products of the other.  The whole warp walks, one lane
+        // issues: what a product takes is then the same for the warp and stays in uniform registers (with a lane alone, a product cost 110
+        // cycles of address arithmetic, twice what it computes).
         fewer();
-        // The whole warp walks, one lane issues: what a product takes is then the same for the warp and stays in uniform registers (with a
-        // lane alone, a product cost 110 cycles of address arithmetic, twice what it computes).
         constexpr uint32_t id_s = ta::tc_idesc<BF>(kKT, false), id_o = ta::tc_idesc<BF>(D, true);
         const bool leader = elect_one();
         const uint64_t qd = kmajor_sw128_desc(smem_addr(smem + L::kQ)), kd = kmajor_sw128_desc(smem_addr(smem + L::kKV)),
@@ -412,66 +413,56 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         uint32_t parts = 0, looks = 0;         // K / V parts, V parts of the items so far
         uint32_t used[2] = {0, 0}, steps[2] = {0, 0}, formed = 0;   // items, key tiles of a row tile so far; S so far
         while (next_item()) {
-            it = items[seen % kItems];
-            const int n[2] = {__shfl_sync(~0u, it.n[0], 0), __shfl_sync(~0u, it.n[1], 0)}, most = max(n[0], n[1]);
-            auto form_s = [&](int w, int i) {
-                if (i >= n[w]) return;
-                if (i == 0) { wait(&qfull[w], used[w] & 1u); used[w]++; }
-                if (formed) wait(sread, (formed - 1) & 1u);
-                formed++;
-                tc_fence_after();
-                const uint32_t slot = (parts + ta::k_part(i)) % L::kRing;
-                const uint64_t a = qd + (uint64_t)(w * (L::kPart >> 4)), b = kd + (uint64_t)(slot * (uint32_t)(L::kPart >> 4));
-                if (leader) {
+            const int n[2] = {__shfl_sync(~0u, items[seen % kItems].n[0], 0), __shfl_sync(~0u, items[seen % kItems].n[1], 0)}, most = max(n[0], n[1]);
+            if (warp == kScores) {
+                for (int i = 0; i < most && !*fault; i++) {
+                    const uint32_t part = parts + ta::k_part(i), slot = part % L::kRing;
+                    const uint64_t b = kd + (uint64_t)(slot * (uint32_t)(L::kPart >> 4));
+                    wait(&full[slot], part / L::kRing & 1u);
                     #pragma unroll
-                    for (int k = 0; k < D / 16; k++)
-                        mma_bf16(tmem, a + (((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4), b + (((k >> 2) * (kKT * 128) + (k & 3) * 32) >> 4), id_s, k ? 1u : 0u);
-                    mma_commit(&sfull[w]);
-                    if (i + 1 == n[w]) mma_commit(&qempty[w]);
-                }
-                __syncwarp();
-            };
-            auto add_pv = [&](int w, int i) {
-                if (i < 0 || i >= n[w]) return;
-                const uint32_t slot = (parts + ta::v_part(i, most)) % L::kRing;
-                const uint64_t b = vd + (uint64_t)(slot * (uint32_t)(L::kPart >> 4));
-                #pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    wait(&pfull[2 * w + half], steps[w] & 1u);
-                    tc_fence_after();
-                    if (leader) {
-                        #pragma unroll
-                        for (int k = 4 * half; k < 4 * half + 4; k++)
-                            ta::tc_mma_ts(tmem + 256 + 128 * w, tmem + 128 + 64 * w + 8 * k, b + (k * 2048 >> 4), id_o, (i | k) ? 1u : 0u);
-                        if (half) mma_commit(&odone[w]);
+                    for (int w = 0; w < 2; w++) {
+                        if (i >= n[w]) continue;
+                        if (i == 0) wait(&qfull[w], used[w]++ & 1u);
+                        if (formed) wait(sread, (formed - 1) & 1u);
+                        formed++;
+                        tc_fence_after();
+                        const uint64_t a = qd + (uint64_t)(w * (L::kPart >> 4));
+                        if (leader) {
+                            #pragma unroll
+                            for (int k = 0; k < D / 16; k++)
+                                mma_bf16(tmem, a + (((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4), b + (((k >> 2) * (kKT * 128) + (k & 3) * 32) >> 4), id_s, k ? 1u : 0u);
+                            mma_commit(&sfull[w]);
+                            if (i + 1 == n[w]) mma_commit(&qempty[w]);
+                        }
+                        __syncwarp();
                     }
+                    if (leader) mma_commit(&empty[slot]);
                     __syncwarp();
                 }
-                steps[w]++;
-            };
-            auto done_with = [&](uint32_t part) {
-                if (leader) mma_commit(&empty[(parts + part) % L::kRing]);
-                __syncwarp();
-            };
-            // S_A(i), P_A(i-1) V, S_B(i), P_B(i-1) V: the order in which the softmax warps come to wait for them
-            for (int i = 0; i <= most && !*fault; i++) {
-                if (i < most) {
-                    const uint32_t p = parts + ta::k_part(i);
-                    wait(&full[p % L::kRing], p / L::kRing & 1u);
-                    form_s(0, i);
-                }
-                if (i >= 1) {
-                    const uint32_t x = looks + i - 1;
+            } else {
+                for (int i = 0; i < most && !*fault; i++) {
+                    const uint32_t slot = (parts + ta::v_part(i, most)) % L::kRing, x = looks + i;
+                    const uint64_t b = vd + (uint64_t)(slot * (uint32_t)(L::kPart >> 4));
                     wait(&clean[x % kClean], x / kClean & 1u);
-                    add_pv(0, i - 1);
-                }
-                if (i < most) {
-                    form_s(1, i);
-                    done_with(ta::k_part(i));
-                }
-                if (i >= 1) {
-                    add_pv(1, i - 1);
-                    done_with(ta::v_part(i - 1, most));
+                    #pragma unroll
+                    for (int w = 0; w < 2; w++) {
+                        if (i >= n[w]) continue;
+                        #pragma unroll
+                        for (int half = 0; half < 2; half++) {
+                            wait(&pfull[2 * w + half], steps[w] & 1u);
+                            tc_fence_after();
+                            if (leader) {
+                                #pragma unroll
+                                for (int k = 4 * half; k < 4 * half + 4; k++)
+                                    ta::tc_mma_ts(tmem + 256 + 128 * w, tmem + 128 + 64 * w + 8 * k, b + (k * 2048 >> 4), id_o, (i | k) ? 1u : 0u);
+                                if (half) mma_commit(&odone[w]);
+                            }
+                            __syncwarp();
+                        }
+                        steps[w]++;
+                    }
+                    if (leader) mma_commit(&empty[slot]);
+                    __syncwarp();
                 }
             }
             parts += 2 * most;
@@ -479,8 +470,8 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             item_done();
         }
         if (leader) {
-            mma_commit(drained);
-            if (!mbar_wait(drained, 0, P.wait_ns)) *fault = 1;
+            mma_commit(&drained[warp - kScores]);
+            if (!mbar_wait(&drained[warp - kScores], 0, P.wait_ns)) *fault = 1;
         }
         __syncwarp();
     } else if (warp == kLooker) {
@@ -521,8 +512,6 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             }
             item_done();
         }
-    } else if (warp > kLooker) {
-        fewer();
     } else {
         // ---------------- softmax and output ----------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
@@ -668,7 +657,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == kIssuer) tmem_dealloc(tmem, 512);
+    if (warp == kScores) tmem_dealloc(tmem, 512);
 }
 
 }  // namespace pr
