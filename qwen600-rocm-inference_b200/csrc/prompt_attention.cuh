@@ -29,9 +29,7 @@
 namespace qb {
 namespace pr {
 
-using ta::add2;
 using ta::exp2_approx;
-using ta::fma2;
 using ta::max3;
 using ta::mul2;
 using ta::pack2;
@@ -115,14 +113,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
     for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
 }
 
-// A place in a ring of barriers, and the parity of its use.
-template <int N>
-struct Ring {
-    uint32_t slot = 0, phase = 0;
-    __device__ __forceinline__ void next() {
-        if (++slot == N) { slot = 0; phase ^= 1u; }
-    }
-};
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
@@ -148,24 +138,41 @@ struct No { static constexpr bool value = false; };
 // interpolates it at the five Chebyshev nodes of [-1/2, 1/2] (within 2^-17), times 2^n from n's bits.  NaN stays NaN; below -125 it
 // is 2^-125.
 constexpr int kByHand = 1;     // of every four pairs
-__device__ __forceinline__ void fma2(float& a, float& b, float x, float y, float s, float t) {   // (a, b) * (x, y) + (s, t)
-    asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmov.b64 r, {%4, %5};\n\tfma.rn.f32x2 p, p, q, r;\n\tmov.b64 {%0, %1}, p;\n\t}"
-        : "+f"(a), "+f"(b) : "f"(x), "f"(y), "f"(s), "f"(t));
+// Two fp32 values in a 64-bit register: one instruction for both, and no moves between separate registers.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
 }
-__device__ __forceinline__ void exp2_by_hand(float& a, float& b) {
+__device__ __forceinline__ void halves(uint64_t x, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x)); }
+__device__ __forceinline__ uint64_t pair_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t pair_mul(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t exp2_by_hand(uint64_t x) {
     constexpr float kC[5] = {1.0f, 0.6931210160255432f, 0.2402234971523285f, 0.055921975523233414f, 0.00966636836528778f};
-    const float x = max_nan(a, -125.0f), y = max_nan(b, -125.0f);
-    float s = x, t = y;
-    add2(s, t, 12582912.0f, 12582912.0f);
-    const uint32_t ns = __float_as_uint(s), nt = __float_as_uint(t);
-    add2(s, t, -12582912.0f, -12582912.0f);
-    fma2(s, t, -1.0f, -1.0f, x, y);
-    float p = kC[4], q = kC[4];
+    float a, b;
+    halves(x, a, b);
+    x = pair(max_nan(a, -125.0f), max_nan(b, -125.0f));
+    const uint64_t s = pair_add(x, pair(12582912.0f, 12582912.0f));
+    halves(s, a, b);
+    const uint64_t scale = pair(__uint_as_float((__float_as_uint(a) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(b) << 23) + 0x3f800000u));
+    const uint64_t f = pair_fma(pair_add(s, pair(-12582912.0f, -12582912.0f)), pair(-1.0f, -1.0f), x);
+    uint64_t p = pair(kC[4], kC[4]);
     #pragma unroll
-    for (int i = 3; i >= 0; i--) fma2(p, q, s, t, kC[i], kC[i]);
-    mul2(p, q, __uint_as_float((ns << 23) + 0x3f800000u), __uint_as_float((nt << 23) + 0x3f800000u));
-    a = p;
-    b = q;
+    for (int i = 3; i >= 0; i--) p = pair_fma(p, f, pair(kC[i], kC[i]));
+    return pair_mul(p, scale);
 }
 
 // The sequences, by all lanes of a warp: where each one's rows and keys lie, and its items.
@@ -310,12 +317,22 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     auto wait = [&](uint64_t* bar, uint32_t parity) {
         if (mbar_try_wait(bar, parity)) return;
         uint64_t since = 0;
-        for (uint32_t n = 0; !*fault && !mbar_try_wait(bar, parity); n++) {
-            if ((n & 255u) == 255u) {
-                const uint64_t now = global_ns();
-                if (!since) since = now;
-                else if (now - since > P.wait_ns) *fault = 1;
-            }
+        while (!*fault) {
+            #pragma unroll 1
+            for (int n = 0; n < 64; n++) if (mbar_try_wait(bar, parity)) return;
+            const uint64_t now = global_ns();
+            if (!since) since = now;
+            else if (now - since > P.wait_ns) *fault = 1;
+        }
+    };
+    // The same for warps that nobody waits for at once: asleep in between, so as to take no issue slots from the others.
+    auto wait_asleep = [&](uint64_t* bar, uint32_t parity) {
+        if (mbar_try_wait(bar, parity)) return;
+        uint64_t since = 0;
+        while (!*fault && !mbar_try_wait_sleep(bar, parity, 2000u)) {
+            const uint64_t now = global_ns();
+            if (!since) since = now;
+            else if (now - since > P.wait_ns) *fault = 1;
         }
     };
     uint32_t seen = 0;                        // items so far
@@ -367,7 +384,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                 const int n = max(it.n[0], it.n[1]);
                 auto rows = [&](int w) {
                     if (!it.n[w]) return;
-                    if (used[w]) wait(&qempty[w], (used[w] - 1) & 1u);
+                    if (used[w]) wait_asleep(&qempty[w], (used[w] - 1) & 1u);
                     if (*fault) return;
                     used[w]++;
                     mbar_arrive_expect_tx(&qfull[w], P.tokens * P.group * D * 2);
@@ -377,7 +394,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                 };
                 auto keys = [&](const CUtensorMap* map, int i) {
                     const uint32_t s = part % L::kRing;
-                    if (part >= (uint32_t)L::kRing) wait(&empty[s], (part / L::kRing - 1) & 1u);
+                    if (part >= (uint32_t)L::kRing) wait_asleep(&empty[s], (part / L::kRing - 1) & 1u);
                     if (*fault) return;
                     mbar_arrive_expect_tx(&full[s], L::kPart);
                     #pragma unroll
@@ -484,7 +501,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             for (int x = 0; x < 2 * n && !*fault; x++, part++) {
                 int value;
                 const int i = ta::part_tile(x, n, value);
-                wait(&full[part % L::kRing], part / L::kRing & 1u);        // (K parts too: a wait that skips a phase may take the one before for it)
+                wait_asleep(&full[part % L::kRing], part / L::kRing & 1u);        // (K parts too: a wait that skips a phase may take the one before for it)
                 if (!value) continue;
                 if (i * kKT + kKT - 1 > it.off) {
                     constexpr uint32_t kExp = BF ? 0x7f807f80u : 0x7c007c00u;
@@ -540,6 +557,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(sread);
+                const bool taken_p = i == 0 || mbar_try_wait(&odone[w], (steps - 1) & 1u);   // P of the tile before has been taken
                 if (flip) {
                     #pragma unroll
                     for (int x = 0; x < 64; x++) v[x] = -v[x];
@@ -568,33 +586,37 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                     base = want;
                 }
                 if (i > 0 && __any_sync(~0u, move)) {
-                    wait(&odone[w], (steps - 1) & 1u);                     // O of the tile before
+                    if (!taken_p) wait(&odone[w], (steps - 1) & 1u);       // O of the tile before
                     tc_fence_after();
                     #pragma unroll 1
                     for (int c0 = 0; c0 < D / 2; c0 += 8) scale8(to + c0, f);
                 }
                 const float from = base == -INFINITY ? 0.f : base;
-                float sum0 = 0.f, sum1 = 0.f;
+                uint64_t sum = pair(0.f, 0.f);
+                const uint64_t c2 = pair(c, c), from2 = pair(-from, -from);
                 uint32_t p[16];
                 auto weights = [&](int c0, auto mixed) {
                     #pragma unroll
                     for (int x = 0; x < 32; x += 2) {
-                        float a = v[c0 + x], b = v[c0 + x + 1];
-                        fma2(a, b, c, -from);
+                        uint64_t y = pair_fma(pair(v[c0 + x], v[c0 + x + 1]), c2, from2);
+                        float a, b;
                         if (decltype(mixed)::value && x % 8 >= 8 - 2 * kByHand) {
-                            exp2_by_hand(a, b);
+                            y = exp2_by_hand(y);
+                            halves(y, a, b);
                         } else {
+                            halves(y, a, b);
                             a = exp2_approx(a);
                             b = exp2_approx(b);
+                            y = pair(a, b);
                         }
-                        add2(sum0, sum1, a, b);
+                        sum = pair_add(sum, y);
                         p[x / 2] = pack2<BF>(a, b);
                     }
                 };
                 // (a column that is not seen has to weigh nothing, which the polynomial cannot say)
                 if (part) weights(0, No());
                 else weights(0, Yes());
-                if (i > 0) wait(&odone[w], (steps - 1) & 1u);              // P of the tile before has been taken
+                if (!taken_p) wait(&odone[w], (steps - 1) & 1u);
                 tc_fence_after();
                 ta::tc_st16(tp, p);
                 if (part) weights(32, No());
@@ -604,6 +626,8 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&pfull[2 * w + half]);
+                float sum0, sum1;
+                halves(sum, sum0, sum1);
                 l += sum0 + sum1;
             }
             // ---- the row: this thread's half of the dims ----
