@@ -131,13 +131,6 @@ __device__ __forceinline__ void scale8(uint32_t taddr, float f) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
                  ::"r"(taddr), "f"(o[0]), "f"(o[1]), "f"(o[2]), "f"(o[3]), "f"(o[4]), "f"(o[5]), "f"(o[6]), "f"(o[7]) : "memory");
 }
-struct Yes { static constexpr bool value = true; };
-struct No { static constexpr bool value = false; };
-// 2^a and 2^b on the fused multiply-add pipe, for part of the weights, whose exponentials are what the softmax warps wait for:
-// a = n + f with the whole number n nearest to a (adding 1.5 * 2^23 rounds to it), 2^f by the polynomial of degree 4 that
-// interpolates it at the five Chebyshev nodes of [-1/2, 1/2] (within 2^-17), times 2^n from n's bits.  NaN stays NaN; below -125 it
-// is 2^-125.
-constexpr int kByHand = 1;     // of every four pairs
 // Two fp32 values in a 64-bit register: one instruction for both, and no moves between separate registers.
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
     uint64_t r;
@@ -155,26 +148,6 @@ __device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-__device__ __forceinline__ uint64_t pair_mul(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t exp2_by_hand(uint64_t x) {
-    constexpr float kC[5] = {1.0f, 0.6931210160255432f, 0.2402234971523285f, 0.055921975523233414f, 0.00966636836528778f};
-    float a, b;
-    halves(x, a, b);
-    x = pair(max_nan(a, -125.0f), max_nan(b, -125.0f));
-    const uint64_t s = pair_add(x, pair(12582912.0f, 12582912.0f));
-    halves(s, a, b);
-    const uint64_t scale = pair(__uint_as_float((__float_as_uint(a) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(b) << 23) + 0x3f800000u));
-    const uint64_t f = pair_fma(pair_add(s, pair(-12582912.0f, -12582912.0f)), pair(-1.0f, -1.0f), x);
-    uint64_t p = pair(kC[4], kC[4]);
-    #pragma unroll
-    for (int i = 3; i >= 0; i--) p = pair_fma(p, f, pair(kC[i], kC[i]));
-    return pair_mul(p, scale);
-}
-
 // The sequences, by all lanes of a warp: where each one's rows and keys lie, and its items.
 // Sequence s has tiles of 2 * tokens queries; tile t's level is t + 1 + the whole tiles that its context
 // would make: tiles of a level have about as many keys.  Items go by falling level,
@@ -595,33 +568,23 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                 uint64_t sum = pair(0.f, 0.f);
                 const uint64_t c2 = pair(c, c), from2 = pair(-from, -from);
                 uint32_t p[16];
-                auto weights = [&](int c0, auto mixed) {
+                #pragma unroll
+                for (int c0 = 0; c0 < 64; c0 += 32) {
                     #pragma unroll
                     for (int x = 0; x < 32; x += 2) {
-                        uint64_t y = pair_fma(pair(v[c0 + x], v[c0 + x + 1]), c2, from2);
                         float a, b;
-                        if (decltype(mixed)::value && x % 8 >= 8 - 2 * kByHand) {
-                            y = exp2_by_hand(y);
-                            halves(y, a, b);
-                        } else {
-                            halves(y, a, b);
-                            a = exp2_approx(a);
-                            b = exp2_approx(b);
-                            y = pair(a, b);
-                        }
-                        sum = pair_add(sum, y);
+                        halves(pair_fma(pair(v[c0 + x], v[c0 + x + 1]), c2, from2), a, b);
+                        a = exp2_approx(a);
+                        b = exp2_approx(b);
+                        sum = pair_add(sum, pair(a, b));
                         p[x / 2] = pack2<BF>(a, b);
                     }
-                };
-                // (a column that is not seen has to weigh nothing, which the polynomial cannot say)
-                if (part) weights(0, No());
-                else weights(0, Yes());
-                if (!taken_p) wait(&odone[w], (steps - 1) & 1u);
-                tc_fence_after();
-                ta::tc_st16(tp, p);
-                if (part) weights(32, No());
-                else weights(32, Yes());
-                ta::tc_st16(tp + 16, p);
+                    if (c0 == 0) {
+                        if (!taken_p) wait(&odone[w], (steps - 1) & 1u);
+                        tc_fence_after();
+                    }
+                    ta::tc_st16(tp + c0 / 2, p);
+                }
                 ta::tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
