@@ -223,8 +223,11 @@ extern "C" int qwen_qk_rope(const void* q, const void* k, const void* v, int dty
     P.out_type = out_dtype;
     P.store = pages ? pages->dtype : -1;
     P.eps = eps;
-    for (int j = 0; j < head_dim / 2; j++)   // (base^0 / 2 pi is the largest: 0.16 turns)
-        P.turn[j] = (unsigned long long)std::llroundl(powl((long double)base, -2.0L * j / head_dim) * (0x1p63L / 3.14159265358979323846264338327950288L));
+    // base^0 / 2 pi is the largest: 0.16 turns.  Factor by factor, each rounding 2^-64: after 63 of them 2^-58, as far below 2^-53 as
+    // the positions' 31 bits need to stay within 2^-22 of a turn at every position.
+    const long double step = powl((long double)base, -2.0L / head_dim);
+    long double turn = 0x1p63L / 3.14159265358979323846264338327950288L;
+    for (int j = 0; j < head_dim / 2; j++, turn *= step) P.turn[j] = (unsigned long long)turn;
     P.tokens = n_rows >= 4096 ? 4 : n_rows >= 1024 ? 2 : 1;
     const cudaStream_t st = (cudaStream_t)stream;
     const bool wide = head_dim == 128;

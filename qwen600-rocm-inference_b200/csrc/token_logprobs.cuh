@@ -26,6 +26,7 @@
 
 #include "../../include/qwen_b200.h"
 #include "ptx.cuh"
+#include "tree_attention.cuh"
 
 namespace qb {
 namespace lp {
@@ -81,32 +82,54 @@ struct Elem {
     }
 };
 
-// A running (m, S, U).
+__device__ __forceinline__ void fma2(float& a, float& b, float x, float y, float s, float t) {   // (a, b) + (x, y) * (s, t)
+    asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmov.b64 r, {%4, %5};\n\tfma.rn.f32x2 p, q, r, p;\n\tmov.b64 {%0, %1}, p;\n\t}"
+        : "+f"(a), "+f"(b) : "f"(x), "f"(y), "f"(s), "f"(t));
+}
+// A running (m, S, U).  S and U take in sums over kAhead pieces, so that the many small terms behind a large one are not lost one by one.
 struct Sums {
     float m, s, u;
-    // elements x follow, the largest of them vm
-    template <int N>
-    __device__ __forceinline__ void add(const float (&x)[N], float vm, float c) {
-        if (vm > m) {
-            const float d = fmaxf((m - vm) * c, -200.0f), f = ex2(d);   // (m = -inf: nothing so far, f = 0)
-            u = (u + s * d) * f;
-            s *= f;
-            m = vm;
-        }
-        const float base = m == -INFINITY ? 0.f : m;   // (no element above -inf so far)
-        #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const float y = max_nan((x[i] - base) * c, -200.0f), p = ex2(y);   // -inf: 0, and 0 to U
-            s += p;
-            u = fmaf(p, y, u);
-        }
-    }
     __device__ __forceinline__ void rise(float to, float c) {
-        if (m == -INFINITY) return;
-        const float d = fmaxf((m - to) * c, -200.0f), f = ex2(d);
+        const float d = fmaxf((m - to) * c, -200.0f), f = ex2(d);   // (m = -inf: nothing so far, f = 0)
         u = (u + s * d) * f;
         s *= f;
         m = to;
+    }
+    // elements x follow, the largest of them vm
+    template <int N>
+    __device__ __forceinline__ void add(const float (&x)[N], float vm, float c) {
+        if (vm > m) rise(vm, c);
+        if (m == -INFINITY) {                  // nothing above -inf so far; a NaN among them, which no maximum shows
+            #pragma unroll
+            for (int i = 0; i < N; i++) if (x[i] != x[i]) s = x[i];
+            return;
+        }
+        float s0 = 0.f, s1 = 0.f, u0 = 0.f, u1 = 0.f;
+        #pragma unroll
+        for (int i = 0; i + 1 < N; i += 2) {
+            float a = x[i], b = x[i + 1];
+            ta::add2(a, b, -m, -m);
+            ta::mul2(a, b, c, c);
+            const float p = ex2(a), q = ex2(b);
+            ta::add2(s0, s1, p, q);
+            fma2(u0, u1, p, q, a, b);
+        }
+        if (N % 2) {
+            const float a = (x[N - 1] - m) * c, p = ex2(a);
+            s0 += p;
+            u0 = fmaf(p, a, u0);
+        }
+        u0 += u1;
+        if (u0 != u0) {                        // an element of -inf: 2^y is 0, and 0 is what it adds (a NaN stays one)
+            u0 = 0.f;
+            #pragma unroll
+            for (int i = 0; i < N; i++) {
+                const float a = max_nan((x[i] - m) * c, -200.0f);
+                u0 = fmaf(ex2(a), a, u0);
+            }
+        }
+        s += s0 + s1;
+        u += u0;
     }
 };
 
@@ -135,28 +158,40 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Params P) {
     const uint4* vecs = reinterpret_cast<const uint4*>(base + (size_t)head * E::kSize);
 
     Sums a{-INFINITY, 0.f, 0.f};
+    auto fetch = [&](int v, uint4 (&w)[kAhead]) {
+        #pragma unroll
+        for (int i = 0; i < kAhead; i++) if (v + i * kThreads < v1) w[i] = __ldg(vecs + v + i * kThreads);
+    };
+    uint4 next[kAhead];
     int v = v0 + tid;
-    for (; v + (kAhead - 1) * kThreads < v1; v += kAhead * kThreads) {
+    fetch(v, next);
+    for (; v < v1; v += kAhead * kThreads) {
         uint4 w[kAhead];
         #pragma unroll
-        for (int i = 0; i < kAhead; i++) w[i] = __ldg(vecs + v + i * kThreads);
-        #pragma unroll
-        for (int i = 0; i < kAhead; i++) {
-            float x[kVec];
-            E::unpack(w[i], x);
-            float vm = x[0];
+        for (int i = 0; i < kAhead; i++) w[i] = next[i];
+        fetch(v + kAhead * kThreads, next);
+        if (v + (kAhead - 1) * kThreads < v1) {
+            float x[kAhead * kVec], vm = -INFINITY;
             #pragma unroll
-            for (int e = 1; e < kVec; e++) vm = fmaxf(vm, x[e]);
+            for (int i = 0; i < kAhead; i++) {
+                float y[kVec];
+                E::unpack(w[i], y);
+                #pragma unroll
+                for (int e = 0; e < kVec; e++) { x[i * kVec + e] = y[e]; vm = fmaxf(vm, y[e]); }
+            }
             a.add(x, vm, P.c);
+        } else {
+            #pragma unroll
+            for (int i = 0; i < kAhead; i++) {
+                if (v + i * kThreads >= v1) break;
+                float x[kVec];
+                E::unpack(w[i], x);
+                float vm = x[0];
+                #pragma unroll
+                for (int e = 1; e < kVec; e++) vm = fmaxf(vm, x[e]);
+                a.add(x, vm, P.c);
+            }
         }
-    }
-    for (; v < v1; v += kThreads) {
-        float x[kVec];
-        E::unpack(__ldg(vecs + v), x);
-        float vm = x[0];
-        #pragma unroll
-        for (int e = 1; e < kVec; e++) vm = fmaxf(vm, x[e]);
-        a.add(x, vm, P.c);
     }
     if (tid < loose) {
         const float x[1] = {E::one(base + (size_t)loose_at(tid) * E::kSize)};
@@ -171,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Params P) {
         float bm = part[0][0];
         #pragma unroll
         for (int i = 1; i < kWarps; i++) bm = fmaxf(bm, part[i][0]);
-        a.rise(bm, P.c);
+        if (a.m != -INFINITY) a.rise(bm, P.c);
         const float s = warp_sum(a.s), u = warp_sum(a.u);
         if (lane == 0) { part[warp][1] = s; part[warp][2] = u; }
         if (tid == 0) { n_chosen = 0; n_cand = 0; }
@@ -298,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Params P) {
             for (int b = 0; b < blocks; b++) {
                 const float* r = cluster.map_shared_rank(sums, b);
                 Sums x{r[0], r[1], r[2]};
-                x.rise(m, P.c);
+                if (x.m != -INFINITY) x.rise(m, P.c);
                 s += x.s;
                 u += x.u;
             }
