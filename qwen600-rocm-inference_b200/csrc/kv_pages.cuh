@@ -37,7 +37,7 @@ struct Pages {
     }
 };
 
-constexpr int kRopeThreads = 256, kRopeTokens = 4;   // tokens of a block at most
+constexpr int kRopeThreads = 256, kRopeTokens = 8;   // tokens of a block at most
 
 struct RopeParams {
     const uint8_t *q, *k, *v;
@@ -69,11 +69,11 @@ __device__ __forceinline__ void store8(uint8_t* p, int type, const float* x) {
     }
 }
 // One head's row to its page: this thread's 8 values of either half, the row's threads together.
-template <int D>
+template <int D, bool Q8>
 __device__ __forceinline__ void to_page(const RopeParams& P, bool value, int page, int row, int h, int part, const float (&x)[16]) {
     const size_t at = (size_t)page * P.pages.page_stride + (size_t)h * P.pages.head_stride + (size_t)row * D;
     uint8_t* base = value ? P.pages.v : P.pages.k;
-    if (P.store == QWEN_BF16 || P.store == QWEN_FP16) {
+    if constexpr (!Q8) {
         if (page < 0) return;
         store8(base + (at + part * 8) * 2, P.store, x);
         store8(base + (at + D / 2 + part * 8) * 2, P.store, x + 8);
@@ -95,8 +95,8 @@ __device__ __forceinline__ void to_page(const RopeParams& P, bool value, int pag
 }
 
 // grid ceil(n_rows / tokens), kRopeThreads threads.
-template <int SRC, int D>
-__global__ void __launch_bounds__(kRopeThreads) qk_rope_kernel(const __grid_constant__ RopeParams P) {
+template <int SRC, int D, bool Q8>   // Q8: 8-bit pages
+__global__ void __launch_bounds__(kRopeThreads, Q8 || SRC == QWEN_FP32 ? 3 : 4) qk_rope_kernel(const __grid_constant__ RopeParams P) {
     constexpr int kLanes = D / 16, kGroups = kRopeThreads / kLanes, kEs = SRC == QWEN_FP32 ? 4 : 2, kN = SRC == QWEN_FP32 ? 2 : 1;
     __shared__ __align__(16) float cosine[kRopeTokens][D / 2], sine[kRopeTokens][D / 2], gains[2][D];
     __shared__ int page_at[kRopeTokens], row_at[kRopeTokens];   // row_at: -1 where the token is left out
@@ -116,63 +116,73 @@ __global__ void __launch_bounds__(kRopeThreads) qk_rope_kernel(const __grid_cons
     }
     if (P.q_gain) for (int i = tid; i < 2 * D; i += kRopeThreads) gains[i / D][i % D] = one_value(i < D ? P.q_gain : P.k_gain, P.gain_type, i % D);
     __syncthreads();
-    const int part = tid % kLanes, per = P.n_heads + (paged ? 2 : 1) * P.n_kv_heads, all = tokens * per;
-    // (a warp's threads stay together: they shuffle)
-    for (int i0 = 0; i0 < all; i0 += kGroups) {
-        const int i = i0 + tid / kLanes, t = min(i / per, tokens - 1), r = i - t * per;
-        const bool in = i < all && row_at[t] >= 0;
+    const int part = tid % kLanes, per = P.n_heads + (paged ? 2 : 1) * P.n_kv_heads;
+    // A thread keeps its head for all of its tokens; where a token's rows are fewer than the threads' groups, several tokens go side by side.
+    // (A warp's threads stay together: they shuffle.)
+    const int beside = max(kGroups / per, 1), own = tid / kLanes / per;
+    for (int r0 = 0; r0 < per; r0 += kGroups) {
+        const int r = beside > 1 ? tid / kLanes - own * per : r0 + tid / kLanes, t0 = beside > 1 ? own : 0;
         const int kind = r < P.n_heads ? 0 : r < P.n_heads + P.n_kv_heads ? 1 : 2;   // q, k, v
         const int h = kind == 0 ? r : kind == 1 ? r - P.n_heads : r - P.n_heads - P.n_kv_heads;
-        const size_t token = (size_t)(first + t);
-        float x[16];
-        {
-            const uint8_t* src = kind == 0 ? P.q + (token * P.ldq + (size_t)h * D) * kEs : kind == 1 ? P.k + (token * P.ldk + (size_t)h * D) * kEs
-                                                                                             : P.v + (token * P.ldv + (size_t)h * D) * kEs;
-            uint4 raw[2 * kN];
+        const long long ld = kind == 0 ? P.ldq : kind == 1 ? P.ldk : P.ldv, ldo = kind == 0 ? P.ldqo : P.ldko;
+        const uint8_t* src = (kind == 0 ? P.q : kind == 1 ? P.k : P.v) + ((size_t)first * ld + (size_t)h * D + part * 8) * kEs;
+        const int es = P.out_type == QWEN_FP32 ? 4 : 2;
+        uint8_t* out = kind == 0 ? P.q_out : kind == 1 ? P.k_out : nullptr;
+        if (out) out += ((size_t)first * ldo + (size_t)h * D + part * 8) * es;
+        const bool mine = r < per && t0 < beside;
+        uint4 next[2 * kN];
+        auto fetch = [&](int t) {
             #pragma unroll
-            for (int n = 0; n < 2 * kN; n++) raw[n] = make_uint4(0, 0, 0, 0);
-            if (in) {
+            for (int n = 0; n < 2 * kN; n++) next[n] = make_uint4(0, 0, 0, 0);
+            if (mine && t < tokens && row_at[t] >= 0) {
+                const uint8_t* p = src + (size_t)t * ld * kEs;
                 #pragma unroll
                 for (int n = 0; n < kN; n++) {
-                    raw[n] = __ldg(reinterpret_cast<const uint4*>(src + part * 8 * kEs) + n);
-                    raw[kN + n] = __ldg(reinterpret_cast<const uint4*>(src + (D / 2 + part * 8) * kEs) + n);
+                    next[n] = __ldg(reinterpret_cast<const uint4*>(p) + n);
+                    next[kN + n] = __ldg(reinterpret_cast<const uint4*>(p + D / 2 * kEs) + n);
                 }
             }
-            kv::unpack16<SRC>(raw, x);
-        }
-        if (P.q_gain) {
-            float sum = 0.f;
-            #pragma unroll
-            for (int e = 0; e < 16; e++) sum = fmaf(x[e], x[e], sum);
-            #pragma unroll
-            for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (kind < 2) {
-                const float inv = 1.0f / sqrtf(fmaf(sum, 1.0f / D, P.eps));
-                const float* g = gains[kind];
+        };
+        fetch(t0);
+        for (int ta = 0; ta < tokens; ta += beside) {
+            const int t = min(ta + t0, tokens - 1);
+            float x[16];
+            kv::unpack16<SRC>(next, x);
+            fetch(ta + t0 + beside);
+            const bool in = mine && ta + t0 < tokens && row_at[t] >= 0;
+            if (P.q_gain) {
+                float sum = 0.f;
                 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    x[e] = x[e] * inv * g[part * 8 + e];
-                    x[8 + e] = x[8 + e] * inv * g[D / 2 + part * 8 + e];
+                for (int e = 0; e < 16; e++) sum = fmaf(x[e], x[e], sum);
+                #pragma unroll
+                for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                const float inv = kind < 2 ? 1.0f / sqrtf(fmaf(sum, 1.0f / D, P.eps)) : 1.0f;
+                #pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const float4 g = *reinterpret_cast<const float4*>(&gains[kind & 1][(e & 8 ? D / 2 - 8 : 0) + part * 8 + e]);
+                    if (kind < 2) { x[e] *= inv * g.x; x[e + 1] *= inv * g.y; x[e + 2] *= inv * g.z; x[e + 3] *= inv * g.w; }
                 }
             }
-        }
-        if (kind < 2) {
-            #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float c = cosine[t][part * 8 + e], s = sine[t][part * 8 + e], a = x[e], b = x[8 + e];
-                x[e] = fmaf(a, c, -(b * s));
-                x[8 + e] = fmaf(b, c, a * s);
+            if (kind < 2) {
+                #pragma unroll
+                for (int e = 0; e < 8; e += 4) {
+                    const float4 c4 = *reinterpret_cast<const float4*>(&cosine[t][part * 8 + e]), s4 = *reinterpret_cast<const float4*>(&sine[t][part * 8 + e]);
+                    const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+                    #pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float a = x[e + j], b = x[8 + e + j];
+                        x[e + j] = fmaf(a, c[j], -(b * s[j]));
+                        x[8 + e + j] = fmaf(b, c[j], a * s[j]);
+                    }
+                }
+                if (in && out) {
+                    uint8_t* p = out + (size_t)t * ldo * es;
+                    store8(p, P.out_type, x);
+                    store8(p + D / 2 * es, P.out_type, x + 8);
+                }
             }
-            const int es = P.out_type == QWEN_FP32 ? 4 : 2;
-            uint8_t* out = kind == 0 ? P.q_out + (token * P.ldqo + (size_t)h * D) * es : P.k_out + (token * P.ldko + (size_t)h * D) * es;
-            if (in && (kind == 0 || P.k_out)) {
-                store8(out + part * 8 * es, P.out_type, x);
-                store8(out + (D / 2 + part * 8) * es, P.out_type, x + 8);
-            }
-        }
-        if (paged) {
             const int page = in && kind > 0 ? page_at[t] : -1;
-            if (__any_sync(0xffffffffu, page >= 0)) to_page<D>(P, kind == 2, page, max(row_at[t], 0), h, part, x);
+            if (__any_sync(0xffffffffu, page >= 0)) to_page<D, Q8>(P, kind == 2, page, max(row_at[t], 0), h, part, x);
         }
     }
 }

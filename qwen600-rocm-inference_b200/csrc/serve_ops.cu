@@ -73,7 +73,9 @@ qb::pg::Pages device_pages(const qwen_kv_pages_t* c) {
 // ---- norms, rotation, rows to pages ----------------------------------------------
 template <int SRC, int D>
 int rope_launch(const qb::pg::RopeParams& P, cudaStream_t st) {
-    qb::pg::qk_rope_kernel<SRC, D><<<(P.n_rows + P.tokens - 1) / P.tokens, qb::pg::kRopeThreads, 0, st>>>(P);
+    const int blocks = (P.n_rows + P.tokens - 1) / P.tokens;
+    if (is8(P.store)) qb::pg::qk_rope_kernel<SRC, D, true><<<blocks, qb::pg::kRopeThreads, 0, st>>>(P);
+    else qb::pg::qk_rope_kernel<SRC, D, false><<<blocks, qb::pg::kRopeThreads, 0, st>>>(P);
     CU(cudaGetLastError());
     return QWEN_OK;
 }
@@ -108,6 +110,9 @@ int prompt_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMa
 }
 
 // ---- attention over pages ------------------------------------------------------------
+// A cluster of 16 CTAs an item where that leaves no SM with more than one CTA and an item is too long for one: one launch, and the parts are joined
+// through distributed shared memory.
+bool paged_clusters(const Plan& p, int nsm) { return p.items * qb::pa::kCluster <= nsm && p.blocks <= 64; }
 int paged_plan(const qwen_kv_pages_t* c, int n_heads, int dev, Plan* p) {
     const int group = n_heads / c->n_kv_heads, keys = qb::pa::tile_keys(c->head_dim * (is8(c->dtype) ? 1 : 2)), capacity = c->max_pages * c->page_size;
     p->rows = group <= 8 ? 8 : 16;
@@ -196,10 +201,11 @@ extern "C" int qwen_qk_rope(const void* q, const void* k, const void* v, int dty
         TRY(check_ld(ldv, n_kv_heads, head_dim, "ldv"));
         if (pages->n_kv_heads != n_kv_heads || pages->head_dim != head_dim) return fail(QWEN_E_ARG, "the pages' heads are not the rows'");
     }
-    int dev = 0;
+    int dev = 0, nsm = 0;
     TRY(check_ptrs({{q, "q", 16, true}, {k, "k", 16, true}, {v, "v", 16, pages != nullptr}, {q_gain, "q_gain", 4, q_gain != nullptr},
                     {k_gain, "k_gain", 4, k_gain != nullptr}, {positions, "positions", 4, true}, {q_out, "q_out", 16, true}, {k_out, "k_out", 16, k_out != nullptr},
                     QB_PAGES_PTRS(c, pages != nullptr), {seqs, "seqs", 4, pages != nullptr}}, &dev));
+    TRY(sm_count(dev, &nsm));
     qb::pg::RopeParams P;
     P.q = (const uint8_t*)q;
     P.k = (const uint8_t*)k;
@@ -228,7 +234,7 @@ extern "C" int qwen_qk_rope(const void* q, const void* k, const void* v, int dty
     const long double step = powl((long double)base, -2.0L / head_dim);
     long double turn = 0x1p63L / 3.14159265358979323846264338327950288L;
     for (int j = 0; j < head_dim / 2; j++, turn *= step) P.turn[j] = (unsigned long long)turn;
-    P.tokens = n_rows >= 4096 ? 4 : n_rows >= 1024 ? 2 : 1;
+    P.tokens = std::min(std::max(n_rows / (4 * nsm), 1), qb::pg::kRopeTokens);   // (four blocks an SM at least)
     const cudaStream_t st = (cudaStream_t)stream;
     const bool wide = head_dim == 128;
     switch (dtype) {
