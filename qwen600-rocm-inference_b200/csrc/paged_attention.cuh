@@ -16,6 +16,8 @@
 // in between need one vote instead of a maximum over the warp.  The page numbers of
 // a tile are loaded a tile before its rows.
 #pragma once
+#include <cooperative_groups.h>
+
 #include "kv_pages.cuh"
 #include "tree_attention.cuh"
 
@@ -33,11 +35,13 @@ using ta::swz;
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kItemCost = 2;   // what an item costs beside its tiles, in tiles
+constexpr int kCluster = 8;    // CTAs that share an item
 constexpr float kRise = 8.0f;  // weights stay below 2^8
 
 struct Params {
     ta::Params t;    // cache.capacity: positions that a table names; q, out, lens, work, shares
     pg::Pages pages;
+    int cluster;     // a cluster of kCluster CTAs has an item
 };
 
 // Keys of a tile, by the bytes of a cache row: 16 or 32 for each warp.
@@ -59,6 +63,7 @@ struct Layout {
     static constexpr int kPitch = D + 4;                       // floats of a row of O at the joining
     static constexpr int kJoin = kWarps * kRows * (kPitch + 2) * 4;
     static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
+    static_assert(kJoin + kRows * (D + 2) * 4 <= kSmem, "a cluster's parts lie behind the warps'");
     static constexpr int kSlot = kRows * (D + 2);              // floats of a workspace slot: O, then (m, l) pairs
     static_assert(kStage % 16 == 0, "rows of 16-byte pieces");
     static_assert(kStages >= 2 && kCtas * (kSmem + 1024) <= 228 * 1024, "kCtas CTAs an SM");
@@ -86,7 +91,22 @@ __global__ void __launch_bounds__(kThreads, 2) paged_kernel(const __grid_constan
     pdl_launch_dependents();   // after the wait: what the joining kernel reads early (lens) is then complete
 
     ta::Items<L::KT, kItemCost, L::kRows> it;
-    if (!it.start(P)) return;
+    const int rank = PP.cluster ? (int)blockIdx.x % kCluster : 0;
+    if (!PP.cluster) {
+        if (!it.start(P)) return;
+    } else {
+        const int unit = (int)blockIdx.x / kCluster, per = P.n_kv_heads * P.row_blocks;
+        it.seq = unit / per;
+        it.h = (unit - it.seq * per) / P.row_blocks;
+        it.r_base = (unit - it.seq * per) % P.row_blocks * L::kRows;
+        it.len = max(P.lens[it.seq], -1);
+        it.end = ta::seq_end(P, it.len);
+        it.n = ta::seq_tiles<L::KT>(P, it.len);
+        it.t0 = (int)((long long)it.n * rank / kCluster);
+        it.t1 = (int)((long long)it.n * (rank + 1) / kCluster);
+        it.at = it.before = 0;                 // (the one item)
+        it.to = it.step = 1;
+    }
     const int in_page = (1 << pages.shift) - 1;
     do {
         const int seq = it.seq, end = it.end, h = it.h, r_base = it.r_base, t0 = it.t0, t1 = it.t1;
@@ -367,12 +387,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_kernel(const __grid_constan
                 }
             }
         __syncthreads();
-        const bool whole = t0 == 0 && t1 == it.n;
-        float* slot = P.work + (size_t)(2 * blockIdx.x + (it.first ? 0 : 1)) * L::kSlot;
-        for (int i = tid; i < L::kRows * (D / 4); i += kThreads) {
-            const int r = i / (D / 4), d = i % (D / 4) * 4, row = r_base + r;
-            if (row >= P.group) break;
-            float mm = -INFINITY, ll = 0.f;
+        auto joined = [&](int r, int d, float& mm, float& ll) {           // dims d .. d + 3 of head r, from the warps
+            mm = -INFINITY;
+            ll = 0.f;
             #pragma unroll
             for (int w = 0; w < kWarps; w++) mm = fmaxf(mm, join_ml[(w * L::kRows + r) * 2]);
             float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -384,10 +401,59 @@ __global__ void __launch_bounds__(kThreads, 2) paged_kernel(const __grid_constan
                 ll += lw * fw;
                 a.x += b.x * fw; a.y += b.y * fw; a.z += b.z * fw; a.w += b.w * fw;
             }
+            return a;
+        };
+        auto write = [&](int row, int d, const float4& a, float ll) {
+            const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+            uint8_t* dst = P.out + ((size_t)seq * P.ldo + (size_t)(h * P.group + row) * D + d) * 2;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(ta::pack2<QT == QWEN_BF16>(a.x * inv, a.y * inv), ta::pack2<QT == QWEN_BF16>(a.z * inv, a.w * inv));
+        };
+        if (PP.cluster) {
+            // this CTA's part, then every CTA joins its share of the outputs from all parts in their order
+            float* own = reinterpret_cast<float*>(smem + L::kJoin);       // [head][D], then (m, l) pairs
+            for (int i = tid; i < L::kRows * (D / 4); i += kThreads) {
+                const int r = i / (D / 4), d = i % (D / 4) * 4;
+                float mm, ll;
+                const float4 a = joined(r, d, mm, ll);
+                *reinterpret_cast<float4*>(own + r * D + d) = a;
+                if (d == 0) *reinterpret_cast<float2*>(own + L::kRows * D + 2 * r) = make_float2(mm, ll);
+            }
+            namespace cg = cooperative_groups;
+            cg::cluster_group group = cg::this_cluster();
+            group.sync();
+            for (int i = rank * kThreads + tid; i < min(L::kRows, P.group - r_base) * (D / 4); i += kCluster * kThreads) {
+                const int r = i / (D / 4), d = i % (D / 4) * 4;
+                float2 ml[kCluster];
+                float4 b[kCluster];
+                float mm = -INFINITY, ll = 0.f;
+                #pragma unroll
+                for (int k = 0; k < kCluster; k++) {
+                    const float* from = group.map_shared_rank(own, k);
+                    ml[k] = *reinterpret_cast<const float2*>(from + L::kRows * D + 2 * r);
+                    b[k] = *reinterpret_cast<const float4*>(from + r * D + d);
+                    mm = fmaxf(mm, ml[k].x);
+                }
+                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+                #pragma unroll
+                for (int k = 0; k < kCluster; k++) {
+                    const float f = mm == -INFINITY ? 1.0f : exp2_approx(ml[k].x - mm);
+                    ll += ml[k].y * f;
+                    a.x += b[k].x * f; a.y += b[k].y * f; a.z += b[k].z * f; a.w += b[k].w * f;
+                }
+                write(r_base + r, d, a, ll);
+            }
+            group.sync();                      // the others read this CTA's part until here
+            return;
+        }
+        const bool whole = t0 == 0 && t1 == it.n;
+        float* slot = P.work + (size_t)(2 * blockIdx.x + (it.first ? 0 : 1)) * L::kSlot;
+        for (int i = tid; i < L::kRows * (D / 4); i += kThreads) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4, row = r_base + r;
+            if (row >= P.group) break;
+            float mm, ll;
+            const float4 a = joined(r, d, mm, ll);
             if (whole) {
-                const float inv = ll == 0.f ? 0.f : 1.0f / ll;
-                uint8_t* dst = P.out + ((size_t)seq * P.ldo + (size_t)(h * P.group + row) * D + d) * 2;
-                *reinterpret_cast<uint2*>(dst) = make_uint2(ta::pack2<QT == QWEN_BF16>(a.x * inv, a.y * inv), ta::pack2<QT == QWEN_BF16>(a.z * inv, a.w * inv));
+                write(row, d, a, ll);
             } else {
                 *reinterpret_cast<float4*>(slot + r * D + d) = a;
                 if (d == 0) *reinterpret_cast<float2*>(slot + L::kRows * D + 2 * r) = make_float2(mm, ll);

@@ -110,10 +110,15 @@ int prompt_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMa
 }
 
 // ---- attention over pages ------------------------------------------------------------
-// A cluster of 16 CTAs an item where that leaves no SM with more than one CTA and an item is too long for one: one launch, and the parts are joined
-// through distributed shared memory.
-bool paged_clusters(const Plan& p, int nsm) { return p.items * qb::pa::kCluster <= nsm && p.blocks <= 64; }
-int paged_plan(const qwen_kv_pages_t* c, int n_heads, int dev, Plan* p) {
+// A CTA for each item, a cluster of eight for each, or shares of the line of tiles.  A cluster needs one launch, its parts are joined through distributed
+// shared memory, but eight CTAs an item leave others idle: clusters where the items' CTAs all fit at once, for tables of up to 32 tiles, or of 96
+// where the items' CTAs are more than half of those that fit.  Measured, clusters / shares, 8 K/V heads of 128, bf16 (tiles of 64): 1 sequence of 500
+// 5.7 / 6.6 us, of 1000 6.8 / 7.6, of 2000 8.5 / 9.5, of 4000 11.9 / 11.6, of 8000 19.1 / 15.8; 4 of 1000 8.1 / 9.8, of 4000 17.2 / 19.6, of 8000
+// 27.7 / 29.8, of 16000 50.0 / 51.9; e4m3 (tiles of 128): 1 of 2000 7.5 / 8.2, of 8000 14.1 / 12.6; 4 of 8000 19.4 / 21.9, of 16000 33.2 / 33.0.
+struct PagedPlan : Plan {
+    int cluster;   // 0: none
+};
+int paged_plan(const qwen_kv_pages_t* c, int n_heads, int dev, PagedPlan* p) {
     const int group = n_heads / c->n_kv_heads, keys = qb::pa::tile_keys(c->head_dim * (is8(c->dtype) ? 1 : 2)), capacity = c->max_pages * c->page_size;
     p->rows = group <= 8 ? 8 : 16;
     p->row_blocks = (group + p->rows - 1) / p->rows;
@@ -121,27 +126,47 @@ int paged_plan(const qwen_kv_pages_t* c, int n_heads, int dev, Plan* p) {
     p->blocks = (capacity + 63) / 64;
     p->items = (long long)c->n_seqs * c->n_kv_heads * p->row_blocks;
     p->spare = 7.0f;
-    p->whole = p->blocks <= p->spare && p->items < 1 << 30;
+    p->cluster = 0;
+    p->whole = p->tiles <= 2 && p->items < 1 << 30;
     int nsm = 0, ctas = 0;
     if (!p->whole) {
         TRY(sm_count(dev, &nsm));
         ctas = 2 * nsm;
-        p->whole = p->blocks <= 16 && p->items < 1 << 30 && (double)p->blocks * std::max(0ll, ctas - p->items) <= (double)p->spare * ctas;
+        const long long all = p->items * qb::pa::kCluster;
+        if (all <= ctas && p->tiles >= qb::pa::kCluster && p->tiles <= (2 * all > ctas ? 96 : 32)) p->cluster = qb::pa::kCluster;
+        p->whole = p->cluster != 0 || (p->blocks <= p->spare && p->items < 1 << 30) ||
+                   (p->blocks <= 16 && p->items < 1 << 30 && (double)p->blocks * std::max(0ll, ctas - p->items) <= (double)p->spare * ctas);
     }
     return plan_shares(p, ctas, c->head_dim);
 }
 template <int QT, int STORE, int D, int NT>
-int paged_launch(const qb::pa::Params& P, const Plan& plan, int dev, cudaStream_t st) {
+int paged_launch(const qb::pa::Params& P, const PagedPlan& plan, int dev, cudaStream_t st) {
     using L = qb::pa::Layout<STORE, D, NT>;
     static std::atomic<uint64_t> done{0};
     auto kernel = qb::pa::paged_kernel<QT, STORE, D, NT>;
     TRY(smem_limit(kernel, done, dev, L::kSmem));
+    if (plan.cluster) {
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = plan.cluster;
+        at[0].val.clusterDim.y = 1;
+        at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        cfg.gridDim = dim3((unsigned)(plan.items * plan.cluster));
+        cfg.blockDim = dim3(qb::pa::kThreads);
+        cfg.dynamicSmemBytes = L::kSmem;
+        cfg.stream = st;
+        CU(cudaLaunchKernelEx(&cfg, kernel, P));
+        return QWEN_OK;
+    }
     kernel<<<plan.shares, qb::pa::kThreads, L::kSmem, st>>>(P);
     CU(cudaGetLastError());
     return join_launch<QT, L::KT, qb::pa::kItemCost, D, L::kRows, false>(P.t, plan, dev, st);
 }
 template <int QT, int STORE>
-int paged_by_shape(int dim, const qb::pa::Params& P, const Plan& plan, int dev, cudaStream_t st) {
+int paged_by_shape(int dim, const qb::pa::Params& P, const PagedPlan& plan, int dev, cudaStream_t st) {
     if (dim == 64) return plan.rows == 8 ? paged_launch<QT, STORE, 64, 1>(P, plan, dev, st) : paged_launch<QT, STORE, 64, 2>(P, plan, dev, st);
     return plan.rows == 8 ? paged_launch<QT, STORE, 128, 1>(P, plan, dev, st) : paged_launch<QT, STORE, 128, 2>(P, plan, dev, st);
 }
@@ -303,8 +328,8 @@ extern "C" int qwen_paged_attention_workspace(const qwen_kv_pages_t* pages, int 
     TRY(check_pages(pages));
     TRY(check_heads(n_heads, pages->n_kv_heads, pages->head_dim));
     int dev = 0;
-    if ((long long)pages->max_pages * pages->page_size > 448) CU(cudaGetDevice(&dev));   // (shorter ones need none on any device)
-    Plan p;
+    if ((long long)pages->max_pages * pages->page_size > 128) CU(cudaGetDevice(&dev));   // (shorter ones need none on any device)
+    PagedPlan p;
     TRY(paged_plan(pages, n_heads, dev, &p));
     *bytes = p.bytes;
     return QWEN_OK;
@@ -322,12 +347,13 @@ extern "C" int qwen_paged_attention(const qwen_kv_pages_t* pages, const void* q,
     if (q == out) return fail(QWEN_E_ARG, "out must not be q");
     int dev = 0;
     TRY(check_ptrs({QB_PAGES_PTRS(pages, true), {q, "q", 16, true}, {out, "out", 16, true}, {lens, "lens", 4, true}, {workspace, "workspace", 16, workspace != nullptr}}, &dev));
-    Plan plan;
+    PagedPlan plan;
     TRY(paged_plan(pages, n_heads, dev, &plan));
     if (plan.bytes && !workspace) return fail(QWEN_E_ARG, "workspace is NULL");
     if (workspace_bytes < plan.bytes) return fail(QWEN_E_ARG, "workspace is smaller than qwen_paged_attention_workspace says");
     qb::pa::Params P;
     P.pages = device_pages(pages);
+    P.cluster = plan.cluster;
     P.t = {};
     P.t.cache.capacity = pages->max_pages * pages->page_size;
     P.t.q = (const uint8_t*)q;
