@@ -212,12 +212,9 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Params P) {
         if (tid == 0) { n_chosen = 0; n_cand = 0; }
         if (tid < kMaxTop) best[tid] = 0;
         __syncthreads();
-        if (tid == 0) {
-            double ds = 0, du = 0;
-            for (int i = 0; i < kWarps; i++) { ds += part[i][1]; du += part[i][2]; }
-            sums[0] = bm;
-            sums[1] = (float)ds;
-            sums[2] = (float)du;
+        if (warp == 0) {
+            const float s2 = warp_sum(lane < kWarps ? part[lane][1] : 0.f), u2 = warp_sum(lane < kWarps ? part[lane][2] : 0.f);
+            if (lane == 0) { sums[0] = bm; sums[1] = s2; sums[2] = u2; }
         }
         __syncthreads();
     }
@@ -326,21 +323,21 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Params P) {
     cluster.sync();
     if (rank == 0) {
         __shared__ double joined[3];                 // m, S, U of the row
-        if (tid == 0) {
-            float m = -INFINITY;
-            for (int b = 0; b < blocks; b++) m = fmaxf(m, cluster.map_shared_rank(sums, b)[0]);
-            double s = 0, u = 0;
-            for (int b = 0; b < blocks; b++) {
-                const float* r = cluster.map_shared_rank(sums, b);
-                Sums x{r[0], r[1], r[2]};
-                if (x.m != -INFINITY) x.rise(m, P.c);
-                s += x.s;
-                u += x.u;
+        if (warp == 0) {                             // lane b has block b's (m, S, U)
+            Sums x{-INFINITY, 0.f, 0.f};
+            if (lane < blocks) {
+                const float* r = cluster.map_shared_rank(sums, lane);
+                x = {r[0], r[1], r[2]};
             }
-            const bool fine = s > 0 && m < INFINITY;  // (false for NaN)
-            joined[0] = fine ? (double)m : NAN;
-            joined[1] = fine ? log2(s) : NAN;
-            joined[2] = fine ? u / s : NAN;
+            const float m = warp_max(x.m);
+            if (x.m != -INFINITY) x.rise(m, P.c);
+            const float s = warp_sum(x.s), u = warp_sum(x.u);
+            if (lane == 0) {
+                const bool fine = s > 0 && m < INFINITY;  // (false for NaN)
+                joined[0] = fine ? (double)m : NAN;
+                joined[1] = fine ? log2((double)s) : NAN;
+                joined[2] = fine ? (double)u / s : NAN;
+            }
         }
         const int n = blocks * P.n_top;
         if (blocks > 1)
