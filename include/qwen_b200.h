@@ -514,11 +514,13 @@ int qwen_tree_verify(const void* logits, int logits_dtype, long long ld, const f
                      const int* parents, const float* uniforms, int n_seqs, int n_nodes, int vocab, float temperature, int* path,
                      int* n_path, int* next, void* stream);
 
-/* Failure testing of the two calls above without a GPU fault: every later call
+/* Failure testing of qwen_tree_attention, qwen_tree_verify and
+ * qwen_prompt_attention without a GPU fault: every later call
  * of the process waits at most wait_ns (>= 1 ms; 0 restores the default 1 s) on
  * the device, and, with part >= 0, one wait can only run out:
  * qwen_tree_attention's for slot `part` of the ring that K and V come through (a
- * call with more than 32 query rows a K/V head), qwen_tree_verify's for the row of
+ * call with more than 32 query rows a K/V head), qwen_prompt_attention's for slot
+ * `part` of its ring (4 slots with heads of 128, 8 with heads of 64), qwen_tree_verify's for the row of
  * node `part` (where rows start on 16 bytes and are held in shared memory).
  * qwen_debug_draft_wait(0, -1) restores normal operation. */
 int qwen_debug_draft_wait(unsigned long long wait_ns, int part);
@@ -604,14 +606,14 @@ int qwen_paged_attention(const qwen_kv_pages_t* pages, const void* q, void* out,
                          const int* lens, float scale, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Log probabilities under p = softmax(logits / temperature) of each of n_rows rows of logits
- * (dtype QWEN_FP32, QWEN_BF16 or QWEN_FP16; vocab columns, rows ld elements apart):
+ * (dtype QWEN_FP32, QWEN_BF16 or QWEN_FP16, aligned to its elements; vocab columns, rows ld elements apart):
  * logprob[r] = log p(tokens[r]) (tokens and logprob may both be NULL; a token outside 0 ..
  * vocab-1 gives NaN), entropy[r] = -sum p log p (may be NULL), and the n_top likeliest tokens
  * (0 .. 64) with their log probabilities, likeliest first, equal logits by the smaller id:
  * top_ids and top_logprobs, [n_rows][n_top]; places beyond the vocabulary hold -1 and -inf.  Logits of
  * -inf are tokens that cannot come.  A row with a NaN, a +inf or nothing above -inf has no
- * distribution: NaN, ids -1.  temperature is within 1e-6 .. 1e6.  Differences between
- * logits below -1e30 count as none in the sums. */
+ * distribution: NaN, ids -1.  temperature is within 1e-6 .. 1e6.  Sums are fp32, in
+ * parts of at most 32 terms a step; the logarithms and differences behind them fp64. */
 int qwen_token_logprobs(const void* logits, int dtype, long long ld, int n_rows, int vocab, const int* tokens, float temperature, int n_top,
                         float* logprob, float* entropy, int* top_ids, float* top_logprobs, void* stream);
 

@@ -14,7 +14,15 @@
 // of cp.async stages, its own sums l and O, and a base for each head that exponents
 // are taken from: it rises only when a score lies 2^8 above it (base-2 exponents), so the tiles
 // in between need one vote instead of a maximum over the warp.  The page numbers of
-// a tile are loaded a tile before its rows.
+// a tile are loaded a tile before its rows.  Weights are rounded to 16 bits for the product
+// with V (off by half a step, 2^-8 or 2^-11 relative); l sums them unrounded.
+//
+// Few sequences: a cluster of eight CTAs an item, each a run of tiles, joined through distributed shared
+// memory, one launch.
+//
+// Measured: 128 ragged sequences up to 8191 over 1.08 GB of e4m3 pages 179 to 187 us (5.8 to 6.0 TB/s, floor 165), bound by memory traffic;
+// 32 over 35 MB of int8 pages, seven heads of 64 each, 16.5 us (floor 5.4), by the plan, the first
+// loads and the joining; one sequence at 1024 6.3 us (floor 0.6), by its latencies (two launches: 8.5 us).
 #pragma once
 #include <cooperative_groups.h>
 

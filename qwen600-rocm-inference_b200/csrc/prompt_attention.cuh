@@ -12,17 +12,30 @@
 // A row of a tile is a (token, query head) pair of one K/V head, head fastest: T = 128 /
 // group tokens of all the K/V head's query heads, so K and V serve the whole group.
 // An item is two such row tiles, A and B, one behind the other, and their common key
-// tiles: while the softmax of one is at work, the tensor cores form the other's products.
-// Tensor memory: S of A and B (128 columns each, P written over them in 16 bits), O of A
-// and B.  The tensor cores take the products in the order in which they are issued: S_A(i+1)
-// follows P_A(i) V(i), which reads what it overwrites.
+// tiles.  Tensor memory: one S (128 columns), which A and B use in turn, P of A and of B
+// (16 bits, 64 columns each), O of A and of B.  S is in registers soon after it is formed, so the
+// next tile's is formed while the softmax is at work, and no chain runs from a tile's P over its product
+// to the next S.
 //
-// Warps: 0-3 softmax and output of A (a thread a row), 4-7 of B, 8 loads (TMA), 9
-// issues the products, 10 finds the items, 11 looks for infinities and NaN among the V
+// Measured (bf16, 16 query heads over 8 K/V heads of 128): one prompt of 8192 224 us, 1,227 TFLOP/s, where a large
+// matrix product has 1,637 for a moment and 1,370 for long (floor 168 us); 2048 38 us; four of 4096 248 us.
+// Heads of 64: one of 8192 208 to 248 us, bound by the softmax in the same way.
+// Bound by the softmax warps: a tile of 256 x 128 takes 3,350 cycles, of which the tensor cores need 2,050 at
+// their rate and 2,500 as they run (both operands of S come from shared memory), the exponentials 2,050; the warps
+// issue in 54 % of the slots, each waiting for its own chain: scores (300 cycles), maximum and its exchange
+// (800), exponentials (1,400), waits that find their barriers ready (100 to 200 each).  Steps on the way: one thread a row, P
+// over S, products issued by a lane alone 374 us; descriptors in uniform registers and registers shared out anew 273; one S for both tiles
+// with two threads a row 255; a warp each for the two products 232; fewer polls 224.  Tried, not kept: a part of the exponentials by a
+// polynomial (as fast or slower: the instructions cost what the special-function unit spares), turns of A and B at the
+// exponentials (235 us).
+//
+// Warps: 0-7 softmax and output of A (two threads a row, 64 keys of a tile and half of the dims each; they agree on
+// the row's maximum through shared memory), 8-15 of B, 16 finds the items and loads (TMA), 17 issues
+// S, 18 issues P V, 19 looks for infinities and NaN among the V
 // rows of tiles that are not seen as a whole: 0 * NaN would reach rows that do not see them,
 // so such values are zeroed in shared memory and added at the end to the rows that see them.
 // Items, heaviest first, are dealt out to the CTAs forwards and backwards in turn; they are found on the device from
-// starts and k_starts.  Every wait is bounded; where one runs out, the CTA's rows become NaN.
+// starts and k_starts.  Every wait on a barrier is bounded; where one runs out, the CTA's rows become NaN.
 #pragma once
 #include "tree_attention_tc.cuh"
 
@@ -37,7 +50,7 @@ using ta::pack2;
 constexpr int kKT = 128;                  // keys of a tile
 constexpr int kSoftmax = 16;              // warps: two threads a row, 64 keys of a tile each
 constexpr int kThreads = 640, kLoader = 16, kScores = 17, kValues = 18, kLooker = 19;
-constexpr int kItems = 4;                 // items between the finder and the slowest warp
+constexpr int kItems = 4;                 // items between the loader and the slowest warp
 constexpr int kClean = 4;                 // V parts that the looker may be ahead
 
 struct Params {
