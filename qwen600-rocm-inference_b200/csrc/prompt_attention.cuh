@@ -51,7 +51,7 @@ constexpr int kKT = 128;                  // keys of a tile
 constexpr int kSoftmax = 16;              // warps: two threads a row, 64 keys of a tile each
 constexpr int kThreads = 640, kLoader = 16, kScores = 17, kValues = 18, kLooker = 19;
 constexpr int kItems = 4;                 // items between the loader and the slowest warp
-constexpr int kClean = 4;                 // V parts that the looker may be ahead
+constexpr int kClean = 8;                 // V parts that the looker may be ahead: no more than the ring holds
 
 struct Params {
     uint8_t* out;
@@ -88,7 +88,7 @@ struct Layout {
     static constexpr int kXm = kItem + kItems * (int)sizeof(Item);       // [row tile][parity][half][row] maxima, then sums
     static constexpr int kMisc = kXm + 2 * 2 * 2 * 128 * 4;
     static constexpr int kSmem = kMisc + 16 + 1024;
-    static_assert(kRing / 2 + kRing % 2 <= kClean, "V parts in flight");
+    static_assert(kRing <= kClean, "V parts in flight (behind a long item, short ones bring V at every other part and two at its end)");
     static_assert(kSmem <= 227 * 1024, "one CTA's shared memory");
     static_assert(2 * kSmem > 228 * 1024, "one CTA an SM: the kernel allocates all of tensor memory");
 };

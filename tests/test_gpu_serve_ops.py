@@ -403,6 +403,38 @@ def test_prompt_more_items_than_multiprocessors(qb):
     _check_prompt(qb, q, k, v, starts, None, 128 ** -0.5)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompt_short_items_behind_long_ones(qb, dim):
+    """CTAs go from items of many key tiles to items of one, where K and V change places in the ring of parts; again and again."""
+    import torch
+    lens = [3000, 1500] + [50] * 500 + [130] * 40
+    starts = np.concatenate([[0], np.cumsum(lens)]).tolist()
+    q, k, v = _rows(17, starts[-1], 8, starts[-1], 4, dim, torch.bfloat16)
+    want = _check_prompt(qb, q, k, v, starts, None, dim ** -0.5)
+    for _ in range(40):
+        assert torch.equal(_prompt(qb, q, k, v, starts, None, dim ** -0.5), want)
+
+
+def test_prompt_repeats_give_the_same_bits(qb):
+    """Many calls one behind the other, with other inputs in between: no order of arrival shows."""
+    import torch
+    sets = [_rows(20 + i, 4096, 16, 4096, 8, 128, torch.bfloat16) for i in range(3)]
+    st = _dev([0, 4096])
+    call = lambda q, k, v, o: qb.prompt_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), qb.BF16, 2048, 1024, 1024, 2048, st.data_ptr(), 0, 1, 4096,  # noqa: E731
+                                                  4096, 16, 8, 128, 0.09, _stream())
+    want = []
+    for s in sets:
+        want.append(torch.empty_like(s[0]))
+        call(*s, want[-1])
+    outs = [torch.empty_like(s[0]) for s in sets]
+    for _ in range(100):
+        for s, o in zip(sets, outs):
+            o.fill_(1)
+            call(*s, o)
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w) and bool(w.isfinite().all())
+
+
 @pytest.mark.parametrize("starts,k_starts", [([0, 500, 90], [0, 500, 90]), ([-5, 60, 10 ** 9], [-(10 ** 9), 70, 2 ** 31 - 1]), ([90, 20, 30], [0, 0, 50])])
 def test_prompt_starts_of_any_value(qb, starts, k_starts):
     """Starts outside the rows count as their ends, a start behind its end as no rows: nothing else is written."""
