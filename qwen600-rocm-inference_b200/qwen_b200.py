@@ -346,7 +346,7 @@ def token_logprobs(logits_ptr, dtype, ld, n_rows, vocab, tokens_ptr, temperature
 
 
 def debug_draft_wait(wait_ns=0, part=-1):
-    """Failure testing of tree_attention and tree_verify: wait limit of later calls (0 = default) and a ring slot or
+    """Failure testing of tree_attention, tree_verify and prompt_attention: wait limit of later calls (0 = default) and a ring slot or
     node whose wait runs out (-1 = none)."""
     _check(load_library().qwen_debug_draft_wait(int(wait_ns), int(part)))
 
