@@ -173,18 +173,13 @@ int paged_by_shape(int dim, const qb::pa::Params& P, const PagedPlan& plan, int 
 
 // ---- log probabilities -----------------------------------------------------------------
 template <int T>
-int logprobs_launch(const qb::lp::Params& P, int n_rows, int nsm, int dev, cudaStream_t st) {
+int logprobs_launch(const qb::lp::Params& P, int n_rows, int nsm, cudaStream_t st) {
     using namespace qb::lp;
-    static std::atomic<uint64_t> done{0};
-    const auto kernel = logprobs_kernel<T>;
-    if (!((done.load() >> dev) & 1)) {
-        CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        done.fetch_or(1ull << dev);
-    }
-    // blocks for a row: as many as keep the SMs' two places busy, each with a few pieces a thread
+    // Blocks for a row: no more in all than the SMs' two places hold, each with a piece a thread at least.  (Twice and four times as many: 64
+    // rows of fp32 16.7 us instead of 11.7, 128 rows 21.9 and 31.9 instead of 17.1.)
     const int vec = T == QWEN_FP32 ? 4 : 8;
     int cluster = 1;
-    while (cluster < 8 && (long long)n_rows * cluster * 2 <= 2 * nsm && P.vocab >= cluster * 2 * kThreads * vec) cluster *= 2;
+    while (cluster < kMaxCluster && (long long)n_rows * cluster * 2 <= 2 * nsm && P.vocab >= cluster * 2 * kThreads * vec) cluster *= 2;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -196,7 +191,7 @@ int logprobs_launch(const qb::lp::Params& P, int n_rows, int nsm, int dev, cudaS
     cfg.gridDim = dim3((unsigned)n_rows * cluster);
     cfg.blockDim = dim3(kThreads);
     cfg.stream = st;
-    CU(cudaLaunchKernelEx(&cfg, kernel, P));
+    CU(cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, P));
     return QWEN_OK;
 }
 
@@ -413,8 +408,8 @@ extern "C" int qwen_token_logprobs(const void* logits, int dtype, long long ld, 
     P.top_ids = top_ids;
     const cudaStream_t st = (cudaStream_t)stream;
     switch (dtype) {
-        case QWEN_BF16: return logprobs_launch<QWEN_BF16>(P, n_rows, nsm, dev, st);
-        case QWEN_FP16: return logprobs_launch<QWEN_FP16>(P, n_rows, nsm, dev, st);
-        default: return logprobs_launch<QWEN_FP32>(P, n_rows, nsm, dev, st);
+        case QWEN_BF16: return logprobs_launch<QWEN_BF16>(P, n_rows, nsm, st);
+        case QWEN_FP16: return logprobs_launch<QWEN_FP16>(P, n_rows, nsm, st);
+        default: return logprobs_launch<QWEN_FP32>(P, n_rows, nsm, st);
     }
 }

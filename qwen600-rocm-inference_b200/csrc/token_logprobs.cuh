@@ -33,7 +33,7 @@
 namespace qb {
 namespace lp {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxTop = 64, kMaxCluster = 16, kCand = 1024;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxTop = 64, kMaxCluster = 8, kCand = 1024;
 constexpr int kAhead = 4;     // 16-byte pieces that a thread loads at once
 
 struct Params {
@@ -135,6 +135,7 @@ struct Sums {
     }
 };
 
+static_assert(kMaxCluster * kMaxTop <= kCand, "the blocks' likeliest are joined in one list");
 // grid n_rows * cluster, kThreads threads, clusters of `cluster` blocks: rows one after the other.
 template <int T>
 __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const Params P) {
