@@ -520,7 +520,8 @@ int qwen_tree_verify(const void* logits, int logits_dtype, long long ld, const f
  * the device, and, with part >= 0, one wait can only run out:
  * qwen_tree_attention's for slot `part` of the ring that K and V come through (a
  * call with more than 32 query rows a K/V head), qwen_prompt_attention's for slot
- * `part` of its ring (4 slots with heads of 128, 8 with heads of 64), qwen_tree_verify's for the row of
+ * `part` of its rings (4 slots with heads of 128, 8 with heads of 64; K's are the even
+ * ones, V's the odd ones), qwen_tree_verify's for the row of
  * node `part` (where rows start on 16 bytes and are held in shared memory).
  * qwen_debug_draft_wait(0, -1) restores normal operation. */
 int qwen_debug_draft_wait(unsigned long long wait_ns, int part);

@@ -51,7 +51,6 @@ constexpr int kKT = 128;                  // keys of a tile
 constexpr int kSoftmax = 16;              // warps: two threads a row, 64 keys of a tile each
 constexpr int kThreads = 640, kLoader = 16, kScores = 17, kValues = 18, kLooker = 19;
 constexpr int kItems = 4;                 // items between the loader and the slowest warp
-constexpr int kClean = 8;                 // V parts that the looker may be ahead: no more than the ring holds
 
 struct Params {
     uint8_t* out;
@@ -79,16 +78,18 @@ struct Item {
 template <int D>
 struct Layout {
     static constexpr int kPart = kKT * D * 2;                 // K or V of a tile, or the rows of a row tile
-    static constexpr int kRing = D == 64 ? 8 : 4;             // K / V parts in flight, in the order in which they are used: K 0, K 1, V 0, K 2, V 1, ...
+    // K / V parts in flight.  K and V have a ring each: K's slots are the even ones, V's the odd ones.  So every warp that waits for a part of
+    // a ring waits for all of them in turn, and a slot is filled anew only when they have: a wait by parity can neither take an
+    // older phase for its own nor be overtaken by two.
+    static constexpr int kRing = D == 64 ? 8 : 4, kSlots = kRing / 2;
     static constexpr int kQ = 0;
     static constexpr int kKV = 2 * kPart;
     static constexpr int kBar = kKV + kRing * kPart;
-    static constexpr int kBars = 2 * kRing + kClean + 2 * kItems + 15;
+    static constexpr int kBars = 2 * kRing + kSlots + 2 * kItems + 15;
     static constexpr int kItem = kBar + (kBars * 8 + 15) / 16 * 16;
     static constexpr int kXm = kItem + kItems * (int)sizeof(Item);       // [row tile][parity][half][row] maxima, then sums
     static constexpr int kMisc = kXm + 2 * 2 * 2 * 128 * 4;
     static constexpr int kSmem = kMisc + 16 + 1024;
-    static_assert(kRing <= kClean, "V parts in flight (behind a long item, short ones bring V at every other part and two at its end)");
     static_assert(kSmem <= 227 * 1024, "one CTA's shared memory");
     static_assert(2 * kSmem > 228 * 1024, "one CTA an SM: the kernel allocates all of tensor memory");
 };
@@ -259,8 +260,8 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBar);   // [kRing] a K or V part has arrived
     uint64_t* empty = full + L::kRing;                              // [kRing] its products are done
-    uint64_t* clean = empty + L::kRing;                             // [kClean] a V part has been looked at
-    uint64_t* given = clean + kClean;                               // [kItems] an item is there
+    uint64_t* clean = empty + L::kRing;                             // [kSlots] a V part has been looked at
+    uint64_t* given = clean + L::kSlots;                            // [kItems] an item is there
     uint64_t* taken = given + kItems;                               // [kItems] all warps are done with it
     // [2]: A, B
     uint64_t* qfull = taken + kItems;                               // the item's rows have arrived
@@ -276,7 +277,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < L::kRing; i++) { mbar_init(&full[i], 1 + (i == P.withheld)); mbar_init(&empty[i], 1); }
-        for (int i = 0; i < kClean; i++) mbar_init(&clean[i], 1);
+        for (int i = 0; i < L::kSlots; i++) mbar_init(&clean[i], 1);
         for (int i = 0; i < kItems; i++) { mbar_init(&given[i], 1); mbar_init(&taken[i], kSoftmax + 3); }   // softmax, products, looker
         for (int w = 0; w < 2; w++) {
             mbar_init(&qfull[w], 1);
@@ -341,7 +342,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         fewer();
         const Finder finder(P);
         const int G = gridDim.x;
-        uint32_t part = 0, used[2] = {0, 0};   // K / V parts so far; items so far that have the row tile
+        uint32_t parts[2] = {0, 0}, used[2] = {0, 0};   // K and V parts so far; items so far that have the row tile
         bool more = true;
         for (int k = 0; more; k++) {
             const long long at = (long long)k * G + (k & 1 ? G - 1 - (int)blockIdx.x : (int)blockIdx.x);   // forwards and backwards
@@ -378,28 +379,31 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                     for (int x = 0; x < D / 64; x++)
                         tma_load_3d(smem + L::kQ + w * L::kPart + x * (128 * 128), &map_q, 64 * x, it.h * P.group, it.q0 + w * P.tokens, &qfull[w]);
                 };
-                auto keys = [&](const CUtensorMap* map, int i) {
-                    const uint32_t s = part % L::kRing;
-                    if (part >= (uint32_t)L::kRing) wait_asleep(&empty[s], (part / L::kRing - 1) & 1u);
+                auto keys = [&](int value, int i) {      // tile i of K or V
+                    const CUtensorMap* map = value ? &map_v : &map_k;
+                    const uint32_t part = parts[value], s = 2 * (part % L::kSlots) + value;
+                    if (part >= (uint32_t)L::kSlots) wait_asleep(&empty[s], (part / L::kSlots - 1) & 1u);
                     if (*fault) return;
                     mbar_arrive_expect_tx(&full[s], L::kPart);
                     #pragma unroll
                     for (int x = 0; x < D / 64; x++)
                         tma_load_2d(smem + L::kKV + s * L::kPart + x * (kKT * 128), map, it.h * D + 64 * x, it.k0 + i * kKT, &full[s]);
-                    part++;
+                    parts[value]++;
                 };
                 rows(0);
-                for (int i = 0; i < n && !*fault; i++) {
-                    keys(&map_k, i);
+                for (int i = 0; i < n && !*fault; i++) {   // in the order in which the products take them
+                    keys(0, i);
                     if (i == 0) rows(1);
-                    else keys(&map_v, i - 1);
+                    else keys(1, i - 1);
                 }
-                if (n) keys(&map_v, n - 1);
+                if (n) keys(1, n - 1);
             }
             __syncwarp();
         }
         if (*fault && lane == 0) {             // nothing may still be on its way when the CTA ends
-            for (uint32_t p = part > (uint32_t)L::kRing ? part - L::kRing : 0; p < part; p++) mbar_wait(&full[p % L::kRing], p / L::kRing & 1u, 10000000ull);
+            for (int v = 0; v < 2; v++)
+                for (uint32_t p = parts[v] > (uint32_t)L::kSlots ? parts[v] - L::kSlots : 0; p < parts[v]; p++)
+                    mbar_wait(&full[2 * (p % L::kSlots) + v], p / L::kSlots & 1u, 10000000ull);
             for (int w = 0; w < 2; w++) if (used[w]) mbar_wait(&qfull[w], (used[w] - 1) & 1u, 10000000ull);
         }
         __syncwarp();
@@ -413,15 +417,15 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         const bool leader = elect_one();
         const uint64_t qd = kmajor_sw128_desc(smem_addr(smem + L::kQ)), kd = kmajor_sw128_desc(smem_addr(smem + L::kKV)),
                        vd = ta::mn_major_sw128_desc(smem_addr(smem + L::kKV), kKT * 128);
-        uint32_t parts = 0, looks = 0;         // K / V parts, V parts of the items so far
+        uint32_t parts = 0;                    // K (or V) parts of the items so far
         uint32_t used[2] = {0, 0}, steps[2] = {0, 0}, formed = 0;   // items, key tiles of a row tile so far; S so far
         while (next_item()) {
             const int n[2] = {__shfl_sync(~0u, items[seen % kItems].n[0], 0), __shfl_sync(~0u, items[seen % kItems].n[1], 0)}, most = max(n[0], n[1]);
             if (warp == kScores) {
                 for (int i = 0; i < most && !*fault; i++) {
-                    const uint32_t part = parts + ta::k_part(i), slot = part % L::kRing;
+                    const uint32_t part = parts + i, slot = 2 * (part % L::kSlots);
                     const uint64_t b = kd + (uint64_t)(slot * (uint32_t)(L::kPart >> 4));
-                    wait(&full[slot], part / L::kRing & 1u);
+                    wait(&full[slot], part / L::kSlots & 1u);
                     #pragma unroll
                     for (int w = 0; w < 2; w++) {
                         if (i >= n[w]) continue;
@@ -444,9 +448,9 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                 }
             } else {
                 for (int i = 0; i < most && !*fault; i++) {
-                    const uint32_t slot = (parts + ta::v_part(i, most)) % L::kRing, x = looks + i;
+                    const uint32_t part = parts + i, place = part % L::kSlots, slot = 2 * place + 1;
                     const uint64_t b = vd + (uint64_t)(slot * (uint32_t)(L::kPart >> 4));
-                    wait(&clean[x % kClean], x / kClean & 1u);
+                    wait(&clean[place], part / L::kSlots & 1u);
                     #pragma unroll
                     for (int w = 0; w < 2; w++) {
                         if (i >= n[w]) continue;
@@ -468,8 +472,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                     __syncwarp();
                 }
             }
-            parts += 2 * most;
-            looks += most;
+            parts += most;
             item_done();
         }
         if (leader) {
@@ -480,18 +483,16 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     } else if (warp == kLooker) {
         // ---------------- infinities and NaN among V rows that not all rows see ----------------
         fewer();
-        uint32_t part = 0, looks = 0;
+        uint32_t part = 0;                     // V parts so far
         while (next_item()) {
             it = items[seen % kItems];
             const int n = max(it.n[0], it.n[1]);
-            for (int x = 0; x < 2 * n && !*fault; x++, part++) {
-                int value;
-                const int i = ta::part_tile(x, n, value);
-                wait_asleep(&full[part % L::kRing], part / L::kRing & 1u);        // (K parts too: a wait that skips a phase may take the one before for it)
-                if (!value) continue;
+            for (int i = 0; i < n && !*fault; i++, part++) {
+                const uint32_t place = part % L::kSlots, slot = 2 * place + 1;
+                wait_asleep(&full[slot], part / L::kSlots & 1u);
                 if (i * kKT + kKT - 1 > it.off) {
                     constexpr uint32_t kExp = BF ? 0x7f807f80u : 0x7c007c00u;
-                    uint4* rows = reinterpret_cast<uint4*>(smem + L::kKV + part % L::kRing * L::kPart);
+                    uint4* rows = reinterpret_cast<uint4*>(smem + L::kKV + slot * L::kPart);
                     bool any = false;
                     #pragma unroll 8
                     for (int x = lane; x < L::kPart / 16; x += 32) {
@@ -510,8 +511,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                     }
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&clean[looks % kClean]);
-                looks++;
+                if (lane == 0) mbar_arrive(&clean[place]);
             }
             item_done();
         }
