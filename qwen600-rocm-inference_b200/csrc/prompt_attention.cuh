@@ -268,7 +268,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     uint64_t* qempty = qfull + 2;                                   // their last S is formed
     uint64_t* sfull = qfull + 4;                                    // S formed
     uint64_t* odone = qfull + 6;                                    // P V added
-    uint64_t* pfull = qfull + 8;                                    // [2][2] a half of P written, O scaled (4 warps)
+    uint64_t* pfull = qfull + 8;                                    // [2][2] a half of P written (4 warps); for the first one O scaled too (all 8)
     uint64_t* sread = qfull + 12;                                   // S is in registers (8 warps)
     uint64_t* drained = qfull + 13;                                 // [2] all products of a warp are done, at the end
     Item* items = reinterpret_cast<Item*>(smem + L::kItem);
@@ -283,7 +283,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             mbar_init(&qfull[w], 1);
             mbar_init(&qempty[w], 1);
             mbar_init(&sfull[w], 1);
-            mbar_init(&pfull[2 * w], 4);
+            mbar_init(&pfull[2 * w], 8);
             mbar_init(&pfull[2 * w + 1], 4);
             mbar_init(&odone[w], 1);
         }
@@ -576,6 +576,12 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                     tc_fence_after();
                     #pragma unroll 1
                     for (int c0 = 0; c0 < D / 2; c0 += 8) scale8(to + c0, f);
+                    ta::tc_wait_st();
+                }
+                if (half) {                                                // the first half's product adds to all columns of O, these warps' too
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&pfull[2 * w]);
                 }
                 const float from = base == -INFINITY ? 0.f : base;
                 uint64_t sum = pair(0.f, 0.f);

@@ -107,9 +107,10 @@ def search(m, limit=3_000_000):
     return len(seen)
 
 
-def kernel(items, slots, one_ring=False):
+def kernel(items, slots, first_half_waits_for_both=True, one_ring=False):
     """The kernel's steps for items (key tiles of A, key tiles of B) with `slots` K and `slots` V parts in flight.  one_ring: K
-    and V through one ring of 2 * slots in the order of use (a form that goes wrong, which the search has to find)."""
+    and V through one ring of 2 * slots in the order of use; first_half_waits_for_both false: the first half of P V
+    does not wait for the second half's scaling of O.  (Forms that go wrong, which the search has to find.)"""
     m = Model()
     loader, scores, values, looker = (m.steps(n) for n in ("loader", "scores", "values", "looker"))
     tiles = [w for w in range(2) if any(it[w] for it in items)]
@@ -145,7 +146,7 @@ def kernel(items, slots, one_ring=False):
         m.bar(f"taken {s}", len(soft) + 3)
     m.bar("sread", 2)
     for w in tiles:
-        for b, n in (("qfull", 1), ("qempty", 1), ("sfull", 1), ("odone", 1), ("pfull 0", 1), ("pfull 1", 1), ("pair", 2)):
+        for b, n in (("qfull", 1), ("qempty", 1), ("sfull", 1), ("odone", 1), ("pfull 0", 2 if first_half_waits_for_both else 1), ("pfull 1", 1), ("pair", 2)):
             m.bar(f"{b} {w}", n)
 
     formed, used, steps, pairs, looked = 0, [0, 0], [0, 0], [0, 0], 0
@@ -201,7 +202,7 @@ def kernel(items, slots, one_ring=False):
                     continue
                 for h in range(2):
                     values.append(("wait", f"pfull {h} {w}", steps[w] + i))
-                    values.append(("mma", [(f"part {s}", ("V", it, i)), (f"P {w} {h}", (it, i))],
+                    values.append(("mma", [(f"part {s}", ("V", it, i)), (f"P {w} {h}", (it, i))] + [(f"scaled {w} {x}", (it, i)) for x in range(2)],
                                    [(f"O {w}", (it, i))] if h else [], [f"odone {w}"] if h else []))
             values[-1][3].append(f"empty {s}")
         if one_ring:                        # the looker waited for K parts too, in the order of use
@@ -221,6 +222,9 @@ def kernel(items, slots, one_ring=False):
                 if i:                       # the base has risen: O of the tile before, times a factor
                     prog.append(("wait", f"odone {w}", steps[w] + i - 1))
                     prog.append(("do", [(f"O {w}", (it, i - 1))], []))
+                prog.append(("do", [], [(f"scaled {w} {h}", (it, i))]))
+                if h and first_half_waits_for_both:
+                    prog.append(("arrive", f"pfull 0 {w}"))
                 prog += [("do", [], [(f"P {w} {h}", (it, i))]), ("arrive", f"pfull {h} {w}")]
             if n[w]:
                 prog += [("arrive", f"pair {w}"), ("wait", f"pair {w}", swap), ("wait", f"odone {w}", steps[w] + n[w] - 1), ("do", [(f"O {w}", (it, n[w] - 1))], [])]
@@ -245,3 +249,10 @@ def test_search_finds_one_ring_for_both(items):
     """A warp that looks at V parts alone, in a ring through which K parts go too, is overtaken."""
     with pytest.raises(Wrong, match="overtaken"):
         search(kernel(items, 2, one_ring=True))
+
+
+@pytest.mark.parametrize("items", [[(2, 0)], [(1, 0)] * 2])
+def test_search_finds_products_beside_scaling(items):
+    """A product that takes the first half's P adds to an O that the second half's warps are still scaling, or reading."""
+    with pytest.raises(Wrong, match="product finds"):
+        search(kernel(items, 2, first_half_waits_for_both=False))

@@ -494,6 +494,22 @@ def test_prompt_large_scores(qb):
     _check_prompt(qb, q, k, v, [0, 700], None, 0.5)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim,heads,kv", [(64, 4, 4), (128, 4, 4), (64, 4, 2), (128, 8, 4)])
+def test_prompt_maximum_that_rises_in_every_tile(qb, dtype, dim, heads, kv):
+    """Keys that grow along each sequence, so that O is scaled in most tiles, beside the products of the tile's first half; several
+    items a CTA, again and again: within the bounds, and always the same bits."""
+    import torch
+    lens = [2600, 1900, 900, 300] + [600] * 40
+    starts = np.concatenate([[0], np.cumsum(lens)]).tolist()
+    q, k, v = _rows(31 + dim + heads, starts[-1], heads, starts[-1], kv, dim, _types(qb)[dtype][1])
+    grow = torch.cat([torch.linspace(0.2, 24 * n / 1000 + 4, n) for n in lens]).cuda()
+    k = (k.float() * grow[:, None, None]).to(k.dtype)
+    want = _check_prompt(qb, q, k, v, starts, None, 0.4)
+    for _ in range(30):
+        assert torch.equal(_prompt(qb, q, k, v, starts, None, 0.4), want)
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 def test_prompt_reports_a_wait_that_ran_out(qb, dim):
     """K and V that are never announced: the bounded waits end, the call's rows are NaN, and the next call is right."""
