@@ -274,6 +274,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     Item* items = reinterpret_cast<Item*>(smem + L::kItem);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
     volatile int* fault = reinterpret_cast<int*>(smem + L::kMisc + 4);
+    volatile uint32_t* beat = reinterpret_cast<uint32_t*>(smem + L::kMisc + 8);   // K and V parts asked for so far
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < L::kRing; i++) { mbar_init(&full[i], 1 + (i == P.withheld)); mbar_init(&empty[i], 1); }
@@ -291,6 +292,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         for (int i = 0; i < 2; i++) mbar_init(&drained[i], 1);
         fence_barrier_init();
         *fault = 0;
+        *beat = 0;
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
@@ -324,10 +326,18 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     };
     uint32_t seen = 0;                        // items so far
     Item it;
-    auto next_item = [&]() {                  // all lanes of a warp; false: no more
+    // All lanes of a warp; false: no more.  A warp whose row tile has no keys may wait here for as long as the block's item takes: the
+    // wait has run out where no part was asked for all the while.
+    auto next_item = [&]() {
         const int slot = seen % kItems;
-        if (!ta::mbar_spin(&given[slot], seen / kItems & 1u, 8 * P.wait_ns)) { *fault = 1; return false; }
-        return !items[slot].stop;
+        for (uint32_t before = 0;;) {
+            if (__all_sync(~0u, ta::mbar_spin(&given[slot], seen / kItems & 1u, 8 * P.wait_ns))) return !items[slot].stop;
+            const uint32_t now = __shfl_sync(~0u, *beat, 0);
+            if (now == before) break;
+            before = now;
+        }
+        *fault = 1;
+        return false;
     };
     auto item_done = [&]() {
         __syncwarp();
@@ -388,7 +398,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                     #pragma unroll
                     for (int x = 0; x < D / 64; x++)
                         tma_load_2d(smem + L::kKV + s * L::kPart + x * (kKT * 128), map, it.h * D + 64 * x, it.k0 + i * kKT, &full[s]);
-                    parts[value]++;
+                    *beat = ++parts[value] + parts[value ^ 1];
                 };
                 rows(0);
                 for (int i = 0; i < n && !*fault; i++) {   // in the order in which the products take them

@@ -510,6 +510,21 @@ def test_prompt_maximum_that_rises_in_every_tile(qb, dtype, dim, heads, kv):
         assert torch.equal(_prompt(qb, q, k, v, starts, None, 0.4), want)
 
 
+def test_prompt_long_items_are_not_waits_that_run_out(qb):
+    """One query over two million keys: the warps of the second row tile have nothing to do for many times the limit of a wait, while
+    the block makes progress all along."""
+    import torch
+    q, k, v = _rows(13, 1, 1, 1 << 21, 1, 64, torch.bfloat16)
+    want = _prompt(qb, q, k, v, [0, 1], [0, 1 << 21], 0.125)
+    assert bool(want.isfinite().all()) and bool((want != 0).any())
+    qb.debug_draft_wait(1_000_000, -1)
+    try:
+        got = _prompt(qb, q, k, v, [0, 1], [0, 1 << 21], 0.125)
+    finally:
+        qb.debug_draft_wait()
+    assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 def test_prompt_reports_a_wait_that_ran_out(qb, dim):
     """K and V that are never announced: the bounded waits end, the call's rows are NaN, and the next call is right."""
