@@ -588,8 +588,9 @@ int qwen_qk_rope(const void* q, const void* k, const void* v, int dtype, long lo
  * start lies behind its end has no rows or keys).  Rows that belong to no sequence stay as they
  * were.  o = sum_j softmax_j(scale * q . k_j) v_j with scores, softmax statistics and sums in fp32; the
  * weights enter the product with V in 16 bits.  What a query does not see (NaN included) has
- * no influence on it.  scale is finite, below 2^127 in magnitude.  The rows of a call whose
- * device-side waits ran out (they are bounded) are NaN. */
+ * no influence on it.  scale is finite, below 2^127 in magnitude.  Device-side waits are bounded:
+ * where one of a thread block runs out, all rows of the items that the block had, of the call's rows a
+ * part, are NaN for the items' heads; the others are right. */
 int qwen_prompt_attention(const void* q, const void* k, const void* v, void* out, int dtype, long long ldq, long long ldk, long long ldv,
                           long long ldo, const int* starts, const int* k_starts, int n_seqs, int n_rows, int n_keys, int n_heads,
                           int n_kv_heads, int head_dim, float scale, void* stream);

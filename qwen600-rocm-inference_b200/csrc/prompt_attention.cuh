@@ -35,7 +35,8 @@
 // rows of tiles that are not seen as a whole: 0 * NaN would reach rows that do not see them,
 // so such values are zeroed in shared memory and added at the end to the rows that see them.
 // Items, heaviest first, are dealt out to the CTAs forwards and backwards in turn; they are found on the device from
-// starts and k_starts.  Every wait on a barrier is bounded; where one runs out, the CTA's rows become NaN.
+// starts and k_starts.  Every wait on a barrier is bounded; where one runs out, the rows of all of the CTA's items become NaN
+// at its end.
 #pragma once
 #include "tree_attention_tc.cuh"
 
@@ -324,6 +325,11 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             else if (now - since > P.wait_ns) *fault = 1;
         }
     };
+    auto failed = [&]() { return __any_sync(~0u, *fault); };   // the same for a warp, whose lanes go on together
+    auto finish = [&]() {                     // a warp's last step: all of the CTA's work is done behind it
+        tc_fence_before();
+        __syncthreads();
+    };
     uint32_t seen = 0;                        // items so far
     Item it;
     // All lanes of a warp; false: no more.  A warp whose row tile has no keys may wait here for as long as the block's item takes: the
@@ -352,29 +358,30 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         fewer();
         const Finder finder(P);
         const int G = gridDim.x;
+        auto deal = [&](int k) {               // item k of this CTA into `it`; false: there are not so many
+            const long long at = (long long)k * G + (k & 1 ? G - 1 - (int)blockIdx.x : (int)blockIdx.x);   // forwards and backwards
+            int seq = 0, tile = 0, q0, nq, k0, nk;
+            it = {};
+            if (at / P.n_kv_heads >= 0x7fffffff || !finder.find(P, (int)(at / P.n_kv_heads), seq, tile)) return false;
+            finder.bounds(P, seq, q0, nq, k0, nk);
+            it.h = (int)(at % P.n_kv_heads);
+            it.q0 = q0 + tile * finder.per;
+            it.nq = min(nq - tile * finder.per, finder.per);
+            it.k0 = k0;
+            it.off = nk - nq + tile * finder.per;
+            for (int w = 0; w < 2; w++) {
+                const int count = min(it.nq - w * P.tokens, P.tokens), last = it.off + w * P.tokens + count - 1;
+                it.n[w] = count <= 0 || last < 0 ? 0 : last / kKT + 1;
+            }
+            return true;
+        };
         uint32_t parts[2] = {0, 0}, used[2] = {0, 0};   // K and V parts so far; items so far that have the row tile
         bool more = true;
         for (int k = 0; more; k++) {
-            const long long at = (long long)k * G + (k & 1 ? G - 1 - (int)blockIdx.x : (int)blockIdx.x);   // forwards and backwards
-            int seq = 0, tile = 0;
-            more = at / P.n_kv_heads < 0x7fffffff && finder.find(P, (int)(at / P.n_kv_heads), seq, tile);
-            it = {};
+            more = deal(k);
             it.stop = !more;
-            if (more) {
-                int q0, nq, k0, nk;
-                finder.bounds(P, seq, q0, nq, k0, nk);
-                it.h = (int)(at % P.n_kv_heads);
-                it.q0 = q0 + tile * finder.per;
-                it.nq = min(nq - tile * finder.per, finder.per);
-                it.k0 = k0;
-                it.off = nk - nq + tile * finder.per;
-                for (int w = 0; w < 2; w++) {
-                    const int count = min(it.nq - w * P.tokens, P.tokens), last = it.off + w * P.tokens + count - 1;
-                    it.n[w] = count <= 0 || last < 0 ? 0 : last / kKT + 1;
-                }
-            }
             const int slot = k % kItems;
-            if (k >= kItems && !ta::mbar_spin(&taken[slot], (k / kItems - 1) & 1u, 8 * P.wait_ns)) { *fault = 1; break; }
+            if (k >= kItems && !__all_sync(~0u, ta::mbar_spin(&taken[slot], (k / kItems - 1) & 1u, 8 * P.wait_ns))) { *fault = 1; break; }
             if (lane == 0) {
                 items[slot] = it;
                 mbar_arrive(&given[slot]);
@@ -417,6 +424,15 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             for (int w = 0; w < 2; w++) if (used[w]) mbar_wait(&qfull[w], (used[w] - 1) & 1u, 10000000ull);
         }
         __syncwarp();
+        finish();
+        if (*fault) {                          // (nobody sets it any more) no row that this CTA had may pass for a result
+            const int pieces = P.group * D / 8;
+            for (int k = 0; deal(k); k++)
+                for (int r = 0; r < it.nq; r++) {
+                    uint4* row = reinterpret_cast<uint4*>(P.out + ((size_t)(it.q0 + r) * P.ldo + (size_t)it.h * P.group * D) * 2);
+                    for (int x = lane; x < pieces; x += 32) row[x] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+                }
+        }
     } else if (warp == kScores || warp == kValues) {
         // ---------------- products ----------------
         // A warp for S and one for P V, so that the waits of one pass under the products of the other.  The whole warp walks, one lane
@@ -432,7 +448,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         while (next_item()) {
             const int n[2] = {__shfl_sync(~0u, items[seen % kItems].n[0], 0), __shfl_sync(~0u, items[seen % kItems].n[1], 0)}, most = max(n[0], n[1]);
             if (warp == kScores) {
-                for (int i = 0; i < most && !*fault; i++) {
+                for (int i = 0; i < most && !failed(); i++) {
                     const uint32_t part = parts + i, slot = 2 * (part % L::kSlots);
                     const uint64_t b = kd + (uint64_t)(slot * (uint32_t)(L::kPart >> 4));
                     wait(&full[slot], part / L::kSlots & 1u);
@@ -457,7 +473,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                     __syncwarp();
                 }
             } else {
-                for (int i = 0; i < most && !*fault; i++) {
+                for (int i = 0; i < most && !failed(); i++) {
                     const uint32_t part = parts + i, place = part % L::kSlots, slot = 2 * place + 1;
                     const uint64_t b = vd + (uint64_t)(slot * (uint32_t)(L::kPart >> 4));
                     wait(&clean[place], part / L::kSlots & 1u);
@@ -490,6 +506,8 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             if (!mbar_wait(&drained[warp - kScores], 0, P.wait_ns)) *fault = 1;
         }
         __syncwarp();
+        finish();
+        if (warp == kScores) tmem_dealloc(tmem, 512);
     } else if (warp == kLooker) {
         // ---------------- infinities and NaN among V rows that not all rows see ----------------
         fewer();
@@ -497,7 +515,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         while (next_item()) {
             it = items[seen % kItems];
             const int n = max(it.n[0], it.n[1]);
-            for (int i = 0; i < n && !*fault; i++, part++) {
+            for (int i = 0; i < n && !failed(); i++, part++) {
                 const uint32_t place = part % L::kSlots, slot = 2 * place + 1;
                 wait_asleep(&full[slot], part / L::kSlots & 1u);
                 if (i * kKT + kKT - 1 > it.off) {
@@ -525,6 +543,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             }
             item_done();
         }
+        finish();
     } else {
         // ---------------- softmax and output ----------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
@@ -632,7 +651,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                 tc_fence_after();
             }
             it = *item;
-            const bool failed = *fault != 0, live = placed && token < it.nq;
+            const bool live = placed && token < it.nq;
             const bool odd = live && *(const volatile int*)&item->odd != 0;
             const float inv = l == 0.f ? 0.f : 1.0f / l;
             uint8_t* dst = P.out + ((size_t)(it.q0 + token) * P.ldo + (size_t)(it.h * P.group + head) * D + half * (D / 2)) * 2;
@@ -654,7 +673,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                 uint32_t b[8];
                 #pragma unroll
                 for (int x = 0; x < 8; x++) {
-                    const float y = failed ? NAN : sees < 0 ? 0.f : o[2 * x] * inv, z = failed ? NAN : sees < 0 ? 0.f : o[2 * x + 1] * inv;
+                    const float y = sees < 0 ? 0.f : o[2 * x] * inv, z = sees < 0 ? 0.f : o[2 * x + 1] * inv;
                     b[x] = pack2<BF>(y, z);
                 }
                 if (live) {
@@ -670,10 +689,8 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             tc_fence_before();
             item_done();
         }
+        finish();
     }
-    tc_fence_before();
-    __syncthreads();
-    if (warp == kScores) tmem_dealloc(tmem, 512);
 }
 
 }  // namespace pr

@@ -539,6 +539,28 @@ def test_prompt_reports_a_wait_that_ran_out(qb, dim):
     _check_prompt(qb, q, k, v, [0, 300], None, 0.1)
 
 
+@pytest.mark.parametrize("part,item", [(0, 1), (3, 2), (6, 4)])
+def test_prompt_wait_that_ran_out_in_a_later_item(qb, part, item):
+    """One-tile prompts, a few blocks more than others with the item whose part is never announced: every row of those blocks is NaN, those
+    of the items before it too, and every other row is right."""
+    import torch
+    blocks = torch.cuda.get_device_properties(0).multi_processor_count
+    n = (item - 1) * blocks + 40
+    q, k, v = _rows(14, 5 * n, 2, 5 * n, 1, 64, torch.bfloat16)
+    starts = list(range(0, 5 * n + 1, 5))
+    want = _prompt(qb, q, k, v, starts, None, 0.1)
+    qb.debug_draft_wait(5_000_000, part)
+    try:
+        got = _prompt(qb, q, k, v, starts, None, 0.1)
+    finally:
+        qb.debug_draft_wait()
+    gone = got.isnan()
+    assert torch.equal(torch.where(gone, 0, got), torch.where(gone, 0, want))
+    rows = gone.view(n, -1)
+    assert bool((rows.all(1) | ~rows.any(1)).all()) and int(rows.any(1).sum()) == 40 * item
+    assert torch.equal(_prompt(qb, q, k, v, starts, None, 0.1), want)
+
+
 # ---------------------------------------------------------------------------
 # attention over pages
 # ---------------------------------------------------------------------------
