@@ -60,6 +60,7 @@ struct Params {
     long long ldv, ldo;
     int n_seqs, n_rows, n_keys, n_kv_heads, group, tokens;   // tokens: of a row tile
     int out32;                            // rows of out start on 32 bytes
+    long long items;                      // no more than these are dealt out: as many as starts in order can have
     int withheld;
     unsigned long long wait_ns;
     float scale_log2;
@@ -191,15 +192,17 @@ struct Finder {
         f = max(nk - nq, 0) / per;
         c = (nq + per - 1) / per;
     }
-    // the tiles above level L
+    // the tiles above level L.  A lane's count ends at 2^26 - 1: what memory holds has fewer tiles, starts that overlap may name more than
+    // 32 bits count, and a rank below 0 would be looked for in front of the starts.
     __device__ __forceinline__ int above(const Params& P, int L) const {
+        constexpr int kMost = (1 << 26) - 1;
         int n = 0;
         #pragma unroll
-        for (int i = 0; i < kHeld; i++) n += min(max(first[i] + count[i] - L, 0), count[i]);
+        for (int i = 0; i < kHeld; i++) n = min(n + min(max(first[i] + count[i] - L, 0), count[i]), kMost);
         for (int s = 32 * kHeld + (threadIdx.x & 31); s < P.n_seqs; s += 32) {
             int f, c;
             levels(P, s, f, c);
-            n += min(max(f + c - L, 0), c);
+            n = min(n + min(max(f + c - L, 0), c), kMost);
         }
         return __reduce_add_sync(~0u, n);
     }
@@ -362,7 +365,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             const long long at = (long long)k * G + (k & 1 ? G - 1 - (int)blockIdx.x : (int)blockIdx.x);   // forwards and backwards
             int seq = 0, tile = 0, q0, nq, k0, nk;
             it = {};
-            if (at / P.n_kv_heads >= 0x7fffffff || !finder.find(P, (int)(at / P.n_kv_heads), seq, tile)) return false;
+            if (at >= P.items || !finder.find(P, (int)(at / P.n_kv_heads), seq, tile)) return false;
             finder.bounds(P, seq, q0, nq, k0, nk);
             it.h = (int)(at % P.n_kv_heads);
             it.q0 = q0 + tile * finder.per;

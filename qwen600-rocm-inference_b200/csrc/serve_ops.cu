@@ -311,8 +311,8 @@ extern "C" int qwen_prompt_attention(const void* q, const void* k, const void* v
     P.withheld = qwen_internal_withheld();
     P.wait_ns = qwen_internal_wait_ns();
     P.scale_log2 = scale * 1.4426950408889634f;
-    const long long most = ((long long)(n_rows + 2 * tokens - 1) / (2 * tokens) + n_seqs) * n_kv_heads;   // items
-    const int grid = (int)std::min((long long)nsm, most);
+    P.items = ((long long)(n_rows + 2 * tokens - 1) / (2 * tokens) + n_seqs) * n_kv_heads;
+    const int grid = (int)std::min((long long)nsm, P.items);
     const cudaStream_t st = (cudaStream_t)stream;
     if (head_dim == 64) return dtype == QWEN_BF16 ? prompt_launch<QWEN_BF16, 64>(mq, mk, mv, P, grid, dev, st) : prompt_launch<QWEN_FP16, 64>(mq, mk, mv, P, grid, dev, st);
     return dtype == QWEN_BF16 ? prompt_launch<QWEN_BF16, 128>(mq, mk, mv, P, grid, dev, st) : prompt_launch<QWEN_FP16, 128>(mq, mk, mv, P, grid, dev, st);

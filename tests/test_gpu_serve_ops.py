@@ -449,6 +449,17 @@ def test_prompt_starts_of_any_value(qb, starts, k_starts):
             assert torch.equal(got[a:b], alone)
 
 
+def test_prompt_starts_that_overlap(qb):
+    """Hundreds of sequences over the same rows, many times the work that starts in order can name: the call ends, writes nothing
+    outside its rows, and the next one is right."""
+    import torch
+    n = 5000
+    q, k, v = _rows(15, n, 2, n, 1, 64, torch.bfloat16)
+    got = _prompt(qb, q, k, v, [0, n] * 300, None, 0.1, pad=8, behind=3)
+    assert bool((got.isfinite()).all())
+    _check_prompt(qb, q, k, v, [0, n], None, 0.1)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("what", ["nan", "inf", "lowest"])
 def test_prompt_unseen_values_do_not_matter(qb, dtype, what):
