@@ -587,7 +587,7 @@ int qwen_qk_rope(const void* q, const void* k, const void* v, int dtype, long lo
  * n_rows and 0 .. n_keys; what lies beyond counts as the nearest end, and a sequence whose
  * start lies behind its end has no rows or keys; where sequences share rows, some rows may stay as they
  * were).  Rows that belong to no sequence stay as they were.  o = sum_j softmax_j(scale * q . k_j) v_j with scores, softmax statistics and sums in fp32; the
- * weights enter the product with V in 16 bits.  What a query does not see (NaN included) has
+ * weights enter the product with V in 16 bits (in fp16 those below 2^-32 of the largest vanish).  What a query does not see (NaN included) has
  * no influence on it.  scale is finite, below 2^127 in magnitude.  Device-side waits are bounded:
  * where one of a thread block runs out, all rows of the items that the block had, of the call's rows a
  * part, are NaN for the items' heads; the others are right. */

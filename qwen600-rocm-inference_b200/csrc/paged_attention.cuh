@@ -12,7 +12,7 @@
 // exponentials, half the registers of O.  P^T reaches the second product by one 8 x 8
 // transposition in registers (movmatrix) each.  A warp owns KW keys of a tile, its own ring
 // of cp.async stages, its own sums l and O, and a base for each head that exponents
-// are taken from: it rises only when a score lies 2^8 above it (base-2 exponents), so the tiles
+// are taken from: it rises only when the maximum has risen by 2^8 (base-2 exponents), so the tiles
 // in between need one vote instead of a maximum over the warp.  The page numbers of
 // a tile are loaded a tile before its rows.  Weights are rounded to 16 bits for the product
 // with V (off by half a step, 2^-8 or 2^-11 relative); l sums them unrounded.
@@ -44,7 +44,7 @@ using ta::swz;
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kItemCost = 2;   // what an item costs beside its tiles, in tiles
 constexpr int kCluster = 8;    // CTAs that share an item
-constexpr float kRise = 8.0f;  // weights stay below 2^8
+constexpr float kRise = 8.0f;  // a base follows when the maximum has risen by 2^8
 
 struct Params {
     ta::Params t;    // cache.capacity: positions that a table names; q, out, lens, work, shares
@@ -88,6 +88,9 @@ template <int QT, int STORE, int D, int NT>
 __global__ void __launch_bounds__(kThreads, 2) paged_kernel(const __grid_constant__ Params PP) {
     using L = Layout<STORE, D, NT>;
     constexpr bool BF = QT == QWEN_BF16 && !L::k8;       // type of the products
+    // A base lies this far below the maximum that it was taken from: fp16 weights use the range up to 2^15, so that what is lost under
+    // fp16's smallest steps is 2^-32 of the largest (of 8-bit caches: times the unit over the value's scale) and less.
+    constexpr float kLift = BF ? 0.0f : 7.0f;
     constexpr int KW = L::KW, KB = KW / 16, KS = D / 16, kStages = L::kStages;
     constexpr int DT = D / 16;                           // tiles of 16 dims
     extern __shared__ __align__(128) uint8_t smem[];
@@ -288,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_kernel(const __grid_constan
                         #pragma unroll
                         for (int kb = 0; kb < KB; kb++) m = fmaxf(m, fmaxf(s[kb][n][e], s[kb][n][2 + e]));
                         mx[n][e] = m;
-                        rise |= m * c[n][e] > base[n][e] + kRise;
+                        rise |= fmaf(m, c[n][e], -kLift) > base[n][e] + kRise;
                     }
                 uint32_t up = 0;                            // the rise of ve
                 if constexpr (L::k8) {
@@ -308,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_kernel(const __grid_constan
                             float m = mx[n][e];
                             #pragma unroll
                             for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, x));
-                            const float to = fmaxf(base[n][e], m == -INFINITY ? m : m * c[n][e]);
+                            const float to = fmaxf(base[n][e], m == -INFINITY ? m : fmaf(m, c[n][e], -kLift));
                             f[e] = to == -INFINITY ? 1.0f : exp2_approx(base[n][e] - to);
                             base[n][e] = to;
                             l[n][e] *= f[e];
@@ -374,7 +377,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_kernel(const __grid_constan
         __syncthreads();    // the rings are free: the warps' results go over them
         float* join = reinterpret_cast<float*>(smem);               // [warp][head][kPitch], then [warp][head][2]
         float* join_ml = join + kWarps * L::kRows * L::kPitch;
-        const float unit_v = L::k8 ? __uint_as_float(ve << 23) : 1.0f;
+        constexpr float kDown = BF ? 1.0f : 0x1p-7f;                // as if from the maximum itself: O and l 2^-kLift
+        const float unit_v = L::k8 ? __uint_as_float(ve << 23) * kDown : kDown;
         #pragma unroll
         for (int n = 0; n < NT; n++)
             #pragma unroll
@@ -384,8 +388,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_kernel(const __grid_constan
                 for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(~0u, sum, x);
                 const int row = warp * L::kRows + 8 * n + 2 * j + e;
                 if (g == 0) {
-                    join_ml[row * 2] = base[n][e];
-                    join_ml[row * 2 + 1] = sum;
+                    join_ml[row * 2] = base[n][e] + kLift;
+                    join_ml[row * 2 + 1] = sum * kDown;
                 }
                 #pragma unroll
                 for (int d = 0; d < DT; d++) {

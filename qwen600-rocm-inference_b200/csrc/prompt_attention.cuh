@@ -6,7 +6,7 @@
 // Mathematics.  Query i of a sequence with n queries and m keys sees keys 0 .. m - n +
 // i.  One pass over tiles of 128 keys with the running maximum and sum of the softmax
 // (base 2, scale * log2 e folded into the exponent): S = Q K^T, P = 2^(S c - base), O += P
-// V.  A row's base follows its maximum only when that lies 2^8 above it, so O is seldom scaled; O
+// V.  A row's base follows its maximum only when that has risen by 2^8, so O is seldom scaled; O
 // / l at the end.
 //
 // A row of a tile is a (token, query head) pair of one K/V head, head fastest: T = 128 /
@@ -260,6 +260,9 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     using namespace qb::tc;
     using L = Layout<D>;
     constexpr bool BF = T == QWEN_BF16;
+    // fp16 weights lie below 2^15: the largest one has at least 2^7, so what is lost under fp16's smallest steps is 2^-32 of it and less
+    // (with 2^0, 8,000 keys of 2^-25 each were nothing).  bf16 has fp32's range.
+    constexpr float kLift = BF ? 0.0f : 7.0f;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBar);   // [kRing] a K or V part has arrived
@@ -595,7 +598,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                 mine[swaps % 2 * 256] = top;
                 named_bar(2 + w, 256);
                 top = fmaxf(top, other[swaps % 2 * 256]);
-                const float want = top == -INFINITY ? top : top * c;       // an all-masked tile stays -inf
+                const float want = top == -INFINITY ? top : fmaf(top, c, -kLift);   // an all-masked tile stays -inf
                 const bool move = want > base + 8.0f;                      // (from -inf: the first tile that has a key)
                 float f = 1.0f;
                 if (move) {

@@ -536,6 +536,28 @@ def test_prompt_long_items_are_not_waits_that_run_out(qb):
     assert torch.equal(got, want)
 
 
+# One key with the weight 1, 8,191 with 2^-tail each and large values: the weights enter the product in fp16, whose steps
+# below 2^-14 are 2^-24, in a unit of at most 2^-7 of the largest weight (8-bit pages: divided by the value's scale, at least a half of the
+# unit's); half a step off each, beside the relative roundings: weight and result 2^-11 each, 2^-18 for exponents and sums.
+def _far_tail(tail, eight_bits):
+    keys, value = 8192, 512.0
+    total = 1 + (keys - 1) * 2.0 ** -tail
+    want = (keys - 1) * 2.0 ** -tail * value / total
+    return keys, value, want, want * (2.0 ** -10 + 2.0 ** -18) + 2.0 ** -32 * keys * value * (2 if eight_bits else 1) + 2.0 ** -25
+
+
+@pytest.mark.parametrize("tail", [12.0, 20.0, 24.5, 25.0, 28.0])
+@pytest.mark.parametrize("first", [0, 100, 8191])
+def test_prompt_many_small_weights_in_fp16(qb, tail, first):
+    import torch
+    keys, value, want, tol = _far_tail(tail, False)
+    q = torch.zeros(1, 1, 64, dtype=torch.float16, device="cuda")
+    k, v = torch.zeros(keys, 1, 64, dtype=torch.float16, device="cuda"), torch.full((keys, 1, 64), value, dtype=torch.float16, device="cuda")
+    q[..., 3], k[..., 3], k[first], v[first] = 1, -tail, 0, 0
+    got = _prompt(qb, q, k, v, [0, 1], [0, keys], math.log(2))
+    assert bool(((got.double() - want).abs() <= tol).all()), (float(got[0, 0, 0]), want)
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 def test_prompt_reports_a_wait_that_ran_out(qb, dim):
     """K and V that are never announced: the bounded waits end, the call's rows are NaN, and the next call is right."""
@@ -718,6 +740,28 @@ def test_paged_large_scores(qb, store):
         q = (torch.randn(1, 4, 128, generator=g, device="cuda") * size).bfloat16()
         _check_paged(qb, pool, q, [1270], 0.5 / size)
         _check_paged(qb, pool, q, [1270], -0.5 / size)
+
+
+@pytest.mark.parametrize("tail", [12.0, 20.0, 24.5, 25.0, 28.0])
+@pytest.mark.parametrize("store", ["fp16", "e4m3", "int8"])
+@pytest.mark.parametrize("copies", [1, 40])
+def test_paged_many_small_weights_in_fp16(qb, store, tail, copies):
+    """Alone (a cluster, or shares of the line, an item) and 40 at once."""
+    import torch
+    keys, value, want, tol = _far_tail(tail, store != "fp16")
+    pool = Pool(qb, np.tile(np.arange(keys // 64), (copies, 1)), keys // 64, 1, 64, 64, store)
+    one = 1.0 if store == "fp16" else TOP[store]            # 8 bits: code times scale
+    pool.k.copy_(torch.zeros(pool.k.shape, device="cuda"))
+    pool.v.copy_(torch.full(pool.v.shape, value if store == "fp16" else one, device="cuda"))
+    pool.k[..., 3] = torch.tensor(-tail if store == "fp16" else -one, device="cuda").to(pool.dtype)
+    pool.k[1, 0, 36], pool.v[1, 0, 36] = (torch.zeros(64, device="cuda").to(pool.dtype) for _ in range(2))
+    if store != "fp16":
+        pool.ks.fill_(tail / one)
+        pool.vs.fill_(value / one)
+    q = torch.zeros(copies, 2, 64, dtype=torch.float16, device="cuda")
+    q[..., 3] = 1
+    got = _attend(qb, pool, q, [keys - 1] * copies, math.log(2))
+    assert bool(((got.double() - want).abs() <= tol).all()), (float(got[0, 0, 0]), want)
 
 
 def test_paged_beyond_32_bit_offsets(qb):
