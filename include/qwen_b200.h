@@ -569,7 +569,7 @@ typedef struct {
  * with pages not NULL, k and v to their pages, 8-bit ones quantised by qwen_kv_append's rule
  * (k from its fp32 values).  Without pages v and seqs are not read and may be NULL.  Tokens
  * whose sequence, position or page is not there reach no page; rows with a negative
- * position are left out altogether.  No two rows may have the same place in the pages.
+ * position are left out altogether.  q_out and k_out lie apart from each other and from what is read.  No two rows may have the same place in the pages.
  * eps is finite and not negative, base finite and at least 1. */
 int qwen_qk_rope(const void* q, const void* k, const void* v, int dtype, long long ldq, long long ldk, long long ldv, int n_rows,
                  int n_heads, int n_kv_heads, int head_dim, const void* q_gain, const void* k_gain, int gain_dtype, float eps, double base,

@@ -31,13 +31,18 @@ struct Ptr {
     size_t align;
     bool used;   // false: may be anything
 };
-// NULL and alignment first (no GPU needed), then: device memory of the current device, *dev.
-int check_ptrs(std::initializer_list<Ptr> ptrs, int* dev) {
+// NULL and alignment (no GPU needed).
+int check_places(std::initializer_list<Ptr> ptrs) {
     for (const Ptr& a : ptrs) {
         if (!a.used) continue;
         if (!a.p) return fail(QWEN_E_ARG, std::string(a.name) + " is NULL");
         if ((uintptr_t)a.p % a.align) return fail(QWEN_E_ARG, std::string(a.name) + " must be " + std::to_string(a.align) + "-byte aligned");
     }
+    return QWEN_OK;
+}
+// These first, then: device memory of the current device, *dev.
+int check_ptrs(std::initializer_list<Ptr> ptrs, int* dev) {
+    TRY(check_places(ptrs));
     CU(cudaGetDevice(dev));
     for (const Ptr& a : ptrs) {
         if (!a.used) continue;

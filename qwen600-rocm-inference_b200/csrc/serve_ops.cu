@@ -73,7 +73,7 @@ qb::pg::Pages device_pages(const qwen_kv_pages_t* c) {
 // ---- norms, rotation, rows to pages ----------------------------------------------
 template <int SRC, int D>
 int rope_launch(const qb::pg::RopeParams& P, cudaStream_t st) {
-    const int blocks = (P.n_rows + P.tokens - 1) / P.tokens;
+    const int blocks = (P.n_rows - 1) / P.tokens + 1;
     if (is8(P.store)) qb::pg::qk_rope_kernel<SRC, D, true><<<blocks, qb::pg::kRopeThreads, 0, st>>>(P);
     else qb::pg::qk_rope_kernel<SRC, D, false><<<blocks, qb::pg::kRopeThreads, 0, st>>>(P);
     CU(cudaGetLastError());
@@ -222,9 +222,14 @@ extern "C" int qwen_qk_rope(const void* q, const void* k, const void* v, int dty
         if (pages->n_kv_heads != n_kv_heads || pages->head_dim != head_dim) return fail(QWEN_E_ARG, "the pages' heads are not the rows'");
     }
     int dev = 0, nsm = 0;
-    TRY(check_ptrs({{q, "q", 16, true}, {k, "k", 16, true}, {v, "v", 16, pages != nullptr}, {q_gain, "q_gain", 4, q_gain != nullptr},
-                    {k_gain, "k_gain", 4, k_gain != nullptr}, {positions, "positions", 4, true}, {q_out, "q_out", 16, true}, {k_out, "k_out", 16, k_out != nullptr},
-                    QB_PAGES_PTRS(c, pages != nullptr), {seqs, "seqs", 4, pages != nullptr}}, &dev));
+    const std::initializer_list<Ptr> ptrs = {{q, "q", 16, true}, {k, "k", 16, true}, {v, "v", 16, pages != nullptr}, {q_gain, "q_gain", 4, q_gain != nullptr},
+                                             {k_gain, "k_gain", 4, k_gain != nullptr}, {positions, "positions", 4, true}, {q_out, "q_out", 16, true},
+                                             {k_out, "k_out", 16, k_out != nullptr}, QB_PAGES_PTRS(c, pages != nullptr), {seqs, "seqs", 4, pages != nullptr}};
+    TRY(check_places(ptrs));
+    for (const void* out : {q_out, k_out})
+        if (out && (out == q || out == k || (pages && out == v))) return fail(QWEN_E_ARG, "q_out and k_out must not be q, k or v");
+    if (q_out == k_out) return fail(QWEN_E_ARG, "q_out must not be k_out");
+    TRY(check_ptrs(ptrs, &dev));
     TRY(sm_count(dev, &nsm));
     qb::pg::RopeParams P;
     P.q = (const uint8_t*)q;

@@ -50,6 +50,20 @@ def test_bad_rope(qb, over, code):
     _raises(qb, code, qb.qk_rope, *{**ROPE, **over}.values(), _view(qb), OK_PTR)
 
 
+@pytest.mark.parametrize("out,other,paged", [("q_out", "q", True), ("q_out", "k", True), ("q_out", "v", True), ("k_out", "q", True), ("k_out", "k", True), ("k_out", "v", True),
+                                             ("q_out", "k_out", True), ("q_out", "q", False), ("k_out", "k", False), ("q_out", "k_out", False)])
+def test_rope_outputs_apart(qb, out, other, paged):
+    """Outputs in the place of an input, or of each other; apart, the call gets as far as the device."""
+    apart = {**ROPE, **{n: OK_PTR + (i << 20) for i, n in enumerate(("q", "k", "v", "q_out", "k_out"))}}
+    pages = (_view(qb), OK_PTR) if paged else ()
+    with pytest.raises(qb.QwenError) as e:
+        qb.qk_rope(*{**apart, out: apart[other]}.values(), *pages)
+    assert e.value.code == -1 and "must not be" in str(e.value)
+    with pytest.raises(qb.QwenError) as e:
+        qb.qk_rope(*apart.values(), *pages)
+    assert "must not be" not in str(e.value)
+
+
 def test_bad_rope_pages(qb):
     _raises(qb, -1, qb.qk_rope, *ROPE.values(), _view(qb), 0)
     _raises(qb, -1, qb.qk_rope, *ROPE.values(), _view(qb, n_kv_heads=1), OK_PTR)
