@@ -588,7 +588,8 @@ int qwen_qk_rope(const void* q, const void* k, const void* v, int dtype, long lo
  * start lies behind its end has no rows or keys; where sequences share rows, some rows may stay as they
  * were).  Rows that belong to no sequence stay as they were.  o = sum_j softmax_j(scale * q . k_j) v_j with scores, softmax statistics and sums in fp32; the
  * weights enter the product with V in 16 bits (in fp16 those below 2^-32 of the largest vanish).  What a query does not see (NaN included) has
- * no influence on it.  scale is finite, below 2^127 in magnitude.  Device-side waits are bounded:
+ * no influence on it; an infinity that it does see, among V, makes its column infinite or NaN (NaN where the weight is 0 in 16 bits),
+ * and where all its scores are -inf it gets zeros.  scale is finite, below 2^127 in magnitude.  Device-side waits are bounded:
  * where one of a thread block runs out, all rows of the items that the block had, of the call's rows a
  * part, are NaN for the items' heads; the others are right. */
 int qwen_prompt_attention(const void* q, const void* k, const void* v, void* out, int dtype, long long ldq, long long ldk, long long ldv,
@@ -603,7 +604,7 @@ int qwen_paged_attention_workspace(const qwen_kv_pages_t* pages, int n_heads, si
  * [n_seqs][n_heads][head_dim], rows ldq and ldo elements apart; types, head layout, scale,
  * roundings and workspace are as for qwen_tree_attention with a single node, 8-bit caches
  * included.  Positions whose page is not there are left out.  lens[s] < 0 or beyond the
- * table, and sequences without any page, give zeros. */
+ * table, sequences without any page and scores that are all -inf give zeros. */
 int qwen_paged_attention(const qwen_kv_pages_t* pages, const void* q, void* out, int dtype, long long ldq, long long ldo, int n_heads,
                          const int* lens, float scale, void* workspace, size_t workspace_bytes, void* stream);
 
@@ -615,7 +616,7 @@ int qwen_paged_attention(const qwen_kv_pages_t* pages, const void* q, void* out,
  * top_ids and top_logprobs, [n_rows][n_top]; places beyond the vocabulary hold -1 and -inf.  Logits of
  * -inf are tokens that cannot come.  A row with a NaN, a +inf or nothing above -inf has no
  * distribution: NaN, ids -1.  temperature is within 1e-6 .. 1e6.  Sums are fp32, in
- * parts of at most 32 terms a step; the logarithms and differences behind them fp64. */
+ * parts of at most 32 terms a step, and so is the factor 1 / temperature; the logarithms and differences behind them are fp64. */
 int qwen_token_logprobs(const void* logits, int dtype, long long ld, int n_rows, int vocab, const int* tokens, float temperature, int n_top,
                         float* logprob, float* entropy, int* top_ids, float* top_logprobs, void* stream);
 

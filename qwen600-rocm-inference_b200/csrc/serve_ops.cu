@@ -111,10 +111,14 @@ int prompt_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMa
 
 // ---- attention over pages ------------------------------------------------------------
 // A CTA for each item, a cluster of eight for each, or shares of the line of tiles.  A cluster needs one launch, its parts are joined through distributed
-// shared memory, but eight CTAs an item leave others idle: clusters where the items' CTAs all fit at once, for tables of up to 32 tiles, or of 96
-// where the items' CTAs are more than half of those that fit.  Measured, clusters / shares, 8 K/V heads of 128, bf16 (tiles of 64): 1 sequence of 500
-// 5.7 / 6.6 us, of 1000 6.8 / 7.6, of 2000 8.5 / 9.5, of 4000 11.9 / 11.6, of 8000 19.1 / 15.8; 4 of 1000 8.1 / 9.8, of 4000 17.2 / 19.6, of 8000
-// 27.7 / 29.8, of 16000 50.0 / 51.9; e4m3 (tiles of 128): 1 of 2000 7.5 / 8.2, of 8000 14.1 / 12.6; 4 of 8000 19.4 / 21.9, of 16000 33.2 / 33.0.
+// shared memory, but eight CTAs an item leave others idle, and where lengths differ the longest sequence has no more than its eight.  So clusters
+// where the items' CTAs all fit at once, for tables of up to 32 tiles, or of 96 where the items' CTAs are more than half of those that fit.  (The
+// host knows the tables' width, not the lengths: short sequences in a wide table take the shares' two launches.)
+// Measured, clusters / shares, 8 K/V heads of 128, rows in the L2.  bf16 (tiles of 64): 1 sequence of 1000 5.9 / 7.6 us, of 2000 7.4 / 9.5, of 4000
+// 10.7 / 11.6, of 8000 17.1 / 14.0; 4 of 4000 13.6 / 15.8, of 6000 18.2 / 20.0, of 16000 49.1 / 51.4, but 4 of which three are half as long: 4000 12.2 /
+// 13.1, 6000 16.2 / 15.3, 16000 38.7 / 35.1, and a sixteenth: 4000 11.3 / 12.0, 6000 14.7 / 13.3, 16000 30.8 / 18.5.  e4m3 (tiles of 128): 1 of
+// 4000 8.1 / 10.1, of 8000 12.4 / 12.4; 4 of 8000 16.2 / 18.7, of 12000 22.2 / 24.6, three of them half as long 14.1 / 15.1 and 19.5 / 17.8, a
+// sixteenth 13.0 / 13.4 and 17.3 / 14.8.
 struct PagedPlan : Plan {
     int cluster;   // 0: none
 };

@@ -536,6 +536,22 @@ def test_prompt_long_items_are_not_waits_that_run_out(qb):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_scores_that_are_all_minus_infinity(qb, dtype):
+    """A query whose scores are all -inf gets zeros, from prompts and from pages; one with a single score above -inf gets that key's values."""
+    import torch
+    dtype = _types(qb)[dtype][1]
+    q, k, v = _rows(16, 200, 2, 200, 1, 64, dtype)
+    q[..., 1], k[..., 1] = 1, -math.inf
+    k[150, 0, 1] = 2
+    got = _prompt(qb, q, k, v, [0, 200], None, 0.1)
+    assert bool((got[:150] == 0).all()) and torch.equal(got[150:], v[150:151].expand(50, 2, 64))
+    pool = Pool(qb, [[0, 1], [0, 1]], 2, 1, 128, 64, "bf16" if dtype == torch.bfloat16 else "fp16").fill(_gen(1))
+    pool.k[0, 0], pool.k[1, 0, :72] = k[:128, 0], k[128:, 0]
+    got = _attend(qb, pool, q[:2].contiguous(), [140, 190], 0.1)
+    assert bool((got[0] == 0).all()) and torch.equal(got[1], pool.v[1, 0, 22].expand(2, 64))
+
+
 # One key with the weight 1, 8,191 with 2^-tail each and large values: the weights enter the product in fp16, whose steps
 # below 2^-14 are 2^-24, in a unit of at most 2^-7 of the largest weight (8-bit pages: divided by the value's scale, at least a half of the
 # unit's); half a step off each, beside the relative roundings: weight and result 2^-11 each, 2^-18 for exponents and sums.
@@ -1097,6 +1113,36 @@ def test_captured_step_follows_its_inputs(qb, store):
             assert torch.equal(s[n], plain[n]), n
         for a, b in zip(s["pool"].raw(), plain["pool"].raw()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("store", ["bf16", "int8"])
+def test_captured_clusters_follow_their_inputs(qb, store):
+    """Attention by clusters (few sequences, no workspace), captured once and replayed with other lengths, tables and queries."""
+    import torch
+    rng, g = np.random.RandomState(21), _gen(21)
+    b, kv, heads, dim, page, most = 2, 4, 12, 128, 16, 2000
+    table, pages = _table(rng, [most] * b, page)
+    pool = Pool(qb, table, pages, kv, page, dim, store).fill(g)
+    assert qb.paged_attention_workspace(pool.view, heads) == 0
+    q, out, lens = torch.zeros(b, heads * dim, device="cuda").bfloat16(), torch.empty(b, heads * dim, device="cuda").bfloat16(), _dev([0, 0])
+    call = lambda o, st: qb.paged_attention(pool.view, q.data_ptr(), o.data_ptr(), qb.BF16, heads * dim, heads * dim, heads, lens.data_ptr(), 0.09, 0, 0, st)  # noqa: E731
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    call(out, stream.cuda_stream)
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        call(out, torch.cuda.current_stream().cuda_stream)
+    for n in ([1999, 3], [-1, 700], [63, 1024], [2 ** 30, 0]):
+        q.copy_(torch.randn(q.shape, generator=g, device="cuda"))
+        lens.copy_(_dev(n))
+        pool.table = table[:, rng.permutation(table.shape[1])]
+        pool.table_dev.copy_(_dev(pool.table))
+        out.fill_(7)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.view(b, heads, dim), _check_paged(qb, pool, q.view(b, heads, dim), n, 0.09))
 
 
 def test_two_streams_and_repeats(qb):
