@@ -38,6 +38,7 @@ using ta::cp_async_commit;
 using ta::cp_async_wait;
 using ta::exp2_approx;
 using ta::fma2;
+using ta::kLeast;
 using ta::mul2;
 using ta::swz;
 
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_kernel(const __grid_constan
                         for (int b = 0; b < 2; b++) qb[n][k][b] = kv::half2_bits(bf_lo(qb[n][k][b]) * down, bf_hi(qb[n][k][b]) * down);
                     f = a * __uint_as_float((uint32_t)e << 23);
                 }
-                f = fmaxf(f, 1e-37f);                                       // (above 0: -inf * 0 would be NaN)
+                f = fmaxf(f, kLeast);                                       // (above 0: -inf * 0 would be NaN)
                 c[n][0] = __shfl_sync(~0u, f, 8 * j);                       // head 2j is lanes 8j .. 8j + 3
                 c[n][1] = __shfl_sync(~0u, f, 8 * j + 4);
             }

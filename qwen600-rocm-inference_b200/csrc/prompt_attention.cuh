@@ -44,6 +44,7 @@ namespace qb {
 namespace pr {
 
 using ta::exp2_approx;
+using ta::kLeast;
 using ta::max3;
 using ta::mul2;
 using ta::pack2;
@@ -557,7 +558,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, ts = tmem + lanes + 64 * half, tp = tmem + lanes + 128 + 64 * w + 32 * half, to = tmem + lanes + 256 + 128 * w + half * (D / 2);
         const int token = w * P.tokens + rl / P.group, head = rl % P.group;
         const bool placed = rl < P.tokens * P.group;
-        const float c = fmaxf(fabsf(P.scale_log2), 1e-37f);                // (above 0: -inf * 0 would be NaN)
+        const float c = fmaxf(fabsf(P.scale_log2), kLeast);                // (above 0: -inf * 0 would be NaN)
         const bool flip = P.scale_log2 < 0.f;
         float* mine = reinterpret_cast<float*>(smem + L::kXm) + w * 512 + half * 128 + rl;   // + 256 for odd steps
         const float* other = reinterpret_cast<const float*>(smem + L::kXm) + w * 512 + (half ^ 1) * 128 + rl;

@@ -31,6 +31,8 @@ namespace qb {
 namespace ta {
 
 constexpr int kMaxNodes = 64;
+// A score's factor is at least this: above 0, as -inf * 0 would be NaN, and too small for any product of a query and a key to show.
+constexpr float kLeast = 0x1p-149f;
 
 struct Params {
     kv::Cache cache;
@@ -537,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, attention_ctas(16 * MT, D)) attentio
         #pragma unroll
         for (int i = 0; i < 2 * MT; i++) {
             const float a = fabsf(P.scale_log2);
-            c[i] = fmaxf(L::k8 ? a * qf[16 * (i >> 1) + g + 8 * (i & 1)] : a, 1e-37f);
+            c[i] = fmaxf(L::k8 ? a * qf[16 * (i >> 1) + g + 8 * (i & 1)] : a, kLeast);
         }
         uint32_t qa[MT == 1 ? KS : 1][4];   // one block of rows: its fragments stay in registers
         auto q_frag = [&](int mt, int ks, uint32_t (&a)[4]) {

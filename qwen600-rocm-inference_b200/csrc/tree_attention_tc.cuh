@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_tc_kernel(const Param
             tc_fence_before();
             named_bar(1, kTcSoftmax + 32);                                 // the masks are there; every thread is behind the item before
             if (tid == 0) odd[(item - 1) & 7] = 0;
-            const float c = fmaxf(fabsf(P.scale_log2) * (L::k8 && QT == QWEN_BF16 ? qf[rl] : 1.0f), 1e-37f);   // (above 0: -inf * 0 would be NaN)
+            const float c = fmaxf(fabsf(P.scale_log2) * (L::k8 && QT == QWEN_BF16 ? qf[rl] : 1.0f), kLeast);   // (above 0: -inf * 0 would be NaN)
             const uint64_t see = live ? anc[node] : 0;
             __syncwarp();
             if (lane == 0) mbar_arrive(qfull);

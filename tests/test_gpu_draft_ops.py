@@ -536,6 +536,18 @@ def test_attention_extreme_values(qb, store):
         _check_attention(qb, c, q, [250, 291], _tree(np.random.RandomState(2), 2, 9), scale)
 
 
+@pytest.mark.parametrize("scale", [0.0, 2e-38, -2e-38])
+@pytest.mark.parametrize("t,group", [(1, 2), (40, 2)])
+def test_attention_scales_at_the_low_end(qb, scale, t, group):
+    """Products of queries and keys up to 10^38, which a scale near the smallest fp32 number, or of 0, brings back."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(t)
+    c = Cache(qb, 2, 2, 331, 128, "bf16").fill(g)
+    c.k *= 1e18
+    q = (torch.randn(2, t, 2 * group, 128, generator=g, device="cuda") * 1e18).bfloat16()
+    _check_attention(qb, c, q, [280, 7], _tree(np.random.RandomState(t), 2, t), scale)
+
+
 def test_attention_many_sequences(qb):
     """More sequences than the shares' search takes in one step, most of them short."""
     import torch

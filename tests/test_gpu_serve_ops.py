@@ -552,6 +552,18 @@ def test_scores_that_are_all_minus_infinity(qb, dtype):
     assert bool((got[0] == 0).all()) and torch.equal(got[1], pool.v[1, 0, 22].expand(2, 64))
 
 
+@pytest.mark.parametrize("scale", [0.0, 2e-38, -2e-38])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_scales_at_the_low_end(qb, scale, dim):
+    """Products of queries and keys up to 10^38, which a scale near the smallest fp32 number, or of 0, brings back."""
+    import torch
+    q, k, v = _rows(18, 260, 4, 260, 2, dim, torch.bfloat16)
+    _check_prompt(qb, q * 1e18, k * 1e18, v, [0, 260], None, scale)
+    pool = Pool(qb, [list(range(20))] * 3, 20, 2, 16, dim, "bf16").fill(_gen(2))
+    pool.k *= 1e18
+    _check_paged(qb, pool, q[:3] * 1e18, [300, 40, 0], scale)
+
+
 # One key with the weight 1, 8,191 with 2^-tail each and large values: the weights enter the product in fp16, whose steps
 # below 2^-14 are 2^-24, in a unit of at most 2^-7 of the largest weight (8-bit pages: divided by the value's scale, at least a half of the
 # unit's); half a step off each, beside the relative roundings: weight and result 2^-11 each, 2^-18 for exponents and sums.
