@@ -21,8 +21,9 @@
 // memory, one launch.
 //
 // Measured: 128 ragged sequences up to 8191 over 1.08 GB of e4m3 pages 179 to 187 us (5.8 to 6.0 TB/s, floor 165), bound by memory traffic;
-// 32 over 35 MB of int8 pages, seven heads of 64 each, 16.5 us (floor 5.4), by the plan, the first
-// loads and the joining; one sequence at 1024 6.3 us (floor 0.6), by its latencies (two launches: 8.5 us).
+// 32 over 35 MB of int8 pages, seven heads of 64 each, 16.5 to 16.9 us (floor 5.4), by the plan, the first
+// loads and the joining; one sequence at 1024 6.3 us (floor 0.6), by its latencies (in a table of more than 2,048 positions, which takes
+// two launches, 8.6 us).
 #pragma once
 #include <cooperative_groups.h>
 

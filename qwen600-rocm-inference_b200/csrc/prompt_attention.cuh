@@ -17,17 +17,18 @@
 // next tile's is formed while the softmax is at work, and no chain runs from a tile's P over its product
 // to the next S.
 //
-// Measured (bf16, 16 query heads over 8 K/V heads of 128): one prompt of 8192 224 us, 1,227 TFLOP/s, where a large
-// matrix product has 1,637 for a moment and 1,370 for long (floor 168 us); 2048 38 us; four of 4096 248 us.
-// Heads of 64: one of 8192 208 to 248 us, bound by the softmax in the same way.
+// Measured (bf16, 16 query heads over 8 K/V heads of 128): one prompt of 8192 220 to 232 us, 1,185 to 1,250
+// TFLOP/s, where a large matrix product has 1,637 for a moment and 1,370 for long (floor 168 us; without a pause for seconds 257 to
+// 263 us); 2048 37 us; four of 4096 245 us.  Heads of 64: one of 8192 205 to 248 us, bound by the softmax in the same way.
+// Many short prompts: 100 of 50 33 us, 500 272, 2000 4,350 (floor 188): an item is found by a search over all sequences, which the
+// other warps wait for.  Few queries over a long context: 5 over 40,000 425 us (floor 25), as keys are not divided.
 // Bound by the softmax warps: a tile of 256 x 128 takes 3,350 cycles, of which the tensor cores need 2,050 at
 // their rate and 2,500 as they run (both operands of S come from shared memory), the exponentials 2,050; the warps
 // issue in 54 % of the slots, each waiting for its own chain: scores (300 cycles), maximum and its exchange
 // (800), exponentials (1,400), waits that find their barriers ready (100 to 200 each).  Steps on the way: one thread a row, P
 // over S, products issued by a lane alone 374 us; descriptors in uniform registers and registers shared out anew 273; one S for both tiles
-// with two threads a row 255; a warp each for the two products 232; fewer polls 224.  Tried, not kept: a part of the exponentials by a
-// polynomial (as fast or slower: the instructions cost what the special-function unit spares), turns of A and B at the
-// exponentials (235 us).
+// with two threads a row 255; a warp each for the two products 232; all exponentials by the special-function unit 224 (a polynomial for a
+// part of them cost more instructions than it spared).  Tried, not kept: turns of A and B at the exponentials (235 us).
 //
 // Warps: 0-7 softmax and output of A (two threads a row, 64 keys of a tile and half of the dims each; they agree on
 // the row's maximum through shared memory), 8-15 of B, 16 finds the items and loads (TMA), 17 issues
