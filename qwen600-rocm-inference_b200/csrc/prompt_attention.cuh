@@ -262,7 +262,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     using namespace qb::tc;
     using L = Layout<D>;
     constexpr bool BF = T == QWEN_BF16;
-    // fp16 weights lie below 2^15: the largest one has at least 2^7, so what is lost under fp16's smallest steps is 2^-32 of it and less
+    // fp16 weights are at most 2^15: the largest one has at least 2^7, so what is lost under fp16's smallest steps is 2^-32 of it and less
     // (with 2^0, 8,000 keys of 2^-25 each were nothing).  bf16 has fp32's range.
     constexpr float kLift = BF ? 0.0f : 7.0f;
     extern __shared__ uint8_t smem_raw[];
@@ -425,16 +425,16 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             }
             __syncwarp();
         }
-        if (*fault && lane == 0) {             // nothing may still be on its way when the CTA ends
-            for (int v = 0; v < 2; v++)
-                for (uint32_t p = parts[v] > (uint32_t)L::kSlots ? parts[v] - L::kSlots : 0; p < parts[v]; p++)
-                    mbar_wait(&full[2 * (p % L::kSlots) + v], p / L::kSlots & 1u, 10000000ull);
-            for (int w = 0; w < 2; w++) if (used[w]) mbar_wait(&qfull[w], (used[w] - 1) & 1u, 10000000ull);
-        }
-        __syncwarp();
         finish();
-        if (*fault) {                          // (nobody sets it any more) no row that this CTA had may pass for a result
-            const int pieces = P.group * D / 8;
+        if (*fault) {                          // (nobody sets it any more)
+            if (lane == 0) {                   // nothing may still be on its way when the CTA ends
+                for (int v = 0; v < 2; v++)
+                    for (uint32_t p = parts[v] > (uint32_t)L::kSlots ? parts[v] - L::kSlots : 0; p < parts[v]; p++)
+                        mbar_wait(&full[2 * (p % L::kSlots) + v], p / L::kSlots & 1u, 10000000ull);
+                for (int w = 0; w < 2; w++) if (used[w]) mbar_wait(&qfull[w], (used[w] - 1) & 1u, 10000000ull);
+            }
+            __syncwarp();
+            const int pieces = P.group * D / 8;   // no row that this CTA had may pass for a result
             for (int k = 0; deal(k); k++)
                 for (int r = 0; r < it.nq; r++) {
                     uint4* row = reinterpret_cast<uint4*>(P.out + ((size_t)(it.q0 + r) * P.ldo + (size_t)it.h * P.group * D) * 2);
